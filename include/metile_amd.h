@@ -43,7 +43,9 @@ typedef enum mt_status {
   MT_ERR_HIP = -3               /* a HIP runtime call failed (launch error) */
 } mt_status;
 
-typedef enum mt_dtype { MT_BF16 = 0, MT_F16 = 1 } mt_dtype;
+/* MT_F32 and MT_FP8 (8-bit floats, e4m3 without infinities) are types of single operands where an
+ * entry point says so; everything else is MT_BF16 or MT_F16. */
+typedef enum mt_dtype { MT_BF16 = 0, MT_F16 = 1, MT_F32 = 2, MT_FP8 = 3 } mt_dtype;
 
 /* Library version string. */
 const char* mt_version(void);
@@ -349,6 +351,96 @@ int mt_plans_clear(void);
  * persistent tuning key that retires decisions when the kernels change, as the reference's
  * source-hash keys do (metile/backends/mlx_quantized.py:1393-1427). */
 const char* mt_source_digest(void);
+
+/* ---- the decode step around the projections: paged key-value cache, norms ------------------ */
+
+/* No counterparts in the reference, whose decode loop leaves these to MLX: they are what a served
+ * decoder needs between its projections. */
+
+/* A paged key-value cache: `pages` pages of `page_size` tokens, `heads` key-value heads of `dim`
+ * values. Strides are in elements, in the order page, token, head; a head's values are contiguous.
+ * Held in 16 bits (dtype MT_BF16 or MT_F16) or as 8-bit floats (MT_FP8), which stand for themselves
+ * times key_scale or value_scale (both 1 otherwise). dim is a multiple of 16 up to 256; pages *
+ * page_size is below 2^31; key, value and all strides are multiples of 16 bytes. */
+typedef struct mt_paged_cache {
+  void* key;
+  void* value;
+  int64_t key_strides[3];
+  int64_t value_strides[3];
+  int pages, page_size, heads, dim;
+  int dtype;
+  float key_scale, value_scale;
+} mt_paged_cache;
+
+/* Block tables and slot maps of a step, from the requests' lengths on the device.
+ *
+ * Request r has cached[r] tokens in the cache and new_tokens[r] in the step (negative counts are 0).
+ * Its table, row r of block_tables ([requests, width], rows table_stride entries apart), holds the
+ * pages of its cached tokens; the pages its new tokens need on top are taken in order from
+ * free_pages ([free_count]), beginning with entry *free_start (NULL: 0), request by request, and
+ * written into the table. Outputs: starts [requests + 1], the first token of each request in the
+ * step's packed batch; lengths [requests], cached + new; for each of the `tokens` tokens of the
+ * batch its slot (page * page_size + place in the page), position in its request and request;
+ * taken [1], the pages that the step needed. Tokens behind the last request's (padding) get slot
+ * -1, position 0, request -1; tokens that the table's width or the free list has no page for get
+ * slot -1 (and an exhausted list writes -1 into the table, with `taken` telling the shortage).
+ * Tokens beyond `tokens` are dropped with the table entries of the pages they open. width *
+ * page_size is below 2^31; sums of counts stop at 2^31 - 1. requests or tokens may be 0. */
+int mt_paged_tables(const int32_t* cached, const int32_t* new_tokens, int requests,
+                    int32_t* block_tables, int64_t table_stride, int width,
+                    const int32_t* free_pages, int free_count, const int32_t* free_start,
+                    int page_size, int64_t* slots, int32_t* positions, int32_t* token_requests,
+                    int tokens, int32_t* starts, int32_t* lengths, int32_t* taken, void* stream);
+
+/* Writes a step's keys and values, [tokens, heads, dim] 16-bit (dtype) with element strides per
+ * token and head, to the cache at slots[token]; tokens whose slot is not in [0, pages * page_size)
+ * are left out. Slots that occur twice get one of their rows or a mixture. 8-bit caches hold
+ * value / scale rounded to nearest even and limited to +-448. A 16-bit cache has the rows' dtype.
+ * Rows and strides are multiples of 16 bytes; tokens * heads * dim / 8 is below 2^31. */
+int mt_paged_append(const mt_paged_cache* cache, const void* key, const void* value,
+                    int64_t key_token_stride, int64_t key_head_stride, int64_t value_token_stride,
+                    int64_t value_head_stride, const int64_t* slots, int64_t tokens, int dtype,
+                    void* stream);
+
+/* Attention of one new token per request over its pages: out[r, h] = sum_t p_t v_t with p =
+ * softmax(scale * q[r, h] . k_t) over the request's last `window` tokens (0: all of them), of the
+ * key-value head h / (heads / cache heads). lengths[r] counts the tokens in the cache, the new one
+ * among them (its key and value are appended first); it is limited to [0, width * page_size]. Rows
+ * without a token give 0. lse (or NULL) [requests, heads] receives log sum exp of the scaled
+ * scores, -inf for such rows. Table entries behind a request's last token are not read; tokens
+ * whose entry is not a page of the cache are left out, and what slots behind the last token hold
+ * does not matter. query [requests, heads, dim] with element strides per request and head
+ * (multiples of 16 bytes), out [requests, heads, dim] contiguous, 16-byte aligned, both in dtype;
+ * a 16-bit cache has the same. Sums are fp32 and in a fixed order: results do not change from run
+ * to run. Results of a call depend on its workgroup count only in that order. */
+size_t mt_paged_attention_workspace_bytes(const mt_paged_cache* cache, int requests, int heads,
+                                          int width, int window);
+int mt_paged_attention(const mt_paged_cache* cache, const void* query, int64_t query_stride,
+                       int64_t query_head_stride, const int32_t* block_tables,
+                       int64_t table_stride, int width, const int32_t* lengths, int requests,
+                       int heads, float scale, int window, void* out, float* lse, int dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+typedef enum mt_norm_kind { MT_NORM_RMS = 0, MT_NORM_LAYER = 1 } mt_norm_kind;
+
+/* The norms around a block, its gate and the scaled residual, [rows, width], in one pass:
+ *
+ *   r = residual_scale * residual + gate * post(block)      normed = pre(r)
+ *
+ * pre and post are rms norms x / sqrt(mean(x^2) + eps) * w (+ b) or layer norms (x - mean) /
+ * sqrt(var + eps) * w (+ b), of all `width` values (up to 65536); without post_weight, post is the
+ * identity. block may be NULL (then r = residual_scale * residual, and post and gate are not read).
+ * gate (or NULL: 1) holds a row of width values, or one value with gate_scalar, for each gate_rows
+ * rows, gate_stride elements apart (0: one for all). residual is in residual_dtype (dtype or
+ * MT_F32), as is residual_out (contiguous; NULL: not written; it may be residual itself where that
+ * is contiguous); everything else is in dtype. All arithmetic is fp32; each output is rounded once,
+ * and pre sees r before its rounding. Pointers need the alignment of their type only. */
+int mt_residual_norm(const void* residual, int64_t residual_stride, const void* block,
+                     int64_t block_stride, const void* weight, const void* bias,
+                     const void* post_weight, const void* post_bias, const void* gate,
+                     int64_t gate_stride, int gate_rows, int gate_scalar, void* residual_out,
+                     void* normed, int rows, int width, float residual_scale, float eps, int kind,
+                     int dtype, int residual_dtype, void* stream);
 
 /* ---- measurement -------------------------------------------------------------------------- */
 

@@ -4,7 +4,8 @@ Affine 4/8-bit quantized QMV, fused SwiGLU, the quantized MLP and dense 16-bit s
 projections, written as hand-written HIP kernels behind a C ABI (``include/metile_amd.h``) and
 exposed here on torch tensors with the reference's call surface
 (``metile/backends/mlx_quantized.py``), with the reference tuner's fidelity gates and native
-compositions for checking kernels against its semantics.
+compositions for checking kernels against its semantics. Around the projections: a paged
+key-value cache with its tables, append and decode attention, and the norms between blocks.
 """
 
 from ._lib import MetileError, version
@@ -18,6 +19,8 @@ from .model import (
     restore_patches,
 )
 from .native import native_affine_matmul, native_affine_residual_qmv, native_affine_swiglu
+from .norms import residual_norm
+from .paged import PagedCache, PagedStep, paged_append, paged_attention, paged_tables
 from .quantize import CompressedDownWeight, affine_quantize
 from .quantized import (
     AffineWeight,
@@ -58,6 +61,12 @@ __all__ = [
     "native_affine_matmul",
     "native_affine_residual_qmv",
     "native_affine_swiglu",
+    "PagedCache",
+    "PagedStep",
+    "paged_append",
+    "paged_attention",
+    "paged_tables",
+    "residual_norm",
     "dense_qmv",
     "dense_swiglu",
     "mlx_dense_residual_qmv",

@@ -19,6 +19,11 @@ MT_ERR_HIP = -3
 
 MT_BF16 = 0
 MT_F16 = 1
+MT_F32 = 2
+MT_FP8 = 3
+
+MT_NORM_RMS = 0
+MT_NORM_LAYER = 1
 
 MT_QMV_STAGED = 1
 MT_QMV_REGISTER = 2
@@ -57,13 +62,26 @@ class DensePlan(ctypes.Structure):
     _fields_ = [("ksplit", ctypes.c_int)]
 
 
+class PagedCacheDesc(ctypes.Structure):
+    """``mt_paged_cache``."""
+
+    _fields_ = [("key", ctypes.c_void_p), ("value", ctypes.c_void_p),
+                ("key_strides", ctypes.c_int64 * 3), ("value_strides", ctypes.c_int64 * 3),
+                ("pages", ctypes.c_int), ("page_size", ctypes.c_int), ("heads", ctypes.c_int),
+                ("dim", ctypes.c_int), ("dtype", ctypes.c_int), ("key_scale", ctypes.c_float),
+                ("value_scale", ctypes.c_float)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_int64
+_F = ctypes.c_float
 _Z = ctypes.c_size_t
 _QP = ctypes.POINTER(QmvPlan)
 _RP = ctypes.POINTER(RowsPlan)
 _GP = ctypes.POINTER(GemmPlan)
 _DP = ctypes.POINTER(DensePlan)
+_CP = ctypes.POINTER(PagedCacheDesc)
 
 # name -> (restype, argtypes); mirrors include/metile_amd.h exactly.
 SIGNATURES = {
@@ -107,6 +125,14 @@ SIGNATURES = {
     "mt_dense_qmv_plan": (_I, [_I, _I, _I, _I, _DP]),
     "mt_dense_qmv_plan_candidates": (_I, [_I, _I, _I, _DP, _I]),
     "mt_dense_qmv_plan_set": (_I, [_I, _I, _I, _I, _DP]),
+    "mt_paged_tables": (_I, [_P, _P, _I, _P, _L, _I, _P, _I, _P, _I, _P, _P, _P, _I, _P, _P, _P,
+                             _P]),
+    "mt_paged_append": (_I, [_CP, _P, _P, _L, _L, _L, _L, _P, _L, _I, _P]),
+    "mt_paged_attention_workspace_bytes": (_Z, [_CP, _I, _I, _I, _I]),
+    "mt_paged_attention": (_I, [_CP, _P, _L, _L, _P, _L, _I, _P, _I, _I, _F, _I, _P, _P, _I, _P,
+                                _Z, _P]),
+    "mt_residual_norm": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _P, _P, _I, _I, _F,
+                              _F, _I, _I, _I, _P]),
     "mt_plans_clear": (_I, []),
     "mt_source_digest": (ctypes.c_char_p, []),
 }

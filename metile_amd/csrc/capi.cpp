@@ -1446,11 +1446,13 @@ int affine_mlp_impl(const char* op, const void* x, const uint32_t* gate_w,
 
 }  // namespace
 
-// Entry points in other source files that bring their own workspace (noalloc.hip) reach the MLP
-// path and the error slot through these.
+// Entry points in other source files (noalloc.hip, decode_capi.cpp) reach the MLP path, the error
+// slot and the device's size through these.
 namespace mt {
 
 int set_last_error(int status, const std::string& msg) { return fail(status, msg); }
+
+int current_device_cus() { return device_cus(); }
 
 size_t affine_mlp_workspace(int M, int H, int I, int group_size, int bits) {
   if (check_affine("mt_affine_mlp", M, H, I, group_size, bits, MT_BF16) ||

@@ -15,6 +15,9 @@ constexpr size_t kWorkspaceCounterBytes = 64 * 1024;
 // Records `msg` as the calling thread's last error (mt_last_error) and returns `status`.
 int set_last_error(int status, const std::string& msg);
 
+// Compute units of the current device.
+int current_device_cus();
+
 // Workspace bytes without which mt_affine_mlp refuses this shape (0 for a shape it rejects).
 size_t affine_mlp_workspace(int M, int H, int I, int group_size, int bits);
 

@@ -1,0 +1,291 @@
+// extern "C" boundary of the decode-step operators around the projections: block tables and slot
+// maps, cache append, paged attention and residual norms. Argument checks and launches only; no
+// allocation of device memory, no synchronisation, no exceptions across the ABI.
+#include "../../include/metile_amd.h"
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "capi_internal.h"
+#include "paged.h"
+#include "residual_norm.h"
+
+namespace {
+
+constexpr int64_t kInt31 = (int64_t)1 << 31;
+constexpr int kMaxHeads = 65536;
+
+int refuse(const char* op, const char* what) {
+  return mt::set_last_error(MT_ERR_INVALID_ARGUMENT, std::string(op) + ": " + what);
+}
+
+int launched(const char* op, hipError_t e) {
+  if (e == hipSuccess) return MT_OK;
+  return mt::set_last_error(MT_ERR_HIP, std::string(op) + ": " + hipGetErrorString(e));
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Strides of `bytes`-wide elements that are whole 16-byte steps and not negative.
+bool stride16(int64_t stride, int bytes) {
+  return stride >= 0 && stride < kInt31 * 256 && stride * bytes % 16 == 0;
+}
+
+int check_cache(const char* op, const mt_paged_cache* c) {
+  if (!c) return refuse(op, "null cache");
+  if (c->dtype != MT_BF16 && c->dtype != MT_F16 && c->dtype != MT_FP8)
+    return refuse(op, "cache dtype must be MT_BF16, MT_F16 or MT_FP8");
+  if (c->pages < 1 || c->page_size < 1 || (int64_t)c->pages * c->page_size >= kInt31)
+    return refuse(op, "pages and page_size must be positive and hold fewer than 2^31 tokens");
+  if (c->heads < 1 || c->heads > kMaxHeads) return refuse(op, "cache heads must be positive");
+  if (c->dim < 16 || c->dim > 256 || c->dim % 16)
+    return refuse(op, "head dim must be a multiple of 16 up to 256");
+  const int bytes = c->dtype == MT_FP8 ? 1 : 2;
+  for (int i = 0; i < 3; ++i)
+    if (!stride16(c->key_strides[i], bytes) || !stride16(c->value_strides[i], bytes))
+      return refuse(op, "cache strides must be multiples of 16 bytes");
+  if (!c->key || !c->value) return refuse(op, "null cache pointer");
+  if (!aligned16(c->key) || !aligned16(c->value))
+    return refuse(op, "cache must be 16-byte aligned");
+  const float scales[2] = {c->key_scale, c->value_scale};
+  for (float s : scales)
+    if (!(s > 0.0f) || !std::isnormal(s) || !std::isnormal(1.0f / s))
+      return refuse(op, "cache scales must be positive and normal");
+  if (c->dtype != MT_FP8 && (c->key_scale != 1.0f || c->value_scale != 1.0f))
+    return refuse(op, "a 16-bit cache has scales of 1");
+  return MT_OK;
+}
+
+// Tiles of the longest request the table holds, and of all requests and heads.
+int64_t most_tiles(int64_t most, int window) {
+  if (window > 0 && window + 31ll < most) most = window + 31ll;
+  const int64_t n = (most + mt::kAttentionTile - 1) / mt::kAttentionTile;
+  return n > 0 ? n : 1;
+}
+
+struct AttentionPlan {
+  int workgroups;
+  size_t bytes;
+};
+
+int plan_attention(const char* op, const mt_paged_cache* c, int requests, int heads, int width,
+                   int window, AttentionPlan* plan) {
+  if (const int st = check_cache(op, c)) return st;
+  if (requests < 1) return refuse(op, "requests must be positive");
+  if (heads < 1 || heads > kMaxHeads || heads % c->heads)
+    return refuse(op, "query heads must be a positive multiple of the cache's");
+  if (width < 1 || (int64_t)width * c->page_size >= kInt31)
+    return refuse(op, "block table width must be positive and hold fewer than 2^31 tokens");
+  if (window < 0) return refuse(op, "window must not be negative");
+  const int group = heads / c->heads, head_tiles = (group + 15) / 16;
+  const int64_t tiles = most_tiles((int64_t)width * c->page_size, window);
+  const int64_t rows = (int64_t)c->heads * head_tiles;
+  if (tiles * rows >= kInt31 || tiles * requests >= kInt31)
+    return refuse(op, "block tables too large");
+  plan->workgroups =
+      mt::paged_attention_workgroups(mt::current_device_cus(), tiles * rows * requests);
+  plan->bytes = mt::kWorkspaceCounterBytes +
+                (size_t)plan->workgroups * 2 * mt::paged_attention_slot_floats(group, c->dim) * 4;
+  return MT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mt_paged_tables(const int32_t* cached, const int32_t* new_tokens, int requests,
+                    int32_t* block_tables, int64_t table_stride, int width,
+                    const int32_t* free_pages, int free_count, const int32_t* free_start,
+                    int page_size, int64_t* slots, int32_t* positions, int32_t* token_requests,
+                    int tokens, int32_t* starts, int32_t* lengths, int32_t* taken, void* stream) {
+  const char* op = "mt_paged_tables";
+  if (requests < 0 || tokens < 0 || free_count < 0)
+    return refuse(op, "counts must not be negative");
+  if (page_size < 1 || width < 1 || (int64_t)width * page_size >= kInt31)
+    return refuse(op, "page_size and width must be positive and hold fewer than 2^31 tokens");
+  if (requests > 1 && table_stride < width) return refuse(op, "block table rows overlap");
+  if ((requests && (!cached || !new_tokens || !block_tables || !lengths)) ||
+      (free_count && !free_pages) || (tokens && (!slots || !positions || !token_requests)) ||
+      !starts || !taken)
+    return refuse(op, "null pointer");
+  mt::PagedTablesArgs a{};
+  a.cached = cached;
+  a.fresh = new_tokens;
+  a.tables = block_tables;
+  a.table_stride = table_stride;
+  a.free_pages = free_pages;
+  a.free_start = free_start;
+  a.slots = slots;
+  a.positions = positions;
+  a.requests = token_requests;
+  a.starts = starts;
+  a.lengths = lengths;
+  a.taken = taken;
+  a.num_requests = requests;
+  a.width = width;
+  a.page_size = page_size;
+  a.free_count = free_count;
+  a.tokens = tokens;
+  return launched(op, mt::launch_paged_tables(a, mt::current_device_cus(),
+                                              static_cast<hipStream_t>(stream)));
+}
+
+int mt_paged_append(const mt_paged_cache* cache, const void* key, const void* value,
+                    int64_t key_token_stride, int64_t key_head_stride, int64_t value_token_stride,
+                    int64_t value_head_stride, const int64_t* slots, int64_t tokens, int dtype,
+                    void* stream) {
+  const char* op = "mt_paged_append";
+  if (const int st = check_cache(op, cache)) return st;
+  if (dtype != MT_BF16 && dtype != MT_F16) return refuse(op, "dtype must be MT_BF16 or MT_F16");
+  if (cache->dtype != MT_FP8 && cache->dtype != dtype)
+    return refuse(op, "a 16-bit cache must have the rows' dtype");
+  if (tokens < 0 || tokens >= kInt31 || tokens * cache->heads * (cache->dim / 8) >= kInt31)
+    return refuse(op, "tokens must not be negative, and tokens * heads * dim / 8 below 2^31");
+  if (tokens == 0) return MT_OK;
+  if (!key || !value || !slots) return refuse(op, "null pointer");
+  if (!aligned16(key) || !aligned16(value) || !stride16(key_token_stride, 2) ||
+      !stride16(key_head_stride, 2) || !stride16(value_token_stride, 2) ||
+      !stride16(value_head_stride, 2))
+    return refuse(op, "rows and their strides must be multiples of 16 bytes");
+  const bool fp8 = cache->dtype == MT_FP8;
+  const int bytes = fp8 ? 1 : 2;
+  mt::PagedAppendArgs a{};
+  for (int i = 0; i < 2; ++i) {
+    mt::PagedSide& s = a.side[i];
+    const int64_t* strides = i ? cache->value_strides : cache->key_strides;
+    s.cache = static_cast<unsigned char*>(i ? cache->value : cache->key);
+    s.page_stride = strides[0] * bytes;
+    s.slot_stride = strides[1] * bytes;
+    s.head_stride = strides[2] * bytes;
+    s.rows = static_cast<const unsigned char*>(i ? value : key);
+    s.row_stride = (i ? value_token_stride : key_token_stride) * 2;
+    s.row_head_stride = (i ? value_head_stride : key_head_stride) * 2;
+    s.scale = i ? cache->value_scale : cache->key_scale;
+    s.inv_scale = 1.0f / s.scale;
+  }
+  a.slots = slots;
+  a.tokens = tokens;
+  a.pages = cache->pages;
+  a.page_size = cache->page_size;
+  a.heads = cache->heads;
+  a.dim = cache->dim;
+  a.by_row = mt::div_magic((uint32_t)(cache->heads * (cache->dim / 8)));
+  a.by_head = mt::div_magic((uint32_t)(cache->dim / 8));
+  a.by_page = mt::div_magic((uint32_t)cache->page_size);
+  return launched(op, mt::launch_paged_append(a, dtype, fp8, static_cast<hipStream_t>(stream)));
+}
+
+size_t mt_paged_attention_workspace_bytes(const mt_paged_cache* cache, int requests, int heads,
+                                          int width, int window) {
+  AttentionPlan plan;
+  if (plan_attention("mt_paged_attention_workspace_bytes", cache, requests, heads, width, window,
+                     &plan))
+    return 0;
+  return plan.bytes;
+}
+
+int mt_paged_attention(const mt_paged_cache* cache, const void* query, int64_t query_stride,
+                       int64_t query_head_stride, const int32_t* block_tables,
+                       int64_t table_stride, int width, const int32_t* lengths, int requests,
+                       int heads, float scale, int window, void* out, float* lse, int dtype,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "mt_paged_attention";
+  AttentionPlan plan;
+  if (const int st = plan_attention(op, cache, requests, heads, width, window, &plan)) return st;
+  if (dtype != MT_BF16 && dtype != MT_F16) return refuse(op, "dtype must be MT_BF16 or MT_F16");
+  if (cache->dtype != MT_FP8 && cache->dtype != dtype)
+    return refuse(op, "a 16-bit cache must have the query's dtype");
+  if (!std::isfinite(scale)) return refuse(op, "scale must be finite");
+  if (!query || !block_tables || !lengths || !out) return refuse(op, "null pointer");
+  if (!aligned16(query) || !aligned16(out) || !stride16(query_stride, 2) ||
+      !stride16(query_head_stride, 2))
+    return refuse(op, "query, its strides and out must be multiples of 16 bytes");
+  if (requests > 1 && table_stride < 0) return refuse(op, "block table rows must be in order");
+  if (!workspace || workspace_bytes < plan.bytes)
+    return mt::set_last_error(MT_ERR_WORKSPACE,
+                              std::string(op) + ": workspace smaller than required");
+  const bool fp8 = cache->dtype == MT_FP8;
+  const int64_t bytes = fp8 ? 1 : 2;
+  mt::PagedAttentionArgs a{};
+  a.query = static_cast<const uint16_t*>(query);
+  a.q_row_stride = query_stride;
+  a.q_head_stride = query_head_stride;
+  a.key = static_cast<const unsigned char*>(cache->key);
+  a.value = static_cast<const unsigned char*>(cache->value);
+  a.k_page = cache->key_strides[0] * bytes;
+  a.k_slot = cache->key_strides[1] * bytes;
+  a.k_head = cache->key_strides[2] * bytes;
+  a.v_page = cache->value_strides[0] * bytes;
+  a.v_slot = cache->value_strides[1] * bytes;
+  a.v_head = cache->value_strides[2] * bytes;
+  a.tables = block_tables;
+  a.table_stride = table_stride;
+  a.lengths = lengths;
+  a.out = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  a.counters = static_cast<uint32_t*>(workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
+                                       mt::kWorkspaceCounterBytes);
+  a.requests = requests;
+  a.kv_heads = cache->heads;
+  a.group = heads / cache->heads;
+  a.head_tiles = (a.group + 15) / 16;
+  a.dim = cache->dim;
+  a.pages = cache->pages;
+  a.page_size = cache->page_size;
+  a.width = width;
+  a.window = window;
+  a.scale_log2 = scale * cache->key_scale * 1.4426950408889634f;
+  a.value_scale = cache->value_scale;
+  a.by_page = mt::div_magic((uint32_t)cache->page_size);
+  return launched(op, mt::launch_paged_attention(a, dtype, fp8, plan.workgroups,
+                                                 static_cast<hipStream_t>(stream)));
+}
+
+int mt_residual_norm(const void* residual, int64_t residual_stride, const void* block,
+                     int64_t block_stride, const void* weight, const void* bias,
+                     const void* post_weight, const void* post_bias, const void* gate,
+                     int64_t gate_stride, int gate_rows, int gate_scalar, void* residual_out,
+                     void* normed, int rows, int width, float residual_scale, float eps, int kind,
+                     int dtype, int residual_dtype, void* stream) {
+  const char* op = "mt_residual_norm";
+  if (dtype != MT_BF16 && dtype != MT_F16) return refuse(op, "dtype must be MT_BF16 or MT_F16");
+  if (residual_dtype != dtype && residual_dtype != MT_F32)
+    return refuse(op, "residual_dtype must be dtype or MT_F32");
+  if (kind != MT_NORM_RMS && kind != MT_NORM_LAYER)
+    return refuse(op, "kind must be MT_NORM_RMS or MT_NORM_LAYER");
+  if (width < 1 || width > mt::kNormMaxWidth) return refuse(op, "width must be 1 to 65536");
+  if (rows < 0) return refuse(op, "rows must not be negative");
+  if (!(eps >= 0.0f) || !std::isfinite(eps)) return refuse(op, "eps must be finite and >= 0");
+  if (!std::isfinite(residual_scale)) return refuse(op, "residual_scale must be finite");
+  if (gate && (gate_rows < 1 || gate_stride < 0))
+    return refuse(op, "gate_rows must be positive and gate_stride not negative");
+  if (rows == 0) return MT_OK;
+  if (!residual || !weight || !normed) return refuse(op, "null pointer");
+  mt::ResidualNormArgs a{};
+  a.residual = residual;
+  a.block = static_cast<const uint16_t*>(block);
+  a.weight = static_cast<const uint16_t*>(weight);
+  a.bias = static_cast<const uint16_t*>(bias);
+  a.post_weight = static_cast<const uint16_t*>(post_weight);
+  a.post_bias = static_cast<const uint16_t*>(post_bias);
+  a.gate = static_cast<const uint16_t*>(gate);
+  a.residual_out = residual_out;
+  a.normed = static_cast<uint16_t*>(normed);
+  a.residual_stride = residual_stride;
+  a.block_stride = block_stride;
+  a.gate_stride = gate_stride;
+  a.rows = rows;
+  a.width = width;
+  a.gate_rows = gate ? gate_rows : 1;
+  a.gate_scalar = gate_scalar;
+  a.scale = residual_scale;
+  a.eps = eps;
+  return launched(op, mt::launch_residual_norm(a, dtype, residual_dtype == MT_F32,
+                                               kind == MT_NORM_LAYER, mt::current_device_cus(),
+                                               static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -1,0 +1,86 @@
+// Host-visible launch interfaces of the paged key-value cache: block tables and slot maps, the
+// append of a step's keys and values, and decode attention over the pages.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace mt {
+
+// Division of n in [0, 2^31) by a constant d in [1, 2^31): n / d = (n * mul) >> shift, exact, since
+// mul = ceil(2^shift / d) with shift = 31 + ceil(log2 d) errs by less than d <= 2^(shift - 31).
+struct DivMagic {
+  uint32_t mul, shift;
+};
+inline DivMagic div_magic(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t n, DivMagic m) {
+  return (uint32_t)(((uint64_t)n * m.mul) >> m.shift);
+}
+
+struct PagedTablesArgs {
+  const int32_t* cached;   // [R] tokens already in the cache
+  const int32_t* fresh;    // [R] new tokens of the step
+  int32_t* tables;         // [R, width], rows `table_stride` entries apart
+  int64_t table_stride;
+  const int32_t* free_pages;  // [free_count]
+  const int32_t* free_start;  // first entry of free_pages to take, or null for 0
+  int64_t* slots;          // [tokens]
+  int32_t* positions;      // [tokens]
+  int32_t* requests;       // [tokens]
+  int32_t* starts;         // [R + 1]
+  int32_t* lengths;        // [R]
+  int32_t* taken;          // [1] pages the step takes
+  int32_t num_requests, width, page_size, free_count, tokens;
+};
+hipError_t launch_paged_tables(const PagedTablesArgs& a, int cus, hipStream_t stream);
+
+// One side (keys or values) of a cache and of the rows written to it. Strides in bytes.
+struct PagedSide {
+  unsigned char* cache;
+  int64_t page_stride, slot_stride, head_stride;
+  const unsigned char* rows;
+  int64_t row_stride, row_head_stride;
+  float scale, inv_scale;  // of an 8-bit cache
+};
+struct PagedAppendArgs {
+  PagedSide side[2];
+  const int64_t* slots;
+  int64_t tokens;
+  int32_t pages, page_size, heads, dim;
+  DivMagic by_row, by_head, by_page;  // chunks of a token, chunks of a head, slots of a page
+};
+hipError_t launch_paged_append(const PagedAppendArgs& a, int dtype, bool fp8, hipStream_t stream);
+
+struct PagedAttentionArgs {
+  const uint16_t* query;           // [R, heads, dim], last dimension contiguous
+  int64_t q_row_stride, q_head_stride;  // elements
+  const unsigned char* key;
+  const unsigned char* value;
+  int64_t k_page, k_slot, k_head;  // bytes
+  int64_t v_page, v_slot, v_head;
+  const int32_t* tables;           // [R, width], rows `table_stride` entries apart
+  int64_t table_stride;
+  const int32_t* lengths;          // [R]
+  uint16_t* out;                   // [R, heads, dim] contiguous
+  float* lse;                      // [R, heads] or null
+  float* partial;
+  uint32_t* counters;
+  int32_t requests, kv_heads, group, head_tiles;  // group: query heads of a kv head
+  int32_t dim, pages, page_size, width, window;   // window 0: none
+  float scale_log2, value_scale;
+  DivMagic by_page;
+};
+// Workgroups of a call and floats of one partial slot (two slots a workgroup).
+int paged_attention_workgroups(int cus, int64_t units);
+size_t paged_attention_slot_floats(int group, int dim);
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, int dtype, bool fp8, int workgroups,
+                                  hipStream_t stream);
+
+constexpr int kAttentionTile = 128;  // tokens a workgroup takes at a time
+
+}  // namespace mt

@@ -1,0 +1,278 @@
+"""The paged key-value cache of a decode step (gfx950 HIP kernels via the C ABI).
+
+A cache is a pool of pages of ``page_size`` tokens; each request has a row of a block table with
+the numbers of its pages, in order. One step of a serving loop:
+
+* :func:`paged_tables` turns the requests' lengths into the pages they need on top, block-table
+  entries and the slot of every new token, on the GPU;
+* :func:`paged_append` writes the step's keys and values to their slots;
+* :func:`paged_attention` attends from one new token of each request over its pages.
+
+The reference has no counterparts: its decode loop leaves cache and attention to MLX.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .quantized import _stream_handle, workspace
+
+_DTYPES = {torch.bfloat16: _lib.MT_BF16, torch.float16: _lib.MT_F16}
+_CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.MT_FP8}
+
+
+def _same_device(device, *tensors):
+    """All tensors on the ROCm device ``device``, which becomes torch's current one if it is not
+    (kernels are launched on the current device's stream)."""
+    if device.type != "cuda":
+        raise ValueError("metile_amd operators take ROCm device tensors")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError("metile_amd operators take tensors of one ROCm device")
+
+
+def _whole16(t):
+    """``t`` with its values in rows of contiguous last dimension whose start and strides are whole
+    16-byte steps, as the kernels read them; a copy only where it is not so already."""
+    size = t.element_size()
+    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1:
+        for i, n in enumerate(t.shape[:-1]):
+            if n > 1 and t.stride(i) * size % 16:
+                break
+        else:
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class PagedCache:
+    """A paged key-value cache over two tensors ``[pages, page_size, kv_heads, head_dim]``.
+
+    ``key`` and ``value`` may have any strides as long as a head's values are contiguous and all
+    strides are whole 16-byte steps; :meth:`allocate` makes them with a head's tokens of a page next
+    to each other. bfloat16, float16 or float8_e4m3fn; an 8-bit cache holds ``key / key_scale`` and
+    ``value / value_scale``. ``head_dim`` is a multiple of 16 up to 256. The object describes the
+    tensors for the kernels and holds no other state.
+    """
+
+    def __init__(self, key, value, *, key_scale=1.0, value_scale=1.0):
+        if key.ndim != 4 or key.shape != value.shape:
+            raise ValueError("cache keys and values must be [pages, page_size, kv_heads, head_dim] "
+                             "of one shape")
+        if key.dtype not in _CACHE_DTYPES or value.dtype != key.dtype:
+            raise ValueError("cache keys and values must both be bfloat16, float16 or "
+                             "float8_e4m3fn")
+        _same_device(key.device, value)
+        pages, page_size, heads, dim = key.shape
+        if min(key.shape) < 1 or pages * page_size >= 1 << 31:
+            raise ValueError("a cache has at least one page, token and head, and fewer than 2^31 "
+                             "tokens")
+        if dim % 16 or dim > 256:
+            raise ValueError("head_dim must be a multiple of 16 up to 256")
+        for t in (key, value):
+            if t.data_ptr() % 16 or t.stride(3) != 1 or any(
+                    n > 1 and s * t.element_size() % 16 for n, s in zip(t.shape, t.stride()[:3])):
+                raise ValueError("a cache's heads must be contiguous and its strides multiples of "
+                                 "16 bytes")
+        if key.dtype != torch.float8_e4m3fn and (key_scale != 1.0 or value_scale != 1.0):
+            raise ValueError("only 8-bit caches have scales")
+        if not (0.0 < key_scale < float("inf") and 0.0 < value_scale < float("inf")):
+            raise ValueError("cache scales must be positive and finite")
+        self.key, self.value = key, value
+        self.key_scale, self.value_scale = float(key_scale), float(value_scale)
+        self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, heads, dim
+        # strides of dimensions of one element do not matter, whatever torch says they are
+        strides = [[s if n > 1 else 0 for n, s in zip(t.shape, t.stride()[:3])]
+                   for t in (key, value)]
+        self._desc = _lib.PagedCacheDesc(
+            key.data_ptr(), value.data_ptr(), (ctypes.c_int64 * 3)(*strides[0]),
+            (ctypes.c_int64 * 3)(*strides[1]), pages, page_size, heads, dim,
+            _CACHE_DTYPES[key.dtype], self.key_scale, self.value_scale)
+        self._ref = ctypes.byref(self._desc)
+        self._device = key.device
+        self._workspaces = {}  # (requests, heads, width, window) -> bytes
+
+    @classmethod
+    def allocate(cls, pages, page_size, kv_heads, head_dim, *, dtype=torch.bfloat16, device="cuda",
+                 key_scale=1.0, value_scale=1.0):
+        """A cache of uninitialised pages. Kept head by head within a page, so that what one
+        attention workgroup reads of a page is one contiguous run."""
+        shape = (pages, kv_heads, page_size, head_dim)
+        key, value = (torch.empty(shape, dtype=dtype, device=device).transpose(1, 2)
+                      for _ in range(2))
+        return cls(key, value, key_scale=key_scale, value_scale=value_scale)
+
+    def _workspace_bytes(self, *shape):
+        need = self._workspaces.get(shape)
+        if need is None:
+            need = _lib.lib().mt_paged_attention_workspace_bytes(self._ref, *shape)
+            if len(self._workspaces) >= 256:
+                self._workspaces.clear()
+            self._workspaces[shape] = need
+        return need
+
+
+class PagedStep(NamedTuple):
+    """What :func:`paged_tables` gives: for each token of the step's packed batch ``slots`` (int64),
+    ``positions`` and ``requests``; ``starts`` (``[requests + 1]``) and ``lengths`` of the requests;
+    ``taken`` (``[1]``), the pages that the step needed. int32 but for the slots."""
+
+    slots: torch.Tensor
+    positions: torch.Tensor
+    requests: torch.Tensor
+    starts: torch.Tensor
+    lengths: torch.Tensor
+    taken: torch.Tensor
+
+
+def _int32(t, what, ndim=1):
+    if t.dtype != torch.int32 or t.ndim != ndim:
+        raise ValueError(f"{what} must be {'a matrix' if ndim == 2 else 'a vector'} of int32")
+    return t
+
+
+def paged_tables(cached, new, block_tables, free_pages, *, page_size, tokens, free_start=None):
+    """Pages, block-table entries and slots of a step whose lengths only the GPU knows.
+
+    ``cached`` and ``new`` (int32 ``[requests]``): each request's tokens in the cache and in the step.
+    ``block_tables`` (int32 ``[requests, width]``) is updated in place: the pages that the new tokens
+    need are taken in order from ``free_pages`` (int32), beginning with entry ``free_start`` (a
+    device int32 tensor of one element; ``None``: the first), request by request. ``tokens``: the
+    size of the packed batch, at least the sum of ``new``; tokens behind that sum are padding (slot
+    -1, request -1, position 0). Tokens without a page (the table too narrow or the list exhausted)
+    have slot -1, and ``taken`` counts the pages wanted, so a caller sees the shortage when it next
+    looks. Returns a :class:`PagedStep`; nothing is synchronised.
+    """
+    device = block_tables.device
+    _same_device(device, cached, new, free_pages, free_start)
+    cached = _int32(cached, "cached").contiguous()
+    new = _int32(new, "new").contiguous()
+    free_pages = _int32(free_pages, "free_pages").contiguous()
+    _int32(block_tables, "block_tables", 2)
+    requests, width = block_tables.shape
+    if cached.shape[0] != requests or new.shape[0] != requests:
+        raise ValueError("cached, new and block_tables must describe the same requests")
+    if width > 1 and block_tables.stride(1) != 1:
+        raise ValueError("block_tables must have contiguous rows")
+    if free_start is not None and (free_start.dtype != torch.int32 or free_start.numel() != 1):
+        raise ValueError("free_start must be an int32 tensor of one element")
+    if not 0 <= tokens < 1 << 31:
+        raise ValueError("tokens must not be negative, and below 2^31")
+    slots = torch.empty(tokens, dtype=torch.int64, device=device)
+    positions, owners, starts, lengths, taken = torch.empty(
+        2 * tokens + 2 * requests + 2, dtype=torch.int32, device=device).split(
+            [tokens, tokens, requests + 1, requests, 1])
+    _launch(device, _lib.lib().mt_paged_tables, (
+        cached.data_ptr(), new.data_ptr(), requests, block_tables.data_ptr(),
+        block_tables.stride(0), width, free_pages.data_ptr(), free_pages.shape[0],
+        None if free_start is None else free_start.data_ptr(), page_size, slots.data_ptr(),
+        positions.data_ptr(), owners.data_ptr(), tokens, starts.data_ptr(), lengths.data_ptr(),
+        taken.data_ptr()))
+    return PagedStep(slots, positions, owners, starts, lengths, taken)
+
+
+def _launch(device, call, args):
+    """``call(*args, stream)`` on torch's current stream of ``device``, checked."""
+    if device.index == torch.cuda.current_device():
+        _lib.check(call(*args, _stream_handle(device)))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(call(*args, _stream_handle(device)))
+
+
+def paged_append(key, value, cache, slots):
+    """Write ``key`` and ``value`` (``[tokens, kv_heads, head_dim]``, bfloat16 or float16) to ``slots``
+    (int64 ``[tokens]``, as :func:`paged_tables` gives them) of ``cache``, in place. Tokens whose slot
+    is negative or past the cache are left out. Rows may be strided (heads of a fused projection's
+    output). An 8-bit cache gets the values over its scales, limited to what 8 bits hold."""
+    if key.dtype not in _DTYPES or value.dtype != key.dtype:
+        raise ValueError("keys and values must both be bfloat16 or float16")
+    if cache.key.dtype not in (key.dtype, torch.float8_e4m3fn):
+        raise ValueError("a 16-bit cache must have the keys' and values' dtype")
+    if key.shape != value.shape or key.ndim != 3 or key.shape[1:] != cache.key.shape[2:]:
+        raise ValueError("keys and values must be [tokens, kv_heads, head_dim] of the cache's heads")
+    if slots.dtype != torch.int64 or slots.shape != key.shape[:1]:
+        raise ValueError("slots must be an int64 vector with one slot per token")
+    _same_device(cache._device, key, value, slots)
+    tokens = key.shape[0]
+    if tokens == 0:
+        return
+    key, value, slots = _whole16(key), _whole16(value), slots.contiguous()
+    _launch(cache._device, _lib.lib().mt_paged_append, (
+        cache._ref, key.data_ptr(), value.data_ptr(), *_strides(key), *_strides(value),
+        slots.data_ptr(), tokens, _DTYPES[key.dtype]))
+
+
+def _strides(t):
+    """Strides of the first two dimensions, 0 where they hold one element."""
+    return (t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def paged_attention(query, cache, block_tables, lengths, *, scale=None, window=None,
+                    return_lse=False):
+    """Attention of one new token of each request over its pages of ``cache``.
+
+    ``query`` ``[requests, heads, head_dim]`` (bfloat16 or float16; ``heads`` a multiple of the
+    cache's: neighbouring query heads share a key-value head). ``block_tables`` int32
+    ``[requests, width]``; ``lengths`` int32 ``[requests]``: tokens in the cache, the new one among
+    them. ``scale``: of the scores (default ``head_dim ** -0.5``). ``window``: attend to the last so
+    many tokens only. Returns the output in ``query``'s shape and dtype and, with ``return_lse``, the
+    log of the sum of exponentials (float32 ``[requests, heads]``). Requests without tokens give
+    zeros and -inf. Table entries behind a request's last token are not read; tokens whose entry is
+    no page of the cache are left out.
+    """
+    if query.dtype not in _DTYPES:
+        raise ValueError("queries must be bfloat16 or float16")
+    if cache.key.dtype not in (query.dtype, torch.float8_e4m3fn):
+        raise ValueError("a 16-bit cache must have the queries' dtype")
+    if query.ndim != 3 or query.shape[2] != cache.head_dim:
+        raise ValueError("queries must be [requests, heads, head_dim] of the cache's head_dim")
+    requests, heads, dim = query.shape
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError("query heads must be a positive multiple of the cache's heads")
+    _int32(block_tables, "block_tables", 2)
+    _int32(lengths, "lengths")
+    if block_tables.shape[0] != requests or lengths.shape[0] != requests:
+        raise ValueError("queries, block_tables and lengths must describe the same requests")
+    if window is None:
+        window = 0
+    elif window < 1:
+        raise ValueError("window must be positive")
+    device = cache._device
+    _same_device(device, query, block_tables, lengths)
+    query = _whole16(query)
+    out = torch.empty((requests, heads, dim), dtype=query.dtype, device=device)
+    lse = torch.empty((requests, heads), dtype=torch.float32, device=device) if return_lse else None
+    width = block_tables.shape[1]
+    if requests and width:
+        if block_tables.stride(1) != 1 and width > 1:
+            block_tables = block_tables.contiguous()
+        lengths = lengths.contiguous()
+        window = min(window, (1 << 31) - 1)
+        if device.index == torch.cuda.current_device():
+            _attend(query, cache, block_tables, lengths, scale, window, out, lse)
+        else:
+            with torch.cuda.device(device):
+                _attend(query, cache, block_tables, lengths, scale, window, out, lse)
+    elif requests:
+        out.zero_()
+        if lse is not None:
+            lse.fill_(-float("inf"))
+    return (out, lse) if return_lse else out
+
+
+def _attend(query, cache, block_tables, lengths, scale, window, out, lse):
+    requests, heads, dim = query.shape
+    width = block_tables.shape[1]
+    stream = _stream_handle(cache._device)
+    need = cache._workspace_bytes(requests, heads, width, window)
+    ws = workspace(cache._device, need, stream)
+    _lib.check(_lib.lib().mt_paged_attention(
+        cache._ref, query.data_ptr(), *_strides(query), block_tables.data_ptr(),
+        block_tables.stride(0), width, lengths.data_ptr(), requests, heads,
+        dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
+        None if lse is None else lse.data_ptr(), _DTYPES[query.dtype], ws.data_ptr(), ws.numel(),
+        stream))
