@@ -361,7 +361,8 @@ const char* mt_source_digest(void);
  * values. Strides are in elements, in the order page, token, head; a head's values are contiguous.
  * Held in 16 bits (dtype MT_BF16 or MT_F16) or as 8-bit floats (MT_FP8), which stand for themselves
  * times key_scale or value_scale (both 1 otherwise). dim is a multiple of 16 up to 256; pages *
- * page_size is below 2^31; key, value and all strides are multiples of 16 bytes. */
+ * page_size is below 2^31; key, value and all strides are multiples of 16 bytes, page and token
+ * strides below 4 GiB. */
 typedef struct mt_paged_cache {
   void* key;
   void* value;
@@ -411,7 +412,8 @@ int mt_paged_append(const mt_paged_cache* cache, const void* key, const void* va
  * whose entry is not a page of the cache are left out, and what slots behind the last token hold
  * does not matter. query [requests, heads, dim] with element strides per request and head
  * (multiples of 16 bytes), out [requests, heads, dim] contiguous, 16-byte aligned, both in dtype;
- * a 16-bit cache has the same. Sums are fp32 and in a fixed order: results do not change from run
+ * a 16-bit cache has the same. requests * cache heads * (query heads of one / 16, rounded up) *
+ * (width * page_size / 32, rounded up, + 4) is below 2^31. Sums are fp32 and in a fixed order: results do not change from run
  * to run. Results of a call depend on its workgroup count only in that order. */
 size_t mt_paged_attention_workspace_bytes(const mt_paged_cache* cache, int requests, int heads,
                                           int width, int window);

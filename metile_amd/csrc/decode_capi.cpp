@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <cstdint>
 #include <string>
 
 #include "capi_internal.h"
@@ -46,6 +47,9 @@ int check_cache(const char* op, const mt_paged_cache* c) {
   for (int i = 0; i < 3; ++i)
     if (!stride16(c->key_strides[i], bytes) || !stride16(c->value_strides[i], bytes))
       return refuse(op, "cache strides must be multiples of 16 bytes");
+  for (int i = 0; i < 2; ++i)  // the kernels multiply page numbers and slots with 32-bit strides
+    if (c->key_strides[i] * bytes > UINT32_MAX || c->value_strides[i] * bytes > UINT32_MAX)
+      return refuse(op, "page and token strides of a cache must be below 4 GiB");
   if (!c->key || !c->value) return refuse(op, "null cache pointer");
   if (!aligned16(c->key) || !aligned16(c->value))
     return refuse(op, "cache must be 16-byte aligned");
@@ -58,11 +62,12 @@ int check_cache(const char* op, const mt_paged_cache* c) {
   return MT_OK;
 }
 
-// Tiles of the longest request the table holds, and of all requests and heads.
-int64_t most_tiles(int64_t most, int window) {
-  if (window > 0 && window + 31ll < most) most = window + 31ll;
-  const int64_t n = (most + mt::kAttentionTile - 1) / mt::kAttentionTile;
-  return n > 0 ? n : 1;
+// Units of the longest request that the table holds.
+int64_t most_units(int64_t most, int window) {
+  if (window > 0 && window + (mt::kAttentionUnit - 1ll) < most)
+    most = window + (mt::kAttentionUnit - 1ll);
+  const int64_t n = (most + mt::kAttentionUnit - 1) / mt::kAttentionUnit;
+  return (n > 0 ? n : 1) + mt::kAttentionRowCost;
 }
 
 struct AttentionPlan {
@@ -80,12 +85,13 @@ int plan_attention(const char* op, const mt_paged_cache* c, int requests, int he
     return refuse(op, "block table width must be positive and hold fewer than 2^31 tokens");
   if (window < 0) return refuse(op, "window must not be negative");
   const int group = heads / c->heads, head_tiles = (group + 15) / 16;
-  const int64_t tiles = most_tiles((int64_t)width * c->page_size, window);
+  const int64_t units = most_units((int64_t)width * c->page_size, window);
   const int64_t rows = (int64_t)c->heads * head_tiles;
-  if (tiles * rows >= kInt31 || tiles * requests >= kInt31)
-    return refuse(op, "block tables too large");
+  if (units * rows >= kInt31 || units * rows * requests >= kInt31)
+    return refuse(op, "requests, heads and table width make more than 2^31 units of 32 tokens");
   plan->workgroups =
-      mt::paged_attention_workgroups(mt::current_device_cus(), tiles * rows * requests);
+      mt::paged_attention_workgroups(mt::current_device_cus(), c->dim, c->page_size,
+                                     units * rows * requests);
   plan->bytes = mt::kWorkspaceCounterBytes +
                 (size_t)plan->workgroups * 2 * mt::paged_attention_slot_floats(group, c->dim) * 4;
   return MT_OK;
@@ -156,8 +162,8 @@ int mt_paged_append(const mt_paged_cache* cache, const void* key, const void* va
     mt::PagedSide& s = a.side[i];
     const int64_t* strides = i ? cache->value_strides : cache->key_strides;
     s.cache = static_cast<unsigned char*>(i ? cache->value : cache->key);
-    s.page_stride = strides[0] * bytes;
-    s.slot_stride = strides[1] * bytes;
+    s.page_stride = (uint32_t)(strides[0] * bytes);
+    s.slot_stride = (uint32_t)(strides[1] * bytes);
     s.head_stride = strides[2] * bytes;
     s.rows = static_cast<const unsigned char*>(i ? value : key);
     s.row_stride = (i ? value_token_stride : key_token_stride) * 2;
@@ -214,11 +220,11 @@ int mt_paged_attention(const mt_paged_cache* cache, const void* query, int64_t q
   a.q_head_stride = query_head_stride;
   a.key = static_cast<const unsigned char*>(cache->key);
   a.value = static_cast<const unsigned char*>(cache->value);
-  a.k_page = cache->key_strides[0] * bytes;
-  a.k_slot = cache->key_strides[1] * bytes;
+  a.k_page = (uint32_t)(cache->key_strides[0] * bytes);
+  a.k_slot = (uint32_t)(cache->key_strides[1] * bytes);
   a.k_head = cache->key_strides[2] * bytes;
-  a.v_page = cache->value_strides[0] * bytes;
-  a.v_slot = cache->value_strides[1] * bytes;
+  a.v_page = (uint32_t)(cache->value_strides[0] * bytes);
+  a.v_slot = (uint32_t)(cache->value_strides[1] * bytes);
   a.v_head = cache->value_strides[2] * bytes;
   a.tables = block_tables;
   a.table_stride = table_stride;

@@ -8,18 +8,19 @@
 
 namespace mt {
 
-// Division of n in [0, 2^31) by a constant d in [1, 2^31): n / d = (n * mul) >> shift, exact, since
-// mul = ceil(2^shift / d) with shift = 31 + ceil(log2 d) errs by less than d <= 2^(shift - 31).
+// Division of n in [0, 2^31) by a constant d in [1, 2^31): n / d = (2 n * mul) >> (32 + shift),
+// exact, since mul = ceil(2^(31 + shift) / d) with shift = ceil(log2 d) errs by less than d <=
+// 2^shift.
 struct DivMagic {
   uint32_t mul, shift;
 };
 inline DivMagic div_magic(uint32_t d) {
   uint32_t s = 0;
   while ((1ull << s) < d) ++s;
-  return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+  return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
 }
 __device__ __forceinline__ uint32_t div_by(uint32_t n, DivMagic m) {
-  return (uint32_t)(((uint64_t)n * m.mul) >> m.shift);
+  return __umulhi(2 * n, m.mul) >> m.shift;
 }
 
 struct PagedTablesArgs {
@@ -42,7 +43,8 @@ hipError_t launch_paged_tables(const PagedTablesArgs& a, int cus, hipStream_t st
 // One side (keys or values) of a cache and of the rows written to it. Strides in bytes.
 struct PagedSide {
   unsigned char* cache;
-  int64_t page_stride, slot_stride, head_stride;
+  uint32_t page_stride, slot_stride;
+  int64_t head_stride;
   const unsigned char* rows;
   int64_t row_stride, row_head_stride;
   float scale, inv_scale;  // of an 8-bit cache
@@ -61,8 +63,8 @@ struct PagedAttentionArgs {
   int64_t q_row_stride, q_head_stride;  // elements
   const unsigned char* key;
   const unsigned char* value;
-  int64_t k_page, k_slot, k_head;  // bytes
-  int64_t v_page, v_slot, v_head;
+  uint32_t k_page, k_slot, v_page, v_slot;  // bytes
+  int64_t k_head, v_head;
   const int32_t* tables;           // [R, width], rows `table_stride` entries apart
   int64_t table_stride;
   const int32_t* lengths;          // [R]
@@ -75,12 +77,15 @@ struct PagedAttentionArgs {
   float scale_log2, value_scale;
   DivMagic by_page;
 };
-// Workgroups of a call and floats of one partial slot (two slots a workgroup).
-int paged_attention_workgroups(int cus, int64_t units);
+// Work is counted in units of 32 tokens of a row, plus kAttentionRowCost a row for what every row
+// costs; a workgroup takes kAttentionLeast at least (two rounds of its waves).
+constexpr int kAttentionUnit = 32;
+constexpr int kAttentionRowCost = 4;
+constexpr int kAttentionLeast = 8;
+// Workgroups of a call of `units` at most, and floats of one partial slot (two slots a workgroup).
+int paged_attention_workgroups(int cus, int dim, int page_size, int64_t units);
 size_t paged_attention_slot_floats(int group, int dim);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, int dtype, bool fp8, int workgroups,
                                   hipStream_t stream);
-
-constexpr int kAttentionTile = 128;  // tokens a workgroup takes at a time
 
 }  // namespace mt

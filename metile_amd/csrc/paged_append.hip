@@ -42,7 +42,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(PagedAppendArgs 
       if (slot >= 0 && slot < (int64_t)limit) {
         const uint32_t page = div_by((uint32_t)slot, a.by_page);
         const uint32_t in_page = (uint32_t)slot - page * (uint32_t)a.page_size;
-        to[i] = s.cache + (int64_t)page * s.page_stride + (int64_t)in_page * s.slot_stride +
+        to[i] = s.cache + (uint64_t)page * s.page_stride + (uint64_t)in_page * s.slot_stride +
                 (int64_t)head * s.head_stride + chunk * (FP8 ? 8 : 16);
         v[i] = *reinterpret_cast<const u32x4*>(s.rows + (int64_t)token * s.row_stride +
                                                (int64_t)head * s.row_head_stride + chunk * 16);

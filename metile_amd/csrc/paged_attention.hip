@@ -3,8 +3,8 @@
 //   s_t = scale * q . k_t      o = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m)      m = max_t s_t
 //
 // in one pass over the pages with a running maximum and sum (in powers of two: the scale holds
-// log2 e). A workgroup takes tiles of 128 tokens of one row (request, key-value head, up to 16
-// query heads that share it), 32 tokens a wave and tile:
+// log2 e). A wave takes 32 tokens of one row (request, key-value head, up to 16 query heads that
+// share it) at a time:
 //  * keys: v_mfma_f32_16x16x32 with the keys as rows and the query heads as columns, so a lane
 //    holds scores of one head, eight consecutive tokens of it in two tiles (row i of tile t is
 //    token 8 (i / 4) + 4 t + i % 4);
@@ -17,10 +17,11 @@
 // second part is zero or negative as often as not, and an infinite value times it is no number: a
 // segment whose sums are not finite is taken again with the first parts alone, which are positive.)
 //
-// Split: all tiles of all rows, laid end to end, are dealt out in equal contiguous runs to a
-// fixed number of workgroups (each finds its place from a scan over the lengths), so ragged
-// batches balance by themselves. Parts of a row that several workgroups share are stored with
-// their maximum and sum and joined, in order, by the last of them to arrive.
+// Split: all rows, laid end to end in units of 32 tokens with a few more for the fixed cost of a
+// row, are dealt out in equal contiguous runs to a fixed number of workgroups (each finds its place
+// from a scan over the lengths), so ragged batches balance by themselves; a workgroup's waves take
+// the units of its run in turn. Parts of a row that several workgroups share are stored with their
+// maximum and sum and joined, in order, by the last of them to arrive (32 parts at a time).
 #include "common.h"
 #include "paged.h"
 
@@ -29,39 +30,48 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kTile = kAttentionTile;
-static_assert(kTile == 32 * kWaves, "a wave takes 32 tokens of a tile");
+constexpr int kUnit = kAttentionUnit;
+constexpr int kRowCost = kAttentionRowCost;
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
+// Inclusive sum over the lanes: within rows of 16, then across them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_add<0x111, 0xF>(v);  // row_shr:1
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<kDppRowBcast15, 0xA>(v);
+  return dpp_add<kDppRowBcast31, 0xC>(v);
 }
 
 __device__ __forceinline__ int readlane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// A request's tokens as they are read: its length, the first token of its window rounded down to
-// 32, and its tiles (one for an empty request, which writes its zeros).
+// A request's tokens as they are read: its length, the first token of its window rounded down to a
+// unit, and its units (one for an empty request, which writes its zeros).
 struct Span {
-  int len, first, base, tiles;
+  int len, first, base, units;
 };
 __device__ __forceinline__ Span span_of(int length, int most, int window) {
   Span s;
   s.len = length < 0 ? 0 : (length > most ? most : length);
   s.first = window > 0 && s.len > window ? s.len - window : 0;
-  s.base = s.first & ~31;
-  const int n = (int)(((unsigned)(s.len - s.base) + kTile - 1) / kTile);
-  s.tiles = n > 0 ? n : 1;
+  s.base = s.first & ~(kUnit - 1);
+  const int n = (int)(((unsigned)(s.len - s.base) + kUnit - 1) / kUnit);
+  s.units = n > 0 ? n : 1;
   return s;
 }
 
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return (uint32_t)f32_to_act<DT>(a) | (uint32_t)f32_to_act<DT>(b) << 16;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT == kBF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
 }
 
 // Two 8-bit floats (half HI of a word) as 16-bit ones: exact.
@@ -80,19 +90,32 @@ __device__ __forceinline__ u32x4 fp8_eight(uint32_t lo, uint32_t hi) {
                  fp8_pair<DT, true>(hi)};
 }
 
+// Where a workgroup's partial sums of a row are kept: [heads][kPartHead + DIM] floats a slot, the
+// maximum and the sum in front of a head's values.
+constexpr int kPartHead = 4;
+// Parts that one workgroup joins; a row of more is joined in two rounds.
+constexpr int kJoin = 32;
+
+// Waves a SIMD (and so workgroups a CU) that the registers are allotted for.
+constexpr int attention_waves(int padded_dim, bool page8) {
+  return padded_dim == 256 ? 1 : padded_dim == 64 && page8 ? 3 : 2;
+}
+
 template <int DT, bool FP8, int DIM, bool PAGE8>
-__global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAttentionArgs a,
-                                                                      int slot_floats) {
+__global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_attention_kernel(PagedAttentionArgs a,
+                                                                      int slot_bytes) {
   constexpr int kElt = FP8 ? 1 : 2;
   constexpr int kMfmas = DIM / 32;               // K depth of a score
   constexpr int kLaneDims = DIM / 16;            // value dimensions of a lane
   constexpr int kKeyLoads = kMfmas * kElt / 2;   // 16-byte loads of a key row a lane makes
   constexpr int kValueWords = kLaneDims * kElt / 4;
+  constexpr int kRow = DIM + 4;                  // floats: heads start four banks apart
+  constexpr int kVecs = DIM / 4;
   // f16 probabilities are scaled up so that small ones, and the second parts, stay above its
   // smallest numbers; the sum carries the same factor.
   constexpr float kShift = DT == kF16 ? 14.0f : 0.0f;
 
-  __shared__ float lds_acc[kWaves][16][DIM];
+  __shared__ __attribute__((aligned(16))) float lds_acc[kWaves][16][kRow];
   __shared__ float lds_m[kWaves][16];
   __shared__ float lds_l[kWaves][16];
   __shared__ int lds_last;
@@ -102,77 +125,73 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
   const int c = lane & 15, g = lane >> 4;
   const int most = a.width * a.page_size;  // the host checks that it fits 31 bits
   const int hr_count = a.kv_heads * a.head_tiles;
-  const int hcnt = a.group < 16 ? a.group : 16;
+  const __amdgpu_buffer_rsrc_t parts_rsrc =
+      make_rsrc(a.partial, (uint32_t)gridDim.x * 2u * (uint32_t)slot_bytes);
 
-  // ---- this workgroup's run of tiles ----
+  // ---- this workgroup's run of units ----
   const int chunk = (a.requests + 63) >> 6;
-  int mine = 0;
+  int mine = 0, len_lane = 0;
   for (int i = 0; i < chunk; ++i) {
     const int r = lane * chunk + i;
-    if (r < a.requests) mine += span_of(a.lengths[r], most, a.window).tiles;
+    len_lane = r < a.requests ? a.lengths[r] : 0;
+    if (r < a.requests) mine += span_of(len_lane, most, a.window).units + kRowCost;
   }
-  const int inc = wave_scan(mine, lane);
-  const int64_t units = (int64_t)readlane(inc, 63) * hr_count;
-  const int64_t per = (units + gridDim.x - 1) / gridDim.x;
-  int64_t u = (int64_t)blockIdx.x * per;
+  const int inc = wave_scan(mine);
+  // (below 2^31, as the host checks; said to be the same in every lane)
+  const unsigned units = (unsigned)readlane(inc, 63) * (unsigned)hr_count;
+  const unsigned per = max((unsigned)uniform((int)((units + gridDim.x - 1) / gridDim.x)),
+                           (unsigned)kAttentionLeast);
+  unsigned u = blockIdx.x * per;
   if (u >= units) return;
-  const int64_t u_end = u + per < units ? u + per : units;
-  const int target = (int)(u / hr_count);
-  const int owner = __ffsll(__ballot(inc > target)) - 1;
-  int prefix = readlane(inc, owner) - readlane(mine, owner);  // tiles of the requests before r
-  int piece = owner * chunk;                                  // 64 requests from `piece` on: lens
-  int len_lane = 0, r = piece;
-  for (;;) {
-    len_lane = piece + lane < a.requests ? a.lengths[piece + lane] : 0;
-    const int t = piece + lane < a.requests ? span_of(len_lane, most, a.window).tiles : 0;
-    const int s = wave_scan(t, lane) + prefix;
-    const uint64_t hit = __ballot(s > target);
-    if (hit) {
-      const int at = __ffsll((unsigned long long)hit) - 1;
-      r = piece + at;
-      prefix = readlane(s, at) - readlane(t, at);
-      break;
+  const unsigned u_end = min(u + per, units);
+  const int target = uniform((int)(u / (unsigned)hr_count));
+  const int owner = __ffsll((unsigned long long)__ballot(inc > target)) - 1;
+  int prefix = readlane(inc, owner) - readlane(mine, owner);  // units of the requests before r
+  int piece = owner * chunk, r = piece;                       // len_lane: 64 requests from `piece`
+  if (chunk == 1) {
+    piece = 0;
+  } else {
+    for (;;) {
+      len_lane = piece + lane < a.requests ? a.lengths[piece + lane] : 0;
+      const int t = piece + lane < a.requests 
+                        ? span_of(len_lane, most, a.window).units + kRowCost : 0;
+      const int s = wave_scan(t) + prefix;
+      const uint64_t hit = __ballot(s > target);
+      if (hit) {
+        const int at = __ffsll((unsigned long long)hit) - 1;
+        r = piece + at;
+        prefix = readlane(s, at) - readlane(t, at);
+        break;
+      }
+      prefix = readlane(s, 63);
+      piece += 64;
+      if (piece >= a.requests) return;  // only if the lengths changed under the scan
     }
-    prefix = readlane(s, 63);
-    piece += 64;
-    if (piece >= a.requests) return;  // only if the lengths changed under the scan
   }
   Span sp = span_of(readlane(len_lane, r - piece), most, a.window);
-  int hr, tile;
-  int64_t row_u;  // unit of the row's first tile
+  int hr;
+  unsigned row_u;  // where the row begins; its units come behind its cost
   {
-    const int off = (int)(u - (int64_t)prefix * hr_count);
-    hr = off / sp.tiles;
-    tile = off - hr * sp.tiles;
-    row_u = u - tile;
+    const unsigned off = u - (unsigned)prefix * (unsigned)hr_count;
+    const unsigned row = (unsigned)(sp.units + kRowCost);
+    hr = uniform((int)(off / row));
+    row_u = u - (off - (unsigned)hr * row);
   }
-
   const int page_size = a.page_size;
 
-  while (u < u_end && r < a.requests) {
-    const int tile_end = sp.tiles - tile <= u_end - u ? sp.tiles : tile + (int)(u_end - u);
-    const int kv = hr / a.head_tiles;
+  for (; r < a.requests; ) {
+    const unsigned data_u = row_u + kRowCost, row_end = data_u + (unsigned)sp.units;
+    if (data_u >= u_end) break;
+    const int unit = u > data_u ? (int)(u - data_u) : 0;  // this workgroup's units of the row
+    const int unit_end = (int)(min(u_end, row_end) - data_u);
+    const int kv = a.head_tiles == 1 ? hr : uniform(hr / a.head_tiles);
     const int head0 = kv * a.group + (hr - kv * a.head_tiles) * 16;
-    const int heads = a.group - (hr - kv * a.head_tiles) * 16 < 16
-                          ? a.group - (hr - kv * a.head_tiles) * 16 : 16;
+    const int left = a.group - (hr - kv * a.head_tiles) * 16;
+    const int heads = left < 16 ? left : 16;
     const int32_t* table = a.tables + (int64_t)r * a.table_stride;
     const unsigned char* kbase = a.key + (int64_t)kv * a.k_head;
     const unsigned char* vbase = a.value + (int64_t)kv * a.v_head;
     const int len = sp.len, first = sp.first, last = len - 1;
-
-    // ---- the query heads, as columns: dimensions in the order of the key loads ----
-    u32x4 q[kMfmas];
-    {
-      const bool has = c < heads;
-      const uint16_t* row = a.query + (int64_t)r * a.q_row_stride +
-                            (int64_t)(head0 + (has ? c : 0)) * a.q_head_stride;
-#pragma unroll
-      for (int k = 0; k < kMfmas; ++k) {
-        const int d = FP8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g;
-        q[k] = (u32x4){0, 0, 0, 0};
-        if (has && d < a.dim) q[k] = *reinterpret_cast<const u32x4*>(row + d);
-      }
-    }
 
     float m = -__builtin_inff(), l = 0.0f;
     f32x4 acc[kLaneDims];
@@ -181,72 +200,136 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
 
     u32x4 kf[2][kKeyLoads];
     uint32_t vf[8][kValueWords];
-    bool v_ok[PAGE8 ? 1 : 8];
 
-    // Tokens past the end read the last one; tokens of a page that is none of the cache's read
-    // page 0. Both are masked.
-    auto page_of = [&](int token, bool& ok) {
-      const int col = (int)div_by((uint32_t)token, a.by_page);
-      const int p = table[col];
-      ok = (uint32_t)p < (uint32_t)a.pages;
-      return (int2){ok ? p : 0, token - col * page_size};
+    // The pages of a tile's tokens: of a lane's key rows (two; one page where pages are whole
+    // groups of eight tokens) and value rows (eight, or one), with the place of the first token in
+    // the page. Tokens past the end stand for the last one; tokens of a page that is none of the
+    // cache's for page 0. Both are masked.
+    constexpr int kKeyPages = PAGE8 ? 1 : 2, kValuePages = PAGE8 ? 1 : 8;
+    struct Pages {
+      int key[kKeyPages], key_at[kKeyPages];
+      int value[kValuePages], value_at[kValuePages];
     };
-    auto load_keys = [&](int tok0) {
+    auto look_up = [&](int tok0, Pages& p) {
+#pragma unroll
+      for (int t = 0; t < kKeyPages; ++t) {
+        int token = tok0 + 8 * (c >> 2) + (PAGE8 ? 0 : 4 * t + (c & 3));
+        token = token < last ? token : last;
+        const int col = (int)div_by((uint32_t)token, a.by_page);
+        p.key[t] = table[col];
+        p.key_at[t] = col * page_size;
+      }
+#pragma unroll
+      for (int j = 0; j < kValuePages; ++j) {
+        int token = tok0 + 8 * g + j;
+        token = token < last ? token : last;
+        const int col = (int)div_by((uint32_t)token, a.by_page);
+        p.value[j] = table[col];
+        p.value_at[j] = col * page_size;
+      }
+    };
+    auto page_or_0 = [&](int p) { return (uint32_t)p < (uint32_t)a.pages ? (uint32_t)p : 0u; };
+    auto load_keys = [&](int tok0, const Pages& p) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        int token = tok0 + 8 * (c >> 2) + 4 * t + (c & 3);
-        token = token < last ? token : last;
-        bool ok;
-        const int2 at = page_of(token, ok);
-        const unsigned char* p = kbase + (int64_t)at.x * a.k_page + (int64_t)at.y * a.k_slot;
+        constexpr int kOne = kKeyPages - 1;
+        const int token = min(tok0 + 8 * (c >> 2) + 4 * t + (c & 3), last);
+        const unsigned char* row = kbase + (uint64_t)page_or_0(p.key[t & kOne]) * a.k_page +
+                                   (uint64_t)(uint32_t)(token - p.key_at[t & kOne]) * a.k_slot;
 #pragma unroll
         for (int k = 0; k < kKeyLoads; ++k) {
           const int d = FP8 ? 64 * k + 16 * g : 32 * k + 8 * g;
-          kf[t][k] = *reinterpret_cast<const u32x4*>(p + (d < a.dim ? d * kElt : 0));
+          kf[t][k] =
+              __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + (d < a.dim ? d * kElt : 0)));
         }
       }
     };
-    auto load_values = [&](int tok0) {
+    auto load_values = [&](int tok0, const Pages& p) {
       const int d = kLaneDims * c;
-      const unsigned char* p0 = vbase + (d < a.dim ? d * kElt : 0);
-      int2 at;
+      const unsigned char* lane_base = vbase + (d < a.dim ? d * kElt : 0);
+      const unsigned char* page = lane_base;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        int token = tok0 + 8 * g + j;
-        token = token < last ? token : last;
-        if (!PAGE8 || j == 0) {
-          at = page_of(token, v_ok[PAGE8 ? 0 : j]);
-          if (PAGE8) at.y -= token;
-        }
-        const int slot = PAGE8 ? at.y + token : at.y;
-        const unsigned char* p = p0 + (int64_t)at.x * a.v_page + (int64_t)slot * a.v_slot;
+        constexpr int kOne = kValuePages - 1;
+        const int token = min(tok0 + 8 * g + j, last);
+        if (j <= kOne) page = lane_base + (uint64_t)page_or_0(p.value[j & kOne]) * a.v_page;
+        const unsigned char* row =
+            page + (uint64_t)(uint32_t)(token - p.value_at[j & kOne]) * a.v_slot;
         if constexpr (kValueWords >= 4) {
 #pragma unroll
           for (int w = 0; w < kValueWords; w += 4) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(p + 4 * w);
+            const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + 4 * w));
             vf[j][w] = v.x, vf[j][w + 1] = v.y, vf[j][w + 2] = v.z, vf[j][w + 3] = v.w;
           }
         } else if constexpr (kValueWords == 2) {
-          const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+          const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(row));
           vf[j][0] = v.x, vf[j][1] = v.y;
         } else {
-          vf[j][0] = *reinterpret_cast<const uint32_t*>(p);
+          vf[j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(row));
         }
       }
     };
 
-    auto start_of = [&](int t) { return sp.base + t * kTile + wave * 32; };
+    auto start_of = [&](int t) { return sp.base + t * kUnit; };
+    // Table entries are looked up one tile further ahead than rows, so that no row waits for one.
+    Pages now, ahead;
+    u32x4 q[kMfmas];
     bool two_parts = true;
     int tok0;
     bool live;
   again:
-    tok0 = start_of(tile);
-    live = tile < tile_end && tok0 < len;
+    // (given values here so that none of an earlier row's is kept through the join of its parts)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int k = 0; k < kKeyLoads; ++k) kf[t][k] = (u32x4){0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int w = 0; w < kValueWords; ++w) vf[j][w] = 0;
+#pragma unroll
+    for (int k = 0; k < kMfmas; ++k) q[k] = (u32x4){0, 0, 0, 0};
+    now = ahead = Pages{};
+    int t = unit + wave;
+    tok0 = start_of(t);
+    live = t < unit_end && tok0 < len;
     if (live) {
-      load_keys(tok0);
-      load_values(tok0);
+      look_up(tok0, now);
+      // the query heads, as columns: dimensions in the order of the key loads
+      const bool has = c < heads;
+      const uint16_t* row = a.query + (int64_t)r * a.q_row_stride +
+                            (int64_t)(head0 + (has ? c : 0)) * a.q_head_stride;
+#pragma unroll
+      for (int k = 0; k < kMfmas; ++k) {
+        const int d = FP8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g;
+        q[k] = *reinterpret_cast<const u32x4*>(row + (d < a.dim ? d : 0));
+        if (!has || d >= a.dim) q[k] = (u32x4){0, 0, 0, 0};
+      }
+      load_keys(tok0, now);
+      load_values(tok0, now);
+      if (t + kWaves < unit_end) look_up(start_of(t + kWaves), ahead);
     }
-    for (int t = tile; live;) {
+    while (live) {
+      const int next = start_of(t + kWaves);
+      const bool more = t + kWaves < unit_end;
+      // whether the lane's eight tokens are all attended to: past the ends of the window and the
+      // request, and on pages that are none, they are not
+      bool page_ok = true;
+#pragma unroll
+      for (int j = 0; j < kValuePages; ++j)
+        page_ok = page_ok && (uint32_t)now.value[j] < (uint32_t)a.pages;
+      const bool all = __all(page_ok) && tok0 >= first && tok0 + 32 <= len;
+      uint32_t ok = 0xffu;
+      if (!all) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int token = tok0 + 8 * g + j;
+          const bool here = (uint32_t)now.value[j & (kValuePages - 1)] < (uint32_t)a.pages &&
+                            token >= first && token < len;
+          ok &= ~((uint32_t)!here << j);
+        }
+      }
+
       // ---- scores ----
       f32x4 s[2];
 #pragma unroll
@@ -268,26 +351,22 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
           s[h] = mfma16<DT>(key, q[k], s[h]);
         }
       }
-      const int next = start_of(t + 1);
-      const bool more = t + 1 < tile_end && next < len;
-      bool ok[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int token = tok0 + 8 * g + j;
-        ok[j] = v_ok[PAGE8 ? 0 : j] && token >= first && token < len;
+      if (more) {
+        load_keys(next, ahead);
+        now = ahead;
+        if (t + 2 * kWaves < unit_end) look_up(start_of(t + 2 * kWaves), ahead);
       }
-      if (more) load_keys(next);
 
       // ---- running maximum and sum ----
       float x[8];
-      float top = -__builtin_inff();
-      bool all = true;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = ok[j] ? s[j >> 2][j & 3] * a.scale_log2 : -__builtin_inff();
-        top = fmaxf(top, x[j]);
-        all = all && ok[j];
+      for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * a.scale_log2;
+      if (!all) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (ok >> j) & 1 ? x[j] : -__builtin_inff();
       }
+      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                        fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       if (__any(top > m)) {
@@ -301,35 +380,34 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
       }
       const float zero_at = (m == -__builtin_inff() ? 0.0f : m) - kShift;
       u32x4 p_hi, p_lo;
+      float sum[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
         const float p0 = __builtin_amdgcn_exp2f(x[j] - zero_at);
         const float p1 = __builtin_amdgcn_exp2f(x[j + 1] - zero_at);
-        l += p0;
-        l += p1;
+        sum[0] += p0;
+        sum[1] += p1;
         const uint32_t hi = pack2<DT>(p0, p1);
         p_hi[j >> 1] = hi;
         p_lo[j >> 1] = pack2<DT>(p0 - lo16<DT>(hi), p1 - hi16<DT>(hi));
       }
+      l += sum[0] + sum[1];
 
       // ---- values ----
-      if (!__all(all)) {  // what masked rows hold must not reach the sums, not even times zero
+      if (!all) {  // what masked rows hold must not reach the sums, not even times zero
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int w = 0; w < kValueWords; ++w) vf[j][w] = ok[j] ? vf[j][w] : 0u;
+          for (int w = 0; w < kValueWords; ++w) vf[j][w] = (ok >> j) & 1 ? vf[j][w] : 0u;
       }
+      u32x4 v[kLaneDims];  // dimension e of the lane's eight tokens
       if constexpr (!FP8) {
 #pragma unroll
-        for (int e = 0; e < kLaneDims; ++e) {
-          u32x4 v;
+        for (int e = 0; e < kLaneDims; ++e)
 #pragma unroll
           for (int j = 0; j < 8; j += 2)
-            v[j >> 1] = __builtin_amdgcn_perm(vf[j + 1][e >> 1], vf[j][e >> 1],
-                                              (e & 1) ? 0x07060302u : 0x05040100u);
-          acc[e] = mfma16<DT>(v, p_hi, acc[e]);
-          if (two_parts) acc[e] = mfma16<DT>(v, p_lo, acc[e]);
-        }
+            v[e][j >> 1] = __builtin_amdgcn_perm(vf[j + 1][e >> 1], vf[j][e >> 1],
+                                                 (e & 1) ? 0x07060302u : 0x05040100u);
       } else {
 #pragma unroll
         for (int w = 0; w < kValueWords; ++w) {
@@ -349,17 +427,19 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
             d[h][3] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const u32x4 v = fp8_eight<DT>(d[0][e], d[1][e]);
-            acc[4 * w + e] = mfma16<DT>(v, p_hi, acc[4 * w + e]);
-            if (two_parts) acc[4 * w + e] = mfma16<DT>(v, p_lo, acc[4 * w + e]);
-          }
+          for (int e = 0; e < 4; ++e) v[4 * w + e] = fp8_eight<DT>(d[0][e], d[1][e]);
         }
       }
-      if (more) load_values(next);
+#pragma unroll
+      for (int e = 0; e < kLaneDims; ++e) acc[e] = mfma16<DT>(v[e], p_hi, acc[e]);
+      if (two_parts) {
+#pragma unroll
+        for (int e = 0; e < kLaneDims; ++e) acc[e] = mfma16<DT>(v[e], p_lo, acc[e]);
+      }
+      if (more) load_values(next, now);
       tok0 = next;
       live = more;
-      ++t;
+      t += kWaves;
     }
     float finite = 0.0f;
 #pragma unroll
@@ -378,25 +458,63 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
     l += __shfl_xor(l, 32);
 
     // ---- the four waves' parts ----
-    if (c < hcnt) {
+    if (c < heads) {
 #pragma unroll
-      for (int e = 0; e < kLaneDims; ++e)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lds_acc[wave][c][kLaneDims * (4 * g + i) + e] = acc[e][i];
+        for (int e = 0; e < kLaneDims; e += 4)
+          *reinterpret_cast<f32x4*>(&lds_acc[wave][c][kLaneDims * (4 * g + i) + e]) =
+              (f32x4){acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]};
       if (g == 0) {
         lds_m[wave][c] = m;
         lds_l[wave][c] = l;
       }
     }
     __syncthreads();
-    const bool whole = tile == 0 && tile_end == sp.tiles;
-    const int64_t row_end = row_u + sp.tiles;
-    const int w_first = whole ? 0 : (int)(row_u / per);
-    const int w_last = whole ? 0 : (int)((row_end - 1) / per);
-    float* slot = a.partial + ((int64_t)blockIdx.x * 2 + ((int)blockIdx.x == w_first ? 1 : 0)) *
-                                  slot_floats;
-    for (int i = tid; i < heads * (DIM / 4); i += kThreads) {
-      const int h = i / (DIM / 4), d = (i - h * (DIM / 4)) * 4;
+    const bool whole = unit == 0 && unit_end == sp.units;
+    const int w_first = whole ? 0 : uniform((int)(data_u / per));
+    const int w_last = whole ? 0 : uniform((int)((row_end - 1) / per));
+    const int parts = w_last - w_first + 1, part = (int)blockIdx.x - w_first;
+
+    // A head's four values of a row: the result, or a part of it.
+    auto write_row = [&](int h, int d, f32x4 o, float top, float sum) {
+      const int64_t row = (int64_t)r * a.kv_heads * a.group + head0 + h;
+      const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
+      if (d < a.dim)
+        *reinterpret_cast<u32x2*>(a.out + row * a.dim + d) =
+            (u32x2){pack2<DT>(o.x * inv, o.y * inv), pack2<DT>(o.z * inv, o.w * inv)};
+      if (a.lse && d == 0)
+        a.lse[row] = sum == 0.0f ? -__builtin_inff()
+                                 : (top - kShift + __builtin_amdgcn_logf(sum)) *
+                                       0.6931471805599453f;
+    };
+    auto slot_of = [&](int n) {  // byte offset of the row's part n
+      return ((uint32_t)(w_first + n) * 2u + (n == 0 ? 1u : 0u)) * (uint32_t)slot_bytes;
+    };
+    auto write_part = [&](int n, int h, int d, f32x4 o, float top, float sum) {
+      const uint32_t at = slot_of(n) + (uint32_t)(h * (kPartHead + DIM)) * 4u;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), parts_rsrc,
+                                             at + (uint32_t)(kPartHead + d) * 4u, 0, kDeviceScope);
+      if (d == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(
+            (u32x2){__float_as_uint(top), __float_as_uint(sum)}, parts_rsrc, at, 0, kDeviceScope);
+    };
+    // Every store of the workgroup has arrived, then one count: true in the last of `of` to come.
+    auto arrived_last = [&](uint32_t* counter, int of) {
+      __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (tid == 0) {
+        const bool is_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
+                                                    __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(of - 1);
+        if (is_last)
+          __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        lds_last = is_last;
+      }
+      __syncthreads();
+      return lds_last != 0;
+    };
+    for (int i = tid; i < heads * kVecs; i += kThreads) {
+      const int h = i / kVecs, d = (i - h * kVecs) * 4;
       float top = lds_m[0][h];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_m[w][h]);
@@ -409,92 +527,75 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
         sum += lds_l[w][h] * f;
         o += *reinterpret_cast<const f32x4*>(&lds_acc[w][h][d]) * f;
       }
-      if (whole) {
-        const int64_t row = (int64_t)r * a.kv_heads * a.group + head0 + h;
-        const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
-        if (d < a.dim) {
-          u32x2 w;
-          w.x = pack2<DT>(o.x * inv, o.y * inv);
-          w.y = pack2<DT>(o.z * inv, o.w * inv);
-          *reinterpret_cast<u32x2*>(a.out + row * a.dim + d) = w;
-        }
-        if (a.lse && d == 0)
-          a.lse[row] = sum == 0.0f ? -__builtin_inff()
-                                   : (top - kShift + __builtin_amdgcn_logf(sum)) *
-                                         0.6931471805599453f;
-      } else {
-        float* to = slot + h * (DIM + 2);
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          __hip_atomic_store(to + 2 + d + v, o[v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (d == 0) {
-          __hip_atomic_store(to, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          __hip_atomic_store(to + 1, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-      }
+      if (whole) write_row(h, d, o, top, sum);
+      else write_part(part, h, d, o, top, sum);
     }
     if (!whole) {
-      // ---- the last workgroup of the row joins its parts, in order ----
-      __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (tid == 0)
-        lds_last = __hip_atomic_fetch_add(&a.counters[w_first], 1u, __ATOMIC_RELAXED,
-                                          __HIP_MEMORY_SCOPE_AGENT) ==
-                   (unsigned)(w_last - w_first);
-      __syncthreads();
-      if (lds_last) {
-        const int parts = w_last - w_first + 1;
-        auto part = [&](int i) {
-          return a.partial + ((int64_t)(w_first + i) * 2 + (i == 0 ? 1 : 0)) * slot_floats;
-        };
-        for (int i = tid; i < heads * (DIM / 4); i += kThreads) {
-          const int h = i / (DIM / 4), d = (i - h * (DIM / 4)) * 4;
-          float top = -__builtin_inff();
-          for (int n = 0; n < parts; ++n)
-            top = fmaxf(top, __hip_atomic_load(part(n) + h * (DIM + 2), __ATOMIC_RELAXED,
-                                               __HIP_MEMORY_SCOPE_AGENT));
-          const float base = top == -__builtin_inff() ? 0.0f : top;
+      // Counters: of a row's first (or only) run of parts by the workgroup the row begins in, of
+      // its other runs by their first workgroup (which continues no other row), of its runs by
+      // the workgroup it begins in again.
+      uint32_t* const of_rows = a.counters;
+      uint32_t* const of_runs = a.counters + gridDim.x;
+      uint32_t* const of_joins = a.counters + 2 * gridDim.x;
+      const int run = part / kJoin;
+      int n0 = run * kJoin, step = 1, n_end = min(parts, n0 + kJoin);
+      bool final = parts <= kJoin;
+      bool last = arrived_last(run == 0 ? of_rows + w_first : of_runs + w_first + n0, n_end - n0);
+#pragma unroll 1
+      while (last) {
+        // parts n0, n0 + step, ... below n_end, in that order, eight requested at a time
+#pragma unroll 1
+        for (int i = tid; i < heads * kVecs; i += kThreads) {
+          const int h = i / kVecs, d = (i - h * kVecs) * 4;
+          const uint32_t in_slot = (uint32_t)(h * (kPartHead + DIM)) * 4u;
+          float top = -__builtin_inff(), sum = 0.0f;
           f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-          float sum = 0.0f;
-          for (int n = 0; n < parts; ++n) {
-            const float* from = part(n) + h * (DIM + 2);
-            float v[6];
+#pragma unroll 1
+          for (int n = n0; n < n_end; n += 8 * step) {
+            u32x4 v[8];
+            u32x2 ml[8];
 #pragma unroll
-            for (int k = 0; k < 6; ++k)
-              v[k] = __hip_atomic_load(from + (k < 2 ? k : d + k), __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_AGENT);
-            const float f = __builtin_amdgcn_exp2f(v[0] - base);
-            sum += v[1] * f;
-            o += (f32x4){v[2], v[3], v[4], v[5]} * f;
+            for (int k = 0; k < 8; ++k) {
+              // parts past the end are not there: the first is read in their place
+              const uint32_t at = slot_of(n + k * step < n_end ? n + k * step : n0) + in_slot;
+              ml[k] = __builtin_amdgcn_raw_buffer_load_b64(parts_rsrc, at, 0, kDeviceScope);
+              v[k] = load16_device(parts_rsrc, at + (uint32_t)(kPartHead + d) * 4u);
+            }
+            float t = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (n + k * step < n_end) t = fmaxf(t, __uint_as_float(ml[k].x));
+            const float base = t == -__builtin_inff() ? 0.0f : t;
+            const float fix = __builtin_amdgcn_exp2f(top - base);
+            o *= fix;
+            sum *= fix;
+            top = t;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t x = ml[k].x, y = ml[k].y;
+              if (n + k * step < n_end) {
+                const float f = __builtin_amdgcn_exp2f(__uint_as_float(x) - base);
+                sum += __uint_as_float(y) * f;
+                o += __builtin_bit_cast(f32x4, v[k]) * f;
+              }
+            }
           }
-          const int64_t row = (int64_t)r * a.kv_heads * a.group + head0 + h;
-          const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
-          if (d < a.dim) {
-            u32x2 w;
-            w.x = pack2<DT>(o.x * inv, o.y * inv);
-            w.y = pack2<DT>(o.z * inv, o.w * inv);
-            *reinterpret_cast<u32x2*>(a.out + row * a.dim + d) = w;
-          }
-          if (a.lse && d == 0)
-            a.lse[row] = sum == 0.0f ? -__builtin_inff()
-                                     : (top - kShift + __builtin_amdgcn_logf(sum)) *
-                                           0.6931471805599453f;
+          if (final) write_row(h, d, o, top, sum);
+          else write_part(n0, h, d, o, top, sum);
         }
-        if (tid == 0)
-          __hip_atomic_store(&a.counters[w_first], 0u, __ATOMIC_RELAXED,
-                             __HIP_MEMORY_SCOPE_AGENT);
+        if (final) break;
+        last = arrived_last(of_joins + w_first, (parts + kJoin - 1) / kJoin);
+        n0 = 0, step = kJoin, n_end = parts, final = true;
       }
     }
     __syncthreads();  // the next segment writes the same LDS
 
     // ---- on to the next row ----
-    u += tile_end - tile;
-    tile = 0;
     row_u = row_end;
     if (++hr == hr_count) {
       hr = 0;
       ++r;
-      if (u < u_end) {
+      if (row_u < u_end) {
         if (r - piece == 64) {
           piece = r;
           len_lane = piece + lane < a.requests ? a.lengths[piece + lane] : 0;
@@ -507,7 +608,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_kernel(PagedAtten
 
 template <int DT, bool FP8, int DIM>
 hipError_t launch(const PagedAttentionArgs& a, int workgroups, hipStream_t stream) {
-  const int slot = (int)paged_attention_slot_floats(a.group, a.dim);
+  const int slot = (int)paged_attention_slot_floats(a.group, a.dim) * 4;
   if (a.page_size % 8 == 0)
     paged_attention_kernel<DT, FP8, DIM, true><<<workgroups, kThreads, 0, stream>>>(a, slot);
   else
@@ -528,13 +629,14 @@ hipError_t launch_dim(const PagedAttentionArgs& a, int workgroups, hipStream_t s
 
 }  // namespace
 
-int paged_attention_workgroups(int cus, int64_t units) {
-  const int64_t most = 2 * (int64_t)cus;
-  return (int)(units < most ? (units > 0 ? units : 1) : most);
+int paged_attention_workgroups(int cus, int dim, int page_size, int64_t units) {
+  const int64_t most = attention_waves(padded_dim(dim), page_size % 8 == 0) * (int64_t)cus;
+  const int64_t runs = (units + kAttentionLeast - 1) / kAttentionLeast;
+  return (int)(runs < most ? (runs > 0 ? runs : 1) : most);
 }
 
 size_t paged_attention_slot_floats(int group, int dim) {
-  return (size_t)(group < 16 ? group : 16) * (padded_dim(dim) + 2);
+  return (size_t)(group < 16 ? group : 16) * (padded_dim(dim) + kPartHead);
 }
 
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, int dtype, bool fp8, int workgroups,

@@ -77,6 +77,9 @@ class PagedCache:
                     n > 1 and s * t.element_size() % 16 for n, s in zip(t.shape, t.stride()[:3])):
                 raise ValueError("a cache's heads must be contiguous and its strides multiples of "
                                  "16 bytes")
+            if any(n > 1 and s * t.element_size() >= 1 << 32
+                   for n, s in zip(t.shape, t.stride()[:2])):
+                raise ValueError("page and token strides of a cache must be below 4 GiB")
         if key.dtype != torch.float8_e4m3fn and (key_scale != 1.0 or value_scale != 1.0):
             raise ValueError("only 8-bit caches have scales")
         if not (0.0 < key_scale < float("inf") and 0.0 < value_scale < float("inf")):

@@ -29,7 +29,7 @@ BAD_CACHES = [(dict(dtype=2), "dtype"), (dict(pages=0), "pages"), (dict(page_siz
               (dict(key_strides=(2048, 12, 128)), "16 bytes"),
               (dict(value_strides=(2048, -128, 128)), "16 bytes"),
               (dict(dtype=_lib.MT_FP8, value_strides=(2048, 128, 8)), "16 bytes"),
-              (dict(key=None), "null"), (dict(value=264), "aligned"),
+              (dict(value_strides=(1 << 31, 128, 128)), "4 GiB"), (dict(key=None), "null"), (dict(value=264), "aligned"),
               (dict(key_scale=2.0), "scales of 1"),
               (dict(dtype=_lib.MT_FP8, key_scale=0.0), "positive"),
               (dict(dtype=_lib.MT_FP8, value_scale=float("inf")), "normal"),
@@ -62,7 +62,8 @@ def test_caches_are_checked(changes, text):
     (dict(dtype=1), "query's dtype"), (dict(scale=float("nan")), "finite"),
     (dict(query=None), "null"), (dict(out=ctypes.c_void_p(264)), "16 bytes"),
     (dict(qh=100), "16 bytes"), (dict(qs=-128), "16 bytes"),
-    (dict(requests=1 << 30, width=1 << 20), "too large")])
+    (dict(requests=1 << 30, width=1 << 20), "2^31 units"),
+    (dict(requests=1 << 20, width=1 << 20), "2^31 units")])
 def test_attention_arguments_are_checked(changes, text):
     assert text in message(attend(cache(), **changes))
 
