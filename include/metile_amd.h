@@ -387,21 +387,38 @@ typedef struct mt_paged_cache {
  * slot -1 (and an exhausted list writes -1 into the table, with `taken` telling the shortage).
  * Tokens beyond `tokens` are dropped with the table entries of the pages they open. width *
  * page_size is below 2^31; sums of counts stop at 2^31 - 1. requests or tokens may be 0. */
-int mt_paged_tables(const int32_t* cached, const int32_t* new_tokens, int requests,
-                    int32_t* block_tables, int64_t table_stride, int width,
-                    const int32_t* free_pages, int free_count, const int32_t* free_start,
-                    int page_size, int64_t* slots, int32_t* positions, int32_t* token_requests,
-                    int tokens, int32_t* starts, int32_t* lengths, int32_t* taken, void* stream);
+typedef struct mt_paged_tables_args {
+  const int32_t* cached;
+  const int32_t* new_tokens;
+  int32_t* block_tables;
+  int64_t table_stride;
+  const int32_t* free_pages;
+  const int32_t* free_start;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* token_requests;
+  int32_t* starts;
+  int32_t* lengths;
+  int32_t* taken;
+  int requests, width, free_count, page_size, tokens;
+} mt_paged_tables_args;
+int mt_paged_tables(const mt_paged_tables_args* args, void* stream);
 
 /* Writes a step's keys and values, [tokens, heads, dim] 16-bit (dtype) with element strides per
  * token and head, to the cache at slots[token]; tokens whose slot is not in [0, pages * page_size)
  * are left out. Slots that occur twice get one of their rows or a mixture. 8-bit caches hold
  * value / scale rounded to nearest even and limited to +-448. A 16-bit cache has the rows' dtype.
  * Rows and strides are multiples of 16 bytes; tokens * heads * dim / 8 is below 2^31. */
-int mt_paged_append(const mt_paged_cache* cache, const void* key, const void* value,
-                    int64_t key_token_stride, int64_t key_head_stride, int64_t value_token_stride,
-                    int64_t value_head_stride, const int64_t* slots, int64_t tokens, int dtype,
-                    void* stream);
+typedef struct mt_paged_append_args {
+  const void* key;
+  const void* value;
+  int64_t key_strides[2];
+  int64_t value_strides[2];
+  const int64_t* slots;
+  int64_t tokens;
+  int dtype;
+} mt_paged_append_args;
+int mt_paged_append(const mt_paged_cache* cache, const mt_paged_append_args* args, void* stream);
 
 /* Attention of one new token per request over its pages: out[r, h] = sum_t p_t v_t with p =
  * softmax(scale * q[r, h] . k_t) over the request's last `window` tokens (0: all of them), of the
@@ -413,14 +430,23 @@ int mt_paged_append(const mt_paged_cache* cache, const void* key, const void* va
  * does not matter. query [requests, heads, dim] with element strides per request and head
  * (multiples of 16 bytes), out [requests, heads, dim] contiguous, 16-byte aligned, both in dtype;
  * a 16-bit cache has the same. requests * cache heads * (query heads of one / 16, rounded up) *
- * (width * page_size / 32, rounded up, + 4) is below 2^31. Sums are fp32 and in a fixed order: results do not change from run
- * to run. Results of a call depend on its workgroup count only in that order. */
+ * (width * page_size / 32, rounded up, + 4) is below 2^31. Sums are fp32 and in a fixed order:
+ * results do not change from run to run. */
+typedef struct mt_paged_attention_args {
+  const void* query;
+  int64_t query_strides[2];
+  const int32_t* block_tables;
+  int64_t table_stride;
+  const int32_t* lengths;
+  void* out;
+  float* lse;
+  int requests, heads, width, window;
+  float scale;
+  int dtype;
+} mt_paged_attention_args;
 size_t mt_paged_attention_workspace_bytes(const mt_paged_cache* cache, int requests, int heads,
                                           int width, int window);
-int mt_paged_attention(const mt_paged_cache* cache, const void* query, int64_t query_stride,
-                       int64_t query_head_stride, const int32_t* block_tables,
-                       int64_t table_stride, int width, const int32_t* lengths, int requests,
-                       int heads, float scale, int window, void* out, float* lse, int dtype,
+int mt_paged_attention(const mt_paged_cache* cache, const mt_paged_attention_args* args,
                        void* workspace, size_t workspace_bytes, void* stream);
 
 typedef enum mt_norm_kind { MT_NORM_RMS = 0, MT_NORM_LAYER = 1 } mt_norm_kind;
@@ -434,15 +460,25 @@ typedef enum mt_norm_kind { MT_NORM_RMS = 0, MT_NORM_LAYER = 1 } mt_norm_kind;
  * identity. block may be NULL (then r = residual_scale * residual, and post and gate are not read).
  * gate (or NULL: 1) holds a row of width values, or one value with gate_scalar, for each gate_rows
  * rows, gate_stride elements apart (0: one for all). residual is in residual_dtype (dtype or
- * MT_F32), as is residual_out (contiguous; NULL: not written; it may be residual itself where that
- * is contiguous); everything else is in dtype. All arithmetic is fp32; each output is rounded once,
- * and pre sees r before its rounding. Pointers need the alignment of their type only. */
-int mt_residual_norm(const void* residual, int64_t residual_stride, const void* block,
-                     int64_t block_stride, const void* weight, const void* bias,
-                     const void* post_weight, const void* post_bias, const void* gate,
-                     int64_t gate_stride, int gate_rows, int gate_scalar, void* residual_out,
-                     void* normed, int rows, int width, float residual_scale, float eps, int kind,
-                     int dtype, int residual_dtype, void* stream);
+ * MT_F32), as is residual_out (contiguous; NULL: not written); everything else is in dtype. All
+ * arithmetic is fp32; each output is rounded once, and pre sees r before its rounding. Outputs
+ * overlap no input. Pointers need the alignment of their type only. */
+typedef struct mt_residual_norm_args {
+  const void* residual;
+  const void* block;
+  const void* weight;
+  const void* bias;
+  const void* post_weight;
+  const void* post_bias;
+  const void* gate;
+  void* residual_out;
+  void* normed;
+  int64_t residual_stride, block_stride, gate_stride;
+  int rows, width, gate_rows, gate_scalar;
+  float residual_scale, eps;
+  int kind, dtype, residual_dtype;
+} mt_residual_norm_args;
+int mt_residual_norm(const mt_residual_norm_args* args, void* stream);
 
 /* ---- measurement -------------------------------------------------------------------------- */
 

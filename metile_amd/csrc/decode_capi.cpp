@@ -101,59 +101,58 @@ int plan_attention(const char* op, const mt_paged_cache* c, int requests, int he
 
 extern "C" {
 
-int mt_paged_tables(const int32_t* cached, const int32_t* new_tokens, int requests,
-                    int32_t* block_tables, int64_t table_stride, int width,
-                    const int32_t* free_pages, int free_count, const int32_t* free_start,
-                    int page_size, int64_t* slots, int32_t* positions, int32_t* token_requests,
-                    int tokens, int32_t* starts, int32_t* lengths, int32_t* taken, void* stream) {
+int mt_paged_tables(const mt_paged_tables_args* args, void* stream) {
   const char* op = "mt_paged_tables";
-  if (requests < 0 || tokens < 0 || free_count < 0)
+  if (!args) return refuse(op, "null arguments");
+  const mt_paged_tables_args& in = *args;
+  if (in.requests < 0 || in.tokens < 0 || in.free_count < 0)
     return refuse(op, "counts must not be negative");
-  if (page_size < 1 || width < 1 || (int64_t)width * page_size >= kInt31)
+  if (in.page_size < 1 || in.width < 1 || (int64_t)in.width * in.page_size >= kInt31)
     return refuse(op, "page_size and width must be positive and hold fewer than 2^31 tokens");
-  if (requests > 1 && table_stride < width) return refuse(op, "block table rows overlap");
-  if ((requests && (!cached || !new_tokens || !block_tables || !lengths)) ||
-      (free_count && !free_pages) || (tokens && (!slots || !positions || !token_requests)) ||
-      !starts || !taken)
+  if (in.requests > 1 && in.table_stride < in.width) return refuse(op, "block table rows overlap");
+  if ((in.requests && (!in.cached || !in.new_tokens || !in.block_tables || !in.lengths)) ||
+      (in.free_count && !in.free_pages) ||
+      (in.tokens && (!in.slots || !in.positions || !in.token_requests)) || !in.starts || !in.taken)
     return refuse(op, "null pointer");
   mt::PagedTablesArgs a{};
-  a.cached = cached;
-  a.fresh = new_tokens;
-  a.tables = block_tables;
-  a.table_stride = table_stride;
-  a.free_pages = free_pages;
-  a.free_start = free_start;
-  a.slots = slots;
-  a.positions = positions;
-  a.requests = token_requests;
-  a.starts = starts;
-  a.lengths = lengths;
-  a.taken = taken;
-  a.num_requests = requests;
-  a.width = width;
-  a.page_size = page_size;
-  a.free_count = free_count;
-  a.tokens = tokens;
+  a.cached = in.cached;
+  a.fresh = in.new_tokens;
+  a.tables = in.block_tables;
+  a.table_stride = in.table_stride;
+  a.free_pages = in.free_pages;
+  a.free_start = in.free_start;
+  a.slots = in.slots;
+  a.positions = in.positions;
+  a.requests = in.token_requests;
+  a.starts = in.starts;
+  a.lengths = in.lengths;
+  a.taken = in.taken;
+  a.num_requests = in.requests;
+  a.width = in.width;
+  a.page_size = in.page_size;
+  a.free_count = in.free_count;
+  a.tokens = in.tokens;
   return launched(op, mt::launch_paged_tables(a, mt::current_device_cus(),
                                               static_cast<hipStream_t>(stream)));
 }
 
-int mt_paged_append(const mt_paged_cache* cache, const void* key, const void* value,
-                    int64_t key_token_stride, int64_t key_head_stride, int64_t value_token_stride,
-                    int64_t value_head_stride, const int64_t* slots, int64_t tokens, int dtype,
-                    void* stream) {
+int mt_paged_append(const mt_paged_cache* cache, const mt_paged_append_args* args, void* stream) {
   const char* op = "mt_paged_append";
   if (const int st = check_cache(op, cache)) return st;
-  if (dtype != MT_BF16 && dtype != MT_F16) return refuse(op, "dtype must be MT_BF16 or MT_F16");
-  if (cache->dtype != MT_FP8 && cache->dtype != dtype)
+  if (!args) return refuse(op, "null arguments");
+  const mt_paged_append_args& in = *args;
+  if (in.dtype != MT_BF16 && in.dtype != MT_F16)
+    return refuse(op, "dtype must be MT_BF16 or MT_F16");
+  if (cache->dtype != MT_FP8 && cache->dtype != in.dtype)
     return refuse(op, "a 16-bit cache must have the rows' dtype");
-  if (tokens < 0 || tokens >= kInt31 || tokens * cache->heads * (cache->dim / 8) >= kInt31)
+  if (in.tokens < 0 || in.tokens >= kInt31 ||
+      in.tokens * cache->heads * (cache->dim / 8) >= kInt31)
     return refuse(op, "tokens must not be negative, and tokens * heads * dim / 8 below 2^31");
-  if (tokens == 0) return MT_OK;
-  if (!key || !value || !slots) return refuse(op, "null pointer");
-  if (!aligned16(key) || !aligned16(value) || !stride16(key_token_stride, 2) ||
-      !stride16(key_head_stride, 2) || !stride16(value_token_stride, 2) ||
-      !stride16(value_head_stride, 2))
+  if (in.tokens == 0) return MT_OK;
+  if (!in.key || !in.value || !in.slots) return refuse(op, "null pointer");
+  if (!aligned16(in.key) || !aligned16(in.value) || !stride16(in.key_strides[0], 2) ||
+      !stride16(in.key_strides[1], 2) || !stride16(in.value_strides[0], 2) ||
+      !stride16(in.value_strides[1], 2))
     return refuse(op, "rows and their strides must be multiples of 16 bytes");
   const bool fp8 = cache->dtype == MT_FP8;
   const int bytes = fp8 ? 1 : 2;
@@ -161,18 +160,19 @@ int mt_paged_append(const mt_paged_cache* cache, const void* key, const void* va
   for (int i = 0; i < 2; ++i) {
     mt::PagedSide& s = a.side[i];
     const int64_t* strides = i ? cache->value_strides : cache->key_strides;
+    const int64_t* row_strides = i ? in.value_strides : in.key_strides;
     s.cache = static_cast<unsigned char*>(i ? cache->value : cache->key);
     s.page_stride = (uint32_t)(strides[0] * bytes);
     s.slot_stride = (uint32_t)(strides[1] * bytes);
     s.head_stride = strides[2] * bytes;
-    s.rows = static_cast<const unsigned char*>(i ? value : key);
-    s.row_stride = (i ? value_token_stride : key_token_stride) * 2;
-    s.row_head_stride = (i ? value_head_stride : key_head_stride) * 2;
+    s.rows = static_cast<const unsigned char*>(i ? in.value : in.key);
+    s.row_stride = row_strides[0] * 2;
+    s.row_head_stride = row_strides[1] * 2;
     s.scale = i ? cache->value_scale : cache->key_scale;
     s.inv_scale = 1.0f / s.scale;
   }
-  a.slots = slots;
-  a.tokens = tokens;
+  a.slots = in.slots;
+  a.tokens = in.tokens;
   a.pages = cache->pages;
   a.page_size = cache->page_size;
   a.heads = cache->heads;
@@ -180,7 +180,7 @@ int mt_paged_append(const mt_paged_cache* cache, const void* key, const void* va
   a.by_row = mt::div_magic((uint32_t)(cache->heads * (cache->dim / 8)));
   a.by_head = mt::div_magic((uint32_t)(cache->dim / 8));
   a.by_page = mt::div_magic((uint32_t)cache->page_size);
-  return launched(op, mt::launch_paged_append(a, dtype, fp8, static_cast<hipStream_t>(stream)));
+  return launched(op, mt::launch_paged_append(a, in.dtype, fp8, static_cast<hipStream_t>(stream)));
 }
 
 size_t mt_paged_attention_workspace_bytes(const mt_paged_cache* cache, int requests, int heads,
@@ -192,32 +192,35 @@ size_t mt_paged_attention_workspace_bytes(const mt_paged_cache* cache, int reque
   return plan.bytes;
 }
 
-int mt_paged_attention(const mt_paged_cache* cache, const void* query, int64_t query_stride,
-                       int64_t query_head_stride, const int32_t* block_tables,
-                       int64_t table_stride, int width, const int32_t* lengths, int requests,
-                       int heads, float scale, int window, void* out, float* lse, int dtype,
+int mt_paged_attention(const mt_paged_cache* cache, const mt_paged_attention_args* args,
                        void* workspace, size_t workspace_bytes, void* stream) {
   const char* op = "mt_paged_attention";
+  if (!args) return refuse(op, "null arguments");
+  const mt_paged_attention_args& in = *args;
   AttentionPlan plan;
-  if (const int st = plan_attention(op, cache, requests, heads, width, window, &plan)) return st;
-  if (dtype != MT_BF16 && dtype != MT_F16) return refuse(op, "dtype must be MT_BF16 or MT_F16");
-  if (cache->dtype != MT_FP8 && cache->dtype != dtype)
+  if (const int st =
+          plan_attention(op, cache, in.requests, in.heads, in.width, in.window, &plan))
+    return st;
+  if (in.dtype != MT_BF16 && in.dtype != MT_F16)
+    return refuse(op, "dtype must be MT_BF16 or MT_F16");
+  if (cache->dtype != MT_FP8 && cache->dtype != in.dtype)
     return refuse(op, "a 16-bit cache must have the query's dtype");
-  if (!std::isfinite(scale)) return refuse(op, "scale must be finite");
-  if (!query || !block_tables || !lengths || !out) return refuse(op, "null pointer");
-  if (!aligned16(query) || !aligned16(out) || !stride16(query_stride, 2) ||
-      !stride16(query_head_stride, 2))
+  if (!std::isfinite(in.scale)) return refuse(op, "scale must be finite");
+  if (!in.query || !in.block_tables || !in.lengths || !in.out) return refuse(op, "null pointer");
+  if (!aligned16(in.query) || !aligned16(in.out) || !stride16(in.query_strides[0], 2) ||
+      !stride16(in.query_strides[1], 2))
     return refuse(op, "query, its strides and out must be multiples of 16 bytes");
-  if (requests > 1 && table_stride < 0) return refuse(op, "block table rows must be in order");
+  if (in.requests > 1 && in.table_stride < 0)
+    return refuse(op, "block table rows must be in order");
   if (!workspace || workspace_bytes < plan.bytes)
     return mt::set_last_error(MT_ERR_WORKSPACE,
                               std::string(op) + ": workspace smaller than required");
   const bool fp8 = cache->dtype == MT_FP8;
   const int64_t bytes = fp8 ? 1 : 2;
   mt::PagedAttentionArgs a{};
-  a.query = static_cast<const uint16_t*>(query);
-  a.q_row_stride = query_stride;
-  a.q_head_stride = query_head_stride;
+  a.query = static_cast<const uint16_t*>(in.query);
+  a.q_row_stride = in.query_strides[0];
+  a.q_head_stride = in.query_strides[1];
   a.key = static_cast<const unsigned char*>(cache->key);
   a.value = static_cast<const unsigned char*>(cache->value);
   a.k_page = (uint32_t)(cache->key_strides[0] * bytes);
@@ -226,71 +229,70 @@ int mt_paged_attention(const mt_paged_cache* cache, const void* query, int64_t q
   a.v_page = (uint32_t)(cache->value_strides[0] * bytes);
   a.v_slot = (uint32_t)(cache->value_strides[1] * bytes);
   a.v_head = cache->value_strides[2] * bytes;
-  a.tables = block_tables;
-  a.table_stride = table_stride;
-  a.lengths = lengths;
-  a.out = static_cast<uint16_t*>(out);
-  a.lse = lse;
+  a.tables = in.block_tables;
+  a.table_stride = in.table_stride;
+  a.lengths = in.lengths;
+  a.out = static_cast<uint16_t*>(in.out);
+  a.lse = in.lse;
   a.counters = static_cast<uint32_t*>(workspace);
   a.partial = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
                                        mt::kWorkspaceCounterBytes);
-  a.requests = requests;
+  a.requests = in.requests;
   a.kv_heads = cache->heads;
-  a.group = heads / cache->heads;
+  a.group = in.heads / cache->heads;
   a.head_tiles = (a.group + 15) / 16;
   a.dim = cache->dim;
   a.pages = cache->pages;
   a.page_size = cache->page_size;
-  a.width = width;
-  a.window = window;
-  a.scale_log2 = scale * cache->key_scale * 1.4426950408889634f;
+  a.width = in.width;
+  a.window = in.window;
+  a.scale_log2 = in.scale * cache->key_scale * 1.4426950408889634f;
   a.value_scale = cache->value_scale;
   a.by_page = mt::div_magic((uint32_t)cache->page_size);
-  return launched(op, mt::launch_paged_attention(a, dtype, fp8, plan.workgroups,
+  return launched(op, mt::launch_paged_attention(a, in.dtype, fp8, plan.workgroups,
                                                  static_cast<hipStream_t>(stream)));
 }
 
-int mt_residual_norm(const void* residual, int64_t residual_stride, const void* block,
-                     int64_t block_stride, const void* weight, const void* bias,
-                     const void* post_weight, const void* post_bias, const void* gate,
-                     int64_t gate_stride, int gate_rows, int gate_scalar, void* residual_out,
-                     void* normed, int rows, int width, float residual_scale, float eps, int kind,
-                     int dtype, int residual_dtype, void* stream) {
+int mt_residual_norm(const mt_residual_norm_args* args, void* stream) {
   const char* op = "mt_residual_norm";
-  if (dtype != MT_BF16 && dtype != MT_F16) return refuse(op, "dtype must be MT_BF16 or MT_F16");
-  if (residual_dtype != dtype && residual_dtype != MT_F32)
+  if (!args) return refuse(op, "null arguments");
+  const mt_residual_norm_args& in = *args;
+  if (in.dtype != MT_BF16 && in.dtype != MT_F16)
+    return refuse(op, "dtype must be MT_BF16 or MT_F16");
+  if (in.residual_dtype != in.dtype && in.residual_dtype != MT_F32)
     return refuse(op, "residual_dtype must be dtype or MT_F32");
-  if (kind != MT_NORM_RMS && kind != MT_NORM_LAYER)
+  if (in.kind != MT_NORM_RMS && in.kind != MT_NORM_LAYER)
     return refuse(op, "kind must be MT_NORM_RMS or MT_NORM_LAYER");
-  if (width < 1 || width > mt::kNormMaxWidth) return refuse(op, "width must be 1 to 65536");
-  if (rows < 0) return refuse(op, "rows must not be negative");
-  if (!(eps >= 0.0f) || !std::isfinite(eps)) return refuse(op, "eps must be finite and >= 0");
-  if (!std::isfinite(residual_scale)) return refuse(op, "residual_scale must be finite");
-  if (gate && (gate_rows < 1 || gate_stride < 0))
+  if (in.width < 1 || in.width > mt::kNormMaxWidth) return refuse(op, "width must be 1 to 65536");
+  if (in.rows < 0) return refuse(op, "rows must not be negative");
+  if (!(in.eps >= 0.0f) || !std::isfinite(in.eps))
+    return refuse(op, "eps must be finite and >= 0");
+  if (!std::isfinite(in.residual_scale)) return refuse(op, "residual_scale must be finite");
+  if (in.gate && (in.gate_rows < 1 || in.gate_stride < 0))
     return refuse(op, "gate_rows must be positive and gate_stride not negative");
-  if (rows == 0) return MT_OK;
-  if (!residual || !weight || !normed) return refuse(op, "null pointer");
+  if (in.rows == 0) return MT_OK;
+  if (!in.residual || !in.weight || !in.normed) return refuse(op, "null pointer");
   mt::ResidualNormArgs a{};
-  a.residual = residual;
-  a.block = static_cast<const uint16_t*>(block);
-  a.weight = static_cast<const uint16_t*>(weight);
-  a.bias = static_cast<const uint16_t*>(bias);
-  a.post_weight = static_cast<const uint16_t*>(post_weight);
-  a.post_bias = static_cast<const uint16_t*>(post_bias);
-  a.gate = static_cast<const uint16_t*>(gate);
-  a.residual_out = residual_out;
-  a.normed = static_cast<uint16_t*>(normed);
-  a.residual_stride = residual_stride;
-  a.block_stride = block_stride;
-  a.gate_stride = gate_stride;
-  a.rows = rows;
-  a.width = width;
-  a.gate_rows = gate ? gate_rows : 1;
-  a.gate_scalar = gate_scalar;
-  a.scale = residual_scale;
-  a.eps = eps;
-  return launched(op, mt::launch_residual_norm(a, dtype, residual_dtype == MT_F32,
-                                               kind == MT_NORM_LAYER, mt::current_device_cus(),
+  a.residual = in.residual;
+  a.block = static_cast<const uint16_t*>(in.block);
+  a.weight = static_cast<const uint16_t*>(in.weight);
+  a.bias = static_cast<const uint16_t*>(in.bias);
+  a.post_weight = static_cast<const uint16_t*>(in.post_weight);
+  a.post_bias = static_cast<const uint16_t*>(in.post_bias);
+  a.gate = static_cast<const uint16_t*>(in.gate);
+  a.residual_out = in.residual_out;
+  a.normed = static_cast<uint16_t*>(in.normed);
+  a.residual_stride = in.residual_stride;
+  a.block_stride = in.block_stride;
+  a.gate_stride = in.gate_stride;
+  a.rows = in.rows;
+  a.width = in.width;
+  a.gate_rows = in.gate ? in.gate_rows : 1;
+  a.gate_scalar = in.gate_scalar;
+  a.scale = in.residual_scale;
+  a.eps = in.eps;
+  return launched(op, mt::launch_residual_norm(a, in.dtype, in.residual_dtype == MT_F32,
+                                               in.kind == MT_NORM_LAYER, mt::current_device_cus(),
                                                static_cast<hipStream_t>(stream)));
 }
 

@@ -15,58 +15,41 @@
 namespace mt {
 namespace {
 
-// Eight values, fewer at a row's end (the others read as zero). Rows need not be aligned to more
-// than their type: the loads are byte-addressed.
+// Eight consecutive values. Rows need not be aligned to more than their type: accesses are
+// byte-addressed.
 template <int DT>
-__device__ __forceinline__ void read8(const uint16_t* p, int n, float (&x)[8]) {
-  if (n >= 8) {
-    u32x4 v;
-    __builtin_memcpy(&v, p, 16);
-    x[0] = lo16<DT>(v.x), x[1] = hi16<DT>(v.x), x[2] = lo16<DT>(v.y), x[3] = hi16<DT>(v.y);
-    x[4] = lo16<DT>(v.z), x[5] = hi16<DT>(v.z), x[6] = lo16<DT>(v.w), x[7] = hi16<DT>(v.w);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < n ? act_to_f32<DT>(p[j]) : 0.0f;
-  }
+__device__ __forceinline__ void read8(const uint16_t* p, float (&x)[8]) {
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  x[0] = lo16<DT>(v.x), x[1] = hi16<DT>(v.x), x[2] = lo16<DT>(v.y), x[3] = hi16<DT>(v.y);
+  x[4] = lo16<DT>(v.z), x[5] = hi16<DT>(v.z), x[6] = lo16<DT>(v.w), x[7] = hi16<DT>(v.w);
 }
 template <int DT>
-__device__ __forceinline__ void read8(const float* p, int n, float (&x)[8]) {
-  if (n >= 8) {
-    __builtin_memcpy(x, p, 32);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : 0.0f;
-  }
+__device__ __forceinline__ void read8(const float* p, float (&x)[8]) {
+  __builtin_memcpy(x, p, 32);
 }
 template <int DT>
-__device__ __forceinline__ void write8(uint16_t* p, int n, const float (&x)[8]) {
-  if (n >= 8) {
-    u32x4 v;
+__device__ __forceinline__ void write8(uint16_t* p, const float (&x)[8]) {
+  u32x4 v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      v[j] = (uint32_t)f32_to_act<DT>(x[2 * j]) | (uint32_t)f32_to_act<DT>(x[2 * j + 1]) << 16;
-    __builtin_memcpy(p, &v, 16);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = f32_to_act<DT>(x[j]);
-  }
+  for (int j = 0; j < 4; ++j)
+    v[j] = (uint32_t)f32_to_act<DT>(x[2 * j]) | (uint32_t)f32_to_act<DT>(x[2 * j + 1]) << 16;
+  __builtin_memcpy(p, &v, 16);
 }
 template <int DT>
-__device__ __forceinline__ void write8(float* p, int n, const float (&x)[8]) {
-  if (n >= 8) {
-    __builtin_memcpy(p, x, 32);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = x[j];
-  }
+__device__ __forceinline__ void write8(float* p, const float (&x)[8]) {
+  __builtin_memcpy(p, x, 32);
 }
 
+// Sum over a wave, the same in every lane: exchanges within rows of 16 lanes, then across them.
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+  v += dpp_read<kDppXor1>(v);
+  v += dpp_read<kDppXor2>(v);
+  v += dpp_read<kDppHalfMirror>(v);
+  v += dpp_read<0x140>(v);  // row_mirror
+  v += dpp_read_rows<kDppRowBcast15, 0xA>(v);
+  v += dpp_read_rows<kDppRowBcast31, 0xC>(v);
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
 }
 
 // Sum over the threads of a row (every one gets it); `turn` alternates the LDS used.
@@ -99,48 +82,62 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_k
 
   const RT* res = static_cast<const RT*>(a.residual) + (int64_t)row * a.residual_stride;
   const uint16_t* blk = a.block ? a.block + (int64_t)row * a.block_stride : nullptr;
-  float x[NV][8], b[NV][8];
+
+  // Vector n of a row is its values 8 n and on; the last one ends with the row and so overlaps the
+  // one before, whose values it computes as well but does not count (`skip` of them). Threads
+  // past the last vector repeat it and count nothing.
+  int at[NV], skip[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int e = 8 * (t + i * kRowThreads);
-    read8<DT>(res + (e < width ? e : 0), e < width ? width - e : 0, x[i]);
-    if (blk) read8<DT>(blk + (e < width ? e : 0), e < width ? width - e : 0, b[i]);
+    at[i] = min(e, width - 8);
+    skip[i] = e < width ? e - at[i] : 8;
+  }
+  // Only the second half of a thread's vectors can be past the end or the last one: with NV of
+  // them, a row has more than NV / 2 (or NV is 1).
+  auto counted = [&](float v, int i, int j) {
+    return i >= NV / 2 && j < skip[i] ? 0.0f : v;
+  };
+
+  float x[NV][8], b[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    read8<DT>(res + at[i], x[i]);
+    if (blk) read8<DT>(blk + at[i], b[i]);
   }
 
-  // in place; values past the row's end stay zero
-  auto norm = [&](float (&v)[NV][8], const uint16_t* weight, const uint16_t* bias) {
+  auto norm = [&](float (&v)[NV][8], const uint16_t* weight, const uint16_t* bias) {  // in place
     if constexpr (LAYER) {
       float s = 0.0f;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += v[i][j];
+        for (int j = 0; j < 8; ++j) s += counted(v[i][j], i, j);
       const float mean = row_sum<WAVES>(s, lds, turn) / (float)width;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int left = width - 8 * (t + i * kRowThreads);
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = j < left ? v[i][j] - mean : 0.0f;
-      }
+        for (int j = 0; j < 8; ++j) v[i][j] -= mean;
     }
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s = fmaf(v[i][j], v[i][j], s);
+      for (int j = 0; j < 8; ++j) {
+        const float c = counted(v[i][j], i, j);
+        s = fmaf(c, c, s);
+      }
     const float mean_sq = row_sum<WAVES>(s, lds, turn) / (float)width;
     const float inv = 1.0f / sqrtf(mean_sq + a.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = 8 * (t + i * kRowThreads);
-      if (e >= width) continue;
       float w[8];
-      read8<DT>(weight + e, width - e, w);
+      read8<DT>(weight + at[i], w);
       if (bias) {
-        float b[8];
-        read8<DT>(bias + e, width - e, b);
+        float c[8];
+        read8<DT>(bias + at[i], c);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = fmaf(v[i][j], inv * w[j], b[j]);
+        for (int j = 0; j < 8; ++j) v[i][j] = fmaf(v[i][j], inv * w[j], c[j]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] *= inv * w[j];
@@ -152,20 +149,13 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_k
     if (a.post_weight) norm(b, a.post_weight, a.post_bias);
     if (a.gate) {
       const uint16_t* gate = a.gate + (int64_t)(row / a.gate_rows) * a.gate_stride;
-      const float one = a.gate_scalar ? act_to_f32<DT>(gate[0]) : 0.0f;
+      const float one = act_to_f32<DT>(gate[0]);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int e = 8 * (t + i * kRowThreads);
-        if (e >= width) continue;
         float w[8];
-        if (a.gate_scalar) {
+        if (!a.gate_scalar) read8<DT>(gate + at[i], w);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = one;
-        } else {
-          read8<DT>(gate + e, width - e, w);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) b[i][j] *= w[j];
+        for (int j = 0; j < 8; ++j) b[i][j] *= a.gate_scalar ? one : w[j];
       }
     }
 #pragma unroll
@@ -179,53 +169,109 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_k
       for (int j = 0; j < 8; ++j) x[i][j] *= a.scale;
   }
   RT* out = static_cast<RT*>(a.residual_out);
+  if (out) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = 8 * (t + i * kRowThreads);
-    if (e >= width) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
-    } else {
-      if (out) write8<DT>(out + (int64_t)row * width + e, width - e, x[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[i][j] = e + j < width ? x[i][j] : 0.0f;
-    }
+    for (int i = 0; i < NV; ++i)
+      if (skip[i] < 8) write8<DT>(out + (int64_t)row * width + at[i], x[i]);
   }
   norm(x, a.weight, a.bias);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = 8 * (t + i * kRowThreads);
-    if (e < width) write8<DT>(a.normed + (int64_t)row * width + e, width - e, x[i]);
-  }
+  for (int i = 0; i < NV; ++i)
+    if (skip[i] < 8) write8<DT>(a.normed + (int64_t)row * width + at[i], x[i]);
 }
 
-template <int DT, typename RT, bool LAYER, int WAVES>
-void launch_vectors(const ResidualNormArgs& a, hipStream_t stream) {
-  const int rows = WAVES == 1 ? 4 : 1, threads = WAVES == 1 ? 256 : 64 * WAVES;
-  const int blocks = (a.rows + rows - 1) / rows;
-  const int vectors = (a.width + 512 * WAVES - 1) / (512 * WAVES);
-  if (vectors <= 1)
-    residual_norm_kernel<DT, RT, LAYER, WAVES, 1><<<blocks, threads, 0, stream>>>(a);
-  else if (vectors <= 2)
-    residual_norm_kernel<DT, RT, LAYER, WAVES, 2><<<blocks, threads, 0, stream>>>(a);
-  else if (vectors <= 4)
-    residual_norm_kernel<DT, RT, LAYER, WAVES, 4><<<blocks, threads, 0, stream>>>(a);
-  else
-    residual_norm_kernel<DT, RT, LAYER, WAVES, 8><<<blocks, threads, 0, stream>>>(a);
-}
-
+// Rows of fewer than eight values: a row a thread, value by value.
 template <int DT, typename RT, bool LAYER>
-void launch_waves(const ResidualNormArgs& a, int cus, hipStream_t stream) {
-  const bool many = a.rows >= 8 * cus;
-  if (a.width <= (many ? 2048 : 512)) launch_vectors<DT, RT, LAYER, 1>(a, stream);
-  else if (a.width <= (many ? 8192 : 2048)) launch_vectors<DT, RT, LAYER, 4>(a, stream);
-  else launch_vectors<DT, RT, LAYER, 16>(a, stream);
+__global__ __launch_bounds__(256) void residual_norm_narrow_kernel(ResidualNormArgs a) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows) return;
+  const int width = a.width;
+  auto value = [](const uint16_t* p, int j) { return act_to_f32<DT>(p[j]); };
+  auto norm = [&](float (&v)[8], const uint16_t* weight, const uint16_t* bias) {
+    float mean = 0.0f, square = 0.0f;
+    if constexpr (LAYER) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mean += j < width ? v[j] : 0.0f;
+      mean /= (float)width;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] -= mean;
+      square = j < width ? fmaf(v[j], v[j], square) : square;
+    }
+    const float inv = 1.0f / sqrtf(square / (float)width + a.eps);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < width) v[j] = fmaf(v[j], inv * value(weight, j), bias ? value(bias, j) : 0.0f);
+  };
+  const RT* res = static_cast<const RT*>(a.residual) + (int64_t)row * a.residual_stride;
+  float x[8], b[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] = b[j] = 0.0f;
+    if (j >= width) continue;
+    if constexpr (sizeof(RT) == 4) x[j] = res[j];
+    else x[j] = value(res, j);
+    if (a.block) b[j] = value(a.block + (int64_t)row * a.block_stride, j);
+  }
+  if (a.block && a.post_weight) norm(b, a.post_weight, a.post_bias);
+  const uint16_t* gate = a.block && a.gate
+                             ? a.gate + (int64_t)(row / a.gate_rows) * a.gate_stride : nullptr;
+  RT* out = static_cast<RT*>(a.residual_out);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j >= width) continue;
+    if (gate) b[j] *= value(gate, a.gate_scalar ? 0 : j);
+    x[j] = fmaf(x[j], a.scale, b[j]);
+    if (!out) continue;
+    if constexpr (sizeof(RT) == 4) out[(int64_t)row * width + j] = x[j];
+    else out[(int64_t)row * width + j] = f32_to_act<DT>(x[j]);
+  }
+  norm(x, a.weight, a.bias);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < width) a.normed[(int64_t)row * width + j] = f32_to_act<DT>(x[j]);
+}
+
+template <int DT, typename RT, bool LAYER, int WAVES, int NV>
+void launch_rows(const ResidualNormArgs& a, hipStream_t stream) {
+  const int rows = WAVES == 1 ? 4 : 1, threads = WAVES == 1 ? 256 : 64 * WAVES;
+  residual_norm_kernel<DT, RT, LAYER, WAVES, NV>
+      <<<(a.rows + rows - 1) / rows, threads, 0, stream>>>(a);
+}
+
+// Waves of a row and vectors of a thread, by width and whether there are rows enough to fill the
+// CUs with several of them. Few rows: a vector a thread, for the shortest chain (one row of 5120
+// takes 2.5 us). Many: two a thread up to 8192 values, so that loads overlap without the registers
+// of four costing half the waves, and sums cross as few waves as that allows. us, bf16, rms norm
+// without and layer norm with a post-norm:
+//   16384 x 4096    1 wave, 8 vectors 126 / 146    4, 2  98 / 98      16, 1  122 / 177
+//   16384 x 2048    1, 4   51 / 56                 2, 2  45 / 47       4, 1   42 / 49
+//    4096 x 8192    4, 4   51 / 58                 8, 2  45 / 49      16, 1   44 / 56
+//    4096 x 896     1, 2   8.4 / 10.0              4, 1   9.4 / 13.1
+// (98 us for 16384 x 4096 are 5.5 TB/s; a copy of 1 GiB reaches 5.1 to 5.2.)
+template <int DT, typename RT, bool LAYER>
+void launch_width(const ResidualNormArgs& a, int cus, hipStream_t stream) {
+  const bool many = a.rows >= 4 * cus;
+  const int w = a.width;
+  if (w < 8)
+    residual_norm_narrow_kernel<DT, RT, LAYER><<<(a.rows + 255) / 256, 256, 0, stream>>>(a);
+  else if (w <= 512) launch_rows<DT, RT, LAYER, 1, 1>(a, stream);
+  else if (w <= 1024 && many) launch_rows<DT, RT, LAYER, 1, 2>(a, stream);
+  else if (w <= 2048 && many && LAYER) launch_rows<DT, RT, LAYER, 2, 2>(a, stream);
+  else if (w <= 2048) launch_rows<DT, RT, LAYER, 4, 1>(a, stream);
+  else if (w <= 4096 && many) launch_rows<DT, RT, LAYER, 4, 2>(a, stream);
+  else if (w <= 8192 && many) launch_rows<DT, RT, LAYER, 8, 2>(a, stream);
+  else if (w <= 8192) launch_rows<DT, RT, LAYER, 16, 1>(a, stream);
+  else if (w <= 16384) launch_rows<DT, RT, LAYER, 16, 2>(a, stream);
+  else if (w <= 32768) launch_rows<DT, RT, LAYER, 16, 4>(a, stream);
+  else launch_rows<DT, RT, LAYER, 16, 8>(a, stream);
 }
 
 template <int DT, typename RT>
 void launch_kind(const ResidualNormArgs& a, bool layer, int cus, hipStream_t stream) {
-  if (layer) launch_waves<DT, RT, true>(a, cus, stream);
-  else launch_waves<DT, RT, false>(a, cus, stream);
+  if (layer) launch_width<DT, RT, true>(a, cus, stream);
+  else launch_width<DT, RT, false>(a, cus, stream);
 }
 
 }  // namespace

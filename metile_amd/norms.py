@@ -72,52 +72,64 @@ def residual_norm(residual, block=None, *, weight, bias=None, post_weight=None, 
     output is rounded once. Widths up to 65536.
     """
     dtype = weight.dtype
+    stream_dtype = residual.dtype
     if dtype not in _DTYPES:
         raise ValueError("norm weights must be bfloat16 or float16")
-    if residual.dtype not in (dtype, torch.float32):
+    if stream_dtype != dtype and stream_dtype != torch.float32:
         raise ValueError("the residual must have the weights' dtype or float32")
-    try:
-        code = _KINDS[kind]
-    except (KeyError, TypeError):
-        raise ValueError("kind must be 'rms' or 'layer'") from None
-    if residual.ndim < 1 or not 1 <= residual.shape[-1] <= 65536:
+    code = _KINDS.get(kind)
+    if code is None:
+        raise ValueError("kind must be 'rms' or 'layer'")
+    shape = residual.shape
+    if not shape or not 1 <= shape[-1] <= 65536:
         raise ValueError("the residual's last dimension must be 1 to 65536")
-    width = residual.shape[-1]
-    if block is None and (post_weight is not None or post_bias is not None or gate is not None):
-        raise ValueError("a post-norm and a gate need a block")
+    width = shape[-1]
+    if block is None:
+        if post_weight is not None or post_bias is not None or gate is not None:
+            raise ValueError("a post-norm and a gate need a block")
+    elif block.shape != shape or block.dtype != dtype:
+        raise ValueError("the block must have the residual's shape and the weights' dtype")
     if post_bias is not None and post_weight is None:
         raise ValueError("a post-norm's bias needs its weight")
-    if block is not None and (block.shape != residual.shape or block.dtype != dtype):
-        raise ValueError("the block must have the residual's shape and the weights' dtype")
-    for t in (weight, bias, post_weight, post_bias):
-        if t is not None and (t.shape != (width,) or t.dtype != dtype):
-            raise ValueError("norm weights and biases must be vectors of the width, of one dtype")
     if gate is not None and gate.dtype != dtype:
         raise ValueError("the gate must have the weights' dtype")
     device = residual.device
     _same_device(device, block, weight, bias, post_weight, post_bias, gate)
-    shape = residual.shape
+    vector = (width,)
+    pointers = []
+    kept = []  # copies must live until the launch
+    for t in (weight, bias, post_weight, post_bias):
+        if t is None:
+            pointers.append(0)
+            continue
+        if t.shape != vector or t.dtype != dtype:
+            raise ValueError("norm weights and biases must be vectors of the width, of one dtype")
+        if not t.is_contiguous():
+            t = t.contiguous()
+            kept.append(t)
+        pointers.append(t.data_ptr())
     rows = residual.numel() // width
     if rows >= 1 << 31:
         raise ValueError("too many rows")
-    normed = torch.empty(shape, dtype=dtype, device=device)
+    whole = residual.is_contiguous()
     keep = block is None and residual_scale == 1.0
-    out = residual if keep else torch.empty(shape, dtype=residual.dtype, device=device)
+    out = (residual if keep else torch.empty_like(residual) if whole
+           else torch.empty(shape, dtype=stream_dtype, device=device))
+    if block is not None and block.is_contiguous():
+        normed = torch.empty_like(block)
+    else:
+        normed = torch.empty(shape, dtype=dtype, device=device)
     if rows == 0:
         return out, normed
-    x, x_stride = _rows(residual, width)
-    b, b_stride = (None, 0) if block is None else _rows(block, width)
-    g, g_stride, g_rows, g_scalar = ((None, 0, 1, False) if gate is None
-                                     else _gate(gate, shape, width, rows))
-    w, wb, pw, pb = (t if t is None or t.stride(0) == 1 or width == 1 else t.contiguous()
-                     for t in (weight, bias, post_weight, post_bias))
-    _launch(device, _lib.lib().mt_residual_norm, (
-        x.data_ptr(), x_stride, _ptr(b), b_stride, w.data_ptr(), _ptr(wb), _ptr(pw), _ptr(pb),
-        _ptr(g), g_stride, g_rows, int(g_scalar), None if keep else out.data_ptr(),
-        normed.data_ptr(), rows, width, residual_scale, eps, code, _DTYPES[dtype],
-        _lib.MT_F32 if residual.dtype == torch.float32 else _DTYPES[dtype]))
+    x, x_stride = (residual, width) if whole else _rows(residual, width)
+    b, b_stride, g, g_stride, g_rows, g_scalar = None, 0, None, 0, 1, False
+    if block is not None:
+        b, b_stride = (block, width) if block.is_contiguous() else _rows(block, width)
+        if gate is not None:
+            g, g_stride, g_rows, g_scalar = _gate(gate, shape, width, rows)
+    _launch(device, _lib.lib().mt_residual_norm, _lib.RESIDUAL_NORM_ARGS.pack(
+        x.data_ptr(), 0 if b is None else b.data_ptr(), *pointers,
+        0 if g is None else g.data_ptr(), 0 if keep else out.data_ptr(), normed.data_ptr(),
+        x_stride, b_stride, g_stride, rows, width, g_rows, g_scalar, residual_scale, eps, code,
+        _DTYPES[dtype], _lib.MT_F32 if stream_dtype == torch.float32 else _DTYPES[dtype]))
     return out, normed
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()

@@ -26,26 +26,26 @@ _CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.MT_FP8}
 
 
 def _same_device(device, *tensors):
-    """All tensors on the ROCm device ``device``, which becomes torch's current one if it is not
-    (kernels are launched on the current device's stream)."""
+    """Refuses tensors that are not all on the ROCm device ``device``."""
     if device.type != "cuda":
         raise ValueError("metile_amd operators take ROCm device tensors")
+    index = device.index
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError("metile_amd operators take tensors of one ROCm device")
 
 
-def _whole16(t):
-    """``t`` with its values in rows of contiguous last dimension whose start and strides are whole
-    16-byte steps, as the kernels read them; a copy only where it is not so already."""
-    size = t.element_size()
-    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1:
-        for i, n in enumerate(t.shape[:-1]):
-            if n > 1 and t.stride(i) * size % 16:
-                break
-        else:
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _rows16(t):
+    """``(t, row stride, head stride)`` of a 16-bit ``[rows, heads, dim]`` tensor whose heads are
+    contiguous and begin at whole 16-byte steps, as the kernels read them; a copy only where it is
+    not so already. Strides of dimensions of one element are 0, whatever torch says they are."""
+    row, head, one = t.stride()
+    rows, heads, dim = t.shape
+    row, head = row if rows > 1 else 0, head if heads > 1 else 0
+    if one != 1 or (t.data_ptr() | 2 * row | 2 * head) & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        row, head = heads * dim, dim
+    return t, row, head
 
 
 class PagedCache:
@@ -95,7 +95,7 @@ class PagedCache:
             (ctypes.c_int64 * 3)(*strides[1]), pages, page_size, heads, dim,
             _CACHE_DTYPES[key.dtype], self.key_scale, self.value_scale)
         self._ref = ctypes.byref(self._desc)
-        self._device = key.device
+        self._device, self._dtype, self._head_shape = key.device, key.dtype, key.shape[2:]
         self._workspaces = {}  # (requests, heads, width, window) -> bytes
 
     @classmethod
@@ -158,32 +158,36 @@ def paged_tables(cached, new, block_tables, free_pages, *, page_size, tokens, fr
     requests, width = block_tables.shape
     if cached.shape[0] != requests or new.shape[0] != requests:
         raise ValueError("cached, new and block_tables must describe the same requests")
-    if width > 1 and block_tables.stride(1) != 1:
+    row, column = block_tables.stride()
+    if width > 1 and column != 1:
         raise ValueError("block_tables must have contiguous rows")
     if free_start is not None and (free_start.dtype != torch.int32 or free_start.numel() != 1):
         raise ValueError("free_start must be an int32 tensor of one element")
     if not 0 <= tokens < 1 << 31:
         raise ValueError("tokens must not be negative, and below 2^31")
+    if not 0 < page_size < 1 << 31:
+        raise ValueError("page_size must be positive, and below 2^31")
     slots = torch.empty(tokens, dtype=torch.int64, device=device)
     positions, owners, starts, lengths, taken = torch.empty(
-        2 * tokens + 2 * requests + 2, dtype=torch.int32, device=device).split(
-            [tokens, tokens, requests + 1, requests, 1])
-    _launch(device, _lib.lib().mt_paged_tables, (
-        cached.data_ptr(), new.data_ptr(), requests, block_tables.data_ptr(),
-        block_tables.stride(0), width, free_pages.data_ptr(), free_pages.shape[0],
-        None if free_start is None else free_start.data_ptr(), page_size, slots.data_ptr(),
-        positions.data_ptr(), owners.data_ptr(), tokens, starts.data_ptr(), lengths.data_ptr(),
-        taken.data_ptr()))
+        2 * tokens + 2 * requests + 2, dtype=torch.int32, device=device).split_with_sizes(
+            (tokens, tokens, requests + 1, requests, 1))
+    _launch(device, _lib.lib().mt_paged_tables, _lib.PAGED_TABLES_ARGS.pack(
+        cached.data_ptr(), new.data_ptr(), block_tables.data_ptr(), row, free_pages.data_ptr(),
+        0 if free_start is None else free_start.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+        owners.data_ptr(), starts.data_ptr(), lengths.data_ptr(), taken.data_ptr(), requests, width,
+        free_pages.shape[0], page_size, tokens))
     return PagedStep(slots, positions, owners, starts, lengths, taken)
 
 
-def _launch(device, call, args):
+def _launch(device, call, *args):
     """``call(*args, stream)`` on torch's current stream of ``device``, checked."""
     if device.index == torch.cuda.current_device():
-        _lib.check(call(*args, _stream_handle(device)))
+        status = call(*args, _stream_handle(device))
     else:
         with torch.cuda.device(device):
-            _lib.check(call(*args, _stream_handle(device)))
+            status = call(*args, _stream_handle(device))
+    if status:
+        _lib.check(status)
 
 
 def paged_append(key, value, cache, slots):
@@ -191,27 +195,26 @@ def paged_append(key, value, cache, slots):
     (int64 ``[tokens]``, as :func:`paged_tables` gives them) of ``cache``, in place. Tokens whose slot
     is negative or past the cache are left out. Rows may be strided (heads of a fused projection's
     output). An 8-bit cache gets the values over its scales, limited to what 8 bits hold."""
-    if key.dtype not in _DTYPES or value.dtype != key.dtype:
+    dtype = key.dtype
+    if dtype not in _DTYPES or value.dtype != dtype:
         raise ValueError("keys and values must both be bfloat16 or float16")
-    if cache.key.dtype not in (key.dtype, torch.float8_e4m3fn):
+    if cache._dtype != dtype and cache._dtype != torch.float8_e4m3fn:
         raise ValueError("a 16-bit cache must have the keys' and values' dtype")
-    if key.shape != value.shape or key.ndim != 3 or key.shape[1:] != cache.key.shape[2:]:
+    shape = key.shape
+    if shape != value.shape or len(shape) != 3 or shape[1:] != cache._head_shape:
         raise ValueError("keys and values must be [tokens, kv_heads, head_dim] of the cache's heads")
-    if slots.dtype != torch.int64 or slots.shape != key.shape[:1]:
+    if slots.dtype != torch.int64 or slots.shape != shape[:1]:
         raise ValueError("slots must be an int64 vector with one slot per token")
     _same_device(cache._device, key, value, slots)
-    tokens = key.shape[0]
+    tokens = shape[0]
     if tokens == 0:
         return
-    key, value, slots = _whole16(key), _whole16(value), slots.contiguous()
-    _launch(cache._device, _lib.lib().mt_paged_append, (
-        cache._ref, key.data_ptr(), value.data_ptr(), *_strides(key), *_strides(value),
-        slots.data_ptr(), tokens, _DTYPES[key.dtype]))
-
-
-def _strides(t):
-    """Strides of the first two dimensions, 0 where they hold one element."""
-    return (t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+    key, key_row, key_head = _rows16(key)
+    value, value_row, value_head = _rows16(value)
+    slots = slots.contiguous()
+    _launch(cache._device, _lib.lib().mt_paged_append, cache._ref, _lib.PAGED_APPEND_ARGS.pack(
+        key.data_ptr(), value.data_ptr(), key_row, key_head, value_row, value_head,
+        slots.data_ptr(), tokens, _DTYPES[dtype]))
 
 
 def paged_attention(query, cache, block_tables, lengths, *, scale=None, window=None,
@@ -227,55 +230,56 @@ def paged_attention(query, cache, block_tables, lengths, *, scale=None, window=N
     zeros and -inf. Table entries behind a request's last token are not read; tokens whose entry is
     no page of the cache are left out.
     """
-    if query.dtype not in _DTYPES:
+    dtype = query.dtype
+    if dtype not in _DTYPES:
         raise ValueError("queries must be bfloat16 or float16")
-    if cache.key.dtype not in (query.dtype, torch.float8_e4m3fn):
+    if cache._dtype != dtype and cache._dtype != torch.float8_e4m3fn:
         raise ValueError("a 16-bit cache must have the queries' dtype")
-    if query.ndim != 3 or query.shape[2] != cache.head_dim:
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim:
         raise ValueError("queries must be [requests, heads, head_dim] of the cache's head_dim")
-    requests, heads, dim = query.shape
+    requests, heads, dim = shape
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError("query heads must be a positive multiple of the cache's heads")
     _int32(block_tables, "block_tables", 2)
     _int32(lengths, "lengths")
+    width = block_tables.shape[1]
     if block_tables.shape[0] != requests or lengths.shape[0] != requests:
         raise ValueError("queries, block_tables and lengths must describe the same requests")
     if window is None:
         window = 0
     elif window < 1:
         raise ValueError("window must be positive")
+    else:
+        window = min(window, (1 << 31) - 1)
     device = cache._device
     _same_device(device, query, block_tables, lengths)
-    query = _whole16(query)
-    out = torch.empty((requests, heads, dim), dtype=query.dtype, device=device)
+    out = torch.empty(shape, dtype=dtype, device=device)
     lse = torch.empty((requests, heads), dtype=torch.float32, device=device) if return_lse else None
-    width = block_tables.shape[1]
-    if requests and width:
-        if block_tables.stride(1) != 1 and width > 1:
-            block_tables = block_tables.contiguous()
-        lengths = lengths.contiguous()
-        window = min(window, (1 << 31) - 1)
-        if device.index == torch.cuda.current_device():
-            _attend(query, cache, block_tables, lengths, scale, window, out, lse)
-        else:
-            with torch.cuda.device(device):
-                _attend(query, cache, block_tables, lengths, scale, window, out, lse)
-    elif requests:
+    if not requests or not width:
         out.zero_()
         if lse is not None:
             lse.fill_(-float("inf"))
+        return (out, lse) if return_lse else out
+    query, row, head = _rows16(query)
+    if width > 1 and block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    lengths = lengths.contiguous()
+    args = _lib.PAGED_ATTENTION_ARGS.pack(
+        query.data_ptr(), row, head, block_tables.data_ptr(), block_tables.stride(0),
+        lengths.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), requests, heads,
+        width, window, dim ** -0.5 if scale is None else scale, _DTYPES[dtype])
+    if device.index == torch.cuda.current_device():
+        _attend(cache, args, requests, heads, width, window)
+    else:
+        with torch.cuda.device(device):
+            _attend(cache, args, requests, heads, width, window)
     return (out, lse) if return_lse else out
 
 
-def _attend(query, cache, block_tables, lengths, scale, window, out, lse):
-    requests, heads, dim = query.shape
-    width = block_tables.shape[1]
+def _attend(cache, args, requests, heads, width, window):
     stream = _stream_handle(cache._device)
-    need = cache._workspace_bytes(requests, heads, width, window)
-    ws = workspace(cache._device, need, stream)
-    _lib.check(_lib.lib().mt_paged_attention(
-        cache._ref, query.data_ptr(), *_strides(query), block_tables.data_ptr(),
-        block_tables.stride(0), width, lengths.data_ptr(), requests, heads,
-        dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
-        None if lse is None else lse.data_ptr(), _DTYPES[query.dtype], ws.data_ptr(), ws.numel(),
-        stream))
+    ws = workspace(cache._device, cache._workspace_bytes(requests, heads, width, window), stream)
+    status = _lib.lib().mt_paged_attention(cache._ref, args, ws.data_ptr(), ws.numel(), stream)
+    if status:
+        _lib.check(status)

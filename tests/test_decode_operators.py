@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -11,7 +13,25 @@ import metile_amd as mt
 from metile_amd import _lib, norms
 from tests import paged_reference as ref
 
-BUF = ctypes.c_void_p(256)  # never dereferenced: every case fails its checks first
+BUF = ctypes.c_void_p(256)  # never dereferenced (nor any 256 below): every case fails its checks
+
+
+def test_argument_blocks_are_laid_out_as_the_header_says():
+    """The struct formats against the header's declarations, field by field."""
+    header = (Path(__file__).resolve().parents[1] / "include" / "metile_amd.h").read_text()
+    for name, packer in (("mt_paged_tables_args", _lib.PAGED_TABLES_ARGS),
+                         ("mt_paged_append_args", _lib.PAGED_APPEND_ARGS),
+                         ("mt_paged_attention_args", _lib.PAGED_ATTENTION_ARGS),
+                         ("mt_residual_norm_args", _lib.RESIDUAL_NORM_ARGS)):
+        body = re.search(r"typedef struct %s \{(.*?)\}" % name, header, re.S).group(1)
+        letters = ""
+        for line in body.strip().split(";")[:-1]:
+            kind, names = re.match(r"\s*(?:const )?(\w+)(.*)", line, re.S).groups()
+            for field in names.split(","):
+                count = int(re.search(r"\[(\d)\]", field).group(1)) if "[" in field else 1
+                letters += ("P" if "*" in field else
+                            {"int64_t": "q", "int": "i", "float": "f"}[kind]) * count
+        assert packer.format == "@" + letters + "0P", name
 
 
 def cache(**changes):
@@ -41,18 +61,22 @@ def message(status):
     return _lib.lib().mt_last_error().decode()
 
 
-def attend(desc, **changes):
-    a = dict(query=BUF, qs=128, qh=128, tables=BUF, ts=4, width=4, lengths=BUF, requests=1, heads=1,
-             scale=1.0, window=0, out=BUF, lse=None, dtype=0, ws=None, nbytes=0)
+def attend(desc, ws=None, nbytes=0, **changes):
+    a = dict(query=256, qs=128, qh=128, tables=256, ts=4, lengths=256, out=256, lse=0, requests=1,
+             heads=1, width=4, window=0, scale=1.0, dtype=0)
     a.update(changes)
-    return _lib.lib().mt_paged_attention(desc, *a.values(), None)
+    return _lib.lib().mt_paged_attention(desc, _lib.PAGED_ATTENTION_ARGS.pack(*a.values()), ws,
+                                         nbytes, None)
+
+
+def append(desc, *args):
+    return _lib.lib().mt_paged_append(desc, _lib.PAGED_APPEND_ARGS.pack(*args), None)
 
 
 @pytest.mark.parametrize("changes,text", BAD_CACHES)
 def test_caches_are_checked(changes, text):
     assert text in message(attend(cache(**changes)))
-    assert text in message(_lib.lib().mt_paged_append(cache(**changes), BUF, BUF, 128, 128, 128, 128,
-                                                      BUF, 1, 0, None))
+    assert text in message(append(cache(**changes), 256, 256, 128, 128, 128, 128, 256, 1, 0))
     assert _lib.lib().mt_paged_attention_workspace_bytes(cache(**changes), 1, 1, 4, 0) == 0
 
 
@@ -60,7 +84,7 @@ def test_caches_are_checked(changes, text):
     (dict(requests=0), "requests"), (dict(heads=0), "heads"), (dict(width=0), "width"),
     (dict(width=1 << 27), "2^31"), (dict(window=-1), "window"), (dict(dtype=2), "dtype"),
     (dict(dtype=1), "query's dtype"), (dict(scale=float("nan")), "finite"),
-    (dict(query=None), "null"), (dict(out=ctypes.c_void_p(264)), "16 bytes"),
+    (dict(query=0), "null"), (dict(out=264), "16 bytes"),
     (dict(qh=100), "16 bytes"), (dict(qs=-128), "16 bytes"),
     (dict(requests=1 << 30, width=1 << 20), "2^31 units"),
     (dict(requests=1 << 20, width=1 << 20), "2^31 units")])
@@ -81,42 +105,47 @@ def test_attention_needs_its_workspace():
 
 def test_append_and_tables_arguments_are_checked():
     lib = _lib.lib()
-    for args, text in (((BUF, BUF, 100, 128, 128, 128, BUF, 1, 0), "16 bytes"),
-                       ((BUF, ctypes.c_void_p(264), 128, 128, 128, 128, BUF, 1, 0), "16 bytes"),
-                       ((None, BUF, 128, 128, 128, 128, BUF, 1, 0), "null"),
-                       ((BUF, BUF, 128, 128, 128, 128, BUF, -1, 0), "tokens"),
-                       ((BUF, BUF, 128, 128, 128, 128, BUF, 1 << 30, 0), "below 2^31"),
-                       ((BUF, BUF, 128, 128, 128, 128, BUF, 1, 1), "rows' dtype"),
-                       ((BUF, BUF, 128, 128, 128, 128, BUF, 1, 2), "dtype")):
-        assert text in message(lib.mt_paged_append(cache(), *args, None))
-    assert lib.mt_paged_append(cache(), None, None, 0, 0, 0, 0, None, 0, 0, None) == _lib.MT_OK
-    good = dict(cached=BUF, new=BUF, requests=2, table=BUF, stride=4, width=4, free=BUF, count=1,
-                start=None, page=16, slots=BUF, positions=BUF, owners=BUF, tokens=1, starts=BUF,
-                lengths=BUF, taken=BUF)
+    for args, text in (((256, 256, 100, 128, 128, 128, 256, 1, 0), "16 bytes"),
+                       ((256, 264, 128, 128, 128, 128, 256, 1, 0), "16 bytes"),
+                       ((0, 256, 128, 128, 128, 128, 256, 1, 0), "null"),
+                       ((256, 256, 128, 128, 128, 128, 256, -1, 0), "tokens"),
+                       ((256, 256, 128, 128, 128, 128, 256, 1 << 30, 0), "below 2^31"),
+                       ((256, 256, 128, 128, 128, 128, 256, 1, 1), "rows' dtype"),
+                       ((256, 256, 128, 128, 128, 128, 256, 1, 2), "dtype")):
+        assert text in message(append(cache(), *args))
+    assert append(cache(), 0, 0, 0, 0, 0, 0, 0, 0, 0) == _lib.MT_OK
+    good = dict(cached=256, new=256, table=256, stride=4, free=256, start=0, slots=256,
+                positions=256, owners=256, starts=256, lengths=256, taken=256, requests=2, width=4,
+                count=1, page=16, tokens=1)
     for changes, text in ((dict(requests=-1), "negative"), (dict(tokens=-1), "negative"),
                           (dict(count=-1), "negative"), (dict(page=0), "page_size"),
                           (dict(width=0), "width"), (dict(width=1 << 27), "2^31"),
-                          (dict(stride=3), "overlap"), (dict(cached=None), "null"),
-                          (dict(free=None), "null"), (dict(slots=None), "null"),
-                          (dict(starts=None), "null"), (dict(taken=None), "null")):
-        assert text in message(lib.mt_paged_tables(*{**good, **changes}.values(), None))
+                          (dict(stride=3), "overlap"), (dict(cached=0), "null"),
+                          (dict(free=0), "null"), (dict(slots=0), "null"),
+                          (dict(starts=0), "null"), (dict(taken=0), "null")):
+        args = _lib.PAGED_TABLES_ARGS.pack(*{**good, **changes}.values())
+        assert text in message(lib.mt_paged_tables(args, None))
 
 
 def test_norm_arguments_are_checked():
-    good = dict(residual=BUF, rs=64, block=BUF, bs=64, weight=BUF, bias=None, pw=None, pb=None,
-                gate=None, gs=0, gr=1, scalar=0, out=BUF, normed=BUF, rows=1, width=64, scale=1.0,
-                eps=1e-6, kind=0, dtype=0, rdtype=0)
-    fn = _lib.lib().mt_residual_norm
+    good = dict(residual=256, block=256, weight=256, bias=0, pw=0, pb=0, gate=0, out=256, normed=256,
+                rs=64, bs=64, gs=0, rows=1, width=64, gr=1, scalar=0, scale=1.0, eps=1e-6, kind=0,
+                dtype=0, rdtype=0)
+
+    def fn(**changes):
+        return _lib.lib().mt_residual_norm(
+            _lib.RESIDUAL_NORM_ARGS.pack(*{**good, **changes}.values()), None)
+
     for changes, text in ((dict(dtype=2), "dtype"), (dict(rdtype=1), "residual_dtype"),
                           (dict(kind=2), "kind"), (dict(width=0), "width"),
                           (dict(width=65537), "width"), (dict(rows=-1), "rows"),
                           (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
                           (dict(scale=float("inf")), "residual_scale"),
-                          (dict(gate=BUF, gr=0), "gate_rows"), (dict(gate=BUF, gs=-1), "gate_"),
-                          (dict(weight=None), "null"), (dict(residual=None), "null"),
-                          (dict(normed=None), "null")):
-        assert text in message(fn(*{**good, **changes}.values(), None))
-    assert fn(*{**good, "rows": 0}.values(), None) == _lib.MT_OK
+                          (dict(gate=256, gr=0), "gate_rows"), (dict(gate=256, gs=-1), "gate_"),
+                          (dict(weight=0), "null"), (dict(residual=0), "null"),
+                          (dict(normed=0), "null")):
+        assert text in message(fn(**changes))
+    assert fn(rows=0) == _lib.MT_OK
 
 
 @pytest.mark.parametrize("shape", [(6, 4), (2, 3, 4), (2, 3, 5, 4), (1, 3, 4), (2, 1, 4), (5, 1),
