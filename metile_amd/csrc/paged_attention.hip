@@ -18,10 +18,12 @@
 // segment whose sums are not finite is taken again with the first parts alone, which are positive.)
 //
 // Split: all rows, laid end to end in units of 32 tokens with a few more for the fixed cost of a
-// row, are dealt out in equal contiguous runs to a fixed number of workgroups (each finds its place
-// from a scan over the lengths), so ragged batches balance by themselves; a workgroup's waves take
-// the units of its run in turn. Parts of a row that several workgroups share are stored with their
-// maximum and sum and joined, in order, by the last of them to arrive (32 parts at a time).
+// row, are dealt out in equal contiguous runs to a fixed number of waves (each finds its place from
+// a scan over the lengths), so ragged batches balance by themselves. A row that lies within one
+// wave's run is written by that wave, with no exchange at all. A wave's parts of other rows (the
+// first and the last of its run) meet in LDS at the end, and the workgroup's parts of rows that go
+// on in other workgroups are stored with their maximum and sum and joined, in order, by the last
+// of those workgroups to arrive (32 parts at a time).
 #include "common.h"
 #include "paged.h"
 
@@ -115,9 +117,13 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
   // smallest numbers; the sum carries the same factor.
   constexpr float kShift = DT == kF16 ? 14.0f : 0.0f;
 
-  __shared__ __attribute__((aligned(16))) float lds_acc[kWaves][16][kRow];
-  __shared__ float lds_m[kWaves][16];
-  __shared__ float lds_l[kWaves][16];
+  // Parts of rows that a wave shares with others: of the row it begins in, of the one it ends in.
+  constexpr int kSlots = 2 * kWaves;
+  __shared__ __attribute__((aligned(16))) float lds_acc[kSlots][16][kRow];
+  __shared__ float lds_m[kSlots][16];
+  __shared__ float lds_l[kSlots][16];
+  __shared__ int lds_row[kSlots], lds_units[kSlots];
+  __shared__ unsigned lds_data[kSlots];
   __shared__ int lds_last;
 
   const int tid = threadIdx.x;
@@ -127,8 +133,13 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
   const int hr_count = a.kv_heads * a.head_tiles;
   const __amdgpu_buffer_rsrc_t parts_rsrc =
       make_rsrc(a.partial, (uint32_t)gridDim.x * 2u * (uint32_t)slot_bytes);
+  // Workgroups go to the XCDs in turn: each XCD takes neighbouring runs, whose rows share lines of
+  // the cache where a head's row of a token is less than one, and all of it where they are query
+  // heads of one key-value head.
+  const int run = gridDim.x % 8 == 0 ? (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8
+                                     : blockIdx.x;
 
-  // ---- this workgroup's run of units ----
+  // ---- this wave's run of units ----
   const int chunk = (a.requests + 63) >> 6;
   int mine = 0, len_lane = 0;
   for (int i = 0; i < chunk; ++i) {
@@ -139,55 +150,69 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
   const int inc = wave_scan(mine);
   // (below 2^31, as the host checks; said to be the same in every lane)
   const unsigned units = (unsigned)readlane(inc, 63) * (unsigned)hr_count;
-  const unsigned per = max((unsigned)uniform((int)((units + gridDim.x - 1) / gridDim.x)),
-                           (unsigned)kAttentionLeast);
-  unsigned u = blockIdx.x * per;
-  if (u >= units) return;
-  const unsigned u_end = min(u + per, units);
-  const int target = uniform((int)(u / (unsigned)hr_count));
-  const int owner = __ffsll((unsigned long long)__ballot(inc > target)) - 1;
-  int prefix = readlane(inc, owner) - readlane(mine, owner);  // units of the requests before r
-  int piece = owner * chunk, r = piece;                       // len_lane: 64 requests from `piece`
-  if (chunk == 1) {
-    piece = 0;
-  } else {
-    for (;;) {
-      len_lane = piece + lane < a.requests ? a.lengths[piece + lane] : 0;
-      const int t = piece + lane < a.requests 
-                        ? span_of(len_lane, most, a.window).units + kRowCost : 0;
-      const int s = wave_scan(t) + prefix;
-      const uint64_t hit = __ballot(s > target);
-      if (hit) {
-        const int at = __ffsll((unsigned long long)hit) - 1;
-        r = piece + at;
-        prefix = readlane(s, at) - readlane(t, at);
-        break;
+  const unsigned waves = gridDim.x * kWaves;
+  const unsigned per_wave =
+      max((unsigned)uniform((int)((units + waves - 1) / waves)), (unsigned)(kAttentionLeast / kWaves));
+  const unsigned per = per_wave * kWaves, wg_u = (unsigned)run * per;
+  if (wg_u >= units) return;
+  const unsigned wg_end = min(wg_u + per, units);
+  const unsigned u = min(wg_u + (unsigned)wave * per_wave, wg_end);
+  const unsigned u_end = min(u + per_wave, wg_end);
+  int piece = 0, r = 0, hr = 0;
+  unsigned row_u = 0;  // where the row begins; its units come behind its cost
+  Span sp{};
+  if (u < u_end) {
+    const int target = uniform((int)(u / (unsigned)hr_count));
+    const int owner = __ffsll((unsigned long long)__ballot(inc > target)) - 1;
+    int prefix = readlane(inc, owner) - readlane(mine, owner);  // units of the requests before r
+    r = owner * chunk;
+    if (chunk > 1) {  // the request is one of the lane's: 64 of them at a time, in len_lane
+      for (piece = r;; piece += 64) {
+        len_lane = piece + lane < a.requests ? a.lengths[piece + lane] : 0;
+        const int t = piece + lane < a.requests
+                          ? span_of(len_lane, most, a.window).units + kRowCost : 0;
+        const int s = wave_scan(t) + prefix;
+        const uint64_t hit = __ballot(s > target);
+        if (hit) {
+          const int at = __ffsll((unsigned long long)hit) - 1;
+          r = piece + at;
+          prefix = readlane(s, at) - readlane(t, at);
+          break;
+        }
+        prefix = readlane(s, 63);
+        if (piece + 64 >= a.requests) break;  // only if the lengths changed under the scan
       }
-      prefix = readlane(s, 63);
-      piece += 64;
-      if (piece >= a.requests) return;  // only if the lengths changed under the scan
     }
-  }
-  Span sp = span_of(readlane(len_lane, r - piece), most, a.window);
-  int hr;
-  unsigned row_u;  // where the row begins; its units come behind its cost
-  {
+    sp = span_of(readlane(len_lane, (r - piece) & 63), most, a.window);
     const unsigned off = u - (unsigned)prefix * (unsigned)hr_count;
     const unsigned row = (unsigned)(sp.units + kRowCost);
-    hr = uniform((int)(off / row));
+    hr = min(uniform((int)(off / row)), hr_count - 1);
     row_u = u - (off - (unsigned)hr * row);
   }
+  if (lane < 2) lds_row[2 * wave + lane] = -1;
   const int page_size = a.page_size;
 
-  for (; r < a.requests; ) {
+  // A row's first query head, and how many of its 16 columns are heads.
+  auto first_head = [&](int hr) {
+    const int kv = a.head_tiles == 1 ? hr : uniform(hr / a.head_tiles);
+    return kv * a.group + (hr - kv * a.head_tiles) * 16;
+  };
+  auto head_count = [&](int hr) {
+    const int kv = a.head_tiles == 1 ? hr : uniform(hr / a.head_tiles);
+    return min(a.group - (hr - kv * a.head_tiles) * 16, 16);
+  };
+  auto lse_of = [&](float top, float sum) {
+    return sum == 0.0f ? -__builtin_inff()
+                       : (top - kShift + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+  };
+
+  while (u < u_end && r < a.requests) {
     const unsigned data_u = row_u + kRowCost, row_end = data_u + (unsigned)sp.units;
     if (data_u >= u_end) break;
-    const int unit = u > data_u ? (int)(u - data_u) : 0;  // this workgroup's units of the row
+    const int unit = u > data_u ? (int)(u - data_u) : 0;  // this wave's units of the row
     const int unit_end = (int)(min(u_end, row_end) - data_u);
     const int kv = a.head_tiles == 1 ? hr : uniform(hr / a.head_tiles);
-    const int head0 = kv * a.group + (hr - kv * a.head_tiles) * 16;
-    const int left = a.group - (hr - kv * a.head_tiles) * 16;
-    const int heads = left < 16 ? left : 16;
+    const int head0 = first_head(hr), heads = head_count(hr);
     const int32_t* table = a.tables + (int64_t)r * a.table_stride;
     const unsigned char* kbase = a.key + (int64_t)kv * a.k_head;
     const unsigned char* vbase = a.value + (int64_t)kv * a.v_head;
@@ -201,7 +226,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
     u32x4 kf[2][kKeyLoads];
     uint32_t vf[8][kValueWords];
 
-    // The pages of a tile's tokens: of a lane's key rows (two; one page where pages are whole
+    // The pages of a unit's tokens: of a lane's key rows (two; one page where pages are whole
     // groups of eight tokens) and value rows (eight, or one), with the place of the first token in
     // the page. Tokens past the end stand for the last one; tokens of a page that is none of the
     // cache's for page 0. Both are masked.
@@ -271,7 +296,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
     };
 
     auto start_of = [&](int t) { return sp.base + t * kUnit; };
-    // Table entries are looked up one tile further ahead than rows, so that no row waits for one.
+    // Table entries are looked up one unit further ahead than rows, so that no row waits for one.
     Pages now, ahead;
     u32x4 q[kMfmas];
     bool two_parts = true;
@@ -290,7 +315,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
 #pragma unroll
     for (int k = 0; k < kMfmas; ++k) q[k] = (u32x4){0, 0, 0, 0};
     now = ahead = Pages{};
-    int t = unit + wave;
+    int t = unit;
     tok0 = start_of(t);
     live = t < unit_end && tok0 < len;
     if (live) {
@@ -307,11 +332,11 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
       }
       load_keys(tok0, now);
       load_values(tok0, now);
-      if (t + kWaves < unit_end) look_up(start_of(t + kWaves), ahead);
+      if (t + 1 < unit_end) look_up(start_of(t + 1), ahead);
     }
     while (live) {
-      const int next = start_of(t + kWaves);
-      const bool more = t + kWaves < unit_end;
+      const int next = start_of(t + 1);
+      const bool more = t + 1 < unit_end;
       // whether the lane's eight tokens are all attended to: past the ends of the window and the
       // request, and on pages that are none, they are not
       bool page_ok = true;
@@ -354,7 +379,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
       if (more) {
         load_keys(next, ahead);
         now = ahead;
-        if (t + 2 * kWaves < unit_end) look_up(start_of(t + 2 * kWaves), ahead);
+        if (t + 2 < unit_end) look_up(start_of(t + 2), ahead);
       }
 
       // ---- running maximum and sum ----
@@ -439,7 +464,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
       if (more) load_values(next, now);
       tok0 = next;
       live = more;
-      t += kWaves;
+      ++t;
     }
     float finite = 0.0f;
 #pragma unroll
@@ -457,145 +482,53 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 
-    // ---- the four waves' parts ----
-    if (c < heads) {
+    if (unit == 0 && unit_end == sp.units) {
+      // the whole row: a lane has 4 kLaneDims consecutive values of its head
+      const int64_t row = (int64_t)r * a.kv_heads * a.group + head0 + c;
+      const float inv = l == 0.0f ? 0.0f : a.value_scale / l;
+      if (c < heads) {
+        uint32_t w[2 * kLaneDims];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < kLaneDims; e += 4)
-          *reinterpret_cast<f32x4*>(&lds_acc[wave][c][kLaneDims * (4 * g + i) + e]) =
-              (f32x4){acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]};
-      if (g == 0) {
-        lds_m[wave][c] = m;
-        lds_l[wave][c] = l;
-      }
-    }
-    __syncthreads();
-    const bool whole = unit == 0 && unit_end == sp.units;
-    const int w_first = whole ? 0 : uniform((int)(data_u / per));
-    const int w_last = whole ? 0 : uniform((int)((row_end - 1) / per));
-    const int parts = w_last - w_first + 1, part = (int)blockIdx.x - w_first;
-
-    // A head's four values of a row: the result, or a part of it.
-    auto write_row = [&](int h, int d, f32x4 o, float top, float sum) {
-      const int64_t row = (int64_t)r * a.kv_heads * a.group + head0 + h;
-      const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
-      if (d < a.dim)
-        *reinterpret_cast<u32x2*>(a.out + row * a.dim + d) =
-            (u32x2){pack2<DT>(o.x * inv, o.y * inv), pack2<DT>(o.z * inv, o.w * inv)};
-      if (a.lse && d == 0)
-        a.lse[row] = sum == 0.0f ? -__builtin_inff()
-                                 : (top - kShift + __builtin_amdgcn_logf(sum)) *
-                                       0.6931471805599453f;
-    };
-    auto slot_of = [&](int n) {  // byte offset of the row's part n
-      return ((uint32_t)(w_first + n) * 2u + (n == 0 ? 1u : 0u)) * (uint32_t)slot_bytes;
-    };
-    auto write_part = [&](int n, int h, int d, f32x4 o, float top, float sum) {
-      const uint32_t at = slot_of(n) + (uint32_t)(h * (kPartHead + DIM)) * 4u;
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), parts_rsrc,
-                                             at + (uint32_t)(kPartHead + d) * 4u, 0, kDeviceScope);
-      if (d == 0)
-        __builtin_amdgcn_raw_buffer_store_b64(
-            (u32x2){__float_as_uint(top), __float_as_uint(sum)}, parts_rsrc, at, 0, kDeviceScope);
-    };
-    // Every store of the workgroup has arrived, then one count: true in the last of `of` to come.
-    auto arrived_last = [&](uint32_t* counter, int of) {
-      __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (tid == 0) {
-        const bool is_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
-                                                    __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(of - 1);
-        if (is_last)
-          __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        lds_last = is_last;
-      }
-      __syncthreads();
-      return lds_last != 0;
-    };
-    for (int i = tid; i < heads * kVecs; i += kThreads) {
-      const int h = i / kVecs, d = (i - h * kVecs) * 4;
-      float top = lds_m[0][h];
+          for (int e = 0; e < kLaneDims; e += 2)
+            w[(i * kLaneDims + e) / 2] = pack2<DT>(acc[e][i] * inv, acc[e + 1][i] * inv);
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds_m[w][h]);
-      const float base = top == -__builtin_inff() ? 0.0f : top;
-      f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-      float sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(lds_m[w][h] - base);
-        sum += lds_l[w][h] * f;
-        o += *reinterpret_cast<const f32x4*>(&lds_acc[w][h][d]) * f;
-      }
-      if (whole) write_row(h, d, o, top, sum);
-      else write_part(part, h, d, o, top, sum);
-    }
-    if (!whole) {
-      // Counters: of a row's first (or only) run of parts by the workgroup the row begins in, of
-      // its other runs by their first workgroup (which continues no other row), of its runs by
-      // the workgroup it begins in again.
-      uint32_t* const of_rows = a.counters;
-      uint32_t* const of_runs = a.counters + gridDim.x;
-      uint32_t* const of_joins = a.counters + 2 * gridDim.x;
-      const int run = part / kJoin;
-      int n0 = run * kJoin, step = 1, n_end = min(parts, n0 + kJoin);
-      bool final = parts <= kJoin;
-      bool last = arrived_last(run == 0 ? of_rows + w_first : of_runs + w_first + n0, n_end - n0);
-#pragma unroll 1
-      while (last) {
-        // parts n0, n0 + step, ... below n_end, in that order, eight requested at a time
-#pragma unroll 1
-        for (int i = tid; i < heads * kVecs; i += kThreads) {
-          const int h = i / kVecs, d = (i - h * kVecs) * 4;
-          const uint32_t in_slot = (uint32_t)(h * (kPartHead + DIM)) * 4u;
-          float top = -__builtin_inff(), sum = 0.0f;
-          f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-          for (int n = n0; n < n_end; n += 8 * step) {
-            u32x4 v[8];
-            u32x2 ml[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              // parts past the end are not there: the first is read in their place
-              const uint32_t at = slot_of(n + k * step < n_end ? n + k * step : n0) + in_slot;
-              ml[k] = __builtin_amdgcn_raw_buffer_load_b64(parts_rsrc, at, 0, kDeviceScope);
-              v[k] = load16_device(parts_rsrc, at + (uint32_t)(kPartHead + d) * 4u);
-            }
-            float t = top;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (n + k * step < n_end) t = fmaxf(t, __uint_as_float(ml[k].x));
-            const float base = t == -__builtin_inff() ? 0.0f : t;
-            const float fix = __builtin_amdgcn_exp2f(top - base);
-            o *= fix;
-            sum *= fix;
-            top = t;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t x = ml[k].x, y = ml[k].y;
-              if (n + k * step < n_end) {
-                const float f = __builtin_amdgcn_exp2f(__uint_as_float(x) - base);
-                sum += __uint_as_float(y) * f;
-                o += __builtin_bit_cast(f32x4, v[k]) * f;
-              }
-            }
-          }
-          if (final) write_row(h, d, o, top, sum);
-          else write_part(n0, h, d, o, top, sum);
+        for (int k = 0; k < 2 * kLaneDims; k += 4) {
+          const int d = 4 * kLaneDims * g + 2 * k;
+          if (d < a.dim)
+            *reinterpret_cast<u32x4*>(a.out + row * a.dim + d) =
+                (u32x4){w[k], w[k + 1], w[k + 2], w[k + 3]};
         }
-        if (final) break;
-        last = arrived_last(of_joins + w_first, (parts + kJoin - 1) / kJoin);
-        n0 = 0, step = kJoin, n_end = parts, final = true;
+        if (a.lse && g == 0) a.lse[row] = lse_of(m, l);
+      }
+    } else {
+      const int s = 2 * wave + (unit == 0 ? 1 : 0);
+      if (c < heads) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < kLaneDims; e += 4)
+            *reinterpret_cast<f32x4*>(&lds_acc[s][c][kLaneDims * (4 * g + i) + e]) =
+                (f32x4){acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]};
+        if (g == 0) {
+          lds_m[s][c] = m;
+          lds_l[s][c] = l;
+        }
+      }
+      if (lane == 0) {
+        lds_row[s] = r * hr_count + hr;
+        lds_units[s] = sp.units;
+        lds_data[s] = data_u;
       }
     }
-    __syncthreads();  // the next segment writes the same LDS
 
     // ---- on to the next row ----
     row_u = row_end;
     if (++hr == hr_count) {
       hr = 0;
       ++r;
-      if (row_u < u_end) {
+      if (row_u < u_end && r < a.requests) {
         if (r - piece == 64) {
           piece = r;
           len_lane = piece + lane < a.requests ? a.lengths[piece + lane] : 0;
@@ -603,6 +536,155 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
         sp = span_of(readlane(len_lane, r - piece), most, a.window);
       }
     }
+  }
+  __syncthreads();
+
+  // ---- rows that waves of this workgroup share ----
+  // A head's four values of a row: the result, or a part of it.
+  auto write_row = [&](int row, int h, int d, f32x4 o, float top, float sum) {
+    const int rr = row / hr_count;
+    const int64_t at = (int64_t)rr * a.kv_heads * a.group + first_head(row - rr * hr_count) + h;
+    const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
+    if (d < a.dim)
+      *reinterpret_cast<u32x2*>(a.out + at * a.dim + d) =
+          (u32x2){pack2<DT>(o.x * inv, o.y * inv), pack2<DT>(o.z * inv, o.w * inv)};
+    if (a.lse && d == 0) a.lse[at] = lse_of(top, sum);
+  };
+  // Byte offset of part n of a row that begins in workgroup w_first.
+  auto slot_of = [&](int w_first, int n) {
+    return ((uint32_t)(w_first + n) * 2u + (n == 0 ? 1u : 0u)) * (uint32_t)slot_bytes;
+  };
+  auto write_part = [&](uint32_t slot, int h, int d, f32x4 o, float top, float sum) {
+    const uint32_t at = slot + (uint32_t)(h * (kPartHead + DIM)) * 4u;
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), parts_rsrc,
+                                           at + (uint32_t)(kPartHead + d) * 4u, 0, kDeviceScope);
+    if (d == 0)
+      __builtin_amdgcn_raw_buffer_store_b64(
+          (u32x2){__float_as_uint(top), __float_as_uint(sum)}, parts_rsrc, at, 0, kDeviceScope);
+  };
+  // The rows that go on in other workgroups: the one this workgroup begins in (0), the one it ends in.
+  int open_row[2] = {-1, -1}, open_first[2] = {0, 0}, open_parts[2] = {0, 0};
+  int done = -1;
+#pragma unroll 1
+  for (int s = 0; s < kSlots; ++s) {
+    const int row = uniform(lds_row[s]);
+    if (row < 0 || row == done) continue;
+    done = row;
+    const unsigned data_u = (unsigned)uniform((int)lds_data[s]);
+    const unsigned row_end = data_u + (unsigned)uniform(lds_units[s]);
+    const bool whole = data_u >= wg_u && row_end <= wg_end;
+    const int w_first = whole ? run : uniform((int)(data_u / per));
+    uint32_t slot = 0;
+    if (!whole) {
+      const int k = w_first == run ? 1 : 0;
+      open_row[k] = row;
+      open_first[k] = w_first;
+      open_parts[k] = uniform((int)((row_end - 1) / per)) - w_first + 1;
+      slot = slot_of(w_first, run - w_first);
+    }
+    const int heads = head_count(uniform(row % hr_count));
+#pragma unroll 1
+    for (int i = tid; i < heads * kVecs; i += kThreads) {
+      const int h = i / kVecs, d = (i - h * kVecs) * 4;
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int k = 0; k < kSlots; ++k)
+        if (lds_row[k] == row) top = fmaxf(top, lds_m[k][h]);
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+      f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kSlots; ++k)
+        if (lds_row[k] == row) {
+          const float f = __builtin_amdgcn_exp2f(lds_m[k][h] - base);
+          sum += lds_l[k][h] * f;
+          o += *reinterpret_cast<const f32x4*>(&lds_acc[k][h][d]) * f;
+        }
+      if (whole) write_row(row, h, d, o, top, sum);
+      else write_part(slot, h, d, o, top, sum);
+    }
+  }
+  if (open_row[0] < 0 && open_row[1] < 0) return;
+
+  // ---- rows that workgroups share: the last to arrive joins their parts, in order ----
+  // Every store of the workgroup has arrived, then one count: true in the last of `of` to come.
+  auto arrived_last = [&](uint32_t* counter, int of) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+      const bool is_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(of - 1);
+      if (is_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      lds_last = is_last;
+    }
+    __syncthreads();
+    return lds_last != 0;
+  };
+  // Counters: of a row's first (or only) run of parts by the workgroup the row begins in, of its
+  // other runs by their first workgroup (which continues no other row), of its runs by the
+  // workgroup it begins in again.
+  uint32_t* const of_rows = a.counters;
+  uint32_t* const of_runs = a.counters + gridDim.x;
+  uint32_t* const of_joins = a.counters + 2 * gridDim.x;
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    const int row = k ? open_row[1] : open_row[0];
+    if (row < 0) continue;
+    const int w_first = k ? open_first[1] : open_first[0];
+    const int parts = k ? open_parts[1] : open_parts[0];
+    const int heads = head_count(uniform(row % hr_count));
+    const int group = (run - w_first) / kJoin;
+    int n0 = group * kJoin, step = 1, n_end = min(parts, n0 + kJoin);
+    bool final = parts <= kJoin;
+    bool last = arrived_last(group == 0 ? of_rows + w_first : of_runs + w_first + n0, n_end - n0);
+#pragma unroll 1
+    while (last) {
+      // parts n0, n0 + step, ... below n_end, in that order, eight requested at a time
+#pragma unroll 1
+      for (int i = tid; i < heads * kVecs; i += kThreads) {
+        const int h = i / kVecs, d = (i - h * kVecs) * 4;
+        const uint32_t in_slot = (uint32_t)(h * (kPartHead + DIM)) * 4u;
+        float top = -__builtin_inff(), sum = 0.0f;
+        f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+        for (int n = n0; n < n_end; n += 8 * step) {
+          u32x4 v[8];
+          u32x2 ml[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            // parts past the end are not there: the first is read in their place
+            const uint32_t at =
+                slot_of(w_first, n + q * step < n_end ? n + q * step : n0) + in_slot;
+            ml[q] = __builtin_amdgcn_raw_buffer_load_b64(parts_rsrc, at, 0, kDeviceScope);
+            v[q] = load16_device(parts_rsrc, at + (uint32_t)(kPartHead + d) * 4u);
+          }
+          float t = top;
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (n + q * step < n_end) t = fmaxf(t, __uint_as_float(ml[q].x));
+          const float base = t == -__builtin_inff() ? 0.0f : t;
+          const float fix = __builtin_amdgcn_exp2f(top - base);
+          o *= fix;
+          sum *= fix;
+          top = t;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t x = ml[q].x, y = ml[q].y;
+            if (n + q * step < n_end) {
+              const float f = __builtin_amdgcn_exp2f(__uint_as_float(x) - base);
+              sum += __uint_as_float(y) * f;
+              o += __builtin_bit_cast(f32x4, v[q]) * f;
+            }
+          }
+        }
+        if (final) write_row(row, h, d, o, top, sum);
+        else write_part(slot_of(w_first, n0), h, d, o, top, sum);
+      }
+      if (final) break;
+      last = arrived_last(of_joins + w_first, (parts + kJoin - 1) / kJoin);
+      n0 = 0, step = kJoin, n_end = parts, final = true;
+    }
+    __syncthreads();  // lds_last
   }
 }
 
