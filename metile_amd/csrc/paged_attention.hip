@@ -23,7 +23,7 @@
 // wave's run is written by that wave, with no exchange at all. A wave's parts of other rows (the
 // first and the last of its run) meet in LDS at the end, and the workgroup's parts of rows that go
 // on in other workgroups are stored with their maximum and sum and joined, in order, by the last
-// of those workgroups to arrive (32 parts at a time).
+// of those workgroups to arrive (8 or 16 parts at a time).
 #include "common.h"
 #include "paged.h"
 
@@ -76,6 +76,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
 }
 
+// Keys and values are read once, with the hint that says so (2 x 131072 tokens of 8 heads of 128
+// values 211 -> 202 us), except where a head's row of a token is less than a line and its
+// neighbours' follow: then other workgroups read the rest of the line.
+template <bool ONCE, typename T>
+__device__ __forceinline__ T stream_load(const T* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 // Two 8-bit floats (half HI of a word) as 16-bit ones: exact.
 template <int DT, bool HI>
 __device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
@@ -95,8 +104,14 @@ __device__ __forceinline__ u32x4 fp8_eight(uint32_t lo, uint32_t hi) {
 // Where a workgroup's partial sums of a row are kept: [heads][kPartHead + DIM] floats a slot, the
 // maximum and the sum in front of a head's values.
 constexpr int kPartHead = 4;
-// Parts that one workgroup joins; a row of more is joined in two rounds.
-constexpr int kJoin = 32;
+// Parts that one workgroup joins at a time; rows of more are joined in levels. Eight where a part is
+// over 8 KiB: one workgroup reads about 50 KB a microsecond. (16 parts of 16 heads of 256 values a
+// join: @FAN@.)
+constexpr int kJoin = 16, kJoinLarge = 8, kLargePart = 8192;
+// The counters of four levels (8^4 parts) of twice so many fit the workspace's region of them.
+constexpr int kMostWorkgroups = 2048;
+static_assert(kMostWorkgroups * 2 * 4 * 4 <= 64 * 1024 && kMostWorkgroups <= 8 * 8 * 8 * 8,
+              "counters of every level");
 
 // Waves a SIMD (and so workgroups a CU) that the registers are allotted for.
 constexpr int attention_waves(int padded_dim, bool page8) {
@@ -153,6 +168,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
   const unsigned waves = gridDim.x * kWaves;
   const unsigned per_wave =
       max((unsigned)uniform((int)((units + waves - 1) / waves)), (unsigned)(kAttentionLeast / kWaves));
+  const int fan = slot_bytes > kLargePart ? kJoinLarge : kJoin;
   const unsigned per = per_wave * kWaves, wg_u = (unsigned)run * per;
   if (wg_u >= units) return;
   const unsigned wg_end = min(wg_u + per, units);
@@ -265,7 +281,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
         for (int k = 0; k < kKeyLoads; ++k) {
           const int d = FP8 ? 64 * k + 16 * g : 32 * k + 8 * g;
           kf[t][k] =
-              __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + (d < a.dim ? d * kElt : 0)));
+              stream_load<!(FP8 && DIM == 64)>(reinterpret_cast<const u32x4*>(row + (d < a.dim ? d * kElt : 0)));
         }
       }
     };
@@ -283,14 +299,14 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
         if constexpr (kValueWords >= 4) {
 #pragma unroll
           for (int w = 0; w < kValueWords; w += 4) {
-            const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + 4 * w));
+            const u32x4 v = stream_load<!(FP8 && DIM == 64)>(reinterpret_cast<const u32x4*>(row + 4 * w));
             vf[j][w] = v.x, vf[j][w + 1] = v.y, vf[j][w + 2] = v.z, vf[j][w + 3] = v.w;
           }
         } else if constexpr (kValueWords == 2) {
-          const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(row));
+          const u32x2 v = stream_load<!(FP8 && DIM == 64)>(reinterpret_cast<const u32x2*>(row));
           vf[j][0] = v.x, vf[j][1] = v.y;
         } else {
-          vf[j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(row));
+          vf[j][0] = stream_load<!(FP8 && DIM == 64)>(reinterpret_cast<const uint32_t*>(row));
         }
       }
     };
@@ -564,14 +580,18 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
   };
   // The rows that go on in other workgroups: the one this workgroup begins in (0), the one it ends in.
   int open_row[2] = {-1, -1}, open_first[2] = {0, 0}, open_parts[2] = {0, 0};
-  int done = -1;
+  const int row_lane = lane < kSlots ? lds_row[lane] : -1;
+  const int units_lane = lane < kSlots ? lds_units[lane] : 0;
+  const int data_lane = lane < kSlots ? (int)lds_data[lane] : 0;
+  uint64_t slots = __ballot(row_lane >= 0);
 #pragma unroll 1
-  for (int s = 0; s < kSlots; ++s) {
-    const int row = uniform(lds_row[s]);
-    if (row < 0 || row == done) continue;
-    done = row;
-    const unsigned data_u = (unsigned)uniform((int)lds_data[s]);
-    const unsigned row_end = data_u + (unsigned)uniform(lds_units[s]);
+  while (slots) {
+    const int s = __ffsll((unsigned long long)slots) - 1;
+    const int row = readlane(row_lane, s);
+    const uint64_t same = __ballot(row_lane == row);  // the row's slots: one wave after another
+    slots &= ~same;
+    const unsigned data_u = (unsigned)readlane(data_lane, s);
+    const unsigned row_end = data_u + (unsigned)readlane(units_lane, s);
     const bool whole = data_u >= wg_u && row_end <= wg_end;
     const int w_first = whole ? run : uniform((int)(data_u / per));
     uint32_t slot = 0;
@@ -586,20 +606,18 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
 #pragma unroll 1
     for (int i = tid; i < heads * kVecs; i += kThreads) {
       const int h = i / kVecs, d = (i - h * kVecs) * 4;
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int k = 0; k < kSlots; ++k)
-        if (lds_row[k] == row) top = fmaxf(top, lds_m[k][h]);
-      const float base = top == -__builtin_inff() ? 0.0f : top;
+      float top = -__builtin_inff(), sum = 0.0f;
       f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-      float sum = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kSlots; ++k)
-        if (lds_row[k] == row) {
-          const float f = __builtin_amdgcn_exp2f(lds_m[k][h] - base);
-          sum += lds_l[k][h] * f;
-          o += *reinterpret_cast<const f32x4*>(&lds_acc[k][h][d]) * f;
-        }
+      for (uint64_t rest = same; rest; rest &= rest - 1) {
+        const int k = __ffsll((unsigned long long)rest) - 1;
+        const float m = lds_m[k][h], l = lds_l[k][h];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(&lds_acc[k][h][d]);
+        const float t = fmaxf(top, m), base = t == -__builtin_inff() ? 0.0f : t;
+        const float old = __builtin_amdgcn_exp2f(top - base), now = __builtin_amdgcn_exp2f(m - base);
+        sum = sum * old + l * now;
+        o = o * old + v * now;
+        top = t;
+      }
       if (whole) write_row(row, h, d, o, top, sum);
       else write_part(slot, h, d, o, top, sum);
     }
@@ -620,12 +638,10 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
     __syncthreads();
     return lds_last != 0;
   };
-  // Counters: of a row's first (or only) run of parts by the workgroup the row begins in, of its
-  // other runs by their first workgroup (which continues no other row), of its runs by the
-  // workgroup it begins in again.
-  uint32_t* const of_rows = a.counters;
-  uint32_t* const of_runs = a.counters + gridDim.x;
-  uint32_t* const of_joins = a.counters + 2 * gridDim.x;
+  // Parts are joined `fan` at a time (level 0), then the results of `fan` such joins (level 1), and
+  // so on. The counter of a join whose first part is n0 belongs to that part's workgroup, two to a
+  // level: a workgroup can hold the first part of one row and a later part of another, no more.
+  const int items = head_count(0) * kVecs;  // the most of a row
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
     const int row = k ? open_row[1] : open_row[0];
@@ -633,56 +649,80 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
     const int w_first = k ? open_first[1] : open_first[0];
     const int parts = k ? open_parts[1] : open_parts[0];
     const int heads = head_count(uniform(row % hr_count));
-    const int group = (run - w_first) / kJoin;
-    int n0 = group * kJoin, step = 1, n_end = min(parts, n0 + kJoin);
-    bool final = parts <= kJoin;
-    bool last = arrived_last(group == 0 ? of_rows + w_first : of_runs + w_first + n0, n_end - n0);
+    int part = run - w_first, step = 1;
+    uint32_t* counters = a.counters;
 #pragma unroll 1
-    while (last) {
+    for (;;) {
+      const int span = step * fan;  // parts under one join of this level
+      const int n0 = part / span * span, n_end = min(parts, n0 + span);
+      const int arrivals = (n_end - n0 + step - 1) / step;
+      if (!arrived_last(counters + (n0 ? gridDim.x : 0) + w_first + n0, arrivals)) break;
       // parts n0, n0 + step, ... below n_end, in that order, eight requested at a time
+      const bool final = n_end - n0 == parts;
+      constexpr int kItems = DIM == 256 ? 4 : 1;  // of a thread at a time
 #pragma unroll 1
-      for (int i = tid; i < heads * kVecs; i += kThreads) {
-        const int h = i / kVecs, d = (i - h * kVecs) * 4;
-        const uint32_t in_slot = (uint32_t)(h * (kPartHead + DIM)) * 4u;
-        float top = -__builtin_inff(), sum = 0.0f;
-        f32x4 o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      for (int first = tid; first < items; first += kItems * kThreads) {
+      float top[kItems], sum[kItems];
+      f32x4 o[kItems];
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        top[i] = -__builtin_inff();
+        sum[i] = 0.0f;
+        o[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      }
 #pragma unroll 1
-        for (int n = n0; n < n_end; n += 8 * step) {
-          u32x4 v[8];
-          u32x2 ml[8];
+      for (int n = n0; n < n_end; n += 8 * step) {
+        u32x4 v[kItems][8];
+        u32x2 ml[kItems][8];
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          const int item = first + i * kThreads, h = item / kVecs, d = (item - h * kVecs) * 4;
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
-            // parts past the end are not there: the first is read in their place
-            const uint32_t at =
-                slot_of(w_first, n + q * step < n_end ? n + q * step : n0) + in_slot;
-            ml[q] = __builtin_amdgcn_raw_buffer_load_b64(parts_rsrc, at, 0, kDeviceScope);
-            v[q] = load16_device(parts_rsrc, at + (uint32_t)(kPartHead + d) * 4u);
+            // (what is not there is not read)
+            const uint32_t at = oob_unless(item < items && n + q * step < n_end,
+                                           slot_of(w_first, n + q * step) +
+                                               (uint32_t)(h * (kPartHead + DIM)) * 4u);
+            ml[i][q] = __builtin_amdgcn_raw_buffer_load_b64(parts_rsrc, at, 0, kDeviceScope);
+            v[i][q] = load16_device(parts_rsrc, at + (uint32_t)(kPartHead + d) * 4u);
           }
-          float t = top;
+        }
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (n + q * step < n_end) t = fmaxf(t, __uint_as_float(ml[q].x));
-          const float base = t == -__builtin_inff() ? 0.0f : t;
-          const float fix = __builtin_amdgcn_exp2f(top - base);
-          o *= fix;
-          sum *= fix;
-          top = t;
+        for (int i = 0; i < kItems; ++i) {
+          float t = top[i];
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
-            const uint32_t x = ml[q].x, y = ml[q].y;
+            const uint32_t x = ml[i][q].x;
+            if (n + q * step < n_end) t = fmaxf(t, __uint_as_float(x));
+          }
+          const float base = t == -__builtin_inff() ? 0.0f : t;
+          const float fix = __builtin_amdgcn_exp2f(top[i] - base);
+          o[i] *= fix;
+          sum[i] *= fix;
+          top[i] = t;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t x = ml[i][q].x, y = ml[i][q].y;
             if (n + q * step < n_end) {
               const float f = __builtin_amdgcn_exp2f(__uint_as_float(x) - base);
-              sum += __uint_as_float(y) * f;
-              o += __builtin_bit_cast(f32x4, v[q]) * f;
+              sum[i] += __uint_as_float(y) * f;
+              o[i] += __builtin_bit_cast(f32x4, v[i][q]) * f;
             }
           }
         }
-        if (final) write_row(row, h, d, o, top, sum);
-        else write_part(slot_of(w_first, n0), h, d, o, top, sum);
+      }
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int item = first + i * kThreads, h = item / kVecs, d = (item - h * kVecs) * 4;
+        if (h >= heads) continue;
+        if (final) write_row(row, h, d, o[i], top[i], sum[i]);
+        else write_part(slot_of(w_first, n0), h, d, o[i], top[i], sum[i]);
+      }
       }
       if (final) break;
-      last = arrived_last(of_joins + w_first, (parts + kJoin - 1) / kJoin);
-      n0 = 0, step = kJoin, n_end = parts, final = true;
+      part = n0;
+      step = span;
+      counters += 2 * gridDim.x;
     }
     __syncthreads();  // lds_last
   }
@@ -714,7 +754,8 @@ hipError_t launch_dim(const PagedAttentionArgs& a, int workgroups, hipStream_t s
 int paged_attention_workgroups(int cus, int dim, int page_size, int64_t units) {
   const int64_t most = attention_waves(padded_dim(dim), page_size % 8 == 0) * (int64_t)cus;
   const int64_t runs = (units + kAttentionLeast - 1) / kAttentionLeast;
-  return (int)(runs < most ? (runs > 0 ? runs : 1) : most);
+  const int64_t n = runs < most ? (runs > 0 ? runs : 1) : most;
+  return (int)(n < kMostWorkgroups ? n : kMostWorkgroups);
 }
 
 size_t paged_attention_slot_floats(int group, int dim) {
