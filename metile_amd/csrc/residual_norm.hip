@@ -93,10 +93,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_k
     at[i] = min(e, width - 8);
     skip[i] = e < width ? e - at[i] : 8;
   }
-  // Only the second half of a thread's vectors can be past the end or the last one: with NV of
-  // them, a row has more than NV / 2 (or NV is 1).
+  // A row has more than kSure vectors a thread (launch_width sees to it): only those behind can be
+  // its last one or past it.
+  constexpr int kSure = NV == 3 ? 2 : NV / 2;
   auto counted = [&](float v, int i, int j) {
-    return i >= NV / 2 && j < skip[i] ? 0.0f : v;
+    return i >= kSure && j < skip[i] ? 0.0f : v;
   };
 
   float x[NV][8], b[NV][8];
@@ -249,6 +250,9 @@ void launch_rows(const ResidualNormArgs& a, hipStream_t stream) {
 //   16384 x 2048    1, 4   51 / 56                 2, 2  45 / 47       4, 1   42 / 49
 //    4096 x 8192    4, 4   51 / 58                 8, 2  45 / 49      16, 1   44 / 56
 //    4096 x 896     1, 2   8.4 / 10.0              4, 1   9.4 / 13.1
+//   16384 x 1133    1, 3  33 / 37                  2, 2   .. / 45       4, 1   36 / ..
+//    4096 x 1536    1, 3  10.7 / 12.5              2, 2   .. / 13.6     4, 1   11.2 / ..
+//    1024 x 1536    1, 3   5.7 / 6.7               2, 2   .. / 6.1      4, 1   4.5 / ..
 // (98 us for 16384 x 4096 are 5.5 TB/s; a copy of 1 GiB reaches 5.1 to 5.2.)
 template <int DT, typename RT, bool LAYER>
 void launch_width(const ResidualNormArgs& a, int cus, hipStream_t stream) {
@@ -258,6 +262,7 @@ void launch_width(const ResidualNormArgs& a, int cus, hipStream_t stream) {
     residual_norm_narrow_kernel<DT, RT, LAYER><<<(a.rows + 255) / 256, 256, 0, stream>>>(a);
   else if (w <= 512) launch_rows<DT, RT, LAYER, 1, 1>(a, stream);
   else if (w <= 1024 && many) launch_rows<DT, RT, LAYER, 1, 2>(a, stream);
+  else if (w <= 1536 && many && LAYER) launch_rows<DT, RT, LAYER, 1, 3>(a, stream);
   else if (w <= 2048 && many && LAYER) launch_rows<DT, RT, LAYER, 2, 2>(a, stream);
   else if (w <= 2048) launch_rows<DT, RT, LAYER, 4, 1>(a, stream);
   else if (w <= 4096 && many) launch_rows<DT, RT, LAYER, 4, 2>(a, stream);

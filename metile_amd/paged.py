@@ -25,6 +25,21 @@ _DTYPES = {torch.bfloat16: _lib.MT_BF16, torch.float16: _lib.MT_F16}
 _CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.MT_FP8}
 
 
+# torch's own getter without the check for initialisation, which a tensor on the device has done
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch(device, call, *args):
+    """``call(*args, stream)`` on torch's current stream of ``device``, checked."""
+    if device.index == _current_device():
+        status = call(*args, _stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            status = call(*args, _stream_handle(device))
+    if status:
+        _lib.check(status)
+
+
 def _same_device(device, *tensors):
     """Refuses tensors that are not all on the ROCm device ``device``."""
     if device.type != "cuda":
@@ -179,17 +194,6 @@ def paged_tables(cached, new, block_tables, free_pages, *, page_size, tokens, fr
     return PagedStep(slots, positions, owners, starts, lengths, taken)
 
 
-def _launch(device, call, *args):
-    """``call(*args, stream)`` on torch's current stream of ``device``, checked."""
-    if device.index == torch.cuda.current_device():
-        status = call(*args, _stream_handle(device))
-    else:
-        with torch.cuda.device(device):
-            status = call(*args, _stream_handle(device))
-    if status:
-        _lib.check(status)
-
-
 def paged_append(key, value, cache, slots):
     """Write ``key`` and ``value`` (``[tokens, kv_heads, head_dim]``, bfloat16 or float16) to ``slots``
     (int64 ``[tokens]``, as :func:`paged_tables` gives them) of ``cache``, in place. Tokens whose slot
@@ -254,7 +258,8 @@ def paged_attention(query, cache, block_tables, lengths, *, scale=None, window=N
         window = min(window, (1 << 31) - 1)
     device = cache._device
     _same_device(device, query, block_tables, lengths)
-    out = torch.empty(shape, dtype=dtype, device=device)
+    out = (torch.empty_like(query) if query.is_contiguous()
+           else torch.empty(shape, dtype=dtype, device=device))
     lse = torch.empty((requests, heads), dtype=torch.float32, device=device) if return_lse else None
     if not requests or not width:
         out.zero_()
@@ -269,7 +274,7 @@ def paged_attention(query, cache, block_tables, lengths, *, scale=None, window=N
         query.data_ptr(), row, head, block_tables.data_ptr(), block_tables.stride(0),
         lengths.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), requests, heads,
         width, window, dim ** -0.5 if scale is None else scale, _DTYPES[dtype])
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():
         _attend(cache, args, requests, heads, width, window)
     else:
         with torch.cuda.device(device):
