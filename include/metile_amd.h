@@ -423,9 +423,9 @@ int mt_paged_append(const mt_paged_cache* cache, const mt_paged_append_args* arg
 /* Attention of one new token per request over its pages: out[r, h] = sum_t p_t v_t with p =
  * softmax(scale * q[r, h] . k_t) over the request's last `window` tokens (0: all of them), of the
  * key-value head h / (heads / cache heads). lengths[r] counts the tokens in the cache, the new one
- * among them (its key and value are appended first); it is limited to [0, width * page_size]. Rows
- * without a token give 0. lse (or NULL) [requests, heads] receives log sum exp of the scaled
- * scores, -inf for such rows. Table entries behind a request's last token are not read; tokens
+ * among them (its key and value are appended first); it is limited to [0, width * page_size], which
+ * is at most 2^31 - 64. Rows without a token give 0. lse (or NULL) [requests, heads] receives log
+ * sum exp of the scaled scores, -inf for such rows. Table entries behind a request's last token are not read; tokens
  * whose entry is not a page of the cache are left out, and what slots behind the last token hold
  * does not matter. query [requests, heads, dim] with element strides per request and head
  * (multiples of 16 bytes), out [requests, heads, dim] contiguous, 16-byte aligned, both in dtype;

@@ -81,8 +81,9 @@ int plan_attention(const char* op, const mt_paged_cache* c, int requests, int he
   if (requests < 1) return refuse(op, "requests must be positive");
   if (heads < 1 || heads > kMaxHeads || heads % c->heads)
     return refuse(op, "query heads must be a positive multiple of the cache's");
-  if (width < 1 || (int64_t)width * c->page_size >= kInt31)
-    return refuse(op, "block table width must be positive and hold fewer than 2^31 tokens");
+  // (64 less than 2^31: the kernel counts to the end of the last unit in 32 bits)
+  if (width < 1 || (int64_t)width * c->page_size > kInt31 - 64)
+    return refuse(op, "block table width must be positive and hold fewer than 2^31 - 64 tokens");
   if (window < 0) return refuse(op, "window must not be negative");
   const int group = heads / c->heads, head_tiles = (group + 15) / 16;
   const int64_t units = most_units((int64_t)width * c->page_size, window);
@@ -205,7 +206,8 @@ int mt_paged_attention(const mt_paged_cache* cache, const mt_paged_attention_arg
     return refuse(op, "dtype must be MT_BF16 or MT_F16");
   if (cache->dtype != MT_FP8 && cache->dtype != in.dtype)
     return refuse(op, "a 16-bit cache must have the query's dtype");
-  if (!std::isfinite(in.scale)) return refuse(op, "scale must be finite");
+  const float scale_log2 = in.scale * cache->key_scale * 1.4426950408889634f;
+  if (!std::isfinite(scale_log2)) return refuse(op, "scale must be finite");
   if (!in.query || !in.block_tables || !in.lengths || !in.out) return refuse(op, "null pointer");
   if (!aligned16(in.query) || !aligned16(in.out) || !stride16(in.query_strides[0], 2) ||
       !stride16(in.query_strides[1], 2))
@@ -246,7 +248,7 @@ int mt_paged_attention(const mt_paged_cache* cache, const mt_paged_attention_arg
   a.page_size = cache->page_size;
   a.width = in.width;
   a.window = in.window;
-  a.scale_log2 = in.scale * cache->key_scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   a.value_scale = cache->value_scale;
   a.by_page = mt::div_magic((uint32_t)cache->page_size);
   return launched(op, mt::launch_paged_attention(a, in.dtype, fp8, plan.workgroups,

@@ -2,9 +2,9 @@
 //
 // Each row is read once and written once; nothing else is to do but the conversion to 8-bit
 // floats (e4m3: the value over the cache's scale, limited to +-448, rounded to nearest even), so
-// memory bounds it. A thread moves eight values (16 bytes in) twice, side by side (16384 tokens of 8
-// heads of 128 into 8 bits, 101 MB: 23.2 us; four times 25.4, once 25.1); keys and values are the two
-// halves of the grid.
+// memory bounds it. A thread moves eight values (16 bytes in) twice, side by side (16384 tokens of
+// 8 heads of 128 into 8 bits, 101 MB: 23.2 us, 4.3 TB/s; four times 25.4, once 25.1); keys and values
+// are the two halves of the grid.
 #include "common.h"
 #include "paged.h"
 

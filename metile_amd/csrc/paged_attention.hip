@@ -24,6 +24,12 @@
 // first and the last of its run) meet in LDS at the end, and the workgroup's parts of rows that go
 // on in other workgroups are stored with their maximum and sum and joined, in order, by the last
 // of those workgroups to arrive (8 or 16 parts at a time).
+//
+// Bound by the bytes of keys and values where there are enough of them: 2 requests of 131072 tokens
+// with 8 key-value heads of 128 bf16 values (1.07 GB) take 185 us, 5.8 TB/s (a copy of 1 GiB
+// reaches 5.2); 64 requests of 1 to 8192 tokens (224 MB) 48 us, 4.6 TB/s. The shortest calls take
+// 5.5 us: the launch, then lengths, table entry and first rows, a memory round trip each after the
+// other; a row that several workgroups share costs about 4 us more for its join.
 #include "common.h"
 #include "paged.h"
 
@@ -104,9 +110,9 @@ __device__ __forceinline__ u32x4 fp8_eight(uint32_t lo, uint32_t hi) {
 // Where a workgroup's partial sums of a row are kept: [heads][kPartHead + DIM] floats a slot, the
 // maximum and the sum in front of a head's values.
 constexpr int kPartHead = 4;
-// Parts that one workgroup joins at a time; rows of more are joined in levels. Eight where a part is
-// over 8 KiB: one workgroup reads about 50 KB a microsecond. (16 parts of 16 heads of 256 values a
-// join: @FAN@.)
+// Parts that one workgroup joins at a time; rows of more are joined in levels. Eight where a part
+// is over 8 KiB: one workgroup reads about 50 KB a microsecond (16 requests of 6 to 13104 tokens,
+// 16 heads of 256 values on one key-value head: 33 us, 37 with 16 parts a join).
 constexpr int kJoin = 16, kJoinLarge = 8, kLargePart = 8192;
 // The counters of four levels (8^4 parts) of twice so many fit the workspace's region of them.
 constexpr int kMostWorkgroups = 2048;
@@ -119,8 +125,8 @@ constexpr int attention_waves(int padded_dim, bool page8) {
 }
 
 template <int DT, bool FP8, int DIM, bool PAGE8>
-__global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_attention_kernel(PagedAttentionArgs a,
-                                                                      int slot_bytes) {
+__global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_attention_kernel(
+    PagedAttentionArgs a, int slot_bytes) {
   constexpr int kElt = FP8 ? 1 : 2;
   constexpr int kMfmas = DIM / 32;               // K depth of a score
   constexpr int kLaneDims = DIM / 16;            // value dimensions of a lane
@@ -128,6 +134,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
   constexpr int kValueWords = kLaneDims * kElt / 4;
   constexpr int kRow = DIM + 4;                  // floats: heads start four banks apart
   constexpr int kVecs = DIM / 4;
+  constexpr bool kOnce = !(FP8 && DIM == 64);
   // f16 probabilities are scaled up so that small ones, and the second parts, stay above its
   // smallest numbers; the sum carries the same factor.
   constexpr float kShift = DT == kF16 ? 14.0f : 0.0f;
@@ -166,8 +173,8 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
   // (below 2^31, as the host checks; said to be the same in every lane)
   const unsigned units = (unsigned)readlane(inc, 63) * (unsigned)hr_count;
   const unsigned waves = gridDim.x * kWaves;
-  const unsigned per_wave =
-      max((unsigned)uniform((int)((units + waves - 1) / waves)), (unsigned)(kAttentionLeast / kWaves));
+  const unsigned per_wave = max((unsigned)uniform((int)((units + waves - 1) / waves)),
+                                (unsigned)(kAttentionLeast / kWaves));
   const int fan = slot_bytes > kLargePart ? kJoinLarge : kJoin;
   const unsigned per = per_wave * kWaves, wg_u = (unsigned)run * per;
   if (wg_u >= units) return;
@@ -280,8 +287,8 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
 #pragma unroll
         for (int k = 0; k < kKeyLoads; ++k) {
           const int d = FP8 ? 64 * k + 16 * g : 32 * k + 8 * g;
-          kf[t][k] =
-              stream_load<!(FP8 && DIM == 64)>(reinterpret_cast<const u32x4*>(row + (d < a.dim ? d * kElt : 0)));
+          kf[t][k] = stream_load<kOnce>(
+              reinterpret_cast<const u32x4*>(row + (d < a.dim ? d * kElt : 0)));
         }
       }
     };
@@ -299,14 +306,15 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
         if constexpr (kValueWords >= 4) {
 #pragma unroll
           for (int w = 0; w < kValueWords; w += 4) {
-            const u32x4 v = stream_load<!(FP8 && DIM == 64)>(reinterpret_cast<const u32x4*>(row + 4 * w));
+            const u32x4 v =
+                stream_load<kOnce>(reinterpret_cast<const u32x4*>(row + 4 * w));
             vf[j][w] = v.x, vf[j][w + 1] = v.y, vf[j][w + 2] = v.z, vf[j][w + 3] = v.w;
           }
         } else if constexpr (kValueWords == 2) {
-          const u32x2 v = stream_load<!(FP8 && DIM == 64)>(reinterpret_cast<const u32x2*>(row));
+          const u32x2 v = stream_load<kOnce>(reinterpret_cast<const u32x2*>(row));
           vf[j][0] = v.x, vf[j][1] = v.y;
         } else {
-          vf[j][0] = stream_load<!(FP8 && DIM == 64)>(reinterpret_cast<const uint32_t*>(row));
+          vf[j][0] = stream_load<kOnce>(reinterpret_cast<const uint32_t*>(row));
         }
       }
     };
@@ -578,7 +586,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
       __builtin_amdgcn_raw_buffer_store_b64(
           (u32x2){__float_as_uint(top), __float_as_uint(sum)}, parts_rsrc, at, 0, kDeviceScope);
   };
-  // The rows that go on in other workgroups: the one this workgroup begins in (0), the one it ends in.
+  // The rows that go on in other workgroups: the one this one begins in (0), the one it ends in.
   int open_row[2] = {-1, -1}, open_first[2] = {0, 0}, open_parts[2] = {0, 0};
   const int row_lane = lane < kSlots ? lds_row[lane] : -1;
   const int units_lane = lane < kSlots ? lds_units[lane] : 0;
@@ -613,7 +621,8 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
         const float m = lds_m[k][h], l = lds_l[k][h];
         const f32x4 v = *reinterpret_cast<const f32x4*>(&lds_acc[k][h][d]);
         const float t = fmaxf(top, m), base = t == -__builtin_inff() ? 0.0f : t;
-        const float old = __builtin_amdgcn_exp2f(top - base), now = __builtin_amdgcn_exp2f(m - base);
+        const float old = __builtin_amdgcn_exp2f(top - base);
+        const float now = __builtin_amdgcn_exp2f(m - base);
         sum = sum * old + l * now;
         o = o * old + v * now;
         top = t;
@@ -662,62 +671,62 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
       constexpr int kItems = DIM == 256 ? 4 : 1;  // of a thread at a time
 #pragma unroll 1
       for (int first = tid; first < items; first += kItems * kThreads) {
-      float top[kItems], sum[kItems];
-      f32x4 o[kItems];
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) {
-        top[i] = -__builtin_inff();
-        sum[i] = 0.0f;
-        o[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-      }
-#pragma unroll 1
-      for (int n = n0; n < n_end; n += 8 * step) {
-        u32x4 v[kItems][8];
-        u32x2 ml[kItems][8];
+        float top[kItems], sum[kItems];
+        f32x4 o[kItems];
 #pragma unroll
         for (int i = 0; i < kItems; ++i) {
-          const int item = first + i * kThreads, h = item / kVecs, d = (item - h * kVecs) * 4;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            // (what is not there is not read)
-            const uint32_t at = oob_unless(item < items && n + q * step < n_end,
-                                           slot_of(w_first, n + q * step) +
-                                               (uint32_t)(h * (kPartHead + DIM)) * 4u);
-            ml[i][q] = __builtin_amdgcn_raw_buffer_load_b64(parts_rsrc, at, 0, kDeviceScope);
-            v[i][q] = load16_device(parts_rsrc, at + (uint32_t)(kPartHead + d) * 4u);
-          }
+          top[i] = -__builtin_inff();
+          sum[i] = 0.0f;
+          o[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
         }
+#pragma unroll 1
+        for (int n = n0; n < n_end; n += 8 * step) {
+          u32x4 v[kItems][8];
+          u32x2 ml[kItems][8];
 #pragma unroll
-        for (int i = 0; i < kItems; ++i) {
-          float t = top[i];
+          for (int i = 0; i < kItems; ++i) {
+            const int item = first + i * kThreads, h = item / kVecs, d = (item - h * kVecs) * 4;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const uint32_t x = ml[i][q].x;
-            if (n + q * step < n_end) t = fmaxf(t, __uint_as_float(x));
+            for (int q = 0; q < 8; ++q) {
+              // (what is not there is not read)
+              const uint32_t at = oob_unless(item < items && n + q * step < n_end,
+                                             slot_of(w_first, n + q * step) +
+                                                 (uint32_t)(h * (kPartHead + DIM)) * 4u);
+              ml[i][q] = __builtin_amdgcn_raw_buffer_load_b64(parts_rsrc, at, 0, kDeviceScope);
+              v[i][q] = load16_device(parts_rsrc, at + (uint32_t)(kPartHead + d) * 4u);
+            }
           }
-          const float base = t == -__builtin_inff() ? 0.0f : t;
-          const float fix = __builtin_amdgcn_exp2f(top[i] - base);
-          o[i] *= fix;
-          sum[i] *= fix;
-          top[i] = t;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const uint32_t x = ml[i][q].x, y = ml[i][q].y;
-            if (n + q * step < n_end) {
-              const float f = __builtin_amdgcn_exp2f(__uint_as_float(x) - base);
-              sum[i] += __uint_as_float(y) * f;
-              o[i] += __builtin_bit_cast(f32x4, v[i][q]) * f;
+          for (int i = 0; i < kItems; ++i) {
+            float t = top[i];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const uint32_t x = ml[i][q].x;
+              if (n + q * step < n_end) t = fmaxf(t, __uint_as_float(x));
+            }
+            const float base = t == -__builtin_inff() ? 0.0f : t;
+            const float fix = __builtin_amdgcn_exp2f(top[i] - base);
+            o[i] *= fix;
+            sum[i] *= fix;
+            top[i] = t;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const uint32_t x = ml[i][q].x, y = ml[i][q].y;
+              if (n + q * step < n_end) {
+                const float f = __builtin_amdgcn_exp2f(__uint_as_float(x) - base);
+                sum[i] += __uint_as_float(y) * f;
+                o[i] += __builtin_bit_cast(f32x4, v[i][q]) * f;
+              }
             }
           }
         }
-      }
 #pragma unroll
-      for (int i = 0; i < kItems; ++i) {
-        const int item = first + i * kThreads, h = item / kVecs, d = (item - h * kVecs) * 4;
-        if (h >= heads) continue;
-        if (final) write_row(row, h, d, o[i], top[i], sum[i]);
-        else write_part(slot_of(w_first, n0), h, d, o[i], top[i], sum[i]);
-      }
+        for (int i = 0; i < kItems; ++i) {
+          const int item = first + i * kThreads, h = item / kVecs, d = (item - h * kVecs) * 4;
+          if (h >= heads) continue;
+          if (final) write_row(row, h, d, o[i], top[i], sum[i]);
+          else write_part(slot_of(w_first, n0), h, d, o[i], top[i], sum[i]);
+        }
       }
       if (final) break;
       part = n0;

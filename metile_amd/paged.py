@@ -155,9 +155,9 @@ def _int32(t, what, ndim=1):
 def paged_tables(cached, new, block_tables, free_pages, *, page_size, tokens, free_start=None):
     """Pages, block-table entries and slots of a step whose lengths only the GPU knows.
 
-    ``cached`` and ``new`` (int32 ``[requests]``): each request's tokens in the cache and in the step.
-    ``block_tables`` (int32 ``[requests, width]``) is updated in place: the pages that the new tokens
-    need are taken in order from ``free_pages`` (int32), beginning with entry ``free_start`` (a
+    ``cached`` and ``new`` (int32 ``[requests]``): each request's tokens in the cache and in the
+    step. ``block_tables`` (int32 ``[requests, width]``) is updated in place: the pages that the new
+    tokens need are taken in order from ``free_pages`` (int32), beginning with entry ``free_start`` (a
     device int32 tensor of one element; ``None``: the first), request by request. ``tokens``: the
     size of the packed batch, at least the sum of ``new``; tokens behind that sum are padding (slot
     -1, request -1, position 0). Tokens without a page (the table too narrow or the list exhausted)
@@ -195,9 +195,9 @@ def paged_tables(cached, new, block_tables, free_pages, *, page_size, tokens, fr
 
 
 def paged_append(key, value, cache, slots):
-    """Write ``key`` and ``value`` (``[tokens, kv_heads, head_dim]``, bfloat16 or float16) to ``slots``
-    (int64 ``[tokens]``, as :func:`paged_tables` gives them) of ``cache``, in place. Tokens whose slot
-    is negative or past the cache are left out. Rows may be strided (heads of a fused projection's
+    """Write ``key`` and ``value`` (``[tokens, kv_heads, head_dim]``, bfloat16 or float16) to
+    ``slots`` (int64 ``[tokens]``, as :func:`paged_tables` gives them) of ``cache``, in place. Tokens
+    whose slot is negative or past the cache are left out. Rows may be strided (heads of a fused projection's
     output). An 8-bit cache gets the values over its scales, limited to what 8 bits hold."""
     dtype = key.dtype
     if dtype not in _DTYPES or value.dtype != dtype:

@@ -82,8 +82,8 @@ def test_caches_are_checked(changes, text):
 
 @pytest.mark.parametrize("changes,text", [
     (dict(requests=0), "requests"), (dict(heads=0), "heads"), (dict(width=0), "width"),
-    (dict(width=1 << 27), "2^31"), (dict(window=-1), "window"), (dict(dtype=2), "dtype"),
-    (dict(dtype=1), "query's dtype"), (dict(scale=float("nan")), "finite"),
+    (dict(width=1 << 27), "2^31"), (dict(width=(1 << 27) - 3), "2^31"), (dict(window=-1), "window"), (dict(dtype=2), "dtype"),
+    (dict(dtype=1), "query's dtype"), (dict(scale=float("nan")), "finite"), (dict(scale=3e38), "finite"),
     (dict(query=0), "null"), (dict(out=264), "16 bytes"),
     (dict(qh=100), "16 bytes"), (dict(qs=-128), "16 bytes"),
     (dict(requests=1 << 30, width=1 << 20), "2^31 units"),

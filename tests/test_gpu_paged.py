@@ -289,6 +289,34 @@ def test_attention_rows_shared_by_many_workgroups(requests):
     check_attention(*attention_case(lengths, 4, 2, 64, 16))
 
 
+@pytest.mark.parametrize("length,heads,kv_heads,dim", [
+    (70000, 2, 1, 64),    # some 270 workgroups a row: three levels of joins of 16
+    (20000, 16, 1, 256),  # some 80 of large parts: three levels of joins of 8
+    (9000, 20, 1, 128)])  # two tiles of query heads, each joined by itself
+def test_attention_joins_of_several_levels(length, heads, kv_heads, dim):
+    case = attention_case([length, 0, 40], heads, kv_heads, dim, 16)
+    first = check_attention(*case)
+    again = mt.paged_attention(*case)
+    assert torch.equal(first.view(torch.int16), again.view(torch.int16))
+    assert not bool(workspace(torch.device("cuda", 0), 1)[:65536].any())
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_random_shapes(seed):
+    rng = random.Random(seed)
+    dtype = rng.choice((torch.bfloat16, torch.float16))
+    kv_heads = rng.choice((1, 2, 3, 8))
+    most = rng.choice((3, 40, 300, 2500))
+    lengths = [rng.choice((0, 1, rng.randint(0, most), rng.randint(0, most)))
+               for _ in range(rng.randint(1, 40))]
+    window = rng.choice((0, 0, rng.randint(1, most + 5)))
+    case = attention_case(lengths, kv_heads * rng.choice((1, 2, 5, 8, 16, 18)), kv_heads,
+                          16 * rng.randint(1, 16), rng.choice((1, 2, 7, 8, 16, 24, 30, 128)),
+                          dtype=dtype, cache=rng.choice((dtype, dtype, FP8)),
+                          layout=rng.choice(("outer", "inner", "mixed")), seed=seed)
+    check_attention(*case, window=window, scale=rng.choice((None, 0.05, 1.0)))
+
+
 def test_attention_more_requests_than_one_scan():
     lengths = [(13 * i) % 5 for i in range(4500)]
     check_attention(*attention_case(lengths, 2, 1, 32, 4))
@@ -341,6 +369,11 @@ def test_attention_infinities_and_nan_of_the_cache():
     assert bool(torch.isfinite(out[0, :2, :5]).all()) and bool(torch.isfinite(out[0, :2, 6:]).all())
     assert bool(torch.isnan(out[1, 2:]).all()) and bool(torch.isfinite(out[1, :2]).all())
     assert bool(torch.isfinite(out[2:]).all())
+    cache.value[table[3][2], 1, 1, 9] = float("nan")
+    cache.value[table[3][0], 4, 1, 10] = -float("inf")
+    out = mt.paged_attention(q, cache, tables, lengths)[3]
+    assert bool(torch.isnan(out[2:, 9]).all()) and bool((out[2:, 10] == -float("inf")).all())
+    assert bool(torch.isfinite(out[:2]).all()) and bool(torch.isfinite(out[2:, 11:]).all())
 
 
 def test_attention_offsets_past_32_bits():
