@@ -430,7 +430,7 @@ int mt_paged_append(const mt_paged_cache* cache, const mt_paged_append_args* arg
  * does not matter. query [requests, heads, dim] with element strides per request and head
  * (multiples of 16 bytes), out [requests, heads, dim] contiguous, 16-byte aligned, both in dtype;
  * a 16-bit cache has the same. requests * cache heads * (query heads of one / 16, rounded up) *
- * (width * page_size / 32, rounded up, + 4) is below 2^31. Sums are fp32 and in a fixed order:
+ * (width * page_size / 32, rounded up, + 4) is at most 2^31 - 2^16. Sums are fp32 and in a fixed order:
  * results do not change from run to run. */
 typedef struct mt_paged_attention_args {
   const void* query;

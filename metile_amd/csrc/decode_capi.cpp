@@ -70,6 +70,8 @@ int64_t most_units(int64_t most, int window) {
   return (n > 0 ? n : 1) + mt::kAttentionRowCost;
 }
 
+constexpr int64_t kMostUnits = kInt31 - 65536;  // the kernel adds up to its waves in 32 bits
+
 struct AttentionPlan {
   int workgroups;
   size_t bytes;
@@ -88,8 +90,8 @@ int plan_attention(const char* op, const mt_paged_cache* c, int requests, int he
   const int group = heads / c->heads, head_tiles = (group + 15) / 16;
   const int64_t units = most_units((int64_t)width * c->page_size, window);
   const int64_t rows = (int64_t)c->heads * head_tiles;
-  if (units * rows >= kInt31 || units * rows * requests >= kInt31)
-    return refuse(op, "requests, heads and table width make more than 2^31 units of 32 tokens");
+  if (units * rows > kMostUnits || units * rows * requests > kMostUnits)
+    return refuse(op, "requests, heads and table width make more than 2^31 - 2^16 units of work");
   plan->workgroups =
       mt::paged_attention_workgroups(mt::current_device_cus(), c->dim, c->page_size,
                                      units * rows * requests);
@@ -250,7 +252,6 @@ int mt_paged_attention(const mt_paged_cache* cache, const mt_paged_attention_arg
   a.window = in.window;
   a.scale_log2 = scale_log2;
   a.value_scale = cache->value_scale;
-  a.by_page = mt::div_magic((uint32_t)cache->page_size);
   return launched(op, mt::launch_paged_attention(a, in.dtype, fp8, plan.workgroups,
                                                  static_cast<hipStream_t>(stream)));
 }

@@ -75,7 +75,7 @@ struct PagedAttentionArgs {
   int32_t requests, kv_heads, group, head_tiles;  // group: query heads of a kv head
   int32_t dim, pages, page_size, width, window;   // window 0: none
   float scale_log2, value_scale;
-  DivMagic by_page;
+  DivMagic by_page, by_waves, by_rows;  // slots of a page, waves of the call, rows of a request
 };
 // Work is counted in units of 32 tokens of a row, plus kAttentionRowCost a row for what every row
 // costs; a workgroup takes kAttentionLeast at least (two rounds of its waves).

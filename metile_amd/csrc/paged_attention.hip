@@ -175,10 +175,10 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
     if (r < a.requests) mine += span_of(len_lane, most, a.window).units + kRowCost;
   }
   const int inc = wave_scan(mine);
-  // (below 2^31, as the host checks; said to be the same in every lane)
+  // (far enough below 2^31, as the host checks; said to be the same in every lane)
   const unsigned units = (unsigned)readlane(inc, 63) * (unsigned)hr_count;
   const unsigned waves = gridDim.x * kWaves;
-  const unsigned per_wave = max((unsigned)uniform((int)((units + waves - 1) / waves)),
+  const unsigned per_wave = max((unsigned)uniform((int)div_by(units + waves - 1, a.by_waves)),
                                 (unsigned)(kAttentionLeast / kWaves));
   const int fan = slot_bytes > kLargePart ? kJoinLarge : kJoin;
   const unsigned per = per_wave * kWaves, wg_u = (unsigned)run * per;
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
   unsigned row_u = 0;  // where the row begins; its units come behind its cost
   Span sp{};
   if (u < u_end) {
-    const int target = uniform((int)(u / (unsigned)hr_count));
+    const int target = uniform((int)div_by(u, a.by_rows));
     const int owner = __ffsll((unsigned long long)__ballot(inc > target)) - 1;
     int prefix = readlane(inc, owner) - readlane(mine, owner);  // units of the requests before r
     r = owner * chunk;
@@ -782,8 +782,12 @@ size_t paged_attention_slot_floats(int group, int dim) {
   return (size_t)(group < 16 ? group : 16) * (padded_dim(dim) + kPartHead);
 }
 
-hipError_t launch_paged_attention(const PagedAttentionArgs& a, int dtype, bool fp8, int workgroups,
-                                  hipStream_t stream) {
+hipError_t launch_paged_attention(const PagedAttentionArgs& args, int dtype, bool fp8,
+                                  int workgroups, hipStream_t stream) {
+  PagedAttentionArgs a = args;
+  a.by_page = div_magic((uint32_t)a.page_size);
+  a.by_waves = div_magic((uint32_t)workgroups * kWaves);
+  a.by_rows = div_magic((uint32_t)(a.kv_heads * a.head_tiles));
   if (dtype == kBF16)
     return fp8 ? launch_dim<kBF16, true>(a, workgroups, stream)
                : launch_dim<kBF16, false>(a, workgroups, stream);
