@@ -78,10 +78,10 @@ struct PagedAttentionArgs {
   DivMagic by_page, by_waves, by_rows;  // slots of a page, waves of the call, rows of a request
 };
 // Work is counted in units of 32 tokens of a row, plus kAttentionRowCost a row for what every row
-// costs; a workgroup takes kAttentionLeast at least (two rounds of its waves).
+// costs; a workgroup takes kAttentionLeast at least (one a wave).
 constexpr int kAttentionUnit = 32;
 constexpr int kAttentionRowCost = 4;
-constexpr int kAttentionLeast = 8;
+constexpr int kAttentionLeast = 4;
 // Workgroups of a call of `units` at most, and floats of one partial slot (two slots a workgroup).
 int paged_attention_workgroups(int cus, int dim, int page_size, int64_t units);
 size_t paged_attention_slot_floats(int group, int dim);

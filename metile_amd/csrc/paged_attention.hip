@@ -23,7 +23,7 @@
 // wave's run is written by that wave, with no exchange at all. A wave's parts of other rows (the
 // first and the last of its run) meet in LDS at the end, and the workgroup's parts of rows that go
 // on in other workgroups are stored with their maximum and sum and joined, in order, by the last
-// of those workgroups to arrive (8 or 16 parts at a time).
+// of those workgroups to arrive (8 or 32 parts at a time).
 //
 // Bound by the bytes of keys and values where there are enough of them: 2 requests of 131072 tokens
 // with 8 key-value heads of 128 bf16 values (1.07 GB) take 185 us, 5.8 TB/s (a copy of 1 GiB
@@ -118,7 +118,7 @@ constexpr int kPartHead = 4;
 // Parts that one workgroup joins at a time; rows of more are joined in levels. Eight where a part
 // is over 8 KiB: one workgroup reads about 50 KB a microsecond (16 requests of 6 to 13104 tokens,
 // 16 heads of 256 values on one key-value head: 33 us, 37 with 16 parts a join).
-constexpr int kJoin = 16, kJoinLarge = 8, kLargePart = 8192;
+constexpr int kJoin = 32, kJoinLarge = 8, kLargePart = 8192;
 // The counters of four levels (8^4 parts) of twice so many fit the workspace's region of them.
 constexpr int kMostWorkgroups = 2048;
 static_assert(kMostWorkgroups * 2 * 4 * 4 <= 64 * 1024 && kMostWorkgroups <= 8 * 8 * 8 * 8,

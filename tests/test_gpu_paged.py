@@ -290,8 +290,8 @@ def test_attention_rows_shared_by_many_workgroups(requests):
 
 
 @pytest.mark.parametrize("length,heads,kv_heads,dim", [
-    (70000, 2, 1, 64),    # some 270 workgroups a row: three levels of joins of 16
-    (20000, 16, 1, 256),  # some 80 of large parts: three levels of joins of 8
+    (70000, 2, 1, 64),    # some 550 workgroups a row: two levels of joins of 32
+    (20000, 16, 1, 256),  # some 160 of large parts: three levels of joins of 8
     (9000, 20, 1, 128)])  # two tiles of query heads, each joined by itself
 def test_attention_joins_of_several_levels(length, heads, kv_heads, dim):
     case = attention_case([length, 0, 40], heads, kv_heads, dim, 16)
