@@ -28,7 +28,14 @@ def _rows(t, width):
 
 
 def _gate(gate, shape, width, rows):
-    """``(gate, stride, rows per gate row, one value a row)`` of a gate that broadcasts to ``shape``."""
+    """``(gate, stride, rows per gate row, one value a row)`` of a gate that broadcasts to
+    ``shape``."""
+    if gate.is_contiguous():  # the ordinary ones: a value a channel, and one for every value
+        own = gate.shape
+        if own == shape:
+            return gate, width, 1, False
+        if len(own) == 1 and own[0] == width:
+            return gate, 0, max(1, rows), False
     if gate.ndim > len(shape) or any(
             g not in (1, n) for g, n in zip(reversed(gate.shape), reversed(shape))):
         raise ValueError("the gate must broadcast to the block's shape")
@@ -95,41 +102,45 @@ def residual_norm(residual, block=None, *, weight, bias=None, post_weight=None, 
         raise ValueError("the gate must have the weights' dtype")
     device = residual.device
     _same_device(device, block, weight, bias, post_weight, post_bias, gate)
-    vector = (width,)
-    pointers = []
-    kept = []  # copies must live until the launch
-    for t in (weight, bias, post_weight, post_bias):
-        if t is None:
-            pointers.append(0)
-            continue
-        if t.shape != vector or t.dtype != dtype:
-            raise ValueError("norm weights and biases must be vectors of the width, of one dtype")
-        if not t.is_contiguous():
-            t = t.contiguous()
-            kept.append(t)
-        pointers.append(t.data_ptr())
+    weight = _vector(weight, width, dtype)
+    if bias is not None:
+        bias = _vector(bias, width, dtype)
+    if post_weight is not None:
+        post_weight = _vector(post_weight, width, dtype)
+    if post_bias is not None:
+        post_bias = _vector(post_bias, width, dtype)
     rows = residual.numel() // width
     if rows >= 1 << 31:
         raise ValueError("too many rows")
     whole = residual.is_contiguous()
+    block_whole = block is not None and block.is_contiguous()
     keep = block is None and residual_scale == 1.0
     out = (residual if keep else torch.empty_like(residual) if whole
            else torch.empty(shape, dtype=stream_dtype, device=device))
-    if block is not None and block.is_contiguous():
-        normed = torch.empty_like(block)
-    else:
-        normed = torch.empty(shape, dtype=dtype, device=device)
+    normed = (torch.empty_like(block) if block_whole
+              else torch.empty(shape, dtype=dtype, device=device))
     if rows == 0:
         return out, normed
     x, x_stride = (residual, width) if whole else _rows(residual, width)
-    b, b_stride, g, g_stride, g_rows, g_scalar = None, 0, None, 0, 1, False
-    if block is not None:
-        b, b_stride = (block, width) if block.is_contiguous() else _rows(block, width)
-        if gate is not None:
-            g, g_stride, g_rows, g_scalar = _gate(gate, shape, width, rows)
+    b, b_stride = ((None, 0) if block is None else (block, width) if block_whole
+                   else _rows(block, width))
+    g, g_stride, g_rows, g_scalar = ((None, 0, 1, False) if gate is None
+                                     else _gate(gate, shape, width, rows))
+    code16 = _DTYPES[dtype]
     _launch(device, _lib.lib().mt_residual_norm, _lib.RESIDUAL_NORM_ARGS.pack(
-        x.data_ptr(), 0 if b is None else b.data_ptr(), *pointers,
-        0 if g is None else g.data_ptr(), 0 if keep else out.data_ptr(), normed.data_ptr(),
-        x_stride, b_stride, g_stride, rows, width, g_rows, g_scalar, residual_scale, eps, code,
-        _DTYPES[dtype], _lib.MT_F32 if stream_dtype == torch.float32 else _DTYPES[dtype]))
+        x.data_ptr(), _ptr(b), weight.data_ptr(), _ptr(bias), _ptr(post_weight), _ptr(post_bias),
+        _ptr(g), 0 if keep else out.data_ptr(), normed.data_ptr(), x_stride, b_stride, g_stride,
+        rows, width, g_rows, g_scalar, residual_scale, eps, code, code16,
+        code16 if stream_dtype == dtype else _lib.MT_F32))
     return out, normed
+
+
+def _vector(t, width, dtype):
+    """A weight or bias, checked, its values next to each other."""
+    if t.dtype != dtype or t.ndim != 1 or t.shape[0] != width:
+        raise ValueError("norm weights and biases must be vectors of the width, of one dtype")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
