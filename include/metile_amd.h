@@ -386,7 +386,8 @@ typedef struct mt_paged_cache {
  * -1, position 0, request -1; tokens that the table's width or the free list has no page for get
  * slot -1 (and an exhausted list writes -1 into the table, with `taken` telling the shortage).
  * Tokens beyond `tokens` are dropped with the table entries of the pages they open. width *
- * page_size is below 2^31; sums of counts stop at 2^31 - 1. requests or tokens may be 0. */
+ * page_size is below 2^31; sums of counts stop at 2^31 - 1. requests or tokens may be 0. Outputs
+ * overlap no input. */
 typedef struct mt_paged_tables_args {
   const int32_t* cached;
   const int32_t* new_tokens;
@@ -425,13 +426,13 @@ int mt_paged_append(const mt_paged_cache* cache, const mt_paged_append_args* arg
  * key-value head h / (heads / cache heads). lengths[r] counts the tokens in the cache, the new one
  * among them (its key and value are appended first); it is limited to [0, width * page_size], which
  * is at most 2^31 - 64. Rows without a token give 0. lse (or NULL) [requests, heads] receives log
- * sum exp of the scaled scores, -inf for such rows. Table entries behind a request's last token are not read; tokens
- * whose entry is not a page of the cache are left out, and what slots behind the last token hold
- * does not matter. query [requests, heads, dim] with element strides per request and head
- * (multiples of 16 bytes), out [requests, heads, dim] contiguous, 16-byte aligned, both in dtype;
- * a 16-bit cache has the same. requests * cache heads * (query heads of one / 16, rounded up) *
- * (width * page_size / 32, rounded up, + 4) is at most 2^31 - 2^16. Sums are fp32 and in a fixed order:
- * results do not change from run to run. */
+ * sum exp of the scaled scores, -inf for such rows. Table entries behind a request's last token are
+ * not read; tokens whose entry is not a page of the cache are left out, and what slots behind the
+ * last token hold does not matter. Lengths must not change while the call runs. query [requests,
+ * heads, dim] with element strides per request and head (multiples of 16 bytes), out [requests,
+ * heads, dim] contiguous, 16-byte aligned, both in dtype; a 16-bit cache has the same. requests *
+ * cache heads * (query heads of one / 16, rounded up) * (width * page_size / 32, rounded up, + 4) is
+ * at most 2^31 - 2^16. Sums are fp32 and in a fixed order: results do not change from run to run. */
 typedef struct mt_paged_attention_args {
   const void* query;
   int64_t query_strides[2];

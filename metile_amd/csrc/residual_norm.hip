@@ -4,11 +4,11 @@
 //   r = scale * residual + gate * post(block)        normed = pre(r)
 //   rms(x) = x / sqrt(mean(x^2) + eps) * w           layer(x) = (x - mean) / sqrt(var + eps) * w
 //
-// each + a bias, if there is one. post and pre are both rms or both layer norms; either input is
-// read once and either output written once, with the row held in registers in fp32 between (the pre-norm sees r before its
-// rounding to the stream's type; the variance is that of deviations, in a second sum). Memory
-// bounds it for many rows, the chain of one read and the row sums for few. A row belongs to
-// one wave, or to a workgroup of 4 or 16: threads take eight consecutive values at a time.
+// each + a bias, if there is one. post and pre are both rms or both layer norms. Either input is read
+// once and either output written once, with the row in fp32 registers between: the pre-norm sees r
+// before its rounding to the stream's type, and the variance is that of deviations, in a second
+// sum. Memory bounds it for many rows, the chain of one read and the row sums for few. A row belongs
+// to one wave, or to a workgroup of 2 to 16: threads take eight consecutive values at a time.
 #include "common.h"
 #include "residual_norm.h"
 

@@ -197,8 +197,9 @@ def paged_tables(cached, new, block_tables, free_pages, *, page_size, tokens, fr
 def paged_append(key, value, cache, slots):
     """Write ``key`` and ``value`` (``[tokens, kv_heads, head_dim]``, bfloat16 or float16) to
     ``slots`` (int64 ``[tokens]``, as :func:`paged_tables` gives them) of ``cache``, in place. Tokens
-    whose slot is negative or past the cache are left out. Rows may be strided (heads of a fused projection's
-    output). An 8-bit cache gets the values over its scales, limited to what 8 bits hold."""
+    whose slot is negative or past the cache are left out. Rows may be strided (heads of a fused
+    projection's output). An 8-bit cache gets the values over its scales, limited to what 8 bits
+    hold."""
     dtype = key.dtype
     if dtype not in _DTYPES or value.dtype != dtype:
         raise ValueError("keys and values must both be bfloat16 or float16")
