@@ -93,7 +93,7 @@ int plan_attention(const char* op, const mt_paged_cache* c, int requests, int he
   if (units * rows > kMostUnits || units * rows * requests > kMostUnits)
     return refuse(op, "requests, heads and table width make more than 2^31 - 2^16 units of work");
   plan->workgroups =
-      mt::paged_attention_workgroups(mt::current_device_cus(), c->dim, c->page_size,
+      mt::paged_attention_workgroups(mt::current_device_cus(), c->dim,
                                      units * rows * requests);
   plan->bytes = mt::kWorkspaceCounterBytes +
                 (size_t)plan->workgroups * 2 * mt::paged_attention_slot_floats(group, c->dim) * 4;

@@ -83,7 +83,7 @@ constexpr int kAttentionUnit = 32;
 constexpr int kAttentionRowCost = 4;
 constexpr int kAttentionLeast = 4;
 // Workgroups of a call of `units` at most, and floats of one partial slot (two slots a workgroup).
-int paged_attention_workgroups(int cus, int dim, int page_size, int64_t units);
+int paged_attention_workgroups(int cus, int dim, int64_t units);
 size_t paged_attention_slot_floats(int group, int dim);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, int dtype, bool fp8, int workgroups,
                                   hipStream_t stream);

@@ -125,12 +125,12 @@ static_assert(kMostWorkgroups * 2 * 4 * 4 <= 64 * 1024 && kMostWorkgroups <= 8 *
               "counters of every level");
 
 // Waves a SIMD (and so workgroups a CU) that the registers are allotted for.
-constexpr int attention_waves(int padded_dim, bool page8) {
-  return padded_dim == 256 ? 1 : padded_dim == 64 && page8 ? 3 : 2;
+constexpr int attention_waves(int padded_dim) {
+  return padded_dim == 256 ? 1 : padded_dim == 64 ? 3 : 2;
 }
 
-template <int DT, bool FP8, int DIM, bool PAGE8>
-__global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_attention_kernel(
+template <int DT, bool FP8, int DIM>
+__global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attention_kernel(
     PagedAttentionArgs a, int slot_bytes) {
   constexpr int kElt = FP8 ? 1 : 2;
   constexpr int kMfmas = DIM / 32;               // K depth of a score
@@ -272,41 +272,33 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
     u32x4 kf[2][kKeyLoads];
     uint32_t vf[8][kValueWords];
 
-    // The pages of a unit's tokens: of a lane's key rows (two; one page where pages are whole
-    // groups of eight tokens) and value rows (eight, or one), with the place of the first token in
-    // the page. Tokens past the end stand for the last one; tokens of a page that is none of the
-    // cache's for page 0. Both are masked.
-    constexpr int kKeyPages = PAGE8 ? 1 : 2, kValuePages = PAGE8 ? 1 : 8;
-    struct Pages {
-      int key[kKeyPages], key_at[kKeyPages];
-      int value[kValuePages], value_at[kValuePages];
+    // Where a unit's tokens are: the page of token lane % 32, and the place in it. Tokens past the end
+    // stand for the last one; tokens of a page that is none of the cache's for page 0. Both are
+    // masked.
+    struct Place {
+      int page, slot;
     };
-    auto look_up = [&](int tok0, Pages& p) {
-#pragma unroll
-      for (int t = 0; t < kKeyPages; ++t) {
-        int token = tok0 + 8 * (c >> 2) + (PAGE8 ? 0 : 4 * t + (c & 3));
-        token = token < last ? token : last;
-        const int col = (int)div_by((uint32_t)token, a.by_page);
-        p.key[t] = table[col];
-        p.key_at[t] = col * page_size;
-      }
-#pragma unroll
-      for (int j = 0; j < kValuePages; ++j) {
-        int token = tok0 + 8 * g + j;
-        token = token < last ? token : last;
-        const int col = (int)div_by((uint32_t)token, a.by_page);
-        p.value[j] = table[col];
-        p.value_at[j] = col * page_size;
-      }
+    auto look_up = [&](int tok0, Place& p) {
+      const int token = min(tok0 + (lane & 31), last);
+      const int col = (int)div_by((uint32_t)token, a.by_page);
+      p.page = table[col];
+      p.slot = token - col * page_size;
     };
-    auto page_or_0 = [&](int p) { return (uint32_t)p < (uint32_t)a.pages ? (uint32_t)p : 0u; };
-    auto load_keys = [&](int tok0, const Pages& p) {
+    // Its row is reckoned once, by that lane; those that load it ask for the offset.
+    auto offset_of = [&](const Place& p, uint32_t page_stride, uint32_t slot_stride) {
+      const uint32_t page = (uint32_t)p.page < (uint32_t)a.pages ? (uint32_t)p.page : 0u;
+      return (uint64_t)page * page_stride + (uint64_t)(uint32_t)p.slot * slot_stride;
+    };
+    auto of_token = [&](uint64_t offset, int i) {
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * i, (int)(uint32_t)offset);
+      const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * i, (int)(offset >> 32));
+      return (uint64_t)hi << 32 | lo;
+    };
+    auto load_keys = [&](const Place& p) {
+      const uint64_t offset = offset_of(p, a.k_page, a.k_slot);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        constexpr int kOne = kKeyPages - 1;
-        const int token = min(tok0 + 8 * (c >> 2) + 4 * t + (c & 3), last);
-        const unsigned char* row = kbase + (uint64_t)page_or_0(p.key[t & kOne]) * a.k_page +
-                                   (uint64_t)(uint32_t)(token - p.key_at[t & kOne]) * a.k_slot;
+        const unsigned char* row = kbase + of_token(offset, 8 * (c >> 2) + 4 * t + (c & 3));
 #pragma unroll
         for (int k = 0; k < kKeyLoads; ++k) {
           const int d = FP8 ? 64 * k + 16 * g : 32 * k + 8 * g;
@@ -315,17 +307,13 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
         }
       }
     };
-    auto load_values = [&](int tok0, const Pages& p) {
+    auto load_values = [&](const Place& p) {
+      const uint64_t offset = offset_of(p, a.v_page, a.v_slot);
       const int d = kLaneDims * c;
       const unsigned char* lane_base = vbase + (d < a.dim ? d * kElt : 0);
-      const unsigned char* page = lane_base;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        constexpr int kOne = kValuePages - 1;
-        const int token = min(tok0 + 8 * g + j, last);
-        if (j <= kOne) page = lane_base + (uint64_t)page_or_0(p.value[j & kOne]) * a.v_page;
-        const unsigned char* row =
-            page + (uint64_t)(uint32_t)(token - p.value_at[j & kOne]) * a.v_slot;
+        const unsigned char* row = lane_base + of_token(offset, 8 * g + j);
         if constexpr (kValueWords >= 4) {
 #pragma unroll
           for (int w = 0; w < kValueWords; w += 4) {
@@ -344,7 +332,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
 
     auto start_of = [&](int t) { return sp.base + t * kUnit; };
     // Table entries are looked up one unit further ahead than rows, so that no row waits for one.
-    Pages now, ahead;
+    Place now, ahead;
     u32x4 q[kMfmas];
     bool two_parts = true;
     int tok0;
@@ -361,7 +349,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
       for (int w = 0; w < kValueWords; ++w) vf[j][w] = 0;
 #pragma unroll
     for (int k = 0; k < kMfmas; ++k) q[k] = (u32x4){0, 0, 0, 0};
-    now = ahead = Pages{};
+    now = ahead = Place{};
     int t = unit;
     tok0 = start_of(t);
     live = t < unit_end && tok0 < len;
@@ -377,30 +365,20 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
         q[k] = *reinterpret_cast<const u32x4*>(row + (d < a.dim ? d : 0));
         if (!has || d >= a.dim) q[k] = (u32x4){0, 0, 0, 0};
       }
-      load_keys(tok0, now);
-      load_values(tok0, now);
+      load_keys(now);
+      load_values(now);
       if (t + 1 < unit_end) look_up(start_of(t + 1), ahead);
     }
     while (live) {
       const int next = start_of(t + 1);
       const bool more = t + 1 < unit_end;
-      // whether the lane's eight tokens are all attended to: past the ends of the window and the
-      // request, and on pages that are none, they are not
-      bool page_ok = true;
-#pragma unroll
-      for (int j = 0; j < kValuePages; ++j)
-        page_ok = page_ok && (uint32_t)now.value[j] < (uint32_t)a.pages;
-      const bool all = __all(page_ok) && tok0 >= first && tok0 + 32 <= len;
-      uint32_t ok = 0xffu;
-      if (!all) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int token = tok0 + 8 * g + j;
-          const bool here = (uint32_t)now.value[j & (kValuePages - 1)] < (uint32_t)a.pages &&
-                            token >= first && token < len;
-          ok &= ~((uint32_t)!here << j);
-        }
-      }
+      // which of the unit's tokens are attended to: past the ends of the window and the request, and
+      // on pages that are none, they are not
+      const int token = tok0 + (lane & 31);
+      const uint32_t here = (uint32_t)__ballot((uint32_t)now.page < (uint32_t)a.pages &&
+                                               token >= first && token < len);
+      const bool all = here == 0xffffffffu;
+      const uint32_t ok = here >> (8 * g);
 
       // ---- scores ----
       f32x4 s[2];
@@ -424,7 +402,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
         }
       }
       if (more) {
-        load_keys(next, ahead);
+        load_keys(ahead);
         now = ahead;
         if (t + 2 < unit_end) look_up(start_of(t + 2), ahead);
       }
@@ -508,7 +486,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
 #pragma unroll
         for (int e = 0; e < kLaneDims; ++e) acc[e] = mfma16<DT>(v[e], p_lo, acc[e]);
       }
-      if (more) load_values(next, now);
+      if (more) load_values(now);
       tok0 = next;
       live = more;
       ++t;
@@ -751,10 +729,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM, PAGE8)) void paged_a
 template <int DT, bool FP8, int DIM>
 hipError_t launch(const PagedAttentionArgs& a, int workgroups, hipStream_t stream) {
   const int slot = (int)paged_attention_slot_floats(a.group, a.dim) * 4;
-  if (a.page_size % 8 == 0)
-    paged_attention_kernel<DT, FP8, DIM, true><<<workgroups, kThreads, 0, stream>>>(a, slot);
-  else
-    paged_attention_kernel<DT, FP8, DIM, false><<<workgroups, kThreads, 0, stream>>>(a, slot);
+  paged_attention_kernel<DT, FP8, DIM><<<workgroups, kThreads, 0, stream>>>(a, slot);
   return hipGetLastError();
 }
 
@@ -771,8 +746,8 @@ hipError_t launch_dim(const PagedAttentionArgs& a, int workgroups, hipStream_t s
 
 }  // namespace
 
-int paged_attention_workgroups(int cus, int dim, int page_size, int64_t units) {
-  const int64_t most = attention_waves(padded_dim(dim), page_size % 8 == 0) * (int64_t)cus;
+int paged_attention_workgroups(int cus, int dim, int64_t units) {
+  const int64_t most = attention_waves(padded_dim(dim)) * (int64_t)cus;
   const int64_t runs = (units + kAttentionLeast - 1) / kAttentionLeast;
   const int64_t n = runs < most ? (runs > 0 ? runs : 1) : most;
   return (int)(n < kMostWorkgroups ? n : kMostWorkgroups);
