@@ -83,8 +83,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // Keys and values are read once, with the hint that says so (2 x 131072 tokens of 8 heads of 128
-// values 211 -> 202 us), except where a head's row of a token is less than a line and its
-// neighbours' follow: then other workgroups read the rest of the line.
+// values 211 -> 202 us), except where a head's row of a token need not be whole lines: then others
+// read the rest of a line (heads of 80 8-bit values, 2 x 68389 tokens: 172 us with it, 122 without).
 template <bool ONCE, typename T>
 __device__ __forceinline__ T stream_load(const T* p) {
   if constexpr (ONCE) return __builtin_nontemporal_load(p);
@@ -115,10 +115,12 @@ constexpr int kWholeUnits = 4;
 // Where a workgroup's partial sums of a row are kept: [heads][kPartHead + DIM] floats a slot, the
 // maximum and the sum in front of a head's values.
 constexpr int kPartHead = 4;
-// Parts that one workgroup joins at a time; rows of more are joined in levels. Eight where a part
-// is over 8 KiB: one workgroup reads about 50 KB a microsecond (16 requests of 6 to 13104 tokens,
-// 16 heads of 256 values on one key-value head: 33 us, 37 with 16 parts a join).
-constexpr int kJoin = 32, kJoinLarge = 8, kLargePart = 8192;
+// Parts that one workgroup joins at a time; rows of more are joined in levels. A level costs two
+// round trips to memory and eight parts a third one, so up to 16 parts are joined at once unless
+// they are large: one workgroup reads about 50 KB a microsecond (2 requests of 3960 to 7057 tokens,
+// 28 heads of 128 values on 4: 32 parts at a time 22.1 us, 8 17.0; 64 requests of 1 to 8192 tokens
+// 8 always 48.9, up to 16 at once 47.9).
+constexpr int kJoin = 8, kJoinAll = 16, kLargePart = 8192;
 // The counters of four levels (8^4 parts) of twice so many fit the workspace's region of them.
 constexpr int kMostWorkgroups = 2048;
 static_assert(kMostWorkgroups * 2 * 4 * 4 <= 64 * 1024 && kMostWorkgroups <= 8 * 8 * 8 * 8,
@@ -129,7 +131,8 @@ constexpr int attention_waves(int padded_dim) {
   return padded_dim == 256 ? 1 : padded_dim == 64 ? 3 : 2;
 }
 
-template <int DT, bool FP8, int DIM>
+// DIM: the head's values, or with PADDED some more (the rest count as zero).
+template <int DT, bool FP8, int DIM, bool PADDED>
 __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attention_kernel(
     PagedAttentionArgs a, int slot_bytes) {
   constexpr int kElt = FP8 ? 1 : 2;
@@ -139,7 +142,8 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
   constexpr int kValueWords = kLaneDims * kElt / 4;
   constexpr int kRow = DIM + 4;                  // floats: heads start four banks apart
   constexpr int kVecs = DIM / 4;
-  constexpr bool kOnce = !(FP8 && DIM == 64);
+  constexpr bool kOnce = !PADDED && !(FP8 && DIM == 64);
+  const int dim = PADDED ? a.dim : DIM;
   // f16 probabilities are scaled up so that small ones, and the second parts, stay above its
   // smallest numbers; the sum carries the same factor.
   constexpr float kShift = DT == kF16 ? 14.0f : 0.0f;
@@ -180,7 +184,6 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
   const unsigned waves = gridDim.x * kWaves;
   const unsigned per_wave = max((unsigned)uniform((int)div_by(units + waves - 1, a.by_waves)),
                                 (unsigned)(kAttentionLeast / kWaves));
-  const int fan = slot_bytes > kLargePart ? kJoinLarge : kJoin;
   const unsigned per = per_wave * kWaves, wg_u = (unsigned)run * per;
   if (wg_u >= units) return;
   const unsigned wg_end = min(wg_u + per, units);
@@ -303,14 +306,14 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
         for (int k = 0; k < kKeyLoads; ++k) {
           const int d = FP8 ? 64 * k + 16 * g : 32 * k + 8 * g;
           kf[t][k] = stream_load<kOnce>(
-              reinterpret_cast<const u32x4*>(row + (d < a.dim ? d * kElt : 0)));
+              reinterpret_cast<const u32x4*>(row + (d < dim ? d * kElt : 0)));
         }
       }
     };
     auto load_values = [&](const Place& p) {
       const uint64_t offset = offset_of(p, a.v_page, a.v_slot);
       const int d = kLaneDims * c;
-      const unsigned char* lane_base = vbase + (d < a.dim ? d * kElt : 0);
+      const unsigned char* lane_base = vbase + (d < dim ? d * kElt : 0);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const unsigned char* row = lane_base + of_token(offset, 8 * g + j);
@@ -362,8 +365,8 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
 #pragma unroll
       for (int k = 0; k < kMfmas; ++k) {
         const int d = FP8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g;
-        q[k] = *reinterpret_cast<const u32x4*>(row + (d < a.dim ? d : 0));
-        if (!has || d >= a.dim) q[k] = (u32x4){0, 0, 0, 0};
+        q[k] = *reinterpret_cast<const u32x4*>(row + (d < dim ? d : 0));
+        if (!has || d >= dim) q[k] = (u32x4){0, 0, 0, 0};
       }
       load_keys(now);
       load_values(now);
@@ -394,9 +397,9 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
           } else {
             key = kf[h][k];
           }
-          if (a.dim != DIM) {  // dimensions that the cache does not have
+          if (PADDED) {  // dimensions that the cache does not have
             const int d = FP8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g;
-            if (d >= a.dim) key = (u32x4){0, 0, 0, 0};
+            if (d >= dim) key = (u32x4){0, 0, 0, 0};
           }
           s[h] = mfma16<DT>(key, q[k], s[h]);
         }
@@ -521,8 +524,8 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
 #pragma unroll
         for (int k = 0; k < 2 * kLaneDims; k += 4) {
           const int d = 4 * kLaneDims * g + 2 * k;
-          if (d < a.dim)
-            *reinterpret_cast<u32x4*>(a.out + row * a.dim + d) =
+          if (d < dim)
+            *reinterpret_cast<u32x4*>(a.out + row * dim + d) =
                 (u32x4){w[k], w[k + 1], w[k + 2], w[k + 3]};
         }
         if (a.lse && g == 0) a.lse[row] = lse_of(m, l);
@@ -558,8 +561,8 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
     const int rr = row / hr_count;
     const int64_t at = (int64_t)rr * a.kv_heads * a.group + first_head(row - rr * hr_count) + h;
     const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
-    if (d < a.dim)
-      *reinterpret_cast<u32x2*>(a.out + at * a.dim + d) =
+    if (d < dim)
+      *reinterpret_cast<u32x2*>(a.out + at * dim + d) =
           (u32x2){pack2<DT>(o.x * inv, o.y * inv), pack2<DT>(o.z * inv, o.w * inv)};
     if (a.lse && d == 0) a.lse[at] = lse_of(top, sum);
   };
@@ -647,6 +650,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
     const int w_first = k ? open_first[1] : open_first[0];
     const int parts = k ? open_parts[1] : open_parts[0];
     const int heads = head_count(uniform(row % hr_count));
+    const int fan = parts <= kJoinAll && slot_bytes <= kLargePart ? kJoinAll : kJoin;
     int part = run - w_first, step = 1;
     uint32_t* counters = a.counters;
 #pragma unroll 1
@@ -729,7 +733,10 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
 template <int DT, bool FP8, int DIM>
 hipError_t launch(const PagedAttentionArgs& a, int workgroups, hipStream_t stream) {
   const int slot = (int)paged_attention_slot_floats(a.group, a.dim) * 4;
-  paged_attention_kernel<DT, FP8, DIM><<<workgroups, kThreads, 0, stream>>>(a, slot);
+  if (a.dim == DIM)
+    paged_attention_kernel<DT, FP8, DIM, false><<<workgroups, kThreads, 0, stream>>>(a, slot);
+  else
+    paged_attention_kernel<DT, FP8, DIM, true><<<workgroups, kThreads, 0, stream>>>(a, slot);
   return hipGetLastError();
 }
 
