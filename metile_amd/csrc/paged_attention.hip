@@ -82,9 +82,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
 }
 
-// Keys and values are read once, with the hint that says so (2 x 131072 tokens of 8 heads of 128
-// values 211 -> 202 us), except where a head's row of a token need not be whole lines: then others
-// read the rest of a line (heads of 80 8-bit values, 2 x 68389 tokens: 172 us with it, 122 without).
+// 16-bit keys and values of whole lines are read with the hint that this happens once (2 x 131072
+// tokens of 8 heads of 128: 190.5 us without it, 183 with), all others are kept in the caches: where
+// a head's row of a token is no whole lines, others read the rest of one (heads of 80 8-bit values,
+// 2 x 68389 tokens: 172 us with the hint, 122 without), and so do further tiles of query heads (48
+// heads on one, 366 requests of up to 5496 tokens: 119, 95). (Heads of 256, 5 x 78518 tokens: 100,
+// 91; 8 bits, 75 x 2086 tokens of 8 heads of 128: 77, 75.)
 template <bool ONCE, typename T>
 __device__ __forceinline__ T stream_load(const T* p) {
   if constexpr (ONCE) return __builtin_nontemporal_load(p);
@@ -131,7 +134,8 @@ constexpr int attention_waves(int padded_dim) {
   return padded_dim == 256 ? 1 : padded_dim == 64 ? 3 : 2;
 }
 
-// DIM: the head's values, or with PADDED some more (the rest count as zero).
+// DIM: the head's values, or with PADDED that many or more (the rest count as zero). Heads in several
+// tiles are such calls too, for the sake of its loads without the hint.
 template <int DT, bool FP8, int DIM, bool PADDED>
 __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attention_kernel(
     PagedAttentionArgs a, int slot_bytes) {
@@ -142,7 +146,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
   constexpr int kValueWords = kLaneDims * kElt / 4;
   constexpr int kRow = DIM + 4;                  // floats: heads start four banks apart
   constexpr int kVecs = DIM / 4;
-  constexpr bool kOnce = !PADDED && !(FP8 && DIM == 64);
+  constexpr bool kOnce = !PADDED && !FP8 && DIM <= 128;
   const int dim = PADDED ? a.dim : DIM;
   // f16 probabilities are scaled up so that small ones, and the second parts, stay above its
   // smallest numbers; the sum carries the same factor.
@@ -733,7 +737,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
 template <int DT, bool FP8, int DIM>
 hipError_t launch(const PagedAttentionArgs& a, int workgroups, hipStream_t stream) {
   const int slot = (int)paged_attention_slot_floats(a.group, a.dim) * 4;
-  if (a.dim == DIM)
+  if (a.dim == DIM && (FP8 || DIM > 128 || a.head_tiles == 1))
     paged_attention_kernel<DT, FP8, DIM, false><<<workgroups, kThreads, 0, stream>>>(a, slot);
   else
     paged_attention_kernel<DT, FP8, DIM, true><<<workgroups, kThreads, 0, stream>>>(a, slot);
