@@ -10,8 +10,11 @@
 //    token 8 (i / 4) + 4 t + i % 4);
 //  * values: a lane loads DIM / 16 dimensions of eight consecutive tokens; eight byte permutes
 //    a dimension pair turn them into operands with the dimensions as rows, and the lane's own
-//    eight probabilities are the other operand as they stand: no exchange between lanes, no LDS.
-//    The result has the head in the lane again, so rescaling is local to the lane.
+//    eight probabilities are the other operand as they stand: no exchange between lanes.
+//    The result has the head in the lane again, so rescaling is local to the lane;
+//  * pages: a lane a token looks up its entry, one unit ahead, and reckons the row's offset, which
+//    the lanes that load the row ask for (pages of one token 10.4 us; with the look-ups and their
+//    divisions in every loading lane 13.2; pages of 16 the same).
 // Probabilities go to the matrix cores as two 16-bit parts (their rounding and the rest of it),
 // so the 16-bit rounding of the result is the only one; sums, maxima and results are fp32. (The
 // second part is zero or negative as often as not, and an infinite value times it is no number: a
@@ -23,12 +26,12 @@
 // wave's run is written by that wave, with no exchange at all. A wave's parts of other rows (the
 // first and the last of its run) meet in LDS at the end, and the workgroup's parts of rows that go
 // on in other workgroups are stored with their maximum and sum and joined, in order, by the last
-// of those workgroups to arrive (8 or 32 parts at a time).
+// of those workgroups to arrive (8 parts at a time, up to 16 at once).
 //
 // Bound by the bytes of keys and values where there are enough of them: 2 requests of 131072 tokens
-// with 8 key-value heads of 128 bf16 values (1.07 GB) take 185 us, 5.8 TB/s (a copy of 1 GiB
-// reaches 5.2); 64 requests of 1 to 8192 tokens (224 MB) 48 us, 4.6 TB/s. The shortest calls take
-// 5.5 us: the launch, then lengths, table entry and first rows, a memory round trip each after the
+// with 8 key-value heads of 128 bf16 values (1.07 GB) take 183 us, 5.9 TB/s (a copy of 1 GiB
+// reaches 5.2); 64 requests of 1 to 8192 tokens (224 MB) 47.5 us, 4.7 TB/s. The shortest calls take
+// 4.7 us: the launch, then lengths, table entry and first rows, a memory round trip each after the
 // other; a row that several workgroups share costs about 4 us more for its join.
 #include "common.h"
 #include "paged.h"
