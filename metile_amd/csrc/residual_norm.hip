@@ -253,11 +253,14 @@ void launch_rows(const ResidualNormArgs& a, hipStream_t stream) {
 //   16384 x 1133    1, 3  33 / 37                  2, 2   .. / 45       4, 1   36 / ..
 //    4096 x 1536    1, 3  10.7 / 12.5              2, 2   .. / 13.6     4, 1   11.2 / ..
 //    1024 x 1536    1, 3   5.7 / 6.7               2, 2   .. / 6.1      4, 1   4.5 / ..
+//     768 x 4096    4, 2   7.3 / 8.7              16, 1   8.1 / 11.8
+//     512 x 4096    4, 2   6.0 / 7.1              16, 1   5.7 / 8.6
+//     768 x 896     1, 2   4.2 / 4.8               4, 1   3.6 / 4.8
 // (98 us for 16384 x 4096 are 5.5 TB/s; a copy of 1 GiB reaches 5.1 to 5.2.)
 template <int DT, typename RT, bool LAYER>
 void launch_width(const ResidualNormArgs& a, int cus, hipStream_t stream) {
-  const bool many = a.rows >= 4 * cus;
   const int w = a.width;
+  const bool many = w > 2048 ? a.rows > 2 * cus : a.rows >= 4 * cus;
   if (w < 8)
     residual_norm_narrow_kernel<DT, RT, LAYER><<<(a.rows + 255) / 256, 256, 0, stream>>>(a);
   else if (w <= 512) launch_rows<DT, RT, LAYER, 1, 1>(a, stream);
