@@ -8,7 +8,8 @@
 // once and either output written once, with the row in fp32 registers between: the pre-norm sees r
 // before its rounding to the stream's type, and the variance is that of deviations, in a second
 // sum. Memory bounds it for many rows, the chain of one read and the row sums for few. A row belongs
-// to one wave, or to a workgroup of 2 to 16: threads take eight consecutive values at a time.
+// to 16 lanes up to a wave, or to a workgroup of 2 to 16 waves: threads take eight consecutive values
+// at a time.
 #include "common.h"
 #include "residual_norm.h"
 
@@ -41,21 +42,25 @@ __device__ __forceinline__ void write8(float* p, const float (&x)[8]) {
   __builtin_memcpy(p, x, 32);
 }
 
-// Sum over a wave, the same in every lane: exchanges within rows of 16 lanes, then across them.
-__device__ __forceinline__ float wave_sum(float v) {
+// Sum over 16, 32 or all lanes, the same in every one of them: exchanges within rows of 16 lanes,
+// then across them.
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
   v += dpp_read<kDppXor1>(v);
   v += dpp_read<kDppXor2>(v);
   v += dpp_read<kDppHalfMirror>(v);
   v += dpp_read<0x140>(v);  // row_mirror
+  if constexpr (LANES == 16) return v;
+  if constexpr (LANES == 32) return v + __shfl_xor(v, 16);
   v += dpp_read_rows<kDppRowBcast15, 0xA>(v);
   v += dpp_read_rows<kDppRowBcast31, 0xC>(v);
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
 }
 
 // Sum over the threads of a row (every one gets it); `turn` alternates the LDS used.
-template <int WAVES>
+template <int WAVES, int LANES>
 __device__ __forceinline__ float row_sum(float v, float (&lds)[2][WAVES], int& turn) {
-  v = wave_sum(v);
+  v = lanes_sum<LANES>(v);
   if constexpr (WAVES > 1) {
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) lds[turn][wave] = v;
@@ -68,15 +73,16 @@ __device__ __forceinline__ float row_sum(float v, float (&lds)[2][WAVES], int& t
   return v;
 }
 
-template <int DT, typename RT, bool LAYER, int WAVES, int NV>
+// LANES: of a wave that a row has to itself (16 or 32 only with one wave and vector).
+template <int DT, typename RT, bool LAYER, int WAVES, int NV, int LANES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_kernel(
     ResidualNormArgs a) {
-  constexpr int kRowThreads = 64 * WAVES;
-  constexpr int kRows = WAVES == 1 ? 4 : 1;  // rows of a workgroup
+  constexpr int kRowThreads = LANES * WAVES;
+  constexpr int kRows = WAVES == 1 ? 256 / LANES : 1;  // rows of a workgroup
   __shared__ float lds[2][WAVES];
   int turn = 0;
-  const int t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int row = blockIdx.x * kRows + (WAVES == 1 ? threadIdx.x >> 6 : 0);
+  const int t = WAVES == 1 ? threadIdx.x & (LANES - 1) : threadIdx.x;
+  const int row = blockIdx.x * kRows + (WAVES == 1 ? threadIdx.x / LANES : 0);
   if (WAVES == 1 && row >= a.rows) return;
   const int width = a.width;
 
@@ -114,7 +120,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_k
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) s += counted(v[i][j], i, j);
-      const float mean = row_sum<WAVES>(s, lds, turn) / (float)width;
+      const float mean = row_sum<WAVES, LANES>(s, lds, turn) / (float)width;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -128,7 +134,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_k
         const float c = counted(v[i][j], i, j);
         s = fmaf(c, c, s);
       }
-    const float mean_sq = row_sum<WAVES>(s, lds, turn) / (float)width;
+    const float mean_sq = row_sum<WAVES, LANES>(s, lds, turn) / (float)width;
     const float inv = 1.0f / sqrtf(mean_sq + a.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -234,10 +240,10 @@ __global__ __launch_bounds__(256) void residual_norm_narrow_kernel(ResidualNormA
     if (j < width) a.normed[(int64_t)row * width + j] = f32_to_act<DT>(x[j]);
 }
 
-template <int DT, typename RT, bool LAYER, int WAVES, int NV>
+template <int DT, typename RT, bool LAYER, int WAVES, int NV, int LANES = 64>
 void launch_rows(const ResidualNormArgs& a, hipStream_t stream) {
-  const int rows = WAVES == 1 ? 4 : 1, threads = WAVES == 1 ? 256 : 64 * WAVES;
-  residual_norm_kernel<DT, RT, LAYER, WAVES, NV>
+  const int rows = WAVES == 1 ? 256 / LANES : 1, threads = WAVES == 1 ? 256 : 64 * WAVES;
+  residual_norm_kernel<DT, RT, LAYER, WAVES, NV, LANES>
       <<<(a.rows + rows - 1) / rows, threads, 0, stream>>>(a);
 }
 
@@ -256,6 +262,11 @@ void launch_rows(const ResidualNormArgs& a, hipStream_t stream) {
 //     768 x 4096    4, 2   7.3 / 8.7              16, 1   8.1 / 11.8
 //     512 x 4096    4, 2   6.0 / 7.1              16, 1   5.7 / 8.6
 //     768 x 896     1, 2   4.2 / 4.8               4, 1   3.6 / 4.8
+// Rows of up to 256 values leave most of a wave idle: 16 lanes take those of up to 128, 32 the others.
+//  100001 x 128    a wave  40 / 54    16 lanes  20 / 21
+//  100001 x 256    a wave  45 / 60    32 lanes  35 / 37
+//       1 x 256    a wave 2.0 / 2.4   32 lanes 2.1 / 2.5
+//  100001 x 448    a wave  65 / 70    32 lanes, two vectors each  68 / 69
 // (98 us for 16384 x 4096 are 5.5 TB/s; a copy of 1 GiB reaches 5.1 to 5.2.)
 template <int DT, typename RT, bool LAYER>
 void launch_width(const ResidualNormArgs& a, int cus, hipStream_t stream) {
@@ -263,6 +274,8 @@ void launch_width(const ResidualNormArgs& a, int cus, hipStream_t stream) {
   const bool many = w > 2048 ? a.rows > 2 * cus : a.rows >= 4 * cus;
   if (w < 8)
     residual_norm_narrow_kernel<DT, RT, LAYER><<<(a.rows + 255) / 256, 256, 0, stream>>>(a);
+  else if (w <= 128) launch_rows<DT, RT, LAYER, 1, 1, 16>(a, stream);
+  else if (w <= 256) launch_rows<DT, RT, LAYER, 1, 1, 32>(a, stream);
   else if (w <= 512) launch_rows<DT, RT, LAYER, 1, 1>(a, stream);
   else if (w <= 1024 && many) launch_rows<DT, RT, LAYER, 1, 2>(a, stream);
   else if (w <= 1536 && many && LAYER) launch_rows<DT, RT, LAYER, 1, 3>(a, stream);

@@ -72,6 +72,15 @@ def test_many_rows(width, kind):
           post_weight=w, kind=kind)
 
 
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("rows,width", [(1, 128), (17, 8), (2051, 64), (2051, 121), (2051, 128),
+                                        (7, 129), (2051, 171), (2051, 256), (9, 257)])
+def test_narrow_rows(rows, width, kind):  # several rows a wave, the last of them not all there
+    w = make(width, torch.bfloat16, 1, 0.2, 1.0)
+    check(make((rows, width), torch.bfloat16, 5), make((rows, width), torch.bfloat16, 6), weight=w,
+          post_weight=w, kind=kind)
+
+
 @pytest.mark.parametrize("post", [False, True])
 @pytest.mark.parametrize("gate", [(), (1,), (1, 1, 1), (96,), (3, 1, 96), (3, 1, 1), (3, 5, 1),
                                   (3, 5, 96), (5, 96), (5, 1), (1, 5, 96), (1, 1, 96)])
