@@ -379,6 +379,7 @@ def section_host(mt, gen, device, stream, args):
         from transformers import Qwen2Config
         from transformers.models.qwen2.modeling_qwen2 import Qwen2MLP
 
+        torch.manual_seed(1234)  # the module's weights: the same in every run
         mlp = Qwen2MLP(Qwen2Config(hidden_size=HIDDEN, intermediate_size=INTER,
                                    hidden_act="silu")).to(device=device, dtype=torch.bfloat16)
         holder = torch.nn.Module()

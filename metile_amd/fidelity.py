@@ -23,9 +23,9 @@ from __future__ import annotations
 import torch
 
 
-def affine_swiglu_compatible(result: torch.Tensor, reference: torch.Tensor) -> bool:
-    if result.shape != reference.shape or result.dtype != reference.dtype:
-        return False
+def affine_deviation(result: torch.Tensor, reference: torch.Tensor) -> tuple[float, float]:
+    """The two figures that ``affine_swiglu_compatible`` limits: RMS of the difference over the
+    reference's RMS, and the largest difference over the reference's largest magnitude."""
     r = result.float()
     ref = reference.float()
     diff = r - ref
@@ -33,10 +33,16 @@ def affine_swiglu_compatible(result: torch.Tensor, reference: torch.Tensor) -> b
     difference_rms = torch.sqrt(torch.mean(diff * diff))
     reference_peak = torch.max(torch.abs(ref))
     difference_peak = torch.max(torch.abs(diff))
-    finite = bool(torch.isfinite(r).all())
     floor = torch.tensor(1e-6, dtype=torch.float32, device=r.device)
-    normalized_rms = float(difference_rms / torch.maximum(reference_rms, floor))
-    normalized_peak = float(difference_peak / torch.maximum(reference_peak, floor))
+    return (float(difference_rms / torch.maximum(reference_rms, floor)),
+            float(difference_peak / torch.maximum(reference_peak, floor)))
+
+
+def affine_swiglu_compatible(result: torch.Tensor, reference: torch.Tensor) -> bool:
+    if result.shape != reference.shape or result.dtype != reference.dtype:
+        return False
+    normalized_rms, normalized_peak = affine_deviation(result, reference)
+    finite = bool(torch.isfinite(result.float()).all())
     return finite and normalized_rms <= 0.005 and normalized_peak <= 0.01
 
 

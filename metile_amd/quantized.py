@@ -630,15 +630,25 @@ def mlx_affine_swiglu_qmv_nax(values, gate_packed, gate_scales, gate_biases, up_
                          up_biases, group_size=group_size, bits=bits)
 
 
-def _fidelity_gate(result, reference, what):
-    """Raise unless ``result`` passes the reference tuner's affine fidelity gate against the
-    native composition (``metile/backends/mlx_quantized.py:1256-1272,1297``). The reference
-    falls back to the native path on failure; here a failure is an error."""
-    from .fidelity import affine_swiglu_compatible
+def _fidelity_gate(result, native, exact, what):
+    """Raise unless ``result`` passes the reference tuner's affine fidelity gate
+    (``metile/backends/mlx_quantized.py:1256-1272,1297``) against ``native``, the native
+    composition, or against what ``exact()`` gives, the same in fp32 and rounded once. The second
+    comparison settles what the first cannot: the kernels round once, the native composition
+    rounds up to four times (gate, up, silu and product), and in bfloat16 these roundings alone
+    can pass the gate's limits (a projection of 8960 values in about one sample of 200). The
+    reference falls back to the native path on failure; here a failure is an error."""
+    from .fidelity import affine_deviation, affine_swiglu_compatible
 
-    if result.numel() and not affine_swiglu_compatible(result, reference):
-        raise RuntimeError(f"{what}: the gfx950 kernel failed the fidelity gate against the "
-                           "native quantized-matmul composition on the sample input")
+    if not result.numel() or affine_swiglu_compatible(result, native):
+        return
+    once = exact()
+    if affine_swiglu_compatible(result, once):
+        return
+    figures = ["rms %.4g peak %.4g" % affine_deviation(result, t) for t in (native, once)]
+    raise RuntimeError(f"{what}: the gfx950 kernel failed the fidelity gate (rms 0.005, peak 0.01) "
+                       f"on the sample input: {figures[0]} from the native quantized-matmul "
+                       f"composition, {figures[1]} from the same in fp32 rounded once")
 
 
 def mlx_affine_swiglu_executor(sample_values, gate_weight, gate_scales, gate_biases, up_weight,
@@ -650,7 +660,7 @@ def mlx_affine_swiglu_executor(sample_values, gate_weight, gate_scales, gate_bia
     (``metile_amd.tuning.ensure_qmv_layout``; cached decisions are reused), checks the kernel
     against the native composition on the sample (the reference tuner's fidelity gate) and
     returns ``execute(values)`` bound to the kept weights."""
-    from .native import native_affine_swiglu
+    from .native import exact_affine_swiglu, native_affine_swiglu
 
     _swiglu_guards(sample_values, gate_weight, gate_scales, gate_biases, up_weight, up_scales,
                    up_biases, group_size, bits)
@@ -666,6 +676,7 @@ def mlx_affine_swiglu_executor(sample_values, gate_weight, gate_scales, gate_bia
     _fidelity_gate(
         affine_swiglu(sample_values, *kept, group_size=group_size, bits=bits),
         native_affine_swiglu(sample_values, *mlx, group_size=group_size, bits=bits),
+        lambda: exact_affine_swiglu(sample_values, *mlx, group_size=group_size, bits=bits),
         "affine SwiGLU")
 
     def execute(values):
@@ -713,10 +724,8 @@ def bind_mlp_executor(sample_values, mlx, packed, sample_residual, *, group_size
     caller's). The
     sample's results are gated against the native compositions. Returns
     ``execute(values, residual)``."""
-    from .native import native_affine_residual_qmv, native_affine_swiglu
+    from . import native
 
-    (gate_weight, gate_scales, gate_biases), (up_weight, up_scales, up_biases), \
-        (down_weight, down_scales, down_biases) = mlx
     chosen = {}  # row bucket -> (gate, up, down) in the layouts picked for it
 
     def bucket(values):  # beyond the chunk the wide kernel's, whose layouts are decided apart
@@ -747,15 +756,16 @@ def bind_mlp_executor(sample_values, mlx, packed, sample_residual, *, group_size
 
     gate, up, down = stages(sample_values)
     hidden = affine_swiglu(sample_values, *gate, *up, group_size=group_size, bits=bits)
+    stage = (sample_values, *mlx[0], *mlx[1])
     _fidelity_gate(
-        hidden,
-        native_affine_swiglu(sample_values, gate_weight, gate_scales, gate_biases, up_weight,
-                             up_scales, up_biases, group_size=group_size, bits=bits),
+        hidden, native.native_affine_swiglu(*stage, group_size=group_size, bits=bits),
+        lambda: native.exact_affine_swiglu(*stage, group_size=group_size, bits=bits),
         "affine SwiGLU")
+    stage = (hidden, *mlx[2], sample_residual)
     _fidelity_gate(
         affine_qmv(hidden, *down, group_size=group_size, bits=bits, residual=sample_residual),
-        native_affine_residual_qmv(hidden, down_weight, down_scales, down_biases,
-                                   sample_residual, group_size=group_size, bits=bits),
+        native.native_affine_residual_qmv(*stage, group_size=group_size, bits=bits),
+        lambda: native.exact_affine_residual_qmv(*stage, group_size=group_size, bits=bits),
         "affine residual QMV")
 
     bound = {}  # row bucket -> BoundMlp over the layouts decided for it
