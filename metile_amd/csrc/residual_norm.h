@@ -21,6 +21,7 @@ struct ResidualNormArgs {
   uint16_t* normed;             // [rows, width] contiguous
   int64_t residual_stride, block_stride, gate_stride;  // of a row (of the gate: of its own rows)
   int32_t rows, width;
+  uint32_t first_row;   // of the launch (its own to set)
   int32_t gate_rows;    // rows of the batch that share one row of the gate
   int32_t gate_scalar;  // the gate's rows hold one value each
   float scale, eps;

@@ -10,6 +10,8 @@
 // sum. Memory bounds it for many rows, the chain of one read and the row sums for few. A row belongs
 // to 16 lanes up to a wave, or to a workgroup of 2 to 16 waves: threads take eight consecutive values
 // at a time.
+#include <algorithm>
+
 #include "common.h"
 #include "residual_norm.h"
 
@@ -82,8 +84,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_k
   __shared__ float lds[2][WAVES];
   int turn = 0;
   const int t = WAVES == 1 ? threadIdx.x & (LANES - 1) : threadIdx.x;
-  const int row = blockIdx.x * kRows + (WAVES == 1 ? threadIdx.x / LANES : 0);
-  if (WAVES == 1 && row >= a.rows) return;
+  const uint32_t row = a.first_row + blockIdx.x * kRows + (WAVES == 1 ? threadIdx.x / LANES : 0);
+  if (WAVES == 1 && row >= (uint32_t)a.rows) return;
   const int width = a.width;
 
   const RT* res = static_cast<const RT*>(a.residual) + (int64_t)row * a.residual_stride;
@@ -155,7 +157,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_k
   if (blk) {
     if (a.post_weight) norm(b, a.post_weight, a.post_bias);
     if (a.gate) {
-      const uint16_t* gate = a.gate + (int64_t)(row / a.gate_rows) * a.gate_stride;
+      const uint16_t* gate = a.gate + (int64_t)(row / (uint32_t)a.gate_rows) * a.gate_stride;
       const float one = act_to_f32<DT>(gate[0]);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -190,8 +192,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void residual_norm_k
 // Rows of fewer than eight values: a row a thread, value by value.
 template <int DT, typename RT, bool LAYER>
 __global__ __launch_bounds__(256) void residual_norm_narrow_kernel(ResidualNormArgs a) {
-  const int row = blockIdx.x * 256 + threadIdx.x;
-  if (row >= a.rows) return;
+  const uint32_t row = a.first_row + blockIdx.x * 256 + threadIdx.x;
+  if (row >= (uint32_t)a.rows) return;
   const int width = a.width;
   auto value = [](const uint16_t* p, int j) { return act_to_f32<DT>(p[j]); };
   auto norm = [&](float (&v)[8], const uint16_t* weight, const uint16_t* bias) {
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(256) void residual_norm_narrow_kernel(ResidualNormA
   }
   if (a.block && a.post_weight) norm(b, a.post_weight, a.post_bias);
   const uint16_t* gate = a.block && a.gate
-                             ? a.gate + (int64_t)(row / a.gate_rows) * a.gate_stride : nullptr;
+                             ? a.gate + (int64_t)(row / (uint32_t)a.gate_rows) * a.gate_stride : nullptr;
   RT* out = static_cast<RT*>(a.residual_out);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -240,11 +242,24 @@ __global__ __launch_bounds__(256) void residual_norm_narrow_kernel(ResidualNormA
     if (j < width) a.normed[(int64_t)row * width + j] = f32_to_act<DT>(x[j]);
 }
 
+// One launch for every kMostBlocks workgroups (of `rows` rows each): the threads of a launch are
+// counted in 32 bits, and those that do not fit are left out without an error.
+constexpr int64_t kMostBlocks = 1 << 21;
+template <typename K>
+void launch_blocks(K kernel, const ResidualNormArgs& args, int rows, int threads,
+                   hipStream_t stream) {
+  ResidualNormArgs a = args;
+  const int64_t blocks = ((int64_t)a.rows + rows - 1) / rows;
+  for (int64_t first = 0; first < blocks; first += kMostBlocks) {
+    a.first_row = (uint32_t)(first * rows);
+    kernel<<<(uint32_t)std::min(blocks - first, kMostBlocks), threads, 0, stream>>>(a);
+  }
+}
+
 template <int DT, typename RT, bool LAYER, int WAVES, int NV, int LANES = 64>
 void launch_rows(const ResidualNormArgs& a, hipStream_t stream) {
-  const int rows = WAVES == 1 ? 256 / LANES : 1, threads = WAVES == 1 ? 256 : 64 * WAVES;
-  residual_norm_kernel<DT, RT, LAYER, WAVES, NV, LANES>
-      <<<(a.rows + rows - 1) / rows, threads, 0, stream>>>(a);
+  launch_blocks(residual_norm_kernel<DT, RT, LAYER, WAVES, NV, LANES>, a,
+                WAVES == 1 ? 256 / LANES : 1, WAVES == 1 ? 256 : 64 * WAVES, stream);
 }
 
 // Waves of a row and vectors of a thread, by width and whether there are rows enough to fill the
@@ -273,7 +288,7 @@ void launch_width(const ResidualNormArgs& a, int cus, hipStream_t stream) {
   const int w = a.width;
   const bool many = w > 2048 ? a.rows > 2 * cus : a.rows >= 4 * cus;
   if (w < 8)
-    residual_norm_narrow_kernel<DT, RT, LAYER><<<(a.rows + 255) / 256, 256, 0, stream>>>(a);
+    launch_blocks(residual_norm_narrow_kernel<DT, RT, LAYER>, a, 256, 256, stream);
   else if (w <= 128) launch_rows<DT, RT, LAYER, 1, 1, 16>(a, stream);
   else if (w <= 256) launch_rows<DT, RT, LAYER, 1, 1, 32>(a, stream);
   else if (w <= 512) launch_rows<DT, RT, LAYER, 1, 1>(a, stream);
