@@ -432,7 +432,9 @@ int mt_paged_append(const mt_paged_cache* cache, const mt_paged_append_args* arg
  * heads, dim] with element strides per request and head (multiples of 16 bytes), out [requests,
  * heads, dim] contiguous, 16-byte aligned, both in dtype; a 16-bit cache has the same. requests *
  * cache heads * (query heads of one / 16, rounded up) * (width * page_size / 32, rounded up, + 4) is
- * at most 2^31 - 2^16. Sums are fp32 and in a fixed order: results do not change from run to run. */
+ * at most 2^31 - 2^16. Scores, maxima and sums are fp32 and in a fixed order: results do not change from
+ * run to run. Probabilities meet the values as two 16-bit parts, off by 2^-18 of each at most (2^-24 in
+ * MT_F16, or 2^-39 of the row's largest), also beside infinities. */
 typedef struct mt_paged_attention_args {
   const void* query;
   int64_t query_strides[2];

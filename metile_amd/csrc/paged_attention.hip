@@ -15,10 +15,13 @@
 //  * pages: a lane a token looks up its entry, one unit ahead, and reckons the row's offset, which
 //    the lanes that load the row ask for (pages of one token 10.4 us; with the look-ups and their
 //    divisions in every loading lane 13.2; pages of 16 the same).
-// Probabilities go to the matrix cores as two 16-bit parts (their rounding and the rest of it),
-// so the 16-bit rounding of the result is the only one; sums, maxima and results are fp32. (The
-// second part is zero or negative as often as not, and an infinite value times it is no number: a
-// segment whose sums are not finite is taken again with the first parts alone, which are positive.)
+// Scores, maxima, sums and results are fp32. Probabilities go to the matrix cores as two 16-bit
+// parts (their rounding and the rest of it): a probability p is off by 2^-18 p at most with bf16, by
+// 2^-24 p or 2^-39 of its row's largest with f16, where the result's own rounding is 2^-9 and 2^-12
+// of it. A third part would add half as many products of values again. (The second part is zero or
+// negative as often as not, and an infinite value times it is no number: a segment with sums that
+// are not finite is taken again, with values that are not finite times the first parts, which are
+// positive, alone.)
 //
 // Split: all rows, laid end to end in units of 32 tokens with a few more for the fixed cost of a
 // row, are dealt out in equal contiguous runs to a fixed number of waves (each finds its place from
@@ -111,6 +114,15 @@ template <int DT>
 __device__ __forceinline__ u32x4 fp8_eight(uint32_t lo, uint32_t hi) {
   return (u32x4){fp8_pair<DT, false>(lo), fp8_pair<DT, true>(lo), fp8_pair<DT, false>(hi),
                  fp8_pair<DT, true>(hi)};
+}
+
+// Two 16-bit floats, 0 in place of infinities and NaN.
+template <int DT>
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
+  constexpr uint32_t kExponent = DT == kBF16 ? 0x7f80u : 0x7c00u;
+  if ((w & kExponent) == kExponent) w &= 0xffff0000u;
+  if ((w >> 16 & kExponent) == kExponent) w &= 0x0000ffffu;
+  return w;
 }
 
 // Rows of up to so many units are not split over waves: a unit costs a wave that has its SIMD to
@@ -344,7 +356,7 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
     // Table entries are looked up one unit further ahead than rows, so that no row waits for one.
     Place now, ahead;
     u32x4 q[kMfmas];
-    bool two_parts = true;
+    bool all_finite = true;
     int tok0;
     bool live;
   again:
@@ -492,10 +504,14 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
       }
 #pragma unroll
       for (int e = 0; e < kLaneDims; ++e) acc[e] = mfma16<DT>(v[e], p_hi, acc[e]);
-      if (two_parts) {
+      if (!all_finite) {
 #pragma unroll
-        for (int e = 0; e < kLaneDims; ++e) acc[e] = mfma16<DT>(v[e], p_lo, acc[e]);
+        for (int e = 0; e < kLaneDims; ++e)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[e][j] = finite_pair<DT>(v[e][j]);
       }
+#pragma unroll
+      for (int e = 0; e < kLaneDims; ++e) acc[e] = mfma16<DT>(v[e], p_lo, acc[e]);
       if (more) load_values(now);
       tok0 = next;
       live = more;
@@ -506,8 +522,8 @@ __global__ __launch_bounds__(kThreads, attention_waves(DIM)) void paged_attentio
     for (int e = 0; e < kLaneDims; ++e)
 #pragma unroll
       for (int i = 0; i < 4; ++i) finite = fmaf(acc[e][i], 0.0f, finite);
-    if (two_parts && __any(finite != 0.0f)) {
-      two_parts = false;
+    if (all_finite && __any(finite != 0.0f)) {
+      all_finite = false;
       m = -__builtin_inff();
       l = 0.0f;
 #pragma unroll
