@@ -65,3 +65,71 @@ def test_heads_that_an_infinite_key_leaves_out(lengths, dtype):
     assert bool(torch.isnan(out[:, ::2]).all())
     assert outside(out[:, 1::2], want[:, 1::2], tol[:, 1::2]) <= 0
     assert outside(lse[:, 1::2], want_lse[:, 1::2], lse_tol[:, 1::2]) <= 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("below", [9.0, 18.0, 26.0, 40.0, 60.0])
+def test_infinite_values_of_small_probability(below, dtype):
+    # exp(-60) is 9e-27, far below float16's range: times infinity it is infinity all the same
+    cache = mt.PagedCache.allocate(8, 16, 1, 64, dtype=dtype)
+    cache.key.zero_(), cache.value.fill_(1.0)
+    cache.key[0, 0, 0, 0] = below
+    cache.value[3, 5, 0, 7], cache.value[5, 1, 0, 8] = float("inf"), -float("inf")
+    q = torch.zeros(1, 2, 64, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    for n in (100, 128):
+        out = mt.paged_attention(q, cache, torch.arange(8, dtype=torch.int32, device="cuda")[None],
+                                 torch.tensor([n], dtype=torch.int32, device="cuda"), scale=1.0)[0]
+        assert bool((out[:, 7] == float("inf")).all()) and bool((out[:, 8] == -float("inf")).all())
+        out[:, 7:9] = 1.0
+        assert bool((out == 1.0).all())
+
+
+@pytest.mark.parametrize("below", [12.0, 18.0, 21.0, 24.0, 27.0])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_small_probabilities_of_large_values_in_f16(infinite, below):
+    # one token far ahead whose value is 0, 127 with 60000: exp(-21) of that counts. A probability is
+    # off by 2^-24 of itself or 2^-39 of the largest, which is 1, in either form of the products
+    n = 128
+    cache = mt.PagedCache.allocate(8, 16, 1, 64, dtype=torch.float16)
+    cache.key.zero_(), cache.value.fill_(60000.0)
+    cache.key[0, 0, 0, 0] = below
+    cache.value[0, 0].zero_()
+    if infinite:
+        cache.value[3, 5, 0, 7] = float("inf")
+    q = torch.zeros(1, 2, 64, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1.0
+    out = mt.paged_attention(q, cache, torch.arange(8, dtype=torch.int32, device="cuda")[None],
+                             torch.tensor([n], dtype=torch.int32, device="cuda"), scale=1.0)[0]
+    if infinite:
+        assert bool((out[:, 7] == float("inf")).all())
+        out[:, 7] = out[:, 8]
+    p = torch.tensor(-below, dtype=torch.float64).exp()
+    want = 60000.0 * (n - 1) * p / (1 + (n - 1) * p)
+    # fp32 exponents and sums: 2^-20 of the result; f16's own rounding, 2^-25 below its normal numbers
+    tol = (2.0 ** -11 + 2.0 ** -20) * want + 60000.0 * (n - 1) * 2.0 ** -39 + 2.0 ** -25
+    assert float((out.double().cpu() - want).abs().max()) <= float(tol)
+
+
+@pytest.mark.parametrize("dtype,cache_dtype", [(torch.bfloat16, torch.bfloat16),
+                                               (torch.float16, torch.float16),
+                                               (torch.bfloat16, torch.float8_e4m3fn),
+                                               (torch.float16, torch.float8_e4m3fn)])
+@pytest.mark.parametrize("lengths", LENGTHS)
+def test_columns_beside_a_value_that_is_no_number(lengths, dtype, cache_dtype):
+    q, cache, tables, n = attention_case(lengths, 6, 2, 64, 16, dtype=dtype, cache=cache_dtype)
+    bits = (lambda t: t.view(torch.uint8) if cache_dtype == torch.float8_e4m3fn else t)
+    key, value = cache.key, bits(cache.value).clone()
+    table = tables.tolist()
+    for r, length in enumerate(lengths):
+        t = length // 2
+        spot = table[r][t // 16], t % 16, 1, 11
+        value[spot] = 0
+        bits(cache.value)[spot] = 0x7f if cache_dtype == torch.float8_e4m3fn else float("nan")
+    out = mt.paged_attention(q, cache, tables, n)
+    want, _, tol, _ = ref.attention(q, key, value.view(cache_dtype), tables.cpu(), lengths,
+                                    64 ** -0.5, 0, cache.key_scale, cache.value_scale)
+    assert bool(torch.isnan(out[:, 3:, 11]).all())
+    out[:, 3:, 11] = 0.0
+    want[:, 3:, 11] = 0.0
+    assert outside(out, want, tol) <= 0
