@@ -129,8 +129,8 @@ class Batch:
         return logits[:requests]
 
     def choose(self, logits):
-        """Greedy next tokens in place."""
-        self.tokens.copy_(logits.argmax(-1))
+        """Greedy next tokens of the active requests in place; idle ones keep theirs."""
+        self.tokens.copy_(torch.where(self.active > 0, logits.argmax(-1), self.tokens))
 
 
 def main():
