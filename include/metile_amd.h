@@ -382,11 +382,12 @@ typedef struct mt_paged_cache {
  * written into the table. Outputs: starts [requests + 1], the first token of each request in the
  * step's packed batch; lengths [requests], cached + new; for each of the `tokens` tokens of the
  * batch its slot (page * page_size + place in the page), position in its request and request;
- * taken [1], the pages that the step needed. Tokens behind the last request's (padding) get slot
- * -1, position 0, request -1; tokens that the table's width or the free list has no page for get
- * slot -1 (and an exhausted list writes -1 into the table, with `taken` telling the shortage).
- * Tokens beyond `tokens` are dropped with the table entries of the pages they open. width *
- * page_size is below 2^31; sums of counts stop at 2^31 - 1. requests or tokens may be 0. Outputs
+ * taken [1], the pages that the step needed as far as the tables reach. Tokens behind the last
+ * request's (padding) get slot -1, position 0, request -1; tokens that the table's width or the free
+ * list has no page for get slot -1. An exhausted list writes -1 into the table, and `taken` tells the
+ * shortage; a table that is too narrow shows in lengths beyond width * page_size alone. Tokens beyond
+ * `tokens` are dropped with the table entries of the pages they open. width * page_size is below
+ * 2^31; sums of counts stop at 2^31 - 1. requests or tokens may be 0. Outputs
  * overlap no input. */
 typedef struct mt_paged_tables_args {
   const int32_t* cached;
@@ -408,7 +409,7 @@ int mt_paged_tables(const mt_paged_tables_args* args, void* stream);
 /* Writes a step's keys and values, [tokens, heads, dim] 16-bit (dtype) with element strides per
  * token and head, to the cache at slots[token]; tokens whose slot is not in [0, pages * page_size)
  * are left out. Slots that occur twice get one of their rows or a mixture. 8-bit caches hold
- * value / scale rounded to nearest even and limited to +-448. A 16-bit cache has the rows' dtype.
+ * the fp32 quotient value / scale rounded to nearest even and limited to +-448. A 16-bit cache has the rows' dtype.
  * Rows and strides are multiples of 16 bytes; tokens * heads * dim / 8 is below 2^31. */
 typedef struct mt_paged_append_args {
   const void* key;

@@ -136,7 +136,8 @@ class PagedCache:
 class PagedStep(NamedTuple):
     """What :func:`paged_tables` gives: for each token of the step's packed batch ``slots`` (int64),
     ``positions`` and ``requests``; ``starts`` (``[requests + 1]``) and ``lengths`` of the requests;
-    ``taken`` (``[1]``), the pages that the step needed. int32 but for the slots."""
+    ``taken`` (``[1]``), the pages that the step needed as far as the tables reach. int32 but for the
+    slots."""
 
     slots: torch.Tensor
     positions: torch.Tensor
@@ -160,9 +161,11 @@ def paged_tables(cached, new, block_tables, free_pages, *, page_size, tokens, fr
     tokens need are taken in order from ``free_pages`` (int32), beginning with entry ``free_start`` (a
     device int32 tensor of one element; ``None``: the first), request by request. ``tokens``: the
     size of the packed batch, at least the sum of ``new``; tokens behind that sum are padding (slot
-    -1, request -1, position 0). Tokens without a page (the table too narrow or the list exhausted)
-    have slot -1, and ``taken`` counts the pages wanted, so a caller sees the shortage when it next
-    looks. Returns a :class:`PagedStep`; nothing is synchronised.
+    -1, request -1, position 0). Tokens without a page have slot -1. Where the list is exhausted,
+    ``taken`` (the pages that the step needs and the tables have room for) is more than the list holds
+    from ``free_start`` on; where a table is too narrow, ``lengths`` is more than ``width *
+    page_size``, and ``taken`` does not count the pages beyond: a caller sees either shortage when it
+    next looks. Returns a :class:`PagedStep`; nothing is synchronised.
     """
     device = block_tables.device
     _same_device(device, cached, new, free_pages, free_start)
@@ -229,8 +232,8 @@ def paged_attention(query, cache, block_tables, lengths, *, scale=None, window=N
     ``query`` ``[requests, heads, head_dim]`` (bfloat16 or float16; ``heads`` a multiple of the
     cache's: neighbouring query heads share a key-value head). ``block_tables`` int32
     ``[requests, width]``; ``lengths`` int32 ``[requests]``: tokens in the cache, the new one among
-    them. ``scale``: of the scores (default ``head_dim ** -0.5``). ``window``: attend to the last so
-    many tokens only. Returns the output in ``query``'s shape and dtype and, with ``return_lse``, the
+    them (what the table has no room for is cut off). ``scale``: of the scores (default ``head_dim **
+    -0.5``). ``window``: attend to the last so many tokens only. Returns the output in ``query``'s shape and dtype and, with ``return_lse``, the
     log of the sum of exponentials (float32 ``[requests, heads]``). Requests without tokens give
     zeros and -inf. Table entries behind a request's last token are not read; tokens whose entry is
     no page of the cache are left out.
