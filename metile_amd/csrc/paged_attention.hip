@@ -32,10 +32,10 @@
 // of those workgroups to arrive (8 parts at a time, up to 16 at once).
 //
 // Bound by the bytes of keys and values where there are enough of them: 2 requests of 131072 tokens
-// with 8 key-value heads of 128 bf16 values (1.07 GB) take 183 us, 5.9 TB/s (a copy of 1 GiB
-// reaches 5.2); 64 requests of 1 to 8192 tokens (224 MB) 47.5 us, 4.7 TB/s. The shortest calls take
-// 4.7 us: the launch, then lengths, table entry and first rows, a memory round trip each after the
-// other; a row that several workgroups share costs about 4 us more for its join.
+// with 8 key-value heads of 128 bf16 values (1.07 GB) take 183 us, 5.9 TB/s (of 1 GiB, reads alone
+// reach 6.3 and a copy 5.2); 64 requests of 1 to 8192 tokens (224 MB) 47.5 us, 4.7 TB/s. The
+// shortest calls take 4.7 us: the launch, then lengths, table entry and first rows, a memory round
+// trip each after the other; a row that several workgroups share costs about 4 us more for its join.
 #include "common.h"
 #include "paged.h"
 
