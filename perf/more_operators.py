@@ -435,6 +435,7 @@ def _plain_compact(s, case):
     open_ = _marked(pages, free[listed_from]) & ~used
     low = (used | open_).cumsum(0) <= used.sum()
     sources, targets = (m.nonzero()[:, 0].to(torch.int32) for m in (used & ~low, open_ & low))
+    sources = sources.flip(0)  # the highest page in use goes to the lowest free one
     number = torch.arange(pages, dtype=torch.int32, device=tables.device)
     number[sources.long()] = targets
     result = torch.where(filled, number[tables.clamp(min=0).long()], tables)
