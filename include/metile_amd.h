@@ -453,6 +453,144 @@ size_t mt_paged_attention_workspace_bytes(const mt_paged_cache* cache, int reque
 int mt_paged_attention(const mt_paged_cache* cache, const mt_paged_attention_args* args,
                        void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention of a chunk of new tokens of each request over its pages: a prompt, a part of one, a draft.
+ * Request r's new tokens are rows starts[r] .. starts[r + 1] - 1 of the packed batch (starts[0] is 0, as
+ * mt_paged_tables writes them) and the last of its lengths[r] tokens in the cache, whose keys and values
+ * are appended first. Each attends to the tokens up to itself, of them the last `window` (0: all):
+ * out[t, h] = sum_j p_j v_j with p = softmax(scale * q[t, h] . k_j), of the key-value head h / (heads /
+ * cache heads). Keys are limited to width * page_size, which is at most 2^31 - 64; tokens whose entry is
+ * not a page of the cache are left out, and neither what slots behind the last token hold nor what
+ * later tokens do matters to a token, NaN and infinities too. Tokens without a key, and rows of the batch
+ * that belong to no request, get 0. lse (or NULL) [tokens, heads] receives log sum exp of the scaled
+ * scores, -inf for such rows. Lengths, starts, tables and the cache must not change while the call runs.
+ * query [tokens, heads, dim] with element strides per token and head (multiples of 16 bytes), out
+ * [tokens, heads, dim] contiguous, 16-byte aligned, both in dtype; a 16-bit cache has the same. tokens *
+ * heads is below 2^31, and tokens * heads / 128 + requests * cache heads below 2^24 - 2^16. Scores, maxima
+ * and sums are fp32 and in a fixed order: results do not change from run to run. Probabilities meet the
+ * values rounded to dtype. The workspace need not be cleared and holds nothing between calls; its size
+ * depends on the shapes alone. */
+typedef struct mt_paged_chunk_attention_args {
+  const void* query;
+  int64_t query_strides[2];
+  const int32_t* block_tables;
+  int64_t table_stride;
+  const int32_t* lengths;
+  const int32_t* starts;
+  void* out;
+  float* lse;
+  int tokens, requests, heads, width, window;
+  float scale;
+  int dtype;
+} mt_paged_chunk_attention_args;
+size_t mt_paged_chunk_attention_workspace_bytes(const mt_paged_cache* cache, int tokens, int requests,
+                                                int heads, int width, int window);
+int mt_paged_chunk_attention(const mt_paged_cache* cache, const mt_paged_chunk_attention_args* args,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copies pages sources[i] to targets[i] (count of them), all tokens and heads of keys and values, in each
+ * of the caches (the layers' of one block table). Pairs with a page that is none of the cache's are left
+ * out. Targets are distinct and none of the sources; others hold one of their sources or a mixture. */
+typedef struct mt_paged_copy_args {
+  const int32_t* sources;
+  const int32_t* targets;
+  int64_t count;
+} mt_paged_copy_args;
+int mt_paged_copy(const mt_paged_cache* const* caches, int num_caches, const mt_paged_copy_args* args,
+                  void* stream);
+
+/* Requests targets[i] go on from the tokens of requests sources[i], the first tokens[i] of them (NULL:
+ * all; at most lengths[sources[i]]). Pages that they fill are shared: entered in the target's row of
+ * block_tables ([requests, width], rows table_stride entries apart; entries behind them stay). A page that
+ * has been begun is the target's own, taken from free_pages ([free_count]) beginning with entry
+ * *free_start (NULL: 0), fork by fork; what it holds is to be copied from page copy_sources[i] to
+ * copy_targets[i] (mt_paged_copy; -1 where nothing is). lengths[targets[i]] is set; taken [1] receives the
+ * pages that were needed. An exhausted list writes -1 as the begun page. Forks with a request that is none
+ * of the batch's are left out. Targets are distinct and none of the sources. width * page_size is below
+ * 2^31, requests below 2^24 (also below) and forks below 2^23. */
+typedef struct mt_paged_fork_args {
+  int32_t* block_tables;
+  int64_t table_stride;
+  int32_t* lengths;
+  const int32_t* sources;
+  const int32_t* targets;
+  const int32_t* tokens;
+  const int32_t* free_pages;
+  const int32_t* free_start;
+  int32_t* copy_sources;
+  int32_t* copy_targets;
+  int32_t* taken;
+  int requests, width, free_count, page_size, forks;
+} mt_paged_fork_args;
+int mt_paged_fork(const mt_paged_fork_args* args, void* stream);
+
+/* Frees the pages of tokens behind the first kept[r] of each request's lengths[r] (0: all of them): those
+ * that no request has among its kept tokens' pages. Their numbers, ascending, are written to free_pages
+ * ([free_count]) in front of entry *free_start (entries before the first are dropped); freed [1] receives
+ * how many there are. Tables and lengths are not changed: the caller sets lengths to kept and takes
+ * `freed` from the start. Entries that are no pages (of `pages`) are left out. The workspace need not be
+ * cleared. width * page_size is below 2^31. */
+typedef struct mt_paged_free_args {
+  const int32_t* block_tables;
+  int64_t table_stride;
+  const int32_t* lengths;
+  const int32_t* kept;
+  int32_t* free_pages;
+  const int32_t* free_start;
+  int32_t* freed;
+  int requests, width, free_count, page_size, pages;
+} mt_paged_free_args;
+size_t mt_paged_free_workspace_bytes(int pages);
+int mt_paged_free(const mt_paged_free_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Plans the pages in use together: of all pages that are in use (among the pages of some request's
+ * lengths[r] tokens) or free (in free_pages from entry *free_start on), those in use get the lowest
+ * numbers. The highest in use moves to the lowest free one, and so on: sources and targets [most_moves]
+ * (at least min(pages / 2, requests * width); -1 behind the last) for mt_paged_copy, moves [1] how many.
+ * new_tables [requests, width] receives the block tables as they are then, new_free [free_count] the free
+ * list (up to *free_start as it was, then ascending; -1 behind the last where a page was listed twice or in use). Inputs are not changed. Pages neither in use nor free are left alone. The
+ * workspace need not be cleared. width * page_size is below 2^31. Outputs overlap no input. */
+typedef struct mt_paged_compact_args {
+  const int32_t* block_tables;
+  int64_t table_stride;
+  const int32_t* lengths;
+  const int32_t* free_pages;
+  const int32_t* free_start;
+  int32_t* new_tables;
+  int32_t* new_free;
+  int32_t* sources;
+  int32_t* targets;
+  int32_t* moves;
+  int requests, width, free_count, page_size, pages, most_moves;
+} mt_paged_compact_args;
+size_t mt_paged_compact_workspace_bytes(int pages);
+int mt_paged_compact(const mt_paged_compact_args* args, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* Log probabilities of softmax(logits / temperature) over logits [rows, vocab] (rows row_stride elements
+ * apart; MT_BF16, MT_F16 or MT_F32): of the given tokens [rows] with their ranks (how many logits are
+ * larger, or as large with a lower index; 0 is the likeliest token), the entropies [rows] in nats, and the
+ * `top` (0 to 32, at most vocab) likeliest tokens [rows, top] in order, equal ones by index. tokens,
+ * logprobs and ranks may be NULL together. Logits of -inf have no probability and no part in the entropy;
+ * a token outside the vocabulary has -inf and rank -1. A row of -inf alone has log probabilities of -inf
+ * and an entropy of 0. A row with NaN or +inf has NaN for both; NaN is no alternative (token -1 where there
+ * are too few others). All sums are fp32 in a fixed order. Logits need the alignment of their type only.
+ * vocab is at most 2^24, temperature 1e-6 to 1e6. The workspace need not be cleared; its size depends on the shapes alone. */
+typedef struct mt_token_logprobs_args {
+  const void* logits;
+  int64_t row_stride;
+  const int64_t* tokens;
+  float* logprobs;
+  float* entropies;
+  int32_t* ranks;
+  float* top_logprobs;
+  int64_t* top_tokens;
+  int rows, vocab, top, dtype;
+  float temperature;
+} mt_token_logprobs_args;
+size_t mt_token_logprobs_workspace_bytes(int rows, int vocab, int top);
+int mt_token_logprobs(const mt_token_logprobs_args* args, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
 typedef enum mt_norm_kind { MT_NORM_RMS = 0, MT_NORM_LAYER = 1 } mt_norm_kind;
 
 /* The norms around a block, its gate and the scaled residual, [rows, width], in one pass:

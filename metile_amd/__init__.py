@@ -5,7 +5,8 @@ projections, written as hand-written HIP kernels behind a C ABI (``include/metil
 exposed here on torch tensors with the reference's call surface
 (``metile/backends/mlx_quantized.py``), with the reference tuner's fidelity gates and native
 compositions for checking kernels against its semantics. Around the projections: a paged
-key-value cache with its tables, append and decode attention, and the norms between blocks.
+key-value cache with its tables, append, attention of one token and of chunks, and its pages' copies,
+forks, freeing and compaction; the norms between blocks; and the tokens' log probabilities.
 """
 
 from ._lib import MetileError, version
@@ -18,9 +19,23 @@ from .model import (
     quantize_mlp,
     restore_patches,
 )
+from .logprobs import TokenLogprobs, token_logprobs
 from .native import native_affine_matmul, native_affine_residual_qmv, native_affine_swiglu
 from .norms import residual_norm
-from .paged import PagedCache, PagedStep, paged_append, paged_attention, paged_tables
+from .paged import (
+    PagedCache,
+    PagedCompaction,
+    PagedFork,
+    PagedStep,
+    paged_append,
+    paged_attention,
+    paged_chunk_attention,
+    paged_compact,
+    paged_copy,
+    paged_fork,
+    paged_free,
+    paged_tables,
+)
 from .quantize import CompressedDownWeight, affine_quantize
 from .quantized import (
     AffineWeight,
@@ -62,10 +77,19 @@ __all__ = [
     "native_affine_residual_qmv",
     "native_affine_swiglu",
     "PagedCache",
+    "PagedCompaction",
+    "PagedFork",
     "PagedStep",
+    "TokenLogprobs",
     "paged_append",
     "paged_attention",
+    "paged_chunk_attention",
+    "paged_compact",
+    "paged_copy",
+    "paged_fork",
+    "paged_free",
     "paged_tables",
+    "token_logprobs",
     "residual_norm",
     "dense_qmv",
     "dense_swiglu",

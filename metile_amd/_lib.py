@@ -79,6 +79,12 @@ class PagedCacheDesc(ctypes.Structure):
 PAGED_TABLES_ARGS = struct.Struct("@PPPqPPPPPPPPiiiii0P")
 PAGED_APPEND_ARGS = struct.Struct("@PPqqqqPqi0P")
 PAGED_ATTENTION_ARGS = struct.Struct("@PqqPqPPPiiiifi0P")
+PAGED_CHUNK_ATTENTION_ARGS = struct.Struct("@PqqPqPPPPiiiiifi0P")
+PAGED_COPY_ARGS = struct.Struct("@PPq0P")
+PAGED_FORK_ARGS = struct.Struct("@PqPPPPPPPPPiiiii0P")
+PAGED_FREE_ARGS = struct.Struct("@PqPPPPPiiiii0P")
+PAGED_COMPACT_ARGS = struct.Struct("@PqPPPPPPPPiiiiii0P")
+TOKEN_LOGPROBS_ARGS = struct.Struct("@PqPPPPPPiiiif0P")
 RESIDUAL_NORM_ARGS = struct.Struct("@PPPPPPPPPqqqiiiiffiii0P")
 
 _P = ctypes.c_void_p
@@ -137,6 +143,16 @@ SIGNATURES = {
     "mt_paged_append": (_I, [_CP, _B, _P]),
     "mt_paged_attention_workspace_bytes": (_Z, [_CP, _I, _I, _I, _I]),
     "mt_paged_attention": (_I, [_CP, _B, _P, _Z, _P]),
+    "mt_paged_chunk_attention_workspace_bytes": (_Z, [_CP, _I, _I, _I, _I, _I]),
+    "mt_paged_chunk_attention": (_I, [_CP, _B, _P, _Z, _P]),
+    "mt_paged_copy": (_I, [_B, _I, _B, _P]),
+    "mt_paged_fork": (_I, [_B, _P]),
+    "mt_paged_free_workspace_bytes": (_Z, [_I]),
+    "mt_paged_free": (_I, [_B, _P, _Z, _P]),
+    "mt_paged_compact_workspace_bytes": (_Z, [_I]),
+    "mt_paged_compact": (_I, [_B, _P, _Z, _P]),
+    "mt_token_logprobs_workspace_bytes": (_Z, [_I, _I, _I]),
+    "mt_token_logprobs": (_I, [_B, _P, _Z, _P]),
     "mt_residual_norm": (_I, [_B, _P]),
     "mt_plans_clear": (_I, []),
     "mt_source_digest": (ctypes.c_char_p, []),

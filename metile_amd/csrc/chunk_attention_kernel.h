@@ -1,0 +1,602 @@
+// The kernels of chunk_attention.hip, a template over types and head size, instantiated in
+// chunk_attention_{bf16,f16}{,_fp8}.hip.
+//
+//   s_j = scale * q . k_j      o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
+//
+// over the keys j up to a token's own position. The rows of a tile are (token, query head) pairs of
+// one request and one key-value head, so that all of them read the same keys. A workgroup takes a
+// tile of 128 rows, 32 a wave, through blocks of 64 keys, with a running reference (near the maximum)
+// and sum:
+//  * keys are the rows of v_mfma_f32_32x32x16 and query rows its columns, so a lane holds scores of
+//    one query row. Key rows are dealt to operand rows so that a lane's registers 8 n .. 8 n + 7 hold
+//    eight consecutive keys, which are the operand of the second product as they stand: no exchange
+//    between lanes but one for the maximum;
+//  * values are read from LDS transposed (ds_read_b64_tr_b16: four rows by sixteen columns a group of
+//    sixteen lanes); the result has the query row in the lane again, so rescaling is local;
+//  * both lie in LDS as 16-bit rows whose 16-byte chunks are exchanged within a row so that every
+//    read touches all banks alike. 8-bit caches are converted on the way in.
+// Probabilities enter the second product rounded to 16 bits (at most 2^-8 of each in bf16, 2^-11 in
+// f16), as the result itself is; a second part of them would add half as many products again. Scores,
+// references, sums and results are fp32, and the sums are of the probabilities before that rounding.
+#pragma once
+
+#include "chunk_attention.h"
+#include "common.h"
+
+namespace mt {
+namespace chunk {
+
+constexpr int kThreads = 256;
+constexpr int kTile = kChunkTile, kBlock = kChunkBlock;
+constexpr float kTiny = 0x1p-126f;
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// A request's new tokens: the packed rows they are, the position of the first (below zero where there
+// are more of them than tokens altogether), and its keys.
+struct Request {
+  int start, count, first, keys;
+};
+__device__ __forceinline__ Request request_of(const ChunkAttentionArgs& a, int r) {
+  Request q;
+  const int s = a.starts[r], e = a.starts[r + 1], n = a.lengths[r];
+  q.start = min(max(s, 0), a.tokens);
+  q.count = max(min(e, a.tokens) - q.start, 0);
+  q.keys = min(max(n, 0), a.width * a.page_size);  // the host checks that it fits 31 bits
+  q.first = max(n, 0) - q.count;
+  return q;
+}
+__device__ __forceinline__ int tiles_of(const ChunkAttentionArgs& a, const Request& q) {
+  return (int)(((int64_t)q.count * a.group + kTile - 1) / kTile);
+}
+// The blocks of keys that tokens t0 .. t1 of a request see, the first one and how many.
+struct Blocks {
+  int first, count;
+};
+__device__ __forceinline__ Blocks blocks_of(const ChunkAttentionArgs& a, const Request& q, int t0,
+                                            int t1) {
+  const int hi = min(q.first + t1 + 1, q.keys);
+  const int lo = a.window ? max(q.first + t0 + 1 - a.window, 0) : 0;
+  Blocks b;
+  b.first = lo / kBlock;
+  b.count = hi > lo ? (hi + kBlock - 1) / kBlock - b.first : 0;
+  return b;
+}
+// Blocks of the tile of a request that has most, or somewhat more.
+__device__ __forceinline__ int most_blocks(const ChunkAttentionArgs& a, const Request& q) {
+  const int all = blocks_of(a, q, 0, q.count - 1).count;
+  if (!a.window) return all;
+  const int64_t tile = (int64_t)a.window + (kTile - 1) / a.group + 1;
+  return (int)min((int64_t)all, (tile + kBlock - 1) / kBlock + 1);
+}
+
+// The last request whose prefix is at most n (prefix[0] = 0, not decreasing): 64 at a time, by a
+// whole wave.
+__device__ __forceinline__ int find(const int32_t* prefix, int requests, int n) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  for (int count = requests; count > 1;) {
+    const int step = (count + 63) / 64;
+    const int at = lo + lane * step;
+    const bool ok = lane * step < count && prefix[at] <= n;
+    const int last = 63 - __clzll((long long)__ballot(ok));
+    lo = uniform(lo + last * step);
+    count = min(step, uniform(count) - last * step);
+  }
+  return lo;
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT == kBF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+}
+
+template <int DT>
+__device__ __forceinline__ u32x4 fp8_eight(u32x2 w) {
+  const uint32_t lo = w.x, hi = w.y;
+  if constexpr (DT == kBF16)
+    return (u32x4){
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)lo, 1.0f, true)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)hi, 1.0f, true))};
+  else
+    return (u32x4){
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, true)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true))};
+}
+
+// Two 16-bit floats, 0 in place of infinities and NaN; and whether there is any.
+template <int DT>
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
+  constexpr uint32_t kExponent = DT == kBF16 ? 0x7f80u : 0x7c00u;
+  if ((w & kExponent) == kExponent) w &= 0xffff0000u;
+  if ((w >> 16 & kExponent) == kExponent) w &= 0x0000ffffu;
+  return w;
+}
+
+// The larger of the two halves' values, in both.
+__device__ __forceinline__ float halves_max(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// Where chunk c (16 bytes) of row `row` lies in its row of CHUNKS: sixteen lanes that read one chunk
+// of sixteen rows (keys), and thirty-two that read four chunks of four rows (values), touch all banks.
+template <int CHUNKS>
+__device__ __forceinline__ int key_place(int c, int row) {
+  if constexpr (CHUNKS % 16 == 0) return c ^ (row & 15);
+  else if constexpr (CHUNKS % 8 == 0) return c ^ ((row >> 1) & 7);
+  else return c ^ ((row >> 2) & 3);
+}
+template <int CHUNKS>
+__device__ __forceinline__ int value_place(int c, int row) {
+  if constexpr (CHUNKS % 16 == 0) return c ^ ((row & 3) << 2);
+  else if constexpr (CHUNKS % 8 == 0) return c ^ ((row >> 1 & 1) << 2);
+  else return c;
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// DIM: the head's values or more, the rest as if zero.
+template <int DT, bool FP8, int DIM>
+__global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel(
+    ChunkAttentionArgs a) {
+  constexpr int kChunks = DIM / 8, kSteps = DIM / 16, kTiles = DIM / 32;
+  constexpr int kLoads = kChunks * kBlock / kThreads;  // of a thread, a side
+  constexpr int kStage = kBlock * DIM;                 // 16-bit values
+  // the narrowest head that is given to this DIM
+  constexpr int kLeastDim = DIM == 64 ? 16 : DIM == 96 ? 80 : DIM == 128 ? 112 : DIM == 192 ? 144 : 208;
+  // p = 2^(x - base) with base kShift below the largest x when it was set; it is set anew once x
+  // passes base + kRoom, so that most blocks need no rescaling. f16 probabilities are scaled up so that
+  // small ones stay above its smallest numbers: 2^15 at most.
+  constexpr float kShift = DT == kF16 ? 11.0f : 0.0f, kRoom = DT == kF16 ? 15.0f : 8.0f;
+
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][2][kStage];  // stage; keys, values
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int dim = a.dim;
+
+  // ---- rows that belong to no request ----
+  {
+    const int from = min(max(a.starts[a.requests], 0), a.tokens);
+    const int row_words = a.kv_heads * a.group * (dim / 8);
+    for (int row = from + (int)blockIdx.x; row < a.tokens; row += (int)gridDim.x) {
+      u32x4* to = reinterpret_cast<u32x4*>(a.out) + (int64_t)row * row_words;
+      for (int i = tid; i < row_words; i += kThreads) to[i] = (u32x4){0, 0, 0, 0};
+      if (a.lse)
+        for (int i = tid; i < a.kv_heads * a.group; i += kThreads)
+          a.lse[(int64_t)row * a.kv_heads * a.group + i] = -__builtin_inff();
+    }
+  }
+
+  // ---- this workgroup's item: a tile of a request, or a part of its keys, for one head ----
+  const int head = (int)(blockIdx.x % (unsigned)a.kv_heads);
+  const int item = (int)(blockIdx.x / (unsigned)a.kv_heads);
+  const int per = a.plan[0];
+  if (item >= a.plan[1]) return;
+  const int32_t* items = a.plan + kPlanHead;
+  const int32_t* part_items = items + a.requests + 1;
+  const int r = find(items, a.requests, item);
+  const Request q = request_of(a, r);
+  const int most = most_blocks(a, q);
+  const int splits = max((most + per - 1) / per, 1);
+  const int tiles = tiles_of(a, q);
+  const int in_request = item - items[r];
+  const int tile = tiles - 1 - in_request / splits;  // the longest first
+  const int split = in_request % splits;
+  if (tile < 0 || (splits > 1 && part_items[r] + in_request >= a.most_parts)) return;
+  const int row0 = tile * kTile, rows = min(kTile, q.count * a.group - row0);
+  const Blocks all = blocks_of(a, q, (int)div_by(row0, a.by_group),
+                               (int)div_by(row0 + rows - 1, a.by_group));
+  const int block0 = all.first + (int)((int64_t)all.count * split / splits);
+  const int block_end = all.first + (int)((int64_t)all.count * (split + 1) / splits);
+
+  // ---- this lane's row, and what the wave's rows see ----
+  const int wave_rows = min(rows - 32 * wave, 32);  // may be none
+  const int my_row = row0 + min(32 * wave + col, rows - 1);
+  const int my_token = (int)div_by(my_row, a.by_group);
+  const int my_head = head * a.group + (my_row - my_token * a.group);
+  const bool has_row = 32 * wave + col < rows;
+  const int my_end = min(q.first + my_token + 1, q.keys);  // keys below
+  const int my_begin = a.window ? max(q.first + my_token + 1 - a.window, 0) : 0;
+  // (rows are in order of their tokens, so the ends of lanes 0 and 31 bound the wave's; readlane of
+  // lanes whose row repeats the last one)
+  const int first_end = __builtin_amdgcn_readlane(my_end, 0);
+  const int last_end = __builtin_amdgcn_readlane(my_end, 31);
+  const int first_begin = __builtin_amdgcn_readlane(my_begin, 0);
+  const int last_begin = __builtin_amdgcn_readlane(my_begin, 31);
+
+  u32x4 query[kSteps];
+  {
+    const uint16_t* p = a.query + (int64_t)(q.start + my_token) * a.q_row_stride +
+                        (int64_t)my_head * a.q_head_stride;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int d = 16 * s + 8 * half;
+      query[s] = *reinterpret_cast<const u32x4*>(p + (d < dim ? d : 0));
+      query[s] ^= a.flip;
+      if (!has_row || d >= dim) query[s] = (u32x4){0, 0, 0, 0};
+    }
+  }
+
+  const int32_t* table = a.tables + (int64_t)r * a.table_stride;
+  const unsigned char* kbase = a.key + (int64_t)head * a.k_head;
+  const unsigned char* vbase = a.value + (int64_t)head * a.v_head;
+  const int last_key = max(q.keys - 1, 0);
+
+  // Where a block's tokens are: a lane a token looks up its entry; those that load the row ask for the
+  // offset. Tokens past the end stand for the last one, tokens on no page of the cache for page 0;
+  // both are masked.
+  auto look_up = [&](int block) {
+    const int token = min(block * kBlock + lane, last_key);
+    return table[div_by((uint32_t)token, a.by_page)];
+  };
+  auto page_ok = [&](int page) { return (uint32_t)page < (uint32_t)a.pages; };
+  auto offset_of = [&](int block, int page, uint32_t page_stride, uint32_t slot_stride) {
+    const uint32_t token = (uint32_t)min(block * kBlock + lane, last_key);
+    const uint32_t slot = token - div_by(token, a.by_page) * (uint32_t)a.page_size;
+    return (uint64_t)(page_ok(page) ? (uint32_t)page : 0u) * page_stride +
+           (uint64_t)slot * slot_stride;
+  };
+  auto of_row = [&](uint64_t offset, int row) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * row, (int)(uint32_t)offset);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * row, (int)(offset >> 32));
+    return (uint64_t)hi << 32 | lo;
+  };
+  // Chunk i of this thread: LDS chunk n of the stage is row n / kChunks, place n % kChunks.
+  u32x2 held8[FP8 ? 2 * kLoads : 1];
+  auto request_rows = [&](int stage, int block, int page) {
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const uint64_t offset = side ? offset_of(block, page, a.v_page, a.v_slot)
+                                   : offset_of(block, page, a.k_page, a.k_slot);
+      const unsigned char* base = side ? vbase : kbase;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int n = (wave * kLoads + i) * 64 + lane;
+        const int row = n / kChunks, place = n % kChunks;
+        const int c = side ? value_place<kChunks>(place, row) : key_place<kChunks>(place, row);
+        const unsigned char* from =
+            base + of_row(offset, row) + (8 * c < dim ? c * (FP8 ? 8 : 16) : 0);
+        if constexpr (FP8) {
+          held8[side * kLoads + i] = *reinterpret_cast<const u32x2*>(from);
+        } else {
+          __builtin_amdgcn_global_load_lds(
+              (const __attribute__((address_space(1))) void*)from,
+              (__attribute__((address_space(3))) void*)(&lds[stage][side][(wave * kLoads + i) * 512]),
+              16, 0, 0);
+        }
+      }
+    }
+  };
+  auto park_rows = [&](int stage) {
+    if constexpr (FP8) {
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          *reinterpret_cast<u32x4*>(&lds[stage][side][((wave * kLoads + i) * 64 + lane) * 8]) =
+              fp8_eight<DT>(held8[side * kLoads + i]);
+    }
+  };
+
+  float base = -__builtin_inff(), sum = 0.0f;
+  f32x16 acc[kTiles];
+  bool all_finite = true;
+again:
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+
+  int page = 0, next_page = 0;
+  if (block0 < block_end) {
+    page = look_up(block0);
+    request_rows(0, block0, page);
+    if (block0 + 1 < block_end) next_page = look_up(block0 + 1);
+    park_rows(0);
+  }
+  for (int block = block0; block < block_end; ++block) {
+    const int stage = (block - block0) & 1;
+    const bool more = block + 1 < block_end;
+    wait_vmcnt<0>();
+    __syncthreads();
+    const uint64_t on_page = __ballot(page_ok(page));
+    if (more) {
+      page = next_page;
+      request_rows(stage ^ 1, block + 1, page);
+      if (block + 2 < block_end) next_page = look_up(block + 2);
+    }
+    const int k0 = block * kBlock;
+    if (wave_rows > 0 && k0 < last_end && k0 + kBlock > first_begin) {
+      const uint16_t* keys = lds[stage][0];
+      const uint16_t* values = lds[stage][1];
+
+      // ---- scores: operand row i is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4 ----
+      f32x16 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = 32 * u + (col & 16) + ((col >> 2) & 1) * 8 + ((col >> 3) & 1) * 4 + (col & 3);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          if (16 * k >= kLeastDim && 16 * k >= dim) break;
+          const int c = 2 * k + half;
+          const u32x4 key = *reinterpret_cast<const u32x4*>(
+              keys + (row * kChunks + key_place<kChunks>(c, row)) * 8);
+          s[u] = mfma32<DT>(key, query[k], s[u]);
+        }
+      }
+
+      // ---- masks ----
+      const bool open = first_end >= k0 + kBlock && last_begin <= k0 && on_page == ~0ull;
+      if (!open) {
+        const int end = my_end - k0, begin = my_begin - k0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = 32 * u + 16 * (i / 8) + 8 * half + i % 8;
+            const bool ok = j < end && j >= begin && (on_page >> j & 1);
+            s[u][i] = ok ? s[u][i] : -__builtin_inff();
+          }
+      }
+
+      // ---- running reference and sum ----
+      float top = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+      top = halves_max(top) * a.scale_log2;
+      if (__any(top > base + kRoom)) {
+        const float next = fmaxf(base, top - kShift);
+        const float at = next == -__builtin_inff() ? 0.0f : next;
+        const float fix = fmaxf(__builtin_amdgcn_exp2f(base - at), kTiny);
+        sum *= fix;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[t][i] *= fix;
+        base = next;
+      }
+      const float zero_at = base == -__builtin_inff() ? 0.0f : base;
+      u32x4 p[4];
+      float sums[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], a.scale_log2, -zero_at));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], a.scale_log2, -zero_at));
+        sums[0] += p0;
+        sums[1] += p1;
+        p[i / 8][i % 8 / 2] = pack2<DT>(p0, p1);
+      }
+      sum += sums[0] + sums[1];
+
+      // ---- values that are not finite: their keys one by one, since products with the zeros of rows
+      // that do not see them would make no numbers ----
+      if (!all_finite) {
+        bool odd_row = false;
+#pragma unroll 1
+        for (int c = 0; c < kChunks; ++c) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(values + (lane * kChunks + c) * 8);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t x = w[j];
+            odd_row |= finite_pair<DT>(x) != x && (8 * value_place<kChunks>(c, lane) < dim);
+          }
+        }
+        uint64_t odd = __ballot(odd_row) & on_page;
+#pragma unroll 1
+        for (; odd; odd &= odd - 1) {
+          const int j = __ffsll((unsigned long long)odd) - 1;
+          const int reg = 16 * (j / 32) + 8 * (j / 16 % 2) + j % 8;
+          float x = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x = i == reg ? s[i / 16][i % 16] : x;
+          x = __shfl(x, col + 32 * (j / 8 % 2));
+          float w = __builtin_amdgcn_exp2f(fmaf(x, a.scale_log2, -zero_at));
+          w = w == 0.0f ? kTiny : w;  // below fp32's range, but not nothing
+          const bool seen = !(x == -__builtin_inff());
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const int d = 32 * t + 2 * i + 4 * half;
+              const u32x2 v = *reinterpret_cast<const u32x2*>(
+                  values + (j * kChunks + value_place<kChunks>(d / 8, j)) * 8 + (d & 7));
+              const uint32_t lo = v.x, hi = v.y;
+              const float f[4] = {lo16<DT>(lo), hi16<DT>(lo), lo16<DT>(hi), hi16<DT>(hi)};
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (seen && !(fabsf(f[e]) < __builtin_inff())) acc[t][i + e] += w * f[e];
+            }
+        }
+      }
+
+      // ---- values: 4 rows by 16 columns a group of 16 lanes, transposed on the way ----
+      const int in_group = lane & 15;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          u32x4 v;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = 16 * k + 8 * half + 4 * e + (in_group >> 2);
+            const int c = 4 * t + ((lane >> 4) & 1) * 2 + ((in_group & 3) >> 1);
+            const uint16_t* at = values + (row * kChunks + value_place<kChunks>(c, row)) * 8 +
+                                 4 * (in_group & 1);
+            const u32x2 w = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (__attribute__((address_space(3))) s16x4*)(at)));
+            v[2 * e] = w.x;
+            v[2 * e + 1] = w.y;
+          }
+          if (!all_finite) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t x = v[j];
+              v[j] = finite_pair<DT>(x);
+            }
+          }
+          acc[t] = mfma32<DT>(v, p[k], acc[t]);
+        }
+    }
+    if (more) park_rows(stage ^ 1);
+  }
+  // A value that is not finite may have met a zero of a row that does not see it: once more, with
+  // care (block by block; for rows that see it the result stays what it is).
+  if (all_finite) {
+    float odd = 0.0f;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) odd = fmaf(acc[t][i], 0.0f, odd);
+    if (__syncthreads_or(odd != 0.0f)) {
+      all_finite = false;
+      base = -__builtin_inff();
+      sum = 0.0f;
+      goto again;
+    }
+  }
+  sum = halves_sum(sum);
+
+  // ---- the result, or this part of it ----
+  if (wave_rows <= 0) return;
+  if (splits > 1) {
+    const int64_t part = (int64_t)(part_items[r] + in_request) * a.kv_heads + head;
+    float* to = a.parts + part * (kTile * (DIM + 2));
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) to[((wave * kTiles + t) * 16 + i) * 64 + lane] = acc[t][i];
+    if (half == 0) {
+      to[kTile * DIM + 32 * wave + col] = base;
+      to[kTile * (DIM + 1) + 32 * wave + col] = sum;
+    }
+    return;
+  }
+  if (!has_row) return;
+  const int64_t row = (int64_t)(q.start + my_token) * a.kv_heads * a.group + my_head;
+  const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = 32 * t + 2 * i + 4 * half;
+      if (d < dim)
+        *reinterpret_cast<u32x2*>(a.out + row * dim + d) =
+            (u32x2){pack2<DT>(acc[t][i] * inv, acc[t][i + 1] * inv),
+                    pack2<DT>(acc[t][i + 2] * inv, acc[t][i + 3] * inv)};
+    }
+  if (a.lse && half == 0)
+    a.lse[row] = sum == 0.0f ? -__builtin_inff()
+                             : (base + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+}
+
+// The parts of tiles whose keys were split, joined in order. Workgroup (part of one head, head, 32
+// dimensions); those of a tile's first part do it, a wave 32 rows, in the layout that they were stored.
+template <int DT, int DIM>
+__global__ __launch_bounds__(kThreads) void join_kernel(ChunkAttentionArgs a) {
+  constexpr int kTiles = DIM / 32, kPart = kTile * (DIM + 2), kBatch = 4;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int head = (int)(blockIdx.x % (unsigned)a.kv_heads);
+  const int part = (int)(blockIdx.x / (unsigned)a.kv_heads), t = blockIdx.y;
+  if (part >= a.plan[2]) return;
+  const int32_t* part_items = a.plan + kPlanHead + a.requests + 1;
+  const int r = find(part_items, a.requests, part);
+  const Request q = request_of(a, r);
+  const int splits = max((most_blocks(a, q) + a.plan[0] - 1) / a.plan[0], 1);
+  const int in_request = part - part_items[r];
+  if (in_request % splits || part + splits > a.most_parts) return;
+  const int tile = tiles_of(a, q) - 1 - in_request / splits;
+  if (tile < 0) return;
+  const int row0 = tile * kTile, rows = min(kTile, q.count * a.group - row0);
+  if (32 * wave >= rows) return;
+  const float* from = a.parts + ((int64_t)part * a.kv_heads + head) * kPart;
+  const int64_t step = (int64_t)a.kv_heads * kPart;
+
+  float base = -__builtin_inff(), sum = 0.0f;
+  float acc[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+  for (int n0 = 0; n0 < splits; n0 += kBatch) {
+    float b[kBatch], l[kBatch], v[kBatch][16];
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n) {
+      const float* p = from + min(n0 + n, splits - 1) * step;
+      b[n] = p[kTile * DIM + 32 * wave + col];
+      l[n] = p[kTile * (DIM + 1) + 32 * wave + col];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[n][i] = p[((wave * kTiles + t) * 16 + i) * 64 + lane];
+    }
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n) {
+      if (n0 + n >= splits || b[n] == -__builtin_inff()) continue;
+      const float next = fmaxf(base, b[n]);
+      const float old = fmaxf(__builtin_amdgcn_exp2f(base - next), kTiny);
+      const float now = fmaxf(__builtin_amdgcn_exp2f(b[n] - next), kTiny);
+      sum = sum * old + l[n] * now;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[i] = acc[i] * old + v[n][i] * now;
+      base = next;
+    }
+  }
+  if (32 * wave + col >= rows) return;
+  const int my_row = row0 + 32 * wave + col;
+  const int token = (int)div_by(my_row, a.by_group);
+  const int64_t row = (int64_t)(q.start + token) * a.kv_heads * a.group + head * a.group +
+                      (my_row - token * a.group);
+  const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const int d = 32 * t + 2 * i + 4 * half;
+    if (d < a.dim)
+      *reinterpret_cast<u32x2*>(a.out + row * a.dim + d) =
+          (u32x2){pack2<DT>(acc[i] * inv, acc[i + 1] * inv),
+                  pack2<DT>(acc[i + 2] * inv, acc[i + 3] * inv)};
+  }
+  if (a.lse && half == 0 && t == 0)
+    a.lse[row] = sum == 0.0f ? -__builtin_inff()
+                             : (base + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+}
+
+template <int DT, bool FP8, int DIM>
+hipError_t launch_dim(const ChunkAttentionArgs& a, hipStream_t stream) {
+  const unsigned items = (unsigned)(a.most_tiles + a.target) * (unsigned)a.kv_heads;
+  attention_kernel<DT, FP8, DIM><<<items, kThreads, 0, stream>>>(a);
+  if (a.most_parts > 0)
+    join_kernel<DT, DIM><<<dim3((unsigned)a.most_parts * (unsigned)a.kv_heads, DIM / 32), kThreads,
+                           0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <int DT, bool FP8>
+hipError_t launch_type(const ChunkAttentionArgs& a, hipStream_t stream) {
+  if (a.dim <= 64) return launch_dim<DT, FP8, 64>(a, stream);
+  if (a.dim <= 96) return launch_dim<DT, FP8, 96>(a, stream);
+  if (a.dim <= 128) return launch_dim<DT, FP8, 128>(a, stream);
+  if (a.dim <= 192) return launch_dim<DT, FP8, 192>(a, stream);
+  return launch_dim<DT, FP8, 256>(a, stream);
+}
+
+hipError_t launch_bf16(const ChunkAttentionArgs& a, hipStream_t stream);
+hipError_t launch_f16(const ChunkAttentionArgs& a, hipStream_t stream);
+hipError_t launch_bf16_fp8(const ChunkAttentionArgs& a, hipStream_t stream);
+hipError_t launch_f16_fp8(const ChunkAttentionArgs& a, hipStream_t stream);
+
+}  // namespace chunk
+}  // namespace mt

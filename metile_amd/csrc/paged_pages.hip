@@ -1,0 +1,435 @@
+// What is done to whole pages of a paged cache: copies, forks of requests, freeing and compaction.
+//
+// Which pages are in use is read from the block tables each time: a page is if any request has it
+// among its tokens' pages. So there are no counts of references to keep, a page that requests share is
+// freed with the last of them, and calls may come in any order. Marks are bytes, set by plain
+// stores of the same value, so that no result goes by the order of threads; lists are made by prefix
+// sums over the pages, in ascending order.
+#include <algorithm>
+
+#include "common.h"
+#include "paged_pages.h"
+
+namespace mt {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
+// ---- copies ----------------------------------------------------------------------------------------
+
+constexpr int kUnroll = 4;
+
+struct CopyMagic {
+  DivMagic units, run, n1;
+};
+
+// Memory bounds it. A thread moves four 16-byte units, a workgroup's next to each other.
+__global__ __launch_bounds__(kThreads) void copy_kernel(PagedCopyArgs a, CopyMagic even, CopyMagic odd,
+                                                         uint32_t units, uint32_t total) {
+  const bool is_odd = blockIdx.y & 1;
+  const PageShape& s = a.shape[is_odd];
+  const CopyMagic magic = is_odd ? odd : even;
+  unsigned char* base = a.side[blockIdx.y];
+  const uint32_t step = gridDim.x * (kThreads * kUnroll);
+  for (uint32_t first = blockIdx.x * (kThreads * kUnroll) + threadIdx.x; first < total;) {
+    u32x4 v[kUnroll];
+    unsigned char* to[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const uint32_t n = min(first + i * kThreads, total - 1);
+      const uint32_t pair = div_by(n, magic.units), u = n - pair * units;
+      const int32_t source = a.sources[pair], target = a.targets[pair];
+      const bool here = first + i * kThreads < total && (uint32_t)source < (uint32_t)a.pages &&
+                        (uint32_t)target < (uint32_t)a.pages;
+      const uint32_t t = div_by(u, magic.run), i0 = div_by(t, magic.n1);
+      const int64_t at = (int64_t)(u - t * s.run) * 16 + (int64_t)(t - i0 * s.n1) * s.s1 +
+                         (int64_t)i0 * s.s0;
+      to[i] = here ? base + (int64_t)target * s.page + at : nullptr;
+      if (here) v[i] = *reinterpret_cast<const u32x4*>(base + (int64_t)source * s.page + at);
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i)
+      if (to[i]) *reinterpret_cast<u32x4*>(to[i]) = v[i];
+    if (total - first <= step) break;
+    first += step;
+  }
+}
+
+// ---- forks -----------------------------------------------------------------------------------------
+
+__device__ __forceinline__ int block_sum(int v, int* lds) {
+  for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) v += lds[w];
+  __syncthreads();
+  return v;
+}
+
+struct Fork {
+  int source, target, tokens;  // source -1: left out
+};
+__device__ __forceinline__ Fork fork_of(const PagedForkArgs& a, int i) {
+  Fork f{a.sources[i], a.targets[i], 0};
+  if ((uint32_t)f.source >= (uint32_t)a.requests || (uint32_t)f.target >= (uint32_t)a.requests) {
+    f.source = -1;
+    return f;
+  }
+  const int most = a.width * a.page_size;  // the host checks that it fits 31 bits
+  f.tokens = min(max(a.lengths[f.source], 0), most);
+  if (a.tokens) f.tokens = min(f.tokens, max(a.tokens[i], 0));
+  return f;
+}
+
+__global__ void zero_int_kernel(int32_t* to) { *to = 0; }
+
+// A workgroup a fork. Each counts the forks before its own that take a page.
+__global__ __launch_bounds__(kThreads) void fork_kernel(PagedForkArgs a, DivMagic by_page) {
+  __shared__ int lds[kWaves];
+  const int i = blockIdx.x, tid = threadIdx.x;
+  const bool last = i == a.forks - 1;
+  auto begun = [&](const Fork& f) {
+    return f.tokens - (int)div_by(f.tokens, by_page) * a.page_size;
+  };
+  int before = 0;
+  for (int j = tid; j < i; j += kThreads) before += begun(fork_of(a, j)) > 0;
+  before = block_sum(before, lds);
+  const Fork f = fork_of(a, i);
+  const int full = (int)div_by(f.tokens, by_page);
+  const bool partial = begun(f) > 0;
+  if (last && tid == 0) *a.taken = before + partial;
+  int32_t fresh = -1, old = -1;
+  if (partial) {
+    const int64_t n = (a.free_start ? (int64_t)*a.free_start : 0) + before;
+    if (n >= 0 && n < a.free_count) fresh = a.free_pages[n];
+    if (fresh >= 0) old = a.tables[(int64_t)f.source * a.table_stride + full];
+  }
+  if (tid == 0) {
+    a.from[i] = old;
+    a.to[i] = fresh;
+  }
+  if (f.source < 0) return;
+  const int32_t* from = a.tables + (int64_t)f.source * a.table_stride;
+  int32_t* to = a.tables + (int64_t)f.target * a.table_stride;
+  for (int c = tid; c < full; c += kThreads) to[c] = from[c];
+  if (tid == 0) {
+    if (partial) to[full] = fresh;
+    a.lengths[f.target] = f.tokens;
+  }
+}
+
+// ---- marks -----------------------------------------------------------------------------------------
+
+constexpr int kScan = 16;                       // pages of a thread
+constexpr int kScanBlock = kThreads * kScan;    // of a workgroup
+
+__host__ __device__ inline int scan_blocks(int pages) {
+  return (int)(((int64_t)pages + kScanBlock - 1) / kScanBlock);
+}
+size_t padded(int pages) { return (size_t)scan_blocks(pages) * kScanBlock; }
+
+__global__ __launch_bounds__(kThreads) void fill_kernel(u32x4* to, int64_t count) {
+  const int64_t step = (int64_t)gridDim.x * kThreads;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += step)
+    to[i] = (u32x4){0, 0, 0, 0};
+}
+
+__device__ __forceinline__ int columns_of(int tokens, DivMagic by_page, int page_size, int width) {
+  const int n = max(tokens, 0), c = (int)div_by(n, by_page);
+  return min(c + (c * page_size != n), width);
+}
+
+// A wave a row of a block table, several side by side for long ones.
+constexpr int kRowPiece = 1024;  // entries
+
+__global__ __launch_bounds__(kThreads) void mark_free_kernel(PagedFreeArgs a, DivMagic by_page,
+                                                              unsigned char* keeps,
+                                                              unsigned char* drops) {
+  const int r = blockIdx.x * kWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= a.requests) return;
+  const int length = a.lengths[r], kept = min(a.kept[r], length);
+  const int used = columns_of(length, by_page, a.page_size, a.width);
+  const int keep = columns_of(kept, by_page, a.page_size, a.width);
+  const int32_t* row = a.tables + (int64_t)r * a.table_stride;
+  for (int c0 = (int)blockIdx.y * kRowPiece; c0 < used; c0 += (int)gridDim.y * kRowPiece)
+    for (int c = c0 + lane; c < min(c0 + kRowPiece, used); c += 64) {
+      const int32_t p = row[c];
+      if ((uint32_t)p < (uint32_t)a.pages) (c < keep ? keeps : drops)[p] = 1;
+    }
+}
+
+// A thread's marks, 16 pages as bytes.
+__device__ __forceinline__ u32x4 marks_of(const unsigned char* marks, int64_t first) {
+  return *reinterpret_cast<const u32x4*>(marks + first);
+}
+__device__ __forceinline__ int count_of(u32x4 v) {  // bytes are 0 or 1
+  return __popc(v.x) + __popc(v.y) + __popc(v.z) + __popc(v.w);
+}
+
+// Exclusive sums over a workgroup's threads of up to two counts, and their totals.
+struct Pair {
+  int a, b;
+};
+__device__ __forceinline__ Pair scan_pair(Pair v, Pair* total, Pair (*lds)) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Pair s = v;
+  for (int d = 1; d < 64; d *= 2) {
+    const int x = __shfl_up(s.a, d), y = __shfl_up(s.b, d);
+    if (lane >= d) s.a += x, s.b += y;
+  }
+  if (lane == 63) lds[wave] = s;
+  __syncthreads();
+  Pair before{0, 0}, all{0, 0};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before.a += lds[w].a, before.b += lds[w].b;
+    all.a += lds[w].a, all.b += lds[w].b;
+  }
+  __syncthreads();
+  *total = all;
+  return {before.a + s.a - v.a, before.b + s.b - v.b};
+}
+// Sums of the blocks' counts before this one, and of all.
+__device__ __forceinline__ Pair blocks_before(const Pair* counts, int blocks, Pair* total, Pair* lds) {
+  Pair before{0, 0}, all{0, 0};
+  for (int i = threadIdx.x; i < blocks; i += kThreads) {
+    const Pair c = counts[i];
+    all.a += c.a, all.b += c.b;
+    if (i < (int)blockIdx.x) before.a += c.a, before.b += c.b;
+  }
+  int* words = reinterpret_cast<int*>(lds);
+  before.a = block_sum(before.a, words);
+  before.b = block_sum(before.b, words);
+  total->a = block_sum(all.a, words);
+  total->b = block_sum(all.b, words);
+  return before;
+}
+
+// Marks of pages to list: `a` those of `first` without those of `second`.
+__device__ __forceinline__ u32x4 without(u32x4 first, u32x4 second) { return first & ~second; }
+
+__global__ __launch_bounds__(kThreads) void count_free_kernel(const unsigned char* keeps,
+                                                               const unsigned char* drops,
+                                                               Pair* counts) {
+  __shared__ int lds[kWaves];
+  const int64_t first = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kScan;
+  const int n = block_sum(count_of(without(marks_of(drops, first), marks_of(keeps, first))), lds);
+  if (threadIdx.x == 0) counts[blockIdx.x] = {n, 0};
+}
+
+__global__ __launch_bounds__(kThreads) void list_free_kernel(PagedFreeArgs a,
+                                                              const unsigned char* keeps,
+                                                              const unsigned char* drops,
+                                                              const Pair* counts) {
+  __shared__ Pair lds[kWaves];
+  Pair total, in_block;
+  const Pair before = blocks_before(counts, gridDim.x, &total, lds);
+  const int64_t first = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kScan;
+  const u32x4 marks = without(marks_of(drops, first), marks_of(keeps, first));
+  const Pair mine = scan_pair({count_of(marks), 0}, &in_block, lds);
+  int64_t at = (int64_t)*a.free_start - total.a + before.a + mine.a;
+#pragma unroll
+  for (int i = 0; i < kScan; ++i) {
+    const uint32_t word = marks[i / 4];
+    if (word >> (8 * (i % 4)) & 1) {
+      if (at >= 0 && at < a.free_count) a.free_pages[at] = (int32_t)(first + i);
+      ++at;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.freed = total.a;
+}
+
+// ---- compaction ------------------------------------------------------------------------------------
+
+// No moves yet, and the free list up to its start.
+__global__ __launch_bounds__(kThreads) void begin_compact_kernel(PagedCompactArgs a, u32x4* marks,
+                                                                  int64_t mark_count) {
+  const int64_t step = (int64_t)gridDim.x * kThreads;
+  const int64_t first = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  for (int64_t i = first; i < mark_count; i += step) marks[i] = (u32x4){0, 0, 0, 0};
+  for (int64_t i = first; i < a.most_moves; i += step) a.sources[i] = a.targets[i] = -1;
+  const int start = *a.free_start;
+  for (int64_t i = first; i < a.free_count; i += step) a.new_free[i] = i < start ? a.free_pages[i] : -1;
+}
+
+__global__ __launch_bounds__(kThreads) void mark_compact_kernel(PagedCompactArgs a, DivMagic by_page,
+                                                                 int row_blocks, unsigned char* used,
+                                                                 unsigned char* open) {
+  const int lane = threadIdx.x & 63;
+  if ((int)blockIdx.x >= row_blocks) {  // the free list
+    const int64_t step = (int64_t)(gridDim.x - row_blocks) * gridDim.y * kThreads;
+    const int64_t start = max(*a.free_start, 0);
+    for (int64_t i = start + ((int64_t)(blockIdx.x - row_blocks) * gridDim.y + blockIdx.y) * kThreads +
+                     threadIdx.x;
+         i < a.free_count; i += step) {
+      const int32_t p = a.free_pages[i];
+      if ((uint32_t)p < (uint32_t)a.pages) open[p] = 1;
+    }
+    return;
+  }
+  const int r = blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (r >= a.requests) return;
+  const int columns = columns_of(a.lengths[r], by_page, a.page_size, a.width);
+  const int32_t* row = a.tables + (int64_t)r * a.table_stride;
+  for (int c0 = (int)blockIdx.y * kRowPiece; c0 < columns; c0 += (int)gridDim.y * kRowPiece)
+    for (int c = c0 + lane; c < min(c0 + kRowPiece, columns); c += 64) {
+      const int32_t p = row[c];
+      if ((uint32_t)p < (uint32_t)a.pages) used[p] = 1;
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void count_compact_kernel(const unsigned char* used,
+                                                                  const unsigned char* open,
+                                                                  Pair* counts) {
+  __shared__ int lds[kWaves];
+  const int64_t first = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kScan;
+  const u32x4 u = marks_of(used, first);
+  const int n = block_sum(count_of(u), lds);
+  const int m = block_sum(count_of(without(marks_of(open, first), u)), lds);
+  if (threadIdx.x == 0) counts[blockIdx.x] = {n, m};
+}
+
+// With U pages in use, those in use beyond the U lowest of all (in use or free) move, the highest to
+// the lowest free page, and so on; `number` says of each page where in the list of moves it is.
+__global__ __launch_bounds__(kThreads) void list_compact_kernel(PagedCompactArgs a,
+                                                                 const unsigned char* used,
+                                                                 const unsigned char* open,
+                                                                 const Pair* counts,
+                                                                 int32_t* number) {
+  __shared__ Pair lds[kWaves];
+  Pair total, in_block;
+  const Pair before = blocks_before(counts, gridDim.x, &total, lds);
+  const int64_t first = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kScan;
+  const u32x4 u = marks_of(used, first), o = without(marks_of(open, first), u);
+  const Pair mine = scan_pair({count_of(u), count_of(o)}, &in_block, lds);
+  int used_before = before.a + mine.a, open_before = before.b + mine.b;
+  const int in_use = total.a, start = max(*a.free_start, 0);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && in_use == 0) *a.moves = 0;
+#pragma unroll
+  for (int i = 0; i < kScan; ++i) {
+    const int32_t page = (int32_t)(first + i);
+    const uint32_t uw = u[i / 4], ow = o[i / 4];
+    const bool is_used = uw >> (8 * (i % 4)) & 1, is_open = ow >> (8 * (i % 4)) & 1;
+    const int rank = used_before + open_before;
+    const bool low = rank < in_use;
+    if (is_used || is_open) {
+      // (moves: as many as there are free pages among the lowest)
+      if (rank == in_use - 1) *a.moves = open_before + is_open;
+      const int move = is_used ? in_use - 1 - used_before : open_before;
+      if (is_used) number[page] = low ? -1 : move;
+      if (is_used && !low && move < a.most_moves) a.sources[move] = page;
+      if (is_open && low && move < a.most_moves) a.targets[move] = page;
+      if (!low && (int64_t)start + rank - in_use < a.free_count)
+        a.new_free[start + rank - in_use] = page;
+      if (is_used) ++used_before;
+      else ++open_before;
+    }
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void apply_compact_kernel(PagedCompactArgs a, DivMagic by_page,
+                                                                  const int32_t* number) {
+  const int r = blockIdx.x * kWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= a.requests) return;
+  const int columns = columns_of(a.lengths[r], by_page, a.page_size, a.width);
+  const int32_t* row = a.tables + (int64_t)r * a.table_stride;
+  int32_t* to = a.new_tables + (int64_t)r * a.width;
+  for (int c0 = (int)blockIdx.y * kRowPiece; c0 < a.width; c0 += (int)gridDim.y * kRowPiece)
+    for (int c = c0 + lane; c < min(c0 + kRowPiece, a.width); c += 64) {
+      int32_t p = row[c];
+      if (c < columns && (uint32_t)p < (uint32_t)a.pages) {
+        const int move = number[p];
+        if (move >= 0) p = a.targets[move];
+      }
+      to[c] = p;
+    }
+}
+
+dim3 row_grid(int requests, int width) {
+  const int rows = (requests + kWaves - 1) / kWaves;
+  const int pieces = (int)(((int64_t)width + kRowPiece - 1) / kRowPiece);
+  return dim3(rows, std::max(1, std::min({pieces, 64, (1 << 20) / std::max(rows, 1)})));
+}
+unsigned fill_grid(int64_t vectors) {
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(1024, (vectors + kThreads - 1) / kThreads));
+}
+
+}  // namespace
+
+hipError_t launch_paged_copy(const PagedCopyArgs& args, int sides, int cus, hipStream_t stream) {
+  const uint32_t units = args.shape[0].run * args.shape[0].n1 * args.shape[0].n0;
+  CopyMagic magic[2];
+  for (int i = 0; i < 2; ++i)
+    magic[i] = {div_magic(units), div_magic(args.shape[i].run), div_magic(args.shape[i].n1)};
+  // pairs of a launch, so that units are counted in 31 bits
+  const int64_t most = std::max<int64_t>(1, 0x7fffffffll / units);
+  for (int64_t at = 0; at < args.count; at += most) {
+    PagedCopyArgs a = args;
+    a.sources += at;
+    a.targets += at;
+    const uint32_t total = (uint32_t)std::min(most, args.count - at) * units;
+    const uint32_t blocks = (total + kThreads * kUnroll - 1) / (kThreads * kUnroll);
+    const uint32_t grid = std::min<uint32_t>(blocks, std::max(1, 32 * cus / sides));
+    copy_kernel<<<dim3(grid, sides), kThreads, 0, stream>>>(a, magic[0], magic[1], units, total);
+    if (const hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_zero_int(int32_t* to, hipStream_t stream) {
+  zero_int_kernel<<<1, 1, 0, stream>>>(to);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_fork(const PagedForkArgs& a, hipStream_t stream) {
+  fork_kernel<<<a.forks, kThreads, 0, stream>>>(a, div_magic((uint32_t)a.page_size));
+  return hipGetLastError();
+}
+
+// Marks of the pages that are kept and that are dropped, then the blocks' counts.
+size_t paged_free_work(int pages) {
+  return 2 * padded(pages) + (size_t)scan_blocks(pages) * sizeof(Pair);
+}
+
+hipError_t launch_paged_free(const PagedFreeArgs& a, hipStream_t stream) {
+  const DivMagic by_page = div_magic((uint32_t)a.page_size);
+  const size_t marks = padded(a.pages);
+  unsigned char *keeps = a.work, *drops = a.work + marks;
+  Pair* counts = reinterpret_cast<Pair*>(a.work + 2 * marks);
+  fill_kernel<<<fill_grid(marks / 8), kThreads, 0, stream>>>(reinterpret_cast<u32x4*>(a.work),
+                                                             (int64_t)marks / 8);
+  if (a.requests)
+    mark_free_kernel<<<row_grid(a.requests, a.width), kThreads, 0, stream>>>(a, by_page, keeps, drops);
+  count_free_kernel<<<scan_blocks(a.pages), kThreads, 0, stream>>>(keeps, drops, counts);
+  list_free_kernel<<<scan_blocks(a.pages), kThreads, 0, stream>>>(a, keeps, drops, counts);
+  return hipGetLastError();
+}
+
+// Marks of the pages in use and of the free ones, the blocks' counts, then each page's move.
+size_t paged_compact_work(int pages) {
+  return 2 * padded(pages) + (size_t)scan_blocks(pages) * sizeof(Pair) + padded(pages) * 4;
+}
+
+hipError_t launch_paged_compact(const PagedCompactArgs& a, hipStream_t stream) {
+  const DivMagic by_page = div_magic((uint32_t)a.page_size);
+  const size_t marks = padded(a.pages);
+  unsigned char *used = a.work, *open = a.work + marks;
+  int32_t* number = reinterpret_cast<int32_t*>(a.work + 2 * marks);
+  Pair* counts = reinterpret_cast<Pair*>(number + marks);
+  const int64_t most = std::max<int64_t>({(int64_t)marks / 8, a.most_moves, a.free_count});
+  begin_compact_kernel<<<fill_grid(most), kThreads, 0, stream>>>(
+      a, reinterpret_cast<u32x4*>(a.work), (int64_t)marks / 8);
+  const dim3 rows = row_grid(a.requests, a.width);
+  const int list = (int)std::max<int64_t>(1, std::min<int64_t>(256, a.free_count / 4096));
+  mark_compact_kernel<<<dim3(rows.x + list, rows.y), kThreads, 0, stream>>>(a, by_page, rows.x, used,
+                                                                            open);
+  count_compact_kernel<<<scan_blocks(a.pages), kThreads, 0, stream>>>(used, open, counts);
+  list_compact_kernel<<<scan_blocks(a.pages), kThreads, 0, stream>>>(a, used, open, counts, number);
+  if (a.requests)
+    apply_compact_kernel<<<rows, kThreads, 0, stream>>>(a, by_page, number);
+  return hipGetLastError();
+}
+
+}  // namespace mt

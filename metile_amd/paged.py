@@ -1,4 +1,4 @@
-"""The paged key-value cache of a decode step (gfx950 HIP kernels via the C ABI).
+"""The paged key-value cache of a served decoder (gfx950 HIP kernels via the C ABI).
 
 A cache is a pool of pages of ``page_size`` tokens; each request has a row of a block table with
 the numbers of its pages, in order. One step of a serving loop:
@@ -6,7 +6,12 @@ the numbers of its pages, in order. One step of a serving loop:
 * :func:`paged_tables` turns the requests' lengths into the pages they need on top, block-table
   entries and the slot of every new token, on the GPU;
 * :func:`paged_append` writes the step's keys and values to their slots;
-* :func:`paged_attention` attends from one new token of each request over its pages.
+* :func:`paged_attention` attends from one new token of each request over its pages,
+  :func:`paged_chunk_attention` from several (a prompt, a part of one, a draft).
+
+Between steps, :func:`paged_fork` lets requests go on from another's tokens, :func:`paged_free` gives
+pages back and :func:`paged_compact` brings those in use together, with :func:`paged_copy` for what the
+pages hold. Which pages are in use the block tables say: there are no counts to keep.
 
 The reference has no counterparts: its decode loop leaves cache and attention to MLX.
 """
@@ -14,6 +19,7 @@ The reference has no counterparts: its decode loop leaves cache and attention to
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
@@ -109,7 +115,7 @@ class PagedCache:
             key.data_ptr(), value.data_ptr(), (ctypes.c_int64 * 3)(*strides[0]),
             (ctypes.c_int64 * 3)(*strides[1]), pages, page_size, heads, dim,
             _CACHE_DTYPES[key.dtype], self.key_scale, self.value_scale)
-        self._ref = ctypes.byref(self._desc)
+        self._ref, self._address = ctypes.byref(self._desc), ctypes.addressof(self._desc)
         self._device, self._dtype, self._head_shape = key.device, key.dtype, key.shape[2:]
         self._workspaces = {}  # (requests, heads, width, window) -> bytes
 
@@ -292,3 +298,253 @@ def _attend(cache, args, requests, heads, width, window):
     status = _lib.lib().mt_paged_attention(cache._ref, args, ws.data_ptr(), ws.numel(), stream)
     if status:
         _lib.check(status)
+
+
+def _scratch(device, nbytes):
+    """Memory for one call, from torch's allocator: a captured call's belongs to its graph."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def paged_chunk_attention(query, cache, block_tables, lengths, starts, *, scale=None, window=None,
+                          return_lse=False):
+    """Attention of a chunk of new tokens of each request over its pages of ``cache``: prompts, parts of
+    them, drafts to verify.
+
+    ``query`` ``[tokens, heads, head_dim]`` (bfloat16 or float16; ``heads`` a multiple of the cache's) is
+    a packed batch: request ``r``'s new tokens are rows ``starts[r]`` to ``starts[r + 1] - 1`` (int32
+    ``[requests + 1]``, beginning with 0) and the last of its ``lengths[r]`` tokens in the cache (int32
+    ``[requests]``), as :func:`paged_tables` gives both. Each attends to its request's tokens up to
+    itself, with ``window`` to the last so many of them only; what later tokens hold does not matter to
+    it. ``block_tables`` and ``scale`` are as in :func:`paged_attention`. Returns the output in
+    ``query``'s shape and dtype and, with ``return_lse``, the log of the sum of exponentials (float32
+    ``[tokens, heads]``). Rows that belong to no request give zeros and -inf.
+    """
+    dtype = query.dtype
+    if dtype not in _DTYPES:
+        raise ValueError("queries must be bfloat16 or float16")
+    if cache._dtype != dtype and cache._dtype != torch.float8_e4m3fn:
+        raise ValueError("a 16-bit cache must have the queries' dtype")
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim:
+        raise ValueError("queries must be [tokens, heads, head_dim] of the cache's head_dim")
+    tokens, heads, dim = shape
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError("query heads must be a positive multiple of the cache's heads")
+    _int32(block_tables, "block_tables", 2)
+    _int32(lengths, "lengths")
+    _int32(starts, "starts")
+    requests, width = block_tables.shape
+    if lengths.shape[0] != requests or starts.shape[0] != requests + 1:
+        raise ValueError("block_tables, lengths and starts (one more) must describe the same requests")
+    if window is None:
+        window = 0
+    elif window < 1:
+        raise ValueError("window must be positive")
+    else:
+        window = min(window, (1 << 31) - 1)
+    device = cache._device
+    _same_device(device, query, block_tables, lengths, starts)
+    out = (torch.empty_like(query) if query.is_contiguous()
+           else torch.empty(shape, dtype=dtype, device=device))
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    if not requests or not width or not tokens:
+        out.zero_()
+        if lse is not None:
+            lse.fill_(-float("inf"))
+        return (out, lse) if return_lse else out
+    query, row, head = _rows16(query)
+    if width > 1 and block_tables.stride(1) != 1:
+        block_tables = block_tables.contiguous()
+    lengths, starts = lengths.contiguous(), starts.contiguous()
+    args = _lib.PAGED_CHUNK_ATTENTION_ARGS.pack(
+        query.data_ptr(), row, head, block_tables.data_ptr(), block_tables.stride(0),
+        lengths.data_ptr(), starts.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        tokens, requests, heads, width, window, dim ** -0.5 if scale is None else scale,
+        _DTYPES[dtype])
+    lib = _lib.lib()
+
+    def call(stream):
+        need = lib.mt_paged_chunk_attention_workspace_bytes(cache._ref, tokens, requests, heads, width,
+                                                            window)
+        ws = _scratch(device, need)
+        return lib.mt_paged_chunk_attention(cache._ref, args, ws.data_ptr(), need, stream)
+
+    _launch(device, call)
+    return (out, lse) if return_lse else out
+
+
+def paged_copy(caches, sources, targets):
+    """Copy pages ``sources[i]`` to ``targets[i]`` (int32 vectors), keys and values, in ``caches`` (one
+    :class:`PagedCache`, or those of all layers that a block table serves). Pairs with a number that is
+    no page of the cache (-1) are left out. Targets must be distinct, and none of them a source."""
+    if isinstance(caches, PagedCache):
+        caches = (caches,)
+    _int32(sources, "sources")
+    _int32(targets, "targets")
+    if sources.shape != targets.shape:
+        raise ValueError("sources and targets must be pairs of pages")
+    if not caches or not sources.shape[0]:
+        return
+    device = caches[0]._device
+    for cache in caches:
+        if cache._device != device:
+            raise ValueError("caches must be on one ROCm device")
+    _same_device(device, sources, targets)
+    sources, targets = sources.contiguous(), targets.contiguous()
+    _launch(device, _lib.lib().mt_paged_copy,
+            struct.pack(f"@{len(caches)}P", *[cache._address for cache in caches]), len(caches),
+            _lib.PAGED_COPY_ARGS.pack(sources.data_ptr(), targets.data_ptr(), sources.shape[0]))
+
+
+class PagedFork(NamedTuple):
+    """What :func:`paged_fork` gives: the pages to copy, ``sources`` to ``targets`` (int32 ``[forks]``, -1
+    where nothing is), and ``taken`` (``[1]``), the pages that the forks needed."""
+
+    sources: torch.Tensor
+    targets: torch.Tensor
+    taken: torch.Tensor
+
+
+def _check_tables(block_tables, page_size):
+    _int32(block_tables, "block_tables", 2)
+    if block_tables.shape[1] == 0:
+        raise ValueError("block_tables must have at least one column")
+    if block_tables.shape[1] > 1 and block_tables.stride(1) != 1:
+        raise ValueError("block_tables must have contiguous rows")
+    if not 0 < page_size < 1 << 31:
+        raise ValueError("page_size must be positive, and below 2^31")
+
+
+def _one_int32(t, what):
+    if t.dtype != torch.int32 or t.numel() != 1:
+        raise ValueError(f"{what} must be an int32 tensor of one element")
+
+
+def _in_place(t, what):
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous: it is changed in place")
+    return t
+
+
+def paged_fork(block_tables, lengths, sources, targets, free_pages, *, page_size, free_start=None,
+               tokens=None):
+    """Let requests ``targets[i]`` go on from the tokens of requests ``sources[i]`` (int32 vectors of rows
+    of ``block_tables``), or the first ``tokens[i]`` (int32) of them.
+
+    Pages that these tokens fill are shared between the requests: nothing writes to them again. One that
+    has been begun is the target's own, taken from ``free_pages`` as :func:`paged_tables` does;
+    ``paged_copy(caches, fork.sources, fork.targets)`` copies what it holds. The targets' rows of
+    ``block_tables`` and their ``lengths`` are set in place; entries behind the last page stay as they
+    were. Where the list is exhausted the begun page is -1, and ``taken`` is more than the list holds.
+    Forks of or onto rows that there are not (-1) are left out. A request may be forked any number of
+    times at once; targets must be distinct, and none of them a source. Pages of a target's former
+    tokens are not freed: :func:`paged_free` does that. Returns a :class:`PagedFork`.
+    """
+    device = block_tables.device
+    _same_device(device, lengths, sources, targets, free_pages, free_start, tokens)
+    _check_tables(block_tables, page_size)
+    _in_place(_int32(lengths, "lengths"), "lengths")
+    free_pages = _int32(free_pages, "free_pages").contiguous()
+    sources = _int32(sources, "sources").contiguous()
+    targets = _int32(targets, "targets").contiguous()
+    requests, width = block_tables.shape
+    forks = sources.shape[0]
+    if lengths.shape[0] != requests:
+        raise ValueError("lengths and block_tables must describe the same requests")
+    if targets.shape[0] != forks or (tokens is not None and
+                                     _int32(tokens, "tokens").shape[0] != forks):
+        raise ValueError("sources, targets and tokens must describe the same forks")
+    if tokens is not None:
+        tokens = tokens.contiguous()
+    if free_start is not None:
+        _one_int32(free_start, "free_start")
+    copy_from, copy_to, taken = torch.empty(2 * forks + 1, dtype=torch.int32,
+                                            device=device).split_with_sizes((forks, forks, 1))
+    _launch(device, _lib.lib().mt_paged_fork, _lib.PAGED_FORK_ARGS.pack(
+        block_tables.data_ptr(), block_tables.stride(0), lengths.data_ptr(), sources.data_ptr(),
+        targets.data_ptr(), 0 if tokens is None else tokens.data_ptr(), free_pages.data_ptr(),
+        0 if free_start is None else free_start.data_ptr(), copy_from.data_ptr(), copy_to.data_ptr(),
+        taken.data_ptr(), requests, width, free_pages.shape[0], page_size, forks))
+    return PagedFork(copy_from, copy_to, taken)
+
+
+def paged_free(block_tables, lengths, kept, free_pages, *, page_size, pages, free_start):
+    """Give back the pages behind the first ``kept[r]`` of each request's ``lengths[r]`` tokens (int32
+    vectors): all of a request that has ended (0), those of tokens that are taken back, none where
+    ``kept`` is the length.
+
+    A page that any request still has among its kept tokens' pages stays. The numbers of the others, in
+    ascending order, are written to ``free_pages`` in place, in front of entry ``free_start`` (a device
+    int32 tensor of one element: how many entries have been taken). Returns how many there are (int32
+    ``[1]``); tables and lengths are not changed. A caller goes on with ``lengths.copy_(kept)`` and
+    ``free_start.sub_(freed)``. ``pages``: of the cache.
+    """
+    device = block_tables.device
+    _same_device(device, lengths, kept, free_pages, free_start)
+    _check_tables(block_tables, page_size)
+    lengths = _int32(lengths, "lengths").contiguous()
+    kept = _int32(kept, "kept").contiguous()
+    _in_place(_int32(free_pages, "free_pages"), "free_pages")
+    _one_int32(free_start, "free_start")
+    requests, width = block_tables.shape
+    if lengths.shape[0] != requests or kept.shape[0] != requests:
+        raise ValueError("lengths, kept and block_tables must describe the same requests")
+    if not 0 < pages < 1 << 31:
+        raise ValueError("pages must be positive, and below 2^31")
+    freed = torch.empty(1, dtype=torch.int32, device=device)
+    lib = _lib.lib()
+    ws = _scratch(device, lib.mt_paged_free_workspace_bytes(pages))
+    _launch(device, lib.mt_paged_free, _lib.PAGED_FREE_ARGS.pack(
+        block_tables.data_ptr(), block_tables.stride(0), lengths.data_ptr(), kept.data_ptr(),
+        free_pages.data_ptr(), free_start.data_ptr(), freed.data_ptr(), requests, width,
+        free_pages.shape[0], page_size, pages), ws.data_ptr(), ws.numel())
+    return freed
+
+
+class PagedCompaction(NamedTuple):
+    """What :func:`paged_compact` gives: the block tables and the free list as they are afterwards, the
+    pages to copy, ``sources`` to ``targets`` (int32, -1 behind the last), and ``moves`` (``[1]``), how
+    many there are."""
+
+    block_tables: torch.Tensor
+    free_pages: torch.Tensor
+    sources: torch.Tensor
+    targets: torch.Tensor
+    moves: torch.Tensor
+
+
+def paged_compact(block_tables, lengths, free_pages, *, page_size, pages, free_start):
+    """Plan the pages in use together, so that a pool can shrink or be read in order.
+
+    Of all pages that are in use (among those of some request's ``lengths[r]`` tokens) or free (in
+    ``free_pages`` from entry ``free_start`` on), those in use get the lowest numbers: the highest in use
+    moves to the lowest free one, and so on. Pages that are neither stay out of it. Nothing is changed in
+    place; a caller goes on with ``paged_copy(caches, plan.sources, plan.targets)``,
+    ``block_tables.copy_(plan.block_tables)`` and ``free_pages.copy_(plan.free_pages)``, whose start is
+    the same as before. Returns a :class:`PagedCompaction`.
+    """
+    device = block_tables.device
+    _same_device(device, lengths, free_pages, free_start)
+    _check_tables(block_tables, page_size)
+    lengths = _int32(lengths, "lengths").contiguous()
+    free_pages = _int32(free_pages, "free_pages").contiguous()
+    _one_int32(free_start, "free_start")
+    requests, width = block_tables.shape
+    if lengths.shape[0] != requests:
+        raise ValueError("lengths and block_tables must describe the same requests")
+    if not 0 < pages < 1 << 31:
+        raise ValueError("pages must be positive, and below 2^31")
+    count = free_pages.shape[0]
+    most = min(pages // 2, requests * width)
+    new_tables = torch.empty((requests, width), dtype=torch.int32, device=device)
+    new_free, sources, targets, moves = torch.empty(
+        count + 2 * most + 1, dtype=torch.int32, device=device).split_with_sizes(
+            (count, most, most, 1))
+    lib = _lib.lib()
+    ws = _scratch(device, lib.mt_paged_compact_workspace_bytes(pages))
+    _launch(device, lib.mt_paged_compact, _lib.PAGED_COMPACT_ARGS.pack(
+        block_tables.data_ptr(), block_tables.stride(0), lengths.data_ptr(), free_pages.data_ptr(),
+        free_start.data_ptr(), new_tables.data_ptr(), new_free.data_ptr(), sources.data_ptr(),
+        targets.data_ptr(), moves.data_ptr(), requests, width, count, page_size, pages, most),
+        ws.data_ptr(), ws.numel())
+    return PagedCompaction(new_tables, new_free, sources, targets, moves)
