@@ -257,7 +257,7 @@ def prepare(case, seed):
     if own:  # a serving program's handles of its caches: the tensors and scales
         import metile_amd as mt
 
-        sides = state.get("caches") or [(state["key"], state["value"])] * ("key" in state)
+        sides = [(state["key"], state["value"])] if "key" in state else state.get("caches", [])
         state["handles"] = [mt.PagedCache(key, value, key_scale=state["scales"][0],
                                           value_scale=state["scales"][1]) for key, value in sides]
     return state
