@@ -1,15 +1,17 @@
 // Log probabilities of given tokens, entropies of their distributions and the likeliest alternatives.
 //
-//   log p_i = (x_i - m) / T - log S      S = sum_j exp((x_j - m) / T)      m = max_j x_j
-//   H = log S - (sum_j exp((x_j - m) / T) (x_j - m) / T) / S
+//   log p_i = (y_i - log2 S) ln 2      y_j = c x_j - R      c = log2 e / T      S = sum_j 2^(y_j)
+//   H = (log2 S - (sum_j 2^(y_j) y_j) / S) ln 2
 //   rank of a token: how many logits are larger, or as large and before it
 //
-// in one pass over the logits: a thread keeps a running maximum, sum and weighted sum of its own, a
-// batch of 32 values at a time. For the alternatives it also keeps each batch's maximum. The k-th
-// largest of those, t, is a lower bound of the k-th largest logit, so all that is larger than t lies in
-// the fewer than k groups of 32 whose maximum is: they alone are read again. What is left to k are the
-// first logits that equal t. Order is by value, then by index, and no sum goes by the order in which
-// threads arrive.
+// in one pass over the logits. R is any whole number near c times the largest logit: exact in fp32, so
+// that y has one rounding, and kept until a logit passes it by four powers of two, so that the sums
+// are hardly ever rescaled. For the alternatives a thread keeps the maximum of each group of 32 values.
+// The k-th largest of the threads' maxima, t, is a lower bound of the k-th largest logit, so all of the k
+// lie in groups whose maximum reaches t: they alone are read again (as many of them as there are
+// alternatives, or a few more; where there are many, for equal logits or a long run of large ones, those
+// above the k-th largest maximum, and then the first logits that equal it). Order is by value, then by
+// index, and no sum goes by the order in which threads arrive.
 //
 // A workgroup takes a row, or with few rows a part of one; the parts are joined by a second launch.
 #include <algorithm>
@@ -25,10 +27,14 @@ constexpr int kUnits = 4;                        // runs of 8 values of a thread
 constexpr int kRun = kThreads * 8;               // values of a unit, next to each other
 constexpr int kBatch = kRun * kUnits;            // values of a batch
 constexpr int kMostBatches = 32;                 // of a part: their maxima fit LDS
+constexpr int kMostGroups = 64;                  // that are read again
 constexpr int kMostTop = kLogprobsMostTop;
 constexpr int kF32 = 2;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kNothing = -0x1p100f;  // the reference before any logit
+constexpr double kNone = -1e300;       // and of a sum of nothing, below that of every logit
+constexpr float kRoom = 4.0f;
 
 // Order of values as unsigned numbers: -0 and +0 alike, NaN below all others.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -40,58 +46,77 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 struct Sums {
-  float m, s, w;  // maximum; sum of exp((x - m) / T), and of that times x - m
+  double ref;  // R
+  float s, w;  // sums of 2^y and 2^y y
 };
-// A weighted sum w beside a sum s once its maximum is |d| smaller than the new one, f = exp(d / T). A sum
+// A weighted sum w beside a sum s once its reference is d (below 0) from the new one, f = 2^d. A sum
 // that does not count any more adds nothing, whatever its distance; sums that are no numbers stay so.
 __device__ __forceinline__ float moved(float w, float s, float d, float f) {
   return f > 0.0f ? f * (w + s * d) : s * 0.0f;
 }
-__device__ __forceinline__ Sums join(Sums a, Sums b, float scale) {
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
   Sums r;
-  r.m = fmaxf(a.m, b.m);
-  const float at = r.m == -__builtin_inff() ? 0.0f : r.m;
-  const float da = fmaxf(a.m - at, kLowest), db = fmaxf(b.m - at, kLowest);
-  const float fa = __builtin_amdgcn_exp2f(da * scale), fb = __builtin_amdgcn_exp2f(db * scale);
+  r.ref = a.ref > b.ref ? a.ref : b.ref;
+  const float da = (float)(a.ref - r.ref), db = (float)(b.ref - r.ref);
+  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
   r.s = a.s * fa + b.s * fb;
   r.w = moved(a.w, a.s, da, fa) + moved(b.w, b.s, db, fb);
   return r;
 }
 
-// What a part of a row hands on: 16 bytes, then its alternatives as (key, index), largest first.
+// What a part of a row hands on, and behind it its alternatives as (key, index), largest first.
 struct Part {
   Sums sums;
-  int32_t larger;
+  int32_t larger, unused;
 };
 
-template <int DT>
-__device__ __forceinline__ void load8(const unsigned char* p, float (&x)[8]) {
-  if constexpr (DT == kF32) {
-    __builtin_memcpy(x, p, 32);
-  } else {
-    u32x4 v;
-    __builtin_memcpy(&v, p, 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = v[j];
-      x[2 * j] = lo16<DT>(w);
-      x[2 * j + 1] = hi16<DT>(w);
-    }
-  }
+// The largest of three, without the instructions that would quiet NaN first.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  __asm__("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
+
+// Eight values as they lie in memory.
+template <int DT>
+struct Raw {
+  u32x4 v[DT == kF32 ? 2 : 1];
+};
 template <int DT>
 __device__ __forceinline__ float load1(const unsigned char* row, int i) {
   if constexpr (DT == kF32) return reinterpret_cast<const float*>(row)[i];
   else return act_to_f32<DT>(reinterpret_cast<const uint16_t*>(row)[i]);
 }
-// Eight values from i on, -inf behind `end`.
+// Addresses need the alignment of a value only.
 template <int DT>
-__device__ __forceinline__ void load8_to(const unsigned char* row, int i, int end, float (&x)[8]) {
+__device__ __forceinline__ Raw<DT> load8(const unsigned char* p) {
+  Raw<DT> r;
+  __builtin_memcpy(&r, p, sizeof r);
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ void values8(const Raw<DT>& r, float (&x)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t w = DT == kF32 ? r.v[j / 4][j % 4] : r.v[0][j / 2];
+    if constexpr (DT == kF32) x[j] = __uint_as_float(w);
+    else x[j] = j % 2 ? hi16<DT>(w) : lo16<DT>(w);
+  }
+}
+// The eight values from i on, -inf behind `end`.
+template <int DT>
+__device__ __forceinline__ void tail8(const unsigned char* row, int i, int end, float (&x)[8]) {
   if (i + 8 <= end) {
-    load8<DT>(row + (int64_t)i * (DT == kF32 ? 4 : 2), x);
+    values8<DT>(load8<DT>(row + (int64_t)i * (DT == kF32 ? 4 : 2)), x);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = i + j < end ? load1<DT>(row, i + j) : -__builtin_inff();
+    for (int j = 0; j < 8; ++j) x[j] = -__builtin_inff();
+#pragma unroll 1
+    for (int j = 0; i + j < end; ++j) {
+      const float v = load1<DT>(row, i + j);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = j == k ? v : x[k];
+    }
   }
 }
 
@@ -103,15 +128,15 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
   return v;
 }
 
-// Sum over the workgroup, in every thread. `lds` holds kWaves words; two barriers.
-__device__ __forceinline__ int block_sum(int v, int* lds) {
-  for (int d = 32; d; d /= 2) v += __shfl_xor(v, d);
+// Sum over the workgroup of its waves' counts, in every thread. `turn` alternates the LDS used, so that
+// one barrier is enough.
+__device__ __forceinline__ int block_sum(int of_wave, int (&lds)[2][kWaves], int& turn) {
+  if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = of_wave;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0;
+  int v = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) v += lds[w];
+  for (int w = 0; w < kWaves; ++w) v += lds[turn][w];
+  turn ^= 1;
   return v;
 }
 
@@ -127,13 +152,14 @@ __device__ __forceinline__ void put_in_order(const uint64_t* from, int count, in
 
 __device__ __forceinline__ void write_row(const LogprobsArgs& a, int row, Sums sums, float given,
                                           bool in_vocab, int larger, const uint64_t* best) {
-  const float log_s = __builtin_amdgcn_logf(sums.s) * kLn2;  // -inf for a row of -inf alone
+  const float scale = a.inv_temperature * kLog2e;
+  const float log_s = __builtin_amdgcn_logf(sums.s);
   auto logprob = [&](float x) {
-    if (sums.s == 0.0f) return -__builtin_inff();
-    return (x - sums.m) * a.inv_temperature - log_s;
+    if (sums.s == 0.0f) return -__builtin_inff();  // a row of -inf alone
+    return (float)(((double)x * (double)scale - sums.ref - (double)log_s) * 0.6931471805599453);
   };
   if (threadIdx.x == 0) {
-    a.entropies[row] = sums.s == 0.0f ? 0.0f : log_s - a.inv_temperature * sums.w / sums.s;
+    a.entropies[row] = sums.s == 0.0f ? 0.0f : (log_s - sums.w / sums.s) * kLn2;
     if (a.tokens) {
       a.logprobs[row] = in_vocab ? logprob(given) : -__builtin_inff();
       a.ranks[row] = in_vocab ? larger : -1;
@@ -149,12 +175,12 @@ __device__ __forceinline__ void write_row(const LogprobsArgs& a, int row, Sums s
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
-  extern __shared__ uint32_t group_keys[];  // [batches][kThreads], with alternatives
-  __shared__ uint64_t larger_than[32 * kMostTop];
-  __shared__ uint64_t best[kMostTop];
+  // each group's maximum, [batches][kThreads]; later the candidates, kMostGroups * 32 of them
+  extern __shared__ __attribute__((aligned(16))) uint32_t group_keys[];
+  __shared__ uint64_t best[kMostTop], flagged;
   __shared__ Sums wave_sums[kWaves];
-  __shared__ int wave_count[kWaves], counts[2], groups[kMostTop];
-  __shared__ uint64_t flagged;
+  __shared__ uint32_t thread_keys[kThreads];
+  __shared__ int wave_count[2][kWaves], counts[2], groups[kMostGroups];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / (unsigned)a.num_parts, part = blockIdx.x % (unsigned)a.num_parts;
@@ -177,36 +203,69 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
   }
 
   // ---- sums, and each group's maximum ----
-  Sums own = {-__builtin_inff(), 0.0f, 0.0f};
-  int larger = 0;  // of the wave
-  for (int b = 0; b < batches; ++b) {
-    const int at = begin + b * kBatch;
-    float x[kUnits][8];
+  constexpr uint32_t kSize = DT == kF32 ? 4 : 2;
+  Raw<DT> next[kUnits];
+  auto request = [&](int b) {  // a batch that is whole
+    const unsigned char* p = x_row + (int64_t)(begin + b * kBatch) * kSize;
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) load8_to<DT>(x_row, at + u * kRun + tid * 8, end, x[u]);
-    float top = x[0][0];
+    for (int u = 0; u < kUnits; ++u) next[u] = load8<DT>(p + (u * kRun + (uint32_t)tid * 8) * kSize);
+  };
+  auto tail = [&](int b, float (&x)[kUnits][8]) {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
+      tail8<DT>(x_row, begin + b * kBatch + u * kRun + tid * 8, end, x[u]);
+  };
+  // Sums of the lanes, then of the waves, in every thread.
+  auto of_all = [&](Sums own) {
+    for (int d = 32; d; d /= 2) {
+      Sums other;
+      other.ref = __shfl_xor(own.ref, d);
+      other.s = __shfl_xor(own.s, d);
+      other.w = __shfl_xor(own.w, d);
+      own = (lane & d) ? join(other, own) : join(own, other);
+    }
+    if (lane == 0) wave_sums[wave] = own;
+    __syncthreads();
+    own = wave_sums[0];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, x[u][j]);
-    if (a.top) group_keys[b * kThreads + tid] = key_of(top);
-    const float m = fmaxf(own.m, top), zero_at = m == -__builtin_inff() ? 0.0f : m;
-    const float step = fmaxf(own.m - zero_at, kLowest);
-    const float fix = __builtin_amdgcn_exp2f(step * scale);
-    float w = moved(own.w, own.s, step, fix), s = own.s * fix;
-    own.m = m;
+    for (int w = 1; w < kWaves; ++w) own = join(own, wave_sums[w]);
+    return own;
+  };
+  float ref = kNothing, s = 0.0f, w = 0.0f, own_top = -__builtin_inff();  // ref is the wave's
+  int larger = 0;                                                        // of the wave
+  auto take = [&](int b, const float (&x)[kUnits][8]) {
+    const int at = begin + b * kBatch;
+    float tops[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) tops[u] = max3(x[u][0], x[u][1], x[u][2]);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) tops[u] = max3(tops[u], x[u][3], x[u][4]);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) tops[u] = max3(tops[u], x[u][5], x[u][6]);
+    float top = max3(tops[0], x[0][7], x[1][7]);
+    top = max3(top, max3(tops[1], x[2][7], x[3][7]), max3(tops[2], tops[2], tops[3]));
+    if (a.top) {
+      group_keys[b * kThreads + tid] = key_of(top);
+      own_top = fmaxf(own_top, top);
+    }
+    if (__any(fmaf(top, scale, -ref) > kRoom)) {
+      float most = top;
+      for (int d = 32; d; d /= 2) most = fmaxf(most, __shfl_xor(most, d));
+      const float to = rintf(most * scale), d = ref - to, f = __builtin_amdgcn_exp2f(d);
+      w = moved(w, s, d, f);
+      s *= f;
+      ref = to;
+    }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float t = x[u][j] - zero_at;
-        const float e = __builtin_amdgcn_exp2f(t * scale);
+        const float y = fmaf(x[u][j], scale, -ref);
+        const float e = __builtin_amdgcn_exp2f(y);
         s += e;
-        w = fmaf(e, fmaxf(t, kLowest), w);  // (0 times -inf is none)
+        w = fmaf(e, fmaxf(y, kLowest), w);  // (0 times -inf is none)
       }
-    own.s = s;
-    own.w = w;
-    if (a.tokens) {
+    if (a.tokens && __any(top >= given)) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int from = at + u * kRun;
@@ -224,75 +283,138 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
         }
       }
     }
+  };
+  const int whole = (end - begin) / kBatch;
+  if (whole) request(0);
+  for (int b = 0; b < whole; ++b) {
+    float x[kUnits][8];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) values8<DT>(next[u], x[u]);
+    if (b + 1 < whole) request(b + 1);
+    take(b, x);
   }
-  for (int d = 32; d; d /= 2) {
-    Sums other;
-    other.m = __shfl_xor(own.m, d);
-    other.s = __shfl_xor(own.s, d);
-    other.w = __shfl_xor(own.w, d);
-    own = (lane & d) ? join(other, own, scale) : join(own, other, scale);
+  if (whole < batches) {
+    float x[kUnits][8];
+    tail(whole, x);
+    take(whole, x);
   }
-  if (lane == 0) {
-    wave_sums[wave] = own;
-    wave_count[wave] = larger;
-  }
+  if (lane == 0) wave_count[0][wave] = larger;
   if (tid < kMostTop) best[tid] = 0;
   if (tid == 0) counts[0] = counts[1] = 0, flagged = 0;
-  __syncthreads();
-  Sums sums = wave_sums[0];
-  larger = wave_count[0];
+  Sums sums = of_all({s == 0.0f ? kNone : (double)ref, s, w});
+  uint32_t own_key = key_of(own_top);
+  if (!(sums.s > 0.0f && sums.s < __builtin_inff())) {
+    // NaN or infinities, logits too large for c times them, or none that is allowed: again, with
+    // references in 64 bits and maxima by whole numbers
+    Sums own = {kNone, 0.0f, 0.0f};
+    own_key = 0;
+#pragma unroll 1
+    for (int b = 0; b < batches; ++b) {
+      float x[kUnits][8];
+      tail(b, x);
+      uint32_t key = 0;
+#pragma unroll 1
+      for (int u = 0; u < kUnits; ++u) {
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    sums = join(sums, wave_sums[w], scale);
-    larger += wave_count[w];
+        for (int j = 0; j < 8; ++j) {
+          const float v = u == 0 ? x[0][j] : u == 1 ? x[1][j] : u == 2 ? x[2][j] : x[3][j];
+          key = max(key, key_of(v));
+          if (v == -__builtin_inff()) continue;
+          const Sums one = {(double)v * (double)scale, v - v == 0.0f ? 1.0f : v - v, 0.0f};
+          own = join(own, one);
+        }
+      }
+      if (a.top) group_keys[b * kThreads + tid] = key;
+      own_key = max(own_key, key);
+    }
+    __syncthreads();
+    sums = of_all(own);
   }
+  larger = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) larger += wave_count[0][w];
 
   // ---- alternatives ----
   if (a.top) {
     const int k = a.top;
-    // the k-th largest of the groups' maxima: the largest key that k of them reach (0: fewer do)
-    uint32_t bound = 0;
     constexpr int kLowBit = DT == kF32 ? 0 : DT == kBF16 ? 16 : 13;  // 16-bit values have no others
-    for (int bit = 31; bit >= kLowBit; --bit) {
-      const uint32_t middle = bound | 1u << bit;
-      int n = 0;
-      for (int b = 0; b < batches; ++b) n += group_keys[b * kThreads + tid] >= middle;
-      if (block_sum(n, wave_count) >= k) bound = middle;
-    }
-    // negative values of 16 bits have ones below: the key itself, not its first bits
-    if (kLowBit && !(bound >> 31)) bound = bound ? bound | ((1u << kLowBit) - 1) : 0;
-    // (fewer than k) groups with larger values, and the batches that have values of the bound
-    for (int b = 0; b < batches; ++b) {
-      const uint32_t key = group_keys[b * kThreads + tid];
-      if (key > bound) groups[atomicAdd(&counts[0], 1)] = b * kThreads + tid;
-      if (key >= bound && bound) atomicOr((unsigned long long*)&flagged, 1ull << b);
-    }
+    auto exact = [&](uint32_t bound) {  // keys of negative values have ones there
+      return kLowBit && bound && !(bound >> 31) ? bound | ((1u << kLowBit) - 1) : bound;
+    };
+    thread_keys[tid] = own_key;
     __syncthreads();
-    const int num_groups = counts[0];
+    // the k-th largest of the threads' maxima: the largest key that k of them reach (0: fewer do)
+    uint32_t bound = 0;
     {
-      const int g = tid / 8, u = tid % 8 / 2, j0 = tid % 2 * 4;
-      if (g < num_groups) {
-        const int group = groups[g];
-        const int at = begin + group / kThreads * kBatch + u * kRun + group % kThreads * 8 + j0;
+      uint32_t keys[kWaves];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t key = at + j < end ? key_of(load1<DT>(x_row, at + j)) : 0;
-          if (key > bound)
-            larger_than[atomicAdd(&counts[1], 1)] = (uint64_t)key << 32 | ~(uint32_t)(at + j);
+      for (int i = 0; i < kWaves; ++i) keys[i] = thread_keys[64 * i + lane];
+      for (int bit = 31; bit >= kLowBit; --bit) {
+        const uint32_t middle = bound | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) n += __popcll(__ballot(keys[i] >= middle));
+        if (n >= k) bound = middle;
+      }
+      bound = exact(bound);
+    }
+    // groups that reach `least`
+    auto collect = [&](uint32_t least) {
+      for (int b = 0; b < batches; ++b)
+        if (group_keys[b * kThreads + tid] >= least) {
+          const int n = atomicAdd(&counts[0], 1);
+          if (n < kMostGroups) groups[n] = b * kThreads + tid;
         }
+      __syncthreads();
+    };
+    uint32_t least = max(bound, 1u);
+    collect(least);
+    const bool many = counts[0] > kMostGroups;
+    if (many) {
+      // Many equal values, or many large ones in one thread's groups: the k-th largest of all groups'
+      // maxima, the fewer than k groups above it, and the batches that have values of it.
+      int turn = 1;
+      uint32_t of_groups = 0;
+      for (int bit = 31; bit >= kLowBit; --bit) {
+        const uint32_t middle = of_groups | 1u << bit;
+        int n = 0;
+        for (int b = 0; b < batches; ++b)
+          n += __popcll(__ballot(group_keys[b * kThreads + tid] >= middle));
+        if (block_sum(n, wave_count, turn) >= k) of_groups = middle;
+      }
+      bound = exact(of_groups);
+      least = bound + 1;
+      __syncthreads();
+      if (tid == 0) counts[0] = 0;
+      for (int b = 0; b < batches; ++b)
+        if (bound && group_keys[b * kThreads + tid] >= bound)
+          atomicOr((unsigned long long*)&flagged, 1ull << b);
+      __syncthreads();
+      collect(least);
+    }
+    const int num_groups = counts[0];
+    uint64_t* candidates = reinterpret_cast<uint64_t*>(group_keys);
+    for (int g = tid / 8; g < num_groups; g += kThreads / 8) {
+      const int u = tid % 8 / 2, j0 = tid % 2 * 4, group = groups[g];
+      const int at = begin + group / kThreads * kBatch + u * kRun + group % kThreads * 8 + j0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t key = at + j < end ? key_of(load1<DT>(x_row, at + j)) : 0;
+        if (key >= least)
+          candidates[atomicAdd(&counts[1], 1)] = (uint64_t)key << 32 | ~(uint32_t)(at + j);
       }
     }
     __syncthreads();
     const int found = counts[1];
-    put_in_order(larger_than, found, k, best);
-    int have = min(found, k);
-    // the first values that equal the bound, unit by unit
-    for (uint64_t rest = flagged; rest && have < k; rest &= rest - 1) {
+    put_in_order(candidates, found, k, best);
+    int have = min(found, k), turn = 1;
+    // with many, the first values that equal the bound, unit by unit
+    for (uint64_t rest = many ? flagged : 0; rest && have < k; rest &= rest - 1) {
       const int b = __ffsll((unsigned long long)rest) - 1;
       for (int u = 0; u < kUnits && have < k; ++u) {
         const int at = begin + b * kBatch + u * kRun + tid * 8;
         float x[8];
-        load8_to<DT>(x_row, at, end, x);
+        tail8<DT>(x_row, at, end, x);
         int n = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) n += at + j < end && key_of(x[j]) == bound;
@@ -302,16 +424,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
           const int o = __shfl_up(before, d);
           if (lane >= d) before += o;
         }
-        __syncthreads();
-        if (lane == 63) wave_count[wave] = before;
+        if (lane == 63) wave_count[turn][wave] = before;
         __syncthreads();
         int all = 0;
         before -= n;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          if (w < wave) before += wave_count[w];
-          all += wave_count[w];
+          if (w < wave) before += wave_count[turn][w];
+          all += wave_count[turn][w];
         }
+        turn ^= 1;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (at + j < end && key_of(x[j]) == bound) {
@@ -330,7 +452,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
     return;
   }
   unsigned char* to = a.parts + (int64_t)blockIdx.x * (sizeof(Part) + a.top * 8);
-  if (tid == 0) *reinterpret_cast<Part*>(to) = Part{sums, larger};
+  if (tid == 0) *reinterpret_cast<Part*>(to) = Part{sums, larger, 0};
   if (tid < a.top) reinterpret_cast<uint64_t*>(to + sizeof(Part))[tid] = best[tid];
 }
 
@@ -343,7 +465,6 @@ __global__ __launch_bounds__(kThreads) void join_kernel(LogprobsArgs a) {
   const int tid = threadIdx.x, row = blockIdx.x;
   const int step = (int)sizeof(Part) + a.top * 8;
   const unsigned char* from = a.parts + (int64_t)row * a.num_parts * step;
-  const float scale = a.inv_temperature * kLog2e;
   const unsigned char* x_row = static_cast<const unsigned char*>(a.logits) +
                                (int64_t)row * a.row_stride * (DT == kF32 ? 4 : 2);
   float given = 0.0f;
@@ -353,11 +474,11 @@ __global__ __launch_bounds__(kThreads) void join_kernel(LogprobsArgs a) {
     in_vocab = t >= 0 && t < a.vocab;
     given = load1<DT>(x_row, in_vocab ? (int)t : 0);
   }
-  Sums sums = {-__builtin_inff(), 0.0f, 0.0f};
+  Sums sums = {kNone, 0.0f, 0.0f};
   int larger = 0;
   for (int p = 0; p < a.num_parts; ++p) {
     const Part part = *reinterpret_cast<const Part*>(from + (int64_t)p * step);
-    sums = join(sums, part.sums, scale);
+    sums = join(sums, part.sums);
     larger += part.larger;
   }
   if (tid < kMostTop) best[tid] = 0;
@@ -387,7 +508,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(LogprobsArgs a) {
 
 template <int DT>
 hipError_t launch(const LogprobsArgs& args, hipStream_t stream) {
-  const int keys = args.top ? std::min(args.part_batches, (args.vocab + kBatch - 1) / kBatch) * kThreads * 4 : 0;
+  const int batches = std::min(args.part_batches, (args.vocab + kBatch - 1) / kBatch);
+  const int keys = args.top ? std::max(batches * kThreads * 4, kMostGroups * 32 * 8) : 0;
   // rows of a launch, so that its threads are counted in 32 bits; the parts of one are joined before
   // those of the next are made
   const int most = std::max(1, (1 << 22) / args.num_parts);
@@ -408,11 +530,11 @@ hipError_t launch(const LogprobsArgs& args, hipStream_t stream) {
 
 }  // namespace
 
-// A workgroup a row, unless that leaves CUs without one: then parts of whole batches, so many that
-// there are four workgroups a CU, at most 64.
+// A workgroup a row, unless that leaves CUs without one: then parts of four batches or more, so many
+// that there are four workgroups a CU, at most 64.
 LogprobsPlan plan_token_logprobs(int rows, int vocab, int cus) {
   const int batches = std::max(1, (int)(((int64_t)vocab + kBatch - 1) / kBatch));
-  int parts = (int)std::min<int64_t>(batches, std::max<int64_t>(1, 4ll * cus / std::max(rows, 1)));
+  int parts = (int)std::min<int64_t>((batches + 3) / 4, std::max<int64_t>(1, 4ll * cus / std::max(rows, 1)));
   parts = std::min(parts, 64);
   const int per = std::min(kMostBatches, (batches + parts - 1) / parts);
   return {per, (batches + per - 1) / per};
