@@ -233,8 +233,12 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
   };
   float ref = kNothing, s = 0.0f, w = 0.0f, own_top = -__builtin_inff();  // ref is the wave's
   int larger = 0;                                                        // of the wave
+  bool masked = false;  // the wave has met -inf
+  // Values as large as the token's count if they are before it: those larger than the next value below.
+  const uint32_t bits = __float_as_uint(given);
+  const float below = __uint_as_float(given == 0.0f ? 0x80000001u : bits >> 31 ? bits + 1 : bits - 1);
   auto take = [&](int b, const float (&x)[kUnits][8]) {
-    const int at = begin + b * kBatch;
+    const int at = begin + b * kBatch + tid * 8;
     float tops[kUnits];
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) tops[u] = max3(x[u][0], x[u][1], x[u][2]);
@@ -256,31 +260,41 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
       s *= f;
       ref = to;
     }
+    // The sums of the batch. (2^y y is no number for y of -inf, which adds nothing: a wave that has met
+    // one bounds y, an instruction more.)
+    const float s0 = s, w0 = w;
+    if (!masked) {
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u)
+      for (int u = 0; u < kUnits; ++u)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float y = fmaf(x[u][j], scale, -ref);
-        const float e = __builtin_amdgcn_exp2f(y);
-        s += e;
-        w = fmaf(e, fmaxf(y, kLowest), w);  // (0 times -inf is none)
-      }
+        for (int j = 0; j < 8; ++j) {
+          const float y = fmaf(x[u][j], scale, -ref);
+          const float e = __builtin_amdgcn_exp2f(y);
+          s += e;
+          w = fmaf(e, y, w);
+        }
+      masked = __any(w != w);
+    }
+    if (masked) {
+      s = s0;
+      w = w0;
+      const float same = opaque(ref);  // (no exponential is to be kept for this)
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float y = fmaf(x[u][j], scale, -same);
+          const float e = __builtin_amdgcn_exp2f(y);
+          s += e;
+          w = fmaf(e, fmaxf(y, kLowest), w);
+        }
+    }
     if (a.tokens && __any(top >= given)) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        const int from = at + u * kRun;
-        if (token >= from + kRun) {  // those before the token count if they are as large
+        const float bound = at + u * kRun + 8 <= token ? below : given;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) larger += __popcll(__ballot(x[u][j] >= given));
-        } else if (token < from) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) larger += __popcll(__ballot(x[u][j] > given));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            larger += __popcll(__ballot(x[u][j] > given ||
-                                        (x[u][j] == given && from + tid * 8 + j < token)));
-        }
+        for (int j = 0; j < 8; ++j) larger += __popcll(__ballot(x[u][j] > bound));
       }
     }
   };
@@ -297,6 +311,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
     float x[kUnits][8];
     tail(whole, x);
     take(whole, x);
+  }
+  if (in_vocab && token >= begin && token < end && tid == 0)  // those of the token's own eight
+    for (int i = token & ~7; i < token; ++i) larger += load1<DT>(x_row, i) == given;
+  if (in_vocab && given == -__builtin_inff()) {
+    // (nothing is below -inf: the larger ones have been counted, those before the token are as large)
+    larger = 0;
+    for (int i = begin + tid; i < end; i += kThreads)
+      larger += __popcll(__ballot(load1<DT>(x_row, i) > given || i < token));
   }
   if (lane == 0) wave_count[0][wave] = larger;
   if (tid < kMostTop) best[tid] = 0;
