@@ -148,8 +148,8 @@ __device__ __forceinline__ int value_place(int c, int row) {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// DIM: the head's values or more, the rest as if zero.
-template <int DT, bool FP8, int DIM>
+// DIM: the head's values, or with PADDED that many or more (the rest count as zero).
+template <int DT, bool FP8, int DIM, bool PADDED>
 __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel(
     ChunkAttentionArgs a) {
   constexpr int kChunks = DIM / 8, kSteps = DIM / 16, kTiles = DIM / 32;
@@ -162,11 +162,13 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   // small ones stay above its smallest numbers: 2^15 at most.
   constexpr float kShift = DT == kF16 ? 11.0f : 0.0f, kRoom = DT == kF16 ? 15.0f : 8.0f;
 
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2][2][kStage];  // stage; keys, values
+  // an array a stage and side: the compiler has to see that reads of one do not wait for loads to another
+  __shared__ __attribute__((aligned(16))) uint16_t keys0[kStage], values0[kStage], keys1[kStage],
+      values1[kStage];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int dim = a.dim;
+  const int dim = PADDED ? a.dim : DIM;
 
   // ---- rows that belong to no request ----
   {
@@ -257,7 +259,7 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   };
   // Chunk i of this thread: LDS chunk n of the stage is row n / kChunks, place n % kChunks.
   u32x2 held8[FP8 ? 2 * kLoads : 1];
-  auto request_rows = [&](int stage, int block, int page) {
+  auto request_rows = [&](uint16_t* keys, uint16_t* values, int block, int page) {
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       const uint64_t offset = side ? offset_of(block, page, a.v_page, a.v_slot)
@@ -269,61 +271,50 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
         const int row = n / kChunks, place = n % kChunks;
         const int c = side ? value_place<kChunks>(place, row) : key_place<kChunks>(place, row);
         const unsigned char* from =
-            base + of_row(offset, row) + (8 * c < dim ? c * (FP8 ? 8 : 16) : 0);
+            base + of_row(offset, row) + (!PADDED || 8 * c < dim ? c * (FP8 ? 8 : 16) : 0);
         if constexpr (FP8) {
           held8[side * kLoads + i] = *reinterpret_cast<const u32x2*>(from);
         } else {
           __builtin_amdgcn_global_load_lds(
               (const __attribute__((address_space(1))) void*)from,
-              (__attribute__((address_space(3))) void*)(&lds[stage][side][(wave * kLoads + i) * 512]),
+              (__attribute__((address_space(3))) void*)((side ? values : keys) +
+                                                        (wave * kLoads + i) * 512),
               16, 0, 0);
         }
       }
     }
   };
-  auto park_rows = [&](int stage) {
+  auto park_rows = [&](uint16_t* keys, uint16_t* values) {
     if constexpr (FP8) {
 #pragma unroll
       for (int side = 0; side < 2; ++side)
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
-          *reinterpret_cast<u32x4*>(&lds[stage][side][((wave * kLoads + i) * 64 + lane) * 8]) =
+          *reinterpret_cast<u32x4*>((side ? values : keys) + ((wave * kLoads + i) * 64 + lane) * 8) =
               fp8_eight<DT>(held8[side * kLoads + i]);
     }
   };
 
   float base = -__builtin_inff(), sum = 0.0f;
   f32x16 acc[kTiles];
-  bool all_finite = true;
-again:
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
-
   int page = 0, next_page = 0;
-  if (block0 < block_end) {
-    page = look_up(block0);
-    request_rows(0, block0, page);
-    if (block0 + 1 < block_end) next_page = look_up(block0 + 1);
-    park_rows(0);
-  }
-  for (int block = block0; block < block_end; ++block) {
-    const int stage = (block - block0) & 1;
+
+  // One block, whose rows are in one stage, while those of the next go to the other. CAREFUL: values that
+  // are not finite are kept out of the products.
+  auto take = [&](auto careful, int block, uint16_t* keys, uint16_t* values, uint16_t* keys_next,
+                  uint16_t* values_next) __attribute__((always_inline)) {
+    constexpr bool kCareful = decltype(careful)::value != 0;
     const bool more = block + 1 < block_end;
     wait_vmcnt<0>();
     __syncthreads();
     const uint64_t on_page = __ballot(page_ok(page));
     if (more) {
       page = next_page;
-      request_rows(stage ^ 1, block + 1, page);
+      request_rows(keys_next, values_next, block + 1, page);
       if (block + 2 < block_end) next_page = look_up(block + 2);
     }
     const int k0 = block * kBlock;
     if (wave_rows > 0 && k0 < last_end && k0 + kBlock > first_begin) {
-      const uint16_t* keys = lds[stage][0];
-      const uint16_t* values = lds[stage][1];
-
       // ---- scores: operand row i is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4 ----
       f32x16 s[2];
 #pragma unroll
@@ -333,7 +324,7 @@ again:
         for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          if (16 * k >= kLeastDim && 16 * k >= dim) break;
+          if (PADDED && 16 * k >= kLeastDim && 16 * k >= dim) break;
           const int c = 2 * k + half;
           const u32x4 key = *reinterpret_cast<const u32x4*>(
               keys + (row * kChunks + key_place<kChunks>(c, row)) * 8);
@@ -386,7 +377,7 @@ again:
 
       // ---- values that are not finite: their keys one by one, since products with the zeros of rows
       // that do not see them would make no numbers ----
-      if (!all_finite) {
+      if constexpr (kCareful) {
         bool odd_row = false;
 #pragma unroll 1
         for (int c = 0; c < kChunks; ++c) {
@@ -444,7 +435,7 @@ again:
             v[2 * e] = w.x;
             v[2 * e + 1] = w.y;
           }
-          if (!all_finite) {
+          if constexpr (kCareful) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const uint32_t x = v[j];
@@ -454,23 +445,36 @@ again:
           acc[t] = mfma32<DT>(v, p[k], acc[t]);
         }
     }
-    if (more) park_rows(stage ^ 1);
-  }
-  // A value that is not finite may have met a zero of a row that does not see it: once more, with
-  // care (block by block; for rows that see it the result stays what it is).
-  if (all_finite) {
-    float odd = 0.0f;
+    if (more) park_rows(keys_next, values_next);
+  };
+  auto take_all = [&](auto careful) __attribute__((always_inline)) {
+    base = -__builtin_inff();
+    sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) odd = fmaf(acc[t][i], 0.0f, odd);
-    if (__syncthreads_or(odd != 0.0f)) {
-      all_finite = false;
-      base = -__builtin_inff();
-      sum = 0.0f;
-      goto again;
+      for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    if (block0 >= block_end) return;
+    page = look_up(block0);
+    request_rows(keys0, values0, block0, page);
+    if (block0 + 1 < block_end) next_page = look_up(block0 + 1);
+    park_rows(keys0, values0);
+    for (int block = block0;;) {
+      take(careful, block, keys0, values0, keys1, values1);
+      if (++block >= block_end) break;
+      take(careful, block, keys1, values1, keys0, values0);
+      if (++block >= block_end) break;
     }
-  }
+  };
+  take_all(IntConst<0>());
+  // A value that is not finite may have met a zero of a row that does not see it: once more, with
+  // care (for rows that see it the result stays what it is).
+  float odd = 0.0f;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) odd = fmaf(acc[t][i], 0.0f, odd);
+  if (__syncthreads_or(odd != 0.0f)) take_all(IntConst<1>());
   sum = halves_sum(sum);
 
   // ---- the result, or this part of it ----
@@ -577,7 +581,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ChunkAttentionArgs a) {
 template <int DT, bool FP8, int DIM>
 hipError_t launch_dim(const ChunkAttentionArgs& a, hipStream_t stream) {
   const unsigned items = (unsigned)(a.most_tiles + a.target) * (unsigned)a.kv_heads;
-  attention_kernel<DT, FP8, DIM><<<items, kThreads, 0, stream>>>(a);
+  if (a.dim == DIM) attention_kernel<DT, FP8, DIM, false><<<items, kThreads, 0, stream>>>(a);
+  else attention_kernel<DT, FP8, DIM, true><<<items, kThreads, 0, stream>>>(a);
   if (a.most_parts > 0)
     join_kernel<DT, DIM><<<dim3((unsigned)a.most_parts * (unsigned)a.kv_heads, DIM / 32), kThreads,
                            0, stream>>>(a);
