@@ -32,6 +32,7 @@ struct ChunkAttentionArgs {
   int32_t target;                       // items that the work is split into, if it can be
   int32_t most_tiles, most_parts;       // of one key-value head
   float scale_log2, value_scale;
+  bool narrow;                          // every row of a head begins less than 4 GiB behind its first
   uint32_t flip;                        // sign bits of a query pair to flip
   DivMagic by_page, by_group;
 };

@@ -148,8 +148,24 @@ __device__ __forceinline__ int value_place(int c, int row) {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// DIM: the head's values, or with PADDED that many or more (the rest count as zero).
-template <int DT, bool FP8, int DIM, bool PADDED>
+// LDS is addressed as such throughout: a pointer of no address space costs two registers and a check.
+typedef __attribute__((address_space(3))) uint16_t Lds;
+typedef __attribute__((address_space(3))) u32x4 Lds16;
+typedef __attribute__((address_space(3))) u32x2 Lds8;
+
+// Bytes to a token's row of one head.
+template <bool GENERAL>
+struct Offset {
+  typedef uint64_t type;
+};
+template <>
+struct Offset<false> {
+  typedef uint32_t type;
+};
+
+// DIM: the head's values. With GENERAL, that many or more (the rest count as zero), in caches of any size;
+// else the offsets of rows fit 32 bits.
+template <int DT, bool FP8, int DIM, bool GENERAL>
 __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel(
     ChunkAttentionArgs a) {
   constexpr int kChunks = DIM / 8, kSteps = DIM / 16, kTiles = DIM / 32;
@@ -163,12 +179,14 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   constexpr float kShift = DT == kF16 ? 11.0f : 0.0f, kRoom = DT == kF16 ? 15.0f : 8.0f;
 
   // an array a stage and side: the compiler has to see that reads of one do not wait for loads to another
-  __shared__ __attribute__((aligned(16))) uint16_t keys0[kStage], values0[kStage], keys1[kStage],
-      values1[kStage];
+  __shared__ __attribute__((aligned(16))) uint16_t lds_k0[kStage], lds_v0[kStage], lds_k1[kStage],
+      lds_v1[kStage];
+  Lds *const keys0 = (Lds*)lds_k0, *const values0 = (Lds*)lds_v0, *const keys1 = (Lds*)lds_k1,
+      *const values1 = (Lds*)lds_v1;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int col = lane & 31, half = lane >> 5;
-  const int dim = PADDED ? a.dim : DIM;
+  const int tid = threadIdx.x, wave = uniform(tid >> 6);
+  int lane = tid & 63, col = lane & 31, half = lane >> 5;
+  const int dim = GENERAL ? a.dim : DIM;
 
   // ---- rows that belong to no request ----
   {
@@ -241,6 +259,7 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   // Where a block's tokens are: a lane a token looks up its entry; those that load the row ask for the
   // offset. Tokens past the end stand for the last one, tokens on no page of the cache for page 0;
   // both are masked.
+  typedef typename Offset<GENERAL>::type RowOffset;
   auto look_up = [&](int block) {
     const int token = min(block * kBlock + lane, last_key);
     return table[div_by((uint32_t)token, a.by_page)];
@@ -249,224 +268,291 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   auto offset_of = [&](int block, int page, uint32_t page_stride, uint32_t slot_stride) {
     const uint32_t token = (uint32_t)min(block * kBlock + lane, last_key);
     const uint32_t slot = token - div_by(token, a.by_page) * (uint32_t)a.page_size;
-    return (uint64_t)(page_ok(page) ? (uint32_t)page : 0u) * page_stride +
-           (uint64_t)slot * slot_stride;
+    return (RowOffset)(page_ok(page) ? (uint32_t)page : 0u) * page_stride +
+           (RowOffset)slot * slot_stride;
   };
-  auto of_row = [&](uint64_t offset, int row) {
+  auto of_row = [&](RowOffset offset, int row) {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * row, (int)(uint32_t)offset);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * row, (int)(offset >> 32));
-    return (uint64_t)hi << 32 | lo;
+    if constexpr (!GENERAL) return lo;
+    else
+      return (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(4 * row, (int)((uint64_t)offset >> 32))
+                 << 32 |
+             lo;
   };
-  // Chunk i of this thread: LDS chunk n of the stage is row n / kChunks, place n % kChunks.
-  u32x2 held8[FP8 ? 2 * kLoads : 1];
-  auto request_rows = [&](uint16_t* keys, uint16_t* values, int block, int page) {
+  // One side of a block to LDS. Chunk i of this thread: LDS chunk n of the stage is row n / kChunks, place
+  // n % kChunks. 8-bit rows wait in registers until they are parked.
+  u32x2 held8[2][FP8 ? kLoads : 1];
+  auto request = [&](int side, Lds* to, int block, int page) __attribute__((always_inline)) {
+    const RowOffset offset = side ? offset_of(block, page, a.v_page, a.v_slot)
+                                  : offset_of(block, page, a.k_page, a.k_slot);
+    const unsigned char* base = side ? vbase : kbase;
+    // (chunks of later rows follow from the first one's: not kept, in registers that are short)
+    constexpr bool kEven = 64 % kChunks == 0;
+    constexpr int kRows = kEven ? 64 / kChunks : 1;  // of a load
+    auto place_of = [&](int c, int row) {
+      return side ? value_place<kChunks>(c, row) : key_place<kChunks>(c, row);
+    };
+    uint32_t chunk0 = (uint32_t)place_of(lane % kChunks, lane / kChunks) * (FP8 ? 8 : 16);
+    int row0 = wave * kLoads * kRows + lane / kChunks;
+    if constexpr (kEven) __asm__("" : "+v"(chunk0), "+v"(row0));
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const uint64_t offset = side ? offset_of(block, page, a.v_page, a.v_slot)
-                                   : offset_of(block, page, a.k_page, a.k_slot);
-      const unsigned char* base = side ? vbase : kbase;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int n = (wave * kLoads + i) * 64 + lane;
-        const int row = n / kChunks, place = n % kChunks;
-        const int c = side ? value_place<kChunks>(place, row) : key_place<kChunks>(place, row);
-        const unsigned char* from =
-            base + of_row(offset, row) + (!PADDED || 8 * c < dim ? c * (FP8 ? 8 : 16) : 0);
-        if constexpr (FP8) {
-          held8[side * kLoads + i] = *reinterpret_cast<const u32x2*>(from);
-        } else {
-          __builtin_amdgcn_global_load_lds(
-              (const __attribute__((address_space(1))) void*)from,
-              (__attribute__((address_space(3))) void*)((side ? values : keys) +
-                                                        (wave * kLoads + i) * 512),
-              16, 0, 0);
-        }
+    for (int i = 0; i < kLoads; ++i) {
+      const int n = (wave * kLoads + i) * 64 + lane;
+      const int row = kEven ? row0 + i * kRows : n / kChunks;
+      const uint32_t chunk = kEven ? chunk0 ^ (uint32_t)place_of(0, i * kRows) * (FP8 ? 8 : 16)
+                                   : (uint32_t)place_of(n % kChunks, row) * (FP8 ? 8 : 16);
+      const unsigned char* from =
+          base + (of_row(offset, row) +
+                  (!GENERAL || chunk / (FP8 ? 1 : 2) < (uint32_t)dim ? chunk : 0u));
+      if constexpr (FP8) {
+        held8[side][i] = *reinterpret_cast<const u32x2*>(from);
+      } else {
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)from,
+            (lds_ptr_t)(to + (wave * kLoads + i) * 512), 16, 0, 0);
       }
     }
   };
-  auto park_rows = [&](uint16_t* keys, uint16_t* values) {
+  auto park = [&](int side, Lds* to) __attribute__((always_inline)) {
     if constexpr (FP8) {
 #pragma unroll
-      for (int side = 0; side < 2; ++side)
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          *reinterpret_cast<u32x4*>((side ? values : keys) + ((wave * kLoads + i) * 64 + lane) * 8) =
-              fp8_eight<DT>(held8[side * kLoads + i]);
+      for (int i = 0; i < kLoads; ++i)
+        *(Lds16*)(to + ((wave * kLoads + i) * 64 + lane) * 8) =
+            fp8_eight<DT>(held8[side][i]);
     }
   };
 
   float base = -__builtin_inff(), sum = 0.0f;
   f32x16 acc[kTiles];
-  int page = 0, next_page = 0;
 
-  // One block, whose rows are in one stage, while those of the next go to the other. CAREFUL: values that
-  // are not finite are kept out of the products.
-  auto take = [&](auto careful, int block, uint16_t* keys, uint16_t* values, uint16_t* keys_next,
-                  uint16_t* values_next) __attribute__((always_inline)) {
-    constexpr bool kCareful = decltype(careful)::value != 0;
-    const bool more = block + 1 < block_end;
-    wait_vmcnt<0>();
-    __syncthreads();
-    const uint64_t on_page = __ballot(page_ok(page));
-    if (more) {
-      page = next_page;
-      request_rows(keys_next, values_next, block + 1, page);
-      if (block + 2 < block_end) next_page = look_up(block + 2);
+  // Scores of a block: operand row i is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4.
+  auto score = [&](const Lds* keys, f32x16 (&s)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = 32 * u + (col & 16) + ((col >> 2) & 1) * 8 + ((col >> 3) & 1) * 4 + (col & 3);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        if (GENERAL && 16 * k >= kLeastDim && 16 * k >= dim) break;
+        const int c = 2 * k + half;
+        const u32x4 key =
+            *(const Lds16*)(keys + (row * kChunks + key_place<kChunks>(c, row)) * 8);
+        s[u] = mfma32<DT>(key, query[k], s[u]);
+      }
     }
+  };
+  // -inf for keys that the row does not see, or that are on no page.
+  auto mask = [&](int block, uint64_t on_page, f32x16 (&s)[2]) __attribute__((always_inline)) {
     const int k0 = block * kBlock;
-    if (wave_rows > 0 && k0 < last_end && k0 + kBlock > first_begin) {
-      // ---- scores: operand row i is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4 ----
-      f32x16 s[2];
+    if (first_end >= k0 + kBlock && last_begin <= k0 && on_page == ~0ull) return;
+    const int end = my_end - k0 - 8 * half, begin = my_begin - k0 - 8 * half;
+    const uint64_t known = on_page >> (8 * half);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int row = 32 * u + (col & 16) + ((col >> 2) & 1) * 8 + ((col >> 3) & 1) * 4 + (col & 3);
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          if (PADDED && 16 * k >= kLeastDim && 16 * k >= dim) break;
-          const int c = 2 * k + half;
-          const u32x4 key = *reinterpret_cast<const u32x4*>(
-              keys + (row * kChunks + key_place<kChunks>(c, row)) * 8);
-          s[u] = mfma32<DT>(key, query[k], s[u]);
-        }
+      for (int i = 0; i < 16; ++i) {
+        const int j = 32 * u + 16 * (i / 8) + i % 8;  // and 8 of the half
+        const bool ok = j < end && j >= begin && (known >> j & 1);
+        s[u][i] = ok ? s[u][i] : -__builtin_inff();
       }
-
-      // ---- masks ----
-      const bool open = first_end >= k0 + kBlock && last_begin <= k0 && on_page == ~0ull;
-      if (!open) {
-        const int end = my_end - k0, begin = my_begin - k0;
+  };
+  auto largest = [&](const f32x16 (&s)[2]) __attribute__((always_inline)) {
+    float top = s[0][0];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int j = 32 * u + 16 * (i / 8) + 8 * half + i % 8;
-            const bool ok = j < end && j >= begin && (on_page >> j & 1);
-            s[u][i] = ok ? s[u][i] : -__builtin_inff();
-          }
-      }
-
-      // ---- running reference and sum ----
-      float top = s[0][0];
-#pragma unroll
-      for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i / 16][i % 16]);
-      top = halves_max(top) * a.scale_log2;
-      if (__any(top > base + kRoom)) {
-        const float next = fmaxf(base, top - kShift);
-        const float at = next == -__builtin_inff() ? 0.0f : next;
-        const float fix = fmaxf(__builtin_amdgcn_exp2f(base - at), kTiny);
-        sum *= fix;
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[t][i] *= fix;
-        base = next;
-      }
-      const float zero_at = base == -__builtin_inff() ? 0.0f : base;
-      u32x4 p[4];
-      float sums[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], a.scale_log2, -zero_at));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], a.scale_log2, -zero_at));
-        sums[0] += p0;
-        sums[1] += p1;
-        p[i / 8][i % 8 / 2] = pack2<DT>(p0, p1);
-      }
-      sum += sums[0] + sums[1];
-
-      // ---- values that are not finite: their keys one by one, since products with the zeros of rows
-      // that do not see them would make no numbers ----
-      if constexpr (kCareful) {
-        bool odd_row = false;
-#pragma unroll 1
-        for (int c = 0; c < kChunks; ++c) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(values + (lane * kChunks + c) * 8);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t x = w[j];
-            odd_row |= finite_pair<DT>(x) != x && (8 * value_place<kChunks>(c, lane) < dim);
-          }
-        }
-        uint64_t odd = __ballot(odd_row) & on_page;
-#pragma unroll 1
-        for (; odd; odd &= odd - 1) {
-          const int j = __ffsll((unsigned long long)odd) - 1;
-          const int reg = 16 * (j / 32) + 8 * (j / 16 % 2) + j % 8;
-          float x = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x = i == reg ? s[i / 16][i % 16] : x;
-          x = __shfl(x, col + 32 * (j / 8 % 2));
-          float w = __builtin_amdgcn_exp2f(fmaf(x, a.scale_log2, -zero_at));
-          w = w == 0.0f ? kTiny : w;  // below fp32's range, but not nothing
-          const bool seen = !(x == -__builtin_inff());
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const int d = 32 * t + 2 * i + 4 * half;
-              const u32x2 v = *reinterpret_cast<const u32x2*>(
-                  values + (j * kChunks + value_place<kChunks>(d / 8, j)) * 8 + (d & 7));
-              const uint32_t lo = v.x, hi = v.y;
-              const float f[4] = {lo16<DT>(lo), hi16<DT>(lo), lo16<DT>(hi), hi16<DT>(hi)};
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (seen && !(fabsf(f[e]) < __builtin_inff())) acc[t][i + e] += w * f[e];
-            }
-        }
-      }
-
-      // ---- values: 4 rows by 16 columns a group of 16 lanes, transposed on the way ----
-      const int in_group = lane & 15;
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+    return halves_max(top) * a.scale_log2;
+  };
+  // A reference near the maximum; what has been summed follows it.
+  auto refer = [&](float top) __attribute__((always_inline)) {
+    if (__any(top > base + kRoom)) {
+      const float next = fmaxf(base, top - kShift);
+      const float at = next == -__builtin_inff() ? 0.0f : next;
+      const float fix = fmaxf(__builtin_amdgcn_exp2f(base - at), kTiny);
+      sum *= fix;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          u32x4 v;
+        for (int i = 0; i < 16; ++i) acc[t][i] *= fix;
+      base = next;
+    }
+  };
+  auto weigh = [&](const f32x16 (&s)[2], u32x4 (&p)[4]) __attribute__((always_inline)) {
+    const float zero_at = base == -__builtin_inff() ? 0.0f : base;
+    float sums[2] = {0.0f, 0.0f};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = 16 * k + 8 * half + 4 * e + (in_group >> 2);
-            const int c = 4 * t + ((lane >> 4) & 1) * 2 + ((in_group & 3) >> 1);
-            const uint16_t* at = values + (row * kChunks + value_place<kChunks>(c, row)) * 8 +
-                                 4 * (in_group & 1);
-            const u32x2 w = __builtin_bit_cast(
-                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                           (__attribute__((address_space(3))) s16x4*)(at)));
-            v[2 * e] = w.x;
-            v[2 * e + 1] = w.y;
-          }
-          if constexpr (kCareful) {
+    for (int i = 0; i < 32; i += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], a.scale_log2, -zero_at));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], a.scale_log2, -zero_at));
+      sums[0] += p0;
+      sums[1] += p1;
+      p[i / 8][i % 8 / 2] = pack2<DT>(p0, p1);
+    }
+    sum += sums[0] + sums[1];
+  };
+  // Values: 4 rows by 16 columns a group of 16 lanes, transposed on the way.
+  auto add = [&](auto careful, const Lds* values, const u32x4 (&p)[4])
+      __attribute__((always_inline)) {
+    const int in_group = lane & 15;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t x = v[j];
-              v[j] = finite_pair<DT>(x);
-            }
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        u32x4 v;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = 16 * k + 8 * half + 4 * e + (in_group >> 2);
+          const int c = 4 * t + ((lane >> 4) & 1) * 2 + ((in_group & 3) >> 1);
+          const Lds* at =
+              values + (row * kChunks + value_place<kChunks>(c, row)) * 8 + 4 * (in_group & 1);
+          const u32x2 w = __builtin_bit_cast(
+              u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                         (__attribute__((address_space(3))) s16x4*)(at)));
+          v[2 * e] = w.x;
+          v[2 * e + 1] = w.y;
+        }
+        if constexpr (decltype(careful)::value != 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t x = v[j];
+            v[j] = finite_pair<DT>(x);
           }
-          acc[t] = mfma32<DT>(v, p[k], acc[t]);
+        }
+        acc[t] = mfma32<DT>(v, p[k], acc[t]);
+      }
+  };
+  // Values that are not finite: their keys one by one, since products with the zeros of rows that do not
+  // see them would make no numbers.
+  auto add_odd = [&](const Lds* values, uint64_t on_page, const f32x16 (&s)[2])
+      __attribute__((always_inline)) {
+    const float zero_at = base == -__builtin_inff() ? 0.0f : base;
+    bool odd_row = false;
+#pragma unroll 1
+    for (int c = 0; c < kChunks; ++c) {
+      const u32x4 w = *(const Lds16*)(values + (lane * kChunks + c) * 8);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x = w[j];
+        odd_row |= finite_pair<DT>(x) != x && (8 * value_place<kChunks>(c, lane) < dim);
+      }
+    }
+    uint64_t odd = __ballot(odd_row) & on_page;
+#pragma unroll 1
+    for (; odd; odd &= odd - 1) {
+      const int j = __ffsll((unsigned long long)odd) - 1;
+      const int reg = 16 * (j / 32) + 8 * (j / 16 % 2) + j % 8;
+      float x = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x = i == reg ? s[i / 16][i % 16] : x;
+      x = __shfl(x, col + 32 * (j / 8 % 2));
+      float w = __builtin_amdgcn_exp2f(fmaf(x, a.scale_log2, -zero_at));
+      w = w == 0.0f ? kTiny : w;  // below fp32's range, but not nothing
+      const bool seen = !(x == -__builtin_inff());
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int d = 32 * t + 2 * i + 4 * half;
+          const u32x2 v = *(const Lds8*)(
+              values + (j * kChunks + value_place<kChunks>(d / 8, j)) * 8 + (d & 7));
+          const uint32_t lo = v.x, hi = v.y;
+          const float f[4] = {lo16<DT>(lo), hi16<DT>(lo), lo16<DT>(hi), hi16<DT>(hi)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (seen && !(fabsf(f[e]) < __builtin_inff())) acc[t][i + e] += w * f[e];
         }
     }
-    if (more) park_rows(keys_next, values_next);
   };
-  auto take_all = [&](auto careful) __attribute__((always_inline)) {
+
+  // ---- the blocks ----
+  // A wave's last block: later ones only pass through it for the others' sake.
+  const int wave_end =
+      wave_rows > 0 ? min(block_end, (last_end + kBlock - 1) / kBlock) : block0;
+  auto clear = [&]() {
     base = -__builtin_inff();
     sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
-    if (block0 >= block_end) return;
-    page = look_up(block0);
-    request_rows(keys0, values0, block0, page);
-    if (block0 + 1 < block_end) next_page = look_up(block0 + 1);
-    park_rows(keys0, values0);
-    for (int block = block0;;) {
-      take(careful, block, keys0, values0, keys1, values1);
-      if (++block >= block_end) break;
-      take(careful, block, keys1, values1, keys0, values0);
-      if (++block >= block_end) break;
-    }
   };
-  take_all(IntConst<0>());
+  // While a block's probabilities are taken, the next one's scores are under way; keys are requested two
+  // blocks ahead, values one, table entries a block before that. (Blocks past the end stand for the last
+  // one: steps have no branches for them.)
+  clear();
+  if (block0 < block_end) {
+    f32x16 s[2];
+    float top = 0.0f;
+    // entries of the block whose values are requested next, whose keys are, and of the one after
+    int page1 = look_up(block0), page2 = look_up(block0 + 1), page3 = look_up(block0 + 2);
+    uint64_t on_page = __ballot(page_ok(page1));  // of the block whose scores come next
+    request(0, keys0, block0, page1);
+    request(1, values0, block0, page1);
+    park(0, keys0);
+    park(1, values0);
+    request(0, keys1, block0 + 1, page2);
+    park(0, keys1);
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (block0 < wave_end) {
+      score(keys0, s);
+      mask(block0, on_page, s);
+      top = largest(s);
+    }
+    // Block `block`, whose values are in `values`, with scores s; the next one's keys in keys_next.
+    auto take = [&](auto next, int block, Lds* keys, Lds* values, Lds* keys_next, Lds* values_next)
+        __attribute__((always_inline)) {
+      constexpr int kNext = decltype(next)::value;  // 1: scores of the next block too, -1: neither
+      wait_vmcnt<0>();
+      __syncthreads();
+      on_page = __ballot(page_ok(page2));
+      request(1, values_next, block + 1, page2);
+      request(0, keys, block + 2, page3);
+      page2 = page3;
+      page3 = look_up(block + 3);
+      if constexpr (kNext >= 0) {
+        refer(top);
+        u32x4 p[4];
+        f32x16 s_next[2];
+        if constexpr (kNext > 0) score(keys_next, s_next);
+        weigh(s, p);
+        if constexpr (kNext > 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) __asm__ volatile("" : "+v"(p[i]));  // (not behind the mask)
+          mask(block + 1, on_page, s_next);
+          top = largest(s_next);
+        }
+        add(IntConst<0>(), values, p);
+        if constexpr (kNext > 0) {
+          s[0] = s_next[0];
+          s[1] = s_next[1];
+        }
+      }
+      park(1, values_next);
+      park(0, keys);
+    };
+    int block = block0;
+#pragma unroll 1
+    for (; block + 2 < wave_end; block += 2) {
+      take(IntConst<1>(), block, keys0, values0, keys1, values1);
+      take(IntConst<1>(), block + 1, keys1, values1, keys0, values0);
+    }
+    bool swapped = false;
+    if (block + 1 < wave_end) {
+      take(IntConst<1>(), block, keys0, values0, keys1, values1);
+      take(IntConst<0>(), block + 1, keys1, values1, keys0, values0);
+      block += 2;
+    } else if (block < wave_end) {
+      take(IntConst<0>(), block, keys0, values0, keys1, values1);
+      ++block;
+      swapped = true;
+    }
+#pragma unroll 1
+    for (; block < block_end; ++block, swapped = !swapped)
+      take(IntConst<-1>(), block, swapped ? keys1 : keys0, swapped ? values1 : values0,
+           swapped ? keys0 : keys1, swapped ? values0 : values1);
+    wait_vmcnt<0>();  // (rows on their way to LDS that is not this workgroup's any more)
+  }
   // A value that is not finite may have met a zero of a row that does not see it: once more, with
   // care (for rows that see it the result stays what it is).
   float odd = 0.0f;
@@ -474,7 +560,33 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) odd = fmaf(acc[t][i], 0.0f, odd);
-  if (__syncthreads_or(odd != 0.0f)) take_all(IntConst<1>());
+  if (__syncthreads_or(odd != 0.0f)) {
+    __asm__ volatile("" : "+v"(lane));  // no address of this is to be reckoned, and kept, before
+    col = lane & 31, half = lane >> 5;
+    clear();
+#pragma unroll 1
+    for (int block = block0; block < block_end; ++block) {
+      const int page = look_up(block);
+      request(0, keys0, block, page);
+      request(1, values0, block, page);
+      park(0, keys0);
+      park(1, values0);
+      wait_vmcnt<0>();
+      __syncthreads();
+      if (block < wave_end) {
+        const uint64_t on_page = __ballot(page_ok(page));
+        f32x16 s[2];
+        score(keys0, s);
+        mask(block, on_page, s);
+        refer(largest(s));
+        u32x4 p[4];
+        weigh(s, p);
+        add_odd(values0, on_page, s);
+        add(IntConst<1>(), values0, p);
+      }
+      __syncthreads();
+    }
+  }
   sum = halves_sum(sum);
 
   // ---- the result, or this part of it ----
@@ -581,7 +693,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ChunkAttentionArgs a) {
 template <int DT, bool FP8, int DIM>
 hipError_t launch_dim(const ChunkAttentionArgs& a, hipStream_t stream) {
   const unsigned items = (unsigned)(a.most_tiles + a.target) * (unsigned)a.kv_heads;
-  if (a.dim == DIM) attention_kernel<DT, FP8, DIM, false><<<items, kThreads, 0, stream>>>(a);
+  if (a.dim == DIM && a.narrow)
+    attention_kernel<DT, FP8, DIM, false><<<items, kThreads, 0, stream>>>(a);
   else attention_kernel<DT, FP8, DIM, true><<<items, kThreads, 0, stream>>>(a);
   if (a.most_parts > 0)
     join_kernel<DT, DIM><<<dim3((unsigned)a.most_parts * (unsigned)a.kv_heads, DIM / 32), kThreads,

@@ -452,6 +452,10 @@ int mt_paged_chunk_attention(const mt_paged_cache* cache, const mt_paged_chunk_a
   a.scale_log2 = std::max(std::fabs(scale_log2), FLT_MIN);
   a.flip = scale_log2 < 0.0f ? 0x80008000u : 0u;
   a.value_scale = cache->value_scale;
+  a.narrow = true;
+  for (const int64_t* strides : {cache->key_strides, cache->value_strides})
+    a.narrow &= ((cache->pages - 1) * strides[0] + (cache->page_size - 1) * strides[1] + cache->dim) *
+                    bytes <= (int64_t)UINT32_MAX;
   return launched(op, mt::launch_chunk_attention(a, in.dtype, fp8, static_cast<hipStream_t>(stream)));
 }
 
