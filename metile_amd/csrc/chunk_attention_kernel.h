@@ -325,21 +325,33 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   float base = -__builtin_inff(), sum = 0.0f;
   f32x16 acc[kTiles];
 
-  // Scores of a block: operand row i is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4.
-  auto score = [&](const Lds* keys, f32x16 (&s)[2]) __attribute__((always_inline)) {
+  // Scores of a block: operand row i is key 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4. Operands
+  // are read kAhead products ahead; `between` is done after each product, in this order: left to itself
+  // the compiler puts all products first, the waves of a SIMD fall into step, and its matrix and vector
+  // units take turns instead of working side by side.
+  constexpr int kAhead = 3, kScores = 2 * kSteps, kSums = 4 * kTiles;
+  auto score = [&](const Lds* keys, f32x16 (&s)[2], auto between) __attribute__((always_inline)) {
+    u32x4 key[kScores];
+    auto read = [&](int n) __attribute__((always_inline)) {
+      const int row =
+          32 * (n & 1) + (col & 16) + ((col >> 2) & 1) * 8 + ((col >> 3) & 1) * 4 + (col & 3);
+      const int c = 2 * (n >> 1) + half;
+      key[n] = *(const Lds16*)(keys + (row * kChunks + key_place<kChunks>(c, row)) * 8);
+    };
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = 32 * u + (col & 16) + ((col >> 2) & 1) * 8 + ((col >> 3) & 1) * 4 + (col & 3);
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        if (GENERAL && 16 * k >= kLeastDim && 16 * k >= dim) break;
-        const int c = 2 * k + half;
-        const u32x4 key =
-            *(const Lds16*)(keys + (row * kChunks + key_place<kChunks>(c, row)) * 8);
-        s[u] = mfma32<DT>(key, query[k], s[u]);
-      }
+    for (int n = 0; n < kAhead; ++n) read(n);
+#pragma unroll
+    for (int n = 0; n < kScores; ++n) {
+      if (n + kAhead < kScores) read(n + kAhead);
+      // (with GENERAL, steps that the head does not have are skipped)
+      if (!GENERAL || 8 * (n & ~1) < kLeastDim || 8 * (n & ~1) < dim)
+        s[n & 1] = mfma32<DT>(key[n], query[n >> 1], s[n & 1]);
+      between(n);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // -inf for keys that the row does not see, or that are on no page.
@@ -361,6 +373,9 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
     float top = s[0][0];
 #pragma unroll
     for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+    return top;
+  };
+  auto of_row_max = [&](float top) __attribute__((always_inline)) {
     return halves_max(top) * a.scale_log2;
   };
   // A reference near the maximum; what has been summed follows it.
@@ -377,50 +392,58 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
       base = next;
     }
   };
-  auto weigh = [&](const f32x16 (&s)[2], u32x4 (&p)[4]) __attribute__((always_inline)) {
-    const float zero_at = base == -__builtin_inff() ? 0.0f : base;
-    float sums[2] = {0.0f, 0.0f};
+  // Probabilities of a row's scores `from` to `to` (two at a time).
+  auto weigh = [&](const f32x16 (&s)[2], u32x4 (&p)[4], float zero_at, float (&sums)[2], int from,
+                   int to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
+    for (int i = from; i < to; i += 2) {
       const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], a.scale_log2, -zero_at));
       const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], a.scale_log2, -zero_at));
       sums[0] += p0;
       sums[1] += p1;
-      p[i / 8][i % 8 / 2] = pack2<DT>(p0, p1);
+      uint32_t pair = pack2<DT>(p0, p1);
+      __asm__ volatile("" : "+v"(pair), "+v"(sums[0]), "+v"(sums[1]));  // (here, and not later)
+      p[i / 8][i % 8 / 2] = pair;
     }
-    sum += sums[0] + sums[1];
   };
   // Values: 4 rows by 16 columns a group of 16 lanes, transposed on the way.
-  auto add = [&](auto careful, const Lds* values, const u32x4 (&p)[4])
+  auto add = [&](auto careful, const Lds* values, const u32x4 (&p)[4], auto between)
       __attribute__((always_inline)) {
     const int in_group = lane & 15;
+    u32x4 v[kSums];
+    auto read = [&](int n) __attribute__((always_inline)) {
+      const int k = n / kTiles, t = n % kTiles;
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        u32x4 v;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = 16 * k + 8 * half + 4 * e + (in_group >> 2);
-          const int c = 4 * t + ((lane >> 4) & 1) * 2 + ((in_group & 3) >> 1);
-          const Lds* at =
-              values + (row * kChunks + value_place<kChunks>(c, row)) * 8 + 4 * (in_group & 1);
-          const u32x2 w = __builtin_bit_cast(
-              u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                         (__attribute__((address_space(3))) s16x4*)(at)));
-          v[2 * e] = w.x;
-          v[2 * e + 1] = w.y;
-        }
-        if constexpr (decltype(careful)::value != 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t x = v[j];
-            v[j] = finite_pair<DT>(x);
-          }
-        }
-        acc[t] = mfma32<DT>(v, p[k], acc[t]);
+      for (int e = 0; e < 2; ++e) {
+        const int row = 16 * k + 8 * half + 4 * e + (in_group >> 2);
+        const int c = 4 * t + ((lane >> 4) & 1) * 2 + ((in_group & 3) >> 1);
+        const Lds* at =
+            values + (row * kChunks + value_place<kChunks>(c, row)) * 8 + 4 * (in_group & 1);
+        const u32x2 w = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                       (__attribute__((address_space(3))) s16x4*)(at)));
+        v[n][2 * e] = w.x;
+        v[n][2 * e + 1] = w.y;
       }
+    };
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) read(n);
+#pragma unroll
+    for (int n = 0; n < kSums; ++n) {
+      if (n + kAhead < kSums) read(n + kAhead);
+      if constexpr (decltype(careful)::value != 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x = v[n][j];
+          v[n][j] = finite_pair<DT>(x);
+        }
+      }
+      acc[n % kTiles] = mfma32<DT>(v[n], p[n / kTiles], acc[n % kTiles]);
+      between(n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
+  auto nothing = [](int) {};
   // Values that are not finite: their keys one by one, since products with the zeros of rows that do not
   // see them would make no numbers.
   auto add_odd = [&](const Lds* values, uint64_t on_page, const f32x16 (&s)[2])
@@ -495,9 +518,9 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
     wait_vmcnt<0>();
     __syncthreads();
     if (block0 < wave_end) {
-      score(keys0, s);
+      score(keys0, s, nothing);
       mask(block0, on_page, s);
-      top = largest(s);
+      top = of_row_max(largest(s));
     }
     // Block `block`, whose values are in `values`, with scores s; the next one's keys in keys_next.
     auto take = [&](auto next, int block, Lds* keys, Lds* values, Lds* keys_next, Lds* values_next)
@@ -506,26 +529,49 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
       wait_vmcnt<0>();
       __syncthreads();
       on_page = __ballot(page_ok(page2));
-      request(1, values_next, block + 1, page2);
-      request(0, keys, block + 2, page3);
-      page2 = page3;
-      page3 = look_up(block + 3);
+      auto request_values = [&]() __attribute__((always_inline)) {
+        request(1, values_next, block + 1, page2);
+      };
+      auto request_keys = [&]() __attribute__((always_inline)) {
+        request(0, keys, block + 2, page3);
+        page2 = page3;
+        page3 = look_up(block + 3);
+      };
+      if constexpr (kNext <= 0) {
+        request_values();
+        request_keys();
+      }
       if constexpr (kNext >= 0) {
         refer(top);
+        const float zero_at = base == -__builtin_inff() ? 0.0f : base;
+        float sums[2] = {0.0f, 0.0f};
         u32x4 p[4];
-        f32x16 s_next[2];
-        if constexpr (kNext > 0) score(keys_next, s_next);
-        weigh(s, p);
         if constexpr (kNext > 0) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) __asm__ volatile("" : "+v"(p[i]));  // (not behind the mask)
+          f32x16 s_next[2];
+          score(keys_next, s_next, [&](int n) __attribute__((always_inline)) {
+            // rows are asked for first, the 32 probabilities follow
+            constexpr int kFirst = kScores / 4;
+            if (n == 0) request_values();
+            if (n == kFirst / 2) request_keys();
+            if (n >= kFirst)
+              weigh(s, p, zero_at, sums, (n - kFirst) * 16 / (kScores - kFirst) * 2,
+                    (n + 1 - kFirst) * 16 / (kScores - kFirst) * 2);
+          });
+          sum += sums[0] + sums[1];
           mask(block + 1, on_page, s_next);
-          top = largest(s_next);
-        }
-        add(IntConst<0>(), values, p);
-        if constexpr (kNext > 0) {
+          float tops[2] = {s_next[0][0], s_next[1][0]};
+          add(IntConst<0>(), values, p, [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = n * 32 / kSums; i < (n + 1) * 32 / kSums; ++i)
+              tops[i / 16] = fmaxf(tops[i / 16], s_next[i / 16][i % 16]);
+          });
+          top = of_row_max(fmaxf(tops[0], tops[1]));
           s[0] = s_next[0];
           s[1] = s_next[1];
+        } else {
+          weigh(s, p, zero_at, sums, 0, 32);
+          sum += sums[0] + sums[1];
+          add(IntConst<0>(), values, p, nothing);
         }
       }
       park(1, values_next);
@@ -576,13 +622,15 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
       if (block < wave_end) {
         const uint64_t on_page = __ballot(page_ok(page));
         f32x16 s[2];
-        score(keys0, s);
+        score(keys0, s, nothing);
         mask(block, on_page, s);
-        refer(largest(s));
+        refer(of_row_max(largest(s)));
         u32x4 p[4];
-        weigh(s, p);
+        float sums[2] = {0.0f, 0.0f};
+        weigh(s, p, base == -__builtin_inff() ? 0.0f : base, sums, 0, 32);
+        sum += sums[0] + sums[1];
         add_odd(values0, on_page, s);
-        add(IntConst<1>(), values0, p);
+        add(IntConst<1>(), values0, p, nothing);
       }
       __syncthreads();
     }
