@@ -12,6 +12,10 @@ namespace mt {
 // Rows (token, query head of a key-value head) of a tile, and keys of a block.
 constexpr int kChunkTile = 128;
 constexpr int kChunkBlock = 64;
+// Blocks that a part of a tile's keys has at least, and requests of a call whose work its workgroups count
+// up themselves.
+constexpr int kChunkLeastBlocks = 4;
+constexpr int kChunkHere = 64;
 
 struct ChunkAttentionArgs {
   const uint16_t* query;                // [tokens, heads, dim], last dimension contiguous

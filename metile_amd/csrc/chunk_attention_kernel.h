@@ -23,6 +23,9 @@
 #include "chunk_attention.h"
 #include "common.h"
 
+#ifndef WAVES64
+#define WAVES64 2
+#endif
 namespace mt {
 namespace chunk {
 
@@ -70,20 +73,95 @@ __device__ __forceinline__ int most_blocks(const ChunkAttentionArgs& a, const Re
   return (int)min((int64_t)all, (tile + kBlock - 1) / kBlock + 1);
 }
 
-// The last request whose prefix is at most n (prefix[0] = 0, not decreasing): 64 at a time, by a
-// whole wave.
-__device__ __forceinline__ int find(const int32_t* prefix, int requests, int n) {
+// Parts of each tile of a request whose tiles have up to `most` blocks.
+__device__ __forceinline__ int splits_of(int most, int per) {
+  return max((int)(((int64_t)most + per - 1) / per), 1);
+}
+
+// An item: a request's tile, or one part of `splits` of its keys; `part` is where a part is kept.
+struct Item {
+  int request, splits, in_request, part;  // request -1: none
+  Request q;
+  __device__ int tile(const ChunkAttentionArgs& a) const {  // the longest first
+    return tiles_of(a, q) - 1 - in_request / splits;
+  }
+};
+
+// Inclusive sums over the lanes: within rows of 16, then across them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_read_int(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  auto from = [](T x, auto read) { return __builtin_bit_cast(T, read(__builtin_bit_cast(int, x))); };
+  v += from(v, dpp_read_int<0x111, 0xF>);  // row_shr:1
+  v += from(v, dpp_read_int<0x112, 0xF>);
+  v += from(v, dpp_read_int<0x114, 0xF>);
+  v += from(v, dpp_read_int<0x118, 0xF>);
+  v += from(v, dpp_read_int<kDppRowBcast15, 0xA>);
+  v += from(v, dpp_read_int<kDppRowBcast31, 0xC>);
+  return v;
+}
+__device__ __forceinline__ int readlane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+
+// Item n, or with PARTS the item that part n is of, of a call of up to 64 requests: each wave counts the
+// work up for itself, a lane a request. `behind` receives the packed row behind the last request's.
+template <bool PARTS>
+__device__ __forceinline__ Item find_here(const ChunkAttentionArgs& a, int n, int* behind) {
+  const int lane = threadIdx.x & 63, r = min(lane, a.requests - 1);
+  const Request q = request_of(a, r);
+  *behind = readlane(min(max(a.starts[r + 1], 0), a.tokens), a.requests - 1);
+  const int tiles = lane < a.requests ? tiles_of(a, q) : 0, most = most_blocks(a, q);
+  // (rounded up, so that there are no more than `target` parts on top of the tiles)
+  const float total =
+      __builtin_bit_cast(float, readlane(__builtin_bit_cast(int, wave_scan((float)tiles * (float)most)),
+                                         63));
+  const int per =
+      max((int)fminf(total * 1.0001f / (float)a.target + 1.0f, 1073741824.0f), kChunkLeastBlocks);
+  const int splits = splits_of(most, per);
+  const int items = tiles * splits, parts = splits > 1 ? items : 0;
+  const int item_sums = wave_scan(items), part_sums = wave_scan(parts);
+  const uint64_t later = __ballot((PARTS ? part_sums : item_sums) > n);
+  Item i{-1, 1, 0, 0, {}};
+  if (!later) return i;
+  const int l = __ffsll((unsigned long long)later) - 1;
+  i.request = l;
+  i.splits = readlane(splits, l);
+  i.in_request = n - readlane(PARTS ? part_sums - parts : item_sums - items, l);
+  i.part = readlane(part_sums - parts, l) + i.in_request;
+  i.q = {readlane(q.start, l), readlane(q.count, l), readlane(q.first, l), readlane(q.keys, l)};
+  return i;
+}
+
+// The same of a call of more requests, from the sums that the plan holds: the last request whose sum of
+// those before it is at most n, 64 at a time, by a whole wave.
+template <bool PARTS>
+__device__ __forceinline__ Item find_planned(const ChunkAttentionArgs& a, int n, int* behind) {
   const int lane = threadIdx.x & 63;
+  const int32_t *items = a.plan + kPlanHead, *parts = items + a.requests + 1;
+  const int32_t* sums = PARTS ? parts : items;
+  *behind = min(max(a.starts[a.requests], 0), a.tokens);
+  Item i{-1, 1, 0, 0, {}};
+  if (n >= a.plan[PARTS ? 2 : 1]) return i;
   int lo = 0;
-  for (int count = requests; count > 1;) {
+  for (int count = a.requests; count > 1;) {
     const int step = (count + 63) / 64;
-    const int at = lo + lane * step;
-    const bool ok = lane * step < count && prefix[at] <= n;
+    const bool ok = lane * step < count && sums[lo + lane * step] <= n;
     const int last = 63 - __clzll((long long)__ballot(ok));
     lo = uniform(lo + last * step);
     count = min(step, uniform(count) - last * step);
   }
-  return lo;
+  i.request = lo;
+  i.q = request_of(a, lo);
+  i.splits = splits_of(most_blocks(a, i.q), a.plan[0]);
+  i.in_request = n - sums[lo];
+  i.part = parts[lo] + i.in_request;
+  return i;
+}
+template <bool PARTS>
+__device__ __forceinline__ Item find(const ChunkAttentionArgs& a, int n, int* behind) {
+  return a.requests <= kChunkHere ? find_here<PARTS>(a, n, behind) : find_planned<PARTS>(a, n, behind);
 }
 
 template <int DT>
@@ -166,7 +244,7 @@ struct Offset<false> {
 // DIM: the head's values. With GENERAL, that many or more (the rest count as zero), in caches of any size;
 // else the offsets of rows fit 32 bits.
 template <int DT, bool FP8, int DIM, bool GENERAL>
-__global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel(
+__global__ __launch_bounds__(kThreads, DIM == 64 ? WAVES64 : DIM <= 128 ? 2 : 1) void attention_kernel(
     ChunkAttentionArgs a) {
   constexpr int kChunks = DIM / 8, kSteps = DIM / 16, kTiles = DIM / 32;
   constexpr int kLoads = kChunks * kBlock / kThreads;  // of a thread, a side
@@ -188,11 +266,15 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   int lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int dim = GENERAL ? a.dim : DIM;
 
+  // ---- this workgroup's item: a tile of a request, or a part of its keys, for one head ----
+  const int head = (int)(blockIdx.x % (unsigned)a.kv_heads);
+  int behind;
+  const Item item = find<false>(a, (int)(blockIdx.x / (unsigned)a.kv_heads), &behind);
+
   // ---- rows that belong to no request ----
   {
-    const int from = min(max(a.starts[a.requests], 0), a.tokens);
     const int row_words = a.kv_heads * a.group * (dim / 8);
-    for (int row = from + (int)blockIdx.x; row < a.tokens; row += (int)gridDim.x) {
+    for (int row = behind + (int)blockIdx.x; row < a.tokens; row += (int)gridDim.x) {
       u32x4* to = reinterpret_cast<u32x4*>(a.out) + (int64_t)row * row_words;
       for (int i = tid; i < row_words; i += kThreads) to[i] = (u32x4){0, 0, 0, 0};
       if (a.lse)
@@ -201,22 +283,11 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
     }
   }
 
-  // ---- this workgroup's item: a tile of a request, or a part of its keys, for one head ----
-  const int head = (int)(blockIdx.x % (unsigned)a.kv_heads);
-  const int item = (int)(blockIdx.x / (unsigned)a.kv_heads);
-  const int per = a.plan[0];
-  if (item >= a.plan[1]) return;
-  const int32_t* items = a.plan + kPlanHead;
-  const int32_t* part_items = items + a.requests + 1;
-  const int r = find(items, a.requests, item);
-  const Request q = request_of(a, r);
-  const int most = most_blocks(a, q);
-  const int splits = max((most + per - 1) / per, 1);
-  const int tiles = tiles_of(a, q);
-  const int in_request = item - items[r];
-  const int tile = tiles - 1 - in_request / splits;  // the longest first
-  const int split = in_request % splits;
-  if (tile < 0 || (splits > 1 && part_items[r] + in_request >= a.most_parts)) return;
+  if (item.request < 0) return;
+  const int r = item.request, splits = item.splits;
+  const Request q = item.q;
+  const int tile = item.tile(a), split = item.in_request % splits;
+  if (tile < 0 || (splits > 1 && item.part >= a.most_parts)) return;
   const int row0 = tile * kTile, rows = min(kTile, q.count * a.group - row0);
   const Blocks all = blocks_of(a, q, (int)div_by(row0, a.by_group),
                                (int)div_by(row0 + rows - 1, a.by_group));
@@ -238,6 +309,7 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   const int first_begin = __builtin_amdgcn_readlane(my_begin, 0);
   const int last_begin = __builtin_amdgcn_readlane(my_begin, 31);
 
+  // (what depends on these is left for later: entries and rows are on their way at the same time)
   u32x4 query[kSteps];
   {
     const uint16_t* p = a.query + (int64_t)(q.start + my_token) * a.q_row_stride +
@@ -246,10 +318,15 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
     for (int s = 0; s < kSteps; ++s) {
       const int d = 16 * s + 8 * half;
       query[s] = *reinterpret_cast<const u32x4*>(p + (d < dim ? d : 0));
-      query[s] ^= a.flip;
-      if (!has_row || d >= dim) query[s] = (u32x4){0, 0, 0, 0};
     }
   }
+  auto finish_query = [&]() {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      query[s] ^= a.flip;
+      if (!has_row || 16 * s + 8 * half >= dim) query[s] = (u32x4){0, 0, 0, 0};
+    }
+  };
 
   const int32_t* table = a.tables + (int64_t)r * a.table_stride;
   const unsigned char* kbase = a.key + (int64_t)head * a.k_head;
@@ -515,6 +592,7 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
     park(1, values0);
     request(0, keys1, block0 + 1, page2);
     park(0, keys1);
+    finish_query();
     wait_vmcnt<0>();
     __syncthreads();
     if (block0 < wave_end) {
@@ -640,7 +718,7 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   // ---- the result, or this part of it ----
   if (wave_rows <= 0) return;
   if (splits > 1) {
-    const int64_t part = (int64_t)(part_items[r] + in_request) * a.kv_heads + head;
+    const int64_t part = (int64_t)item.part * a.kv_heads + head;
     float* to = a.parts + part * (kTile * (DIM + 2));
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
@@ -679,14 +757,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ChunkAttentionArgs a) {
   const int col = lane & 31, half = lane >> 5;
   const int head = (int)(blockIdx.x % (unsigned)a.kv_heads);
   const int part = (int)(blockIdx.x / (unsigned)a.kv_heads), t = blockIdx.y;
-  if (part >= a.plan[2]) return;
-  const int32_t* part_items = a.plan + kPlanHead + a.requests + 1;
-  const int r = find(part_items, a.requests, part);
-  const Request q = request_of(a, r);
-  const int splits = max((most_blocks(a, q) + a.plan[0] - 1) / a.plan[0], 1);
-  const int in_request = part - part_items[r];
-  if (in_request % splits || part + splits > a.most_parts) return;
-  const int tile = tiles_of(a, q) - 1 - in_request / splits;
+  int behind;
+  const Item item = find<true>(a, part, &behind);
+  if (item.request < 0) return;
+  const Request q = item.q;
+  const int splits = item.splits, tile = item.tile(a);
+  if (item.in_request % splits || part + splits > a.most_parts) return;
   if (tile < 0) return;
   const int row0 = tile * kTile, rows = min(kTile, q.count * a.group - row0);
   if (32 * wave >= rows) return;
