@@ -291,8 +291,8 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? WAVES64 : DIM <= 128 ? 2 : 1)
   const int row0 = tile * kTile, rows = min(kTile, q.count * a.group - row0);
   const Blocks all = blocks_of(a, q, (int)div_by(row0, a.by_group),
                                (int)div_by(row0 + rows - 1, a.by_group));
-  const int block0 = all.first + (int)((int64_t)all.count * split / splits);
-  const int block_end = all.first + (int)((int64_t)all.count * (split + 1) / splits);
+  const int block0 = uniform(all.first + (int)((int64_t)all.count * split / splits));
+  const int block_end = uniform(all.first + (int)((int64_t)all.count * (split + 1) / splits));
 
   // ---- this lane's row, and what the wave's rows see ----
   const int wave_rows = min(rows - 32 * wave, 32);  // may be none
@@ -337,16 +337,23 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? WAVES64 : DIM <= 128 ? 2 : 1)
   // offset. Tokens past the end stand for the last one, tokens on no page of the cache for page 0;
   // both are masked.
   typedef typename Offset<GENERAL>::type RowOffset;
-  auto look_up = [&](int block) {
-    const int token = min(block * kBlock + lane, last_key);
-    return table[div_by((uint32_t)token, a.by_page)];
+  struct Place {
+    int page;
+    uint32_t slot;
   };
-  auto page_ok = [&](int page) { return (uint32_t)page < (uint32_t)a.pages; };
-  auto offset_of = [&](int block, int page, uint32_t page_stride, uint32_t slot_stride) {
+  auto look_up = [&](int block) __attribute__((always_inline)) {
     const uint32_t token = (uint32_t)min(block * kBlock + lane, last_key);
-    const uint32_t slot = token - div_by(token, a.by_page) * (uint32_t)a.page_size;
-    return (RowOffset)(page_ok(page) ? (uint32_t)page : 0u) * page_stride +
-           (RowOffset)slot * slot_stride;
+    const uint32_t column = div_by(token, a.by_page);
+    return Place{table[column], token - column * (uint32_t)a.page_size};
+  };
+  struct Offsets {
+    RowOffset key, value;
+    uint64_t on_page;  // of the block's tokens, which are on a page of the cache
+  };
+  auto offsets_of = [&](const Place& p) __attribute__((always_inline)) {
+    const bool ok = (uint32_t)p.page < (uint32_t)a.pages;
+    const RowOffset page = ok ? (uint32_t)p.page : 0u, slot = p.slot;
+    return Offsets{page * a.k_page + slot * a.k_slot, page * a.v_page + slot * a.v_slot, __ballot(ok)};
   };
   auto of_row = [&](RowOffset offset, int row) {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * row, (int)(uint32_t)offset);
@@ -359,9 +366,7 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? WAVES64 : DIM <= 128 ? 2 : 1)
   // One side of a block to LDS. Chunk i of this thread: LDS chunk n of the stage is row n / kChunks, place
   // n % kChunks. 8-bit rows wait in registers until they are parked.
   u32x2 held8[2][FP8 ? kLoads : 1];
-  auto request = [&](int side, Lds* to, int block, int page) __attribute__((always_inline)) {
-    const RowOffset offset = side ? offset_of(block, page, a.v_page, a.v_slot)
-                                  : offset_of(block, page, a.k_page, a.k_slot);
+  auto request = [&](int side, Lds* to, RowOffset offset) __attribute__((always_inline)) {
     const unsigned char* base = side ? vbase : kbase;
     // (chunks of later rows follow from the first one's: not kept, in registers that are short)
     constexpr bool kEven = 64 % kChunks == 0;
@@ -583,37 +588,38 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? WAVES64 : DIM <= 128 ? 2 : 1)
   if (block0 < block_end) {
     f32x16 s[2];
     float top = 0.0f;
-    // entries of the block whose values are requested next, whose keys are, and of the one after
-    int page1 = look_up(block0), page2 = look_up(block0 + 1), page3 = look_up(block0 + 2);
-    uint64_t on_page = __ballot(page_ok(page1));  // of the block whose scores come next
-    request(0, keys0, block0, page1);
-    request(1, values0, block0, page1);
+    Place ahead = look_up(block0), second = look_up(block0 + 1), third = look_up(block0 + 2);
+    const Offsets first = offsets_of(ahead);
+    request(0, keys0, first.key);
+    request(1, values0, first.value);
     park(0, keys0);
     park(1, values0);
-    request(0, keys1, block0 + 1, page2);
+    Offsets next = offsets_of(second);  // of the block whose values are requested next
+    request(0, keys1, next.key);
     park(0, keys1);
+    ahead = third;  // of the block whose keys are
     finish_query();
     wait_vmcnt<0>();
     __syncthreads();
     if (block0 < wave_end) {
       score(keys0, s, nothing);
-      mask(block0, on_page, s);
+      mask(block0, first.on_page, s);
       top = of_row_max(largest(s));
     }
     // Block `block`, whose values are in `values`, with scores s; the next one's keys in keys_next.
-    auto take = [&](auto next, int block, Lds* keys, Lds* values, Lds* keys_next, Lds* values_next)
+    auto take = [&](auto which, int block, Lds* keys, Lds* values, Lds* keys_next, Lds* values_next)
         __attribute__((always_inline)) {
-      constexpr int kNext = decltype(next)::value;  // 1: scores of the next block too, -1: neither
+      constexpr int kNext = decltype(which)::value;  // 1: scores of the next block too, -1: neither
       wait_vmcnt<0>();
       __syncthreads();
-      on_page = __ballot(page_ok(page2));
+      const uint64_t on_page = next.on_page;
       auto request_values = [&]() __attribute__((always_inline)) {
-        request(1, values_next, block + 1, page2);
+        request(1, values_next, next.value);
       };
       auto request_keys = [&]() __attribute__((always_inline)) {
-        request(0, keys, block + 2, page3);
-        page2 = page3;
-        page3 = look_up(block + 3);
+        next = offsets_of(ahead);
+        request(0, keys, next.key);
+        ahead = look_up(block + 3);
       };
       if constexpr (kNext <= 0) {
         request_values();
@@ -690,24 +696,23 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? WAVES64 : DIM <= 128 ? 2 : 1)
     clear();
 #pragma unroll 1
     for (int block = block0; block < block_end; ++block) {
-      const int page = look_up(block);
-      request(0, keys0, block, page);
-      request(1, values0, block, page);
+      const Offsets at = offsets_of(look_up(block));
+      request(0, keys0, at.key);
+      request(1, values0, at.value);
       park(0, keys0);
       park(1, values0);
       wait_vmcnt<0>();
       __syncthreads();
       if (block < wave_end) {
-        const uint64_t on_page = __ballot(page_ok(page));
         f32x16 s[2];
         score(keys0, s, nothing);
-        mask(block, on_page, s);
+        mask(block, at.on_page, s);
         refer(of_row_max(largest(s)));
         u32x4 p[4];
         float sums[2] = {0.0f, 0.0f};
         weigh(s, p, base == -__builtin_inff() ? 0.0f : base, sums, 0, 32);
         sum += sums[0] + sums[1];
-        add_odd(values0, on_page, s);
+        add_odd(values0, at.on_page, s);
         add(IntConst<1>(), values0, p, nothing);
       }
       __syncthreads();
