@@ -598,7 +598,7 @@ int mt_token_logprobs(const mt_token_logprobs_args* args, void* workspace, size_
   if (need && !aligned16(workspace)) return refuse(op, "workspace must be 16-byte aligned");
   mt::LogprobsArgs a{in.logits, in.row_stride, in.tokens, in.logprobs, in.entropies, in.ranks,
                      in.top_logprobs, in.top_tokens, static_cast<unsigned char*>(workspace), in.rows,
-                     in.vocab, in.top, plan.part_batches, plan.num_parts, inverse};
+                     in.vocab, in.top, plan.threads, plan.part_batches, plan.num_parts, inverse};
   return launched(op, mt::launch_token_logprobs(a, in.dtype, static_cast<hipStream_t>(stream)));
 }
 

@@ -20,13 +20,13 @@ struct LogprobsArgs {
   int64_t* top_tokens;    // [rows, top]
   unsigned char* parts;   // of rows in several parts
   int32_t rows, vocab, top;
-  int32_t part_batches, num_parts;  // batches of a part, parts of a row
+  int32_t threads, part_batches, num_parts;  // of a workgroup; batches of a part, parts of a row
   float inv_temperature;
 };
 
-// How a call's rows are split: batches of a part, parts of a row.
+// How a call's rows are split: threads of a workgroup, batches of a part, parts of a row.
 struct LogprobsPlan {
-  int part_batches, num_parts;
+  int threads, part_batches, num_parts;
 };
 LogprobsPlan plan_token_logprobs(int rows, int vocab, int cus);
 size_t logprobs_part_bytes(int top);

@@ -22,11 +22,14 @@
 namespace mt {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
+// Threads of a workgroup. With as many rows as CUs or fewer and more than 16384 values in each, 16 waves
+// take a row with fewer parts to join (us with 4 waves -> 16, top 20 of 152064 values: 1 row 23.2 -> 21.7,
+// 64 rows 25.7 -> 23.7, 256 rows 34.7 -> 26.1); below that 4 have less to exchange (1 row of 1000 values
+// 8.0, with 16 waves 11.0).
+constexpr int kFew = 1024, kMany = 256;
 constexpr int kUnits = 4;                        // runs of 8 values of a thread in a batch
-constexpr int kRun = kThreads * 8;               // values of a unit, next to each other
-constexpr int kBatch = kRun * kUnits;            // values of a batch
-constexpr int kMostBatches = 32;                 // of a part: their maxima fit LDS
+constexpr int kMostKept = 8192;                  // groups of a part: their maxima fit LDS
+constexpr int kBounds = 256;                     // maxima that the bound is found from
 constexpr int kMostGroups = 64;                  // that are read again
 constexpr int kMostTop = kLogprobsMostTop;
 constexpr int kF32 = 2;
@@ -45,20 +48,22 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
 }
 
+// (In 64 bits: beside the sum of a likely token the others' are small, and round alike.)
 struct Sums {
-  double ref;  // R
-  float s, w;  // sums of 2^y and 2^y y
+  double ref;   // R
+  double s, w;  // sums of 2^y and 2^y y
 };
 // A weighted sum w beside a sum s once its reference is d (below 0) from the new one, f = 2^d. A sum
 // that does not count any more adds nothing, whatever its distance; sums that are no numbers stay so.
-__device__ __forceinline__ float moved(float w, float s, float d, float f) {
-  return f > 0.0f ? f * (w + s * d) : s * 0.0f;
+template <typename F>
+__device__ __forceinline__ F moved(F w, F s, F d, F f) {
+  return f > 0 ? f * (w + s * d) : s * 0;
 }
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
   Sums r;
   r.ref = a.ref > b.ref ? a.ref : b.ref;
-  const float da = (float)(a.ref - r.ref), db = (float)(b.ref - r.ref);
-  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+  const double da = a.ref - r.ref, db = b.ref - r.ref;
+  const double fa = __builtin_amdgcn_exp2f((float)da), fb = __builtin_amdgcn_exp2f((float)db);
   r.s = a.s * fa + b.s * fb;
   r.w = moved(a.w, a.s, da, fa) + moved(b.w, b.s, db, fb);
   return r;
@@ -67,7 +72,7 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
 // What a part of a row hands on, and behind it its alternatives as (key, index), largest first.
 struct Part {
   Sums sums;
-  int32_t larger, unused;
+  int64_t larger;
 };
 
 // The largest of three, without the instructions that would quiet NaN first.
@@ -130,6 +135,7 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
 
 // Sum over the workgroup of its waves' counts, in every thread. `turn` alternates the LDS used, so that
 // one barrier is enough.
+template <int kWaves>
 __device__ __forceinline__ int block_sum(int of_wave, int (&lds)[2][kWaves], int& turn) {
   if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = of_wave;
   __syncthreads();
@@ -142,7 +148,7 @@ __device__ __forceinline__ int block_sum(int of_wave, int (&lds)[2][kWaves], int
 
 // The n (at most kMostTop) largest of `count` different numbers in LDS, put in order into best[].
 __device__ __forceinline__ void put_in_order(const uint64_t* from, int count, int n, uint64_t* best) {
-  for (int i = threadIdx.x; i < count; i += kThreads) {
+  for (int i = threadIdx.x; i < count; i += blockDim.x) {
     const uint64_t v = from[i];
     int rank = 0;
     for (int j = 0; j < count && rank < n; ++j) rank += from[j] > v;
@@ -153,19 +159,21 @@ __device__ __forceinline__ void put_in_order(const uint64_t* from, int count, in
 __device__ __forceinline__ void write_row(const LogprobsArgs& a, int row, Sums sums, float given,
                                           bool in_vocab, int larger, const uint64_t* best) {
   const float scale = a.inv_temperature * kLog2e;
-  const float log_s = __builtin_amdgcn_logf(sums.s);
+  const float log_s = __builtin_amdgcn_logf((float)sums.s);
   auto logprob = [&](float x) {
-    if (sums.s == 0.0f) return -__builtin_inff();  // a row of -inf alone
-    return (float)(((double)x * (double)scale - sums.ref - (double)log_s) * 0.6931471805599453);
+    if (sums.s == 0.0) return -__builtin_inff();  // a row of -inf alone
+    const float l = (float)(((double)x * (double)scale - sums.ref - (double)log_s) * 0.6931471805599453);
+    return l > 0.0f ? 0.0f : l;
   };
   if (threadIdx.x == 0) {
-    a.entropies[row] = sums.s == 0.0f ? 0.0f : (log_s - sums.w / sums.s) * kLn2;
+    const float h = sums.s == 0.0 ? 0.0f : (log_s - (float)(sums.w / sums.s)) * kLn2;
+    a.entropies[row] = h < 0.0f ? 0.0f : h;
     if (a.tokens) {
       a.logprobs[row] = in_vocab ? logprob(given) : -__builtin_inff();
       a.ranks[row] = in_vocab ? larger : -1;
     }
   }
-  for (int i = threadIdx.x; i < a.top; i += kThreads) {
+  for (int i = threadIdx.x; i < a.top; i += blockDim.x) {
     const uint32_t key = (uint32_t)(best[i] >> 32);
     a.top_logprobs[(int64_t)row * a.top + i] =
         key ? logprob(value_of(key)) : __builtin_nanf("");
@@ -173,13 +181,15 @@ __device__ __forceinline__ void write_row(const LogprobsArgs& a, int row, Sums s
   }
 }
 
-template <int DT>
+template <int DT, int kThreads>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
+  constexpr int kWaves = kThreads / 64;
+  constexpr int kRun = kThreads * 8, kBatch = kRun * kUnits;  // values of a unit, next to each other
   // each group's maximum, [batches][kThreads]; later the candidates, kMostGroups * 32 of them
   extern __shared__ __attribute__((aligned(16))) uint32_t group_keys[];
   __shared__ uint64_t best[kMostTop], flagged;
   __shared__ Sums wave_sums[kWaves];
-  __shared__ uint32_t thread_keys[kThreads];
+  __shared__ uint32_t thread_keys[kBounds];
   __shared__ int wave_count[2][kWaves], counts[2], groups[kMostGroups];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -192,6 +202,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
   const int batches = (end - begin + kBatch - 1) / kBatch;
   const float scale = a.inv_temperature * kLog2e;
 
+  // ---- sums, and each group's maximum ----
+  constexpr uint32_t kSize = DT == kF32 ? 4 : 2;
+  Raw<DT> next[kUnits];
+  auto request = [&](int b) {  // a batch that is whole
+    const unsigned char* p = x_row + (int64_t)(begin + b * kBatch) * kSize;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) next[u] = load8<DT>(p + (u * kRun + (uint32_t)tid * 8) * kSize);
+  };
+  const int whole = (end - begin) / kBatch;
+  if (whole) request(0);
   int token = -1;
   float given = 0.0f;
   bool in_vocab = false;
@@ -201,35 +221,26 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
     token = in_vocab ? (int)t : 0;
     given = load1<DT>(x_row, token);
   }
-
-  // ---- sums, and each group's maximum ----
-  constexpr uint32_t kSize = DT == kF32 ? 4 : 2;
-  Raw<DT> next[kUnits];
-  auto request = [&](int b) {  // a batch that is whole
-    const unsigned char* p = x_row + (int64_t)(begin + b * kBatch) * kSize;
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) next[u] = load8<DT>(p + (u * kRun + (uint32_t)tid * 8) * kSize);
-  };
   auto tail = [&](int b, float (&x)[kUnits][8]) {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
       tail8<DT>(x_row, begin + b * kBatch + u * kRun + tid * 8, end, x[u]);
   };
-  // Sums of the lanes, then of the waves, in every thread.
-  auto of_all = [&](Sums own) {
-    for (int d = 32; d; d /= 2) {
+  // Sums of 2 d lanes, in each of them.
+  auto of_lanes = [&](Sums own, int d) {
+    for (; d; d /= 2) {
       Sums other;
       other.ref = __shfl_xor(own.ref, d);
       other.s = __shfl_xor(own.s, d);
       other.w = __shfl_xor(own.w, d);
       own = (lane & d) ? join(other, own) : join(own, other);
     }
+    return own;
+  };
+  auto of_waves = [&](Sums own) {
     if (lane == 0) wave_sums[wave] = own;
     __syncthreads();
-    own = wave_sums[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) own = join(own, wave_sums[w]);
-    return own;
+    return of_lanes(wave_sums[lane % kWaves], kWaves / 2);
   };
   float ref = kNothing, s = 0.0f, w = 0.0f, own_top = -__builtin_inff();  // ref is the wave's
   int larger = 0;                                                        // of the wave
@@ -298,8 +309,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
       }
     }
   };
-  const int whole = (end - begin) / kBatch;
-  if (whole) request(0);
   for (int b = 0; b < whole; ++b) {
     float x[kUnits][8];
 #pragma unroll
@@ -323,12 +332,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
   if (lane == 0) wave_count[0][wave] = larger;
   if (tid < kMostTop) best[tid] = 0;
   if (tid == 0) counts[0] = counts[1] = 0, flagged = 0;
-  Sums sums = of_all({s == 0.0f ? kNone : (double)ref, s, w});
+  double wave_s = s, wave_w = w;
+  for (int d = 32; d; d /= 2) wave_s += __shfl_xor(wave_s, d), wave_w += __shfl_xor(wave_w, d);
+  Sums sums = of_waves({wave_s == 0.0 ? kNone : (double)ref, wave_s, wave_w});
   uint32_t own_key = key_of(own_top);
-  if (!(sums.s > 0.0f && sums.s < __builtin_inff())) {
+  if (!(sums.s > 0.0 && sums.s < (double)__builtin_inff())) {
     // NaN or infinities, logits too large for c times them, or none that is allowed: again, with
     // references in 64 bits and maxima by whole numbers
-    Sums own = {kNone, 0.0f, 0.0f};
+    Sums own = {kNone, 0.0, 0.0};
     own_key = 0;
 #pragma unroll 1
     for (int b = 0; b < batches; ++b) {
@@ -342,7 +353,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
           const float v = u == 0 ? x[0][j] : u == 1 ? x[1][j] : u == 2 ? x[2][j] : x[3][j];
           key = max(key, key_of(v));
           if (v == -__builtin_inff()) continue;
-          const Sums one = {(double)v * (double)scale, v - v == 0.0f ? 1.0f : v - v, 0.0f};
+          const Sums one = {(double)v * (double)scale, v - v == 0.0f ? 1.0 : (double)(v - v), 0.0};
           own = join(own, one);
         }
       }
@@ -350,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
       own_key = max(own_key, key);
     }
     __syncthreads();
-    sums = of_all(own);
+    sums = of_waves(of_lanes(own, 32));
   }
   larger = 0;
 #pragma unroll
@@ -363,19 +374,22 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
     auto exact = [&](uint32_t bound) {  // keys of negative values have ones there
       return kLowBit && bound && !(bound >> 31) ? bound | ((1u << kLowBit) - 1) : bound;
     };
-    thread_keys[tid] = own_key;
+    // the k-th largest of the threads' maxima (of 16 waves, the fours of threads'): the largest key
+    // that k of them reach (0: fewer do)
+    constexpr int kEach = kThreads / kBounds, kKeys = kBounds / 64;
+    for (int d = 1; d < kEach; d *= 2) own_key = max(own_key, (uint32_t)__shfl_xor((int)own_key, d));
+    if (tid % kEach == 0) thread_keys[tid / kEach] = own_key;
     __syncthreads();
-    // the k-th largest of the threads' maxima: the largest key that k of them reach (0: fewer do)
     uint32_t bound = 0;
     {
-      uint32_t keys[kWaves];
+      uint32_t keys[kKeys];
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) keys[i] = thread_keys[64 * i + lane];
+      for (int i = 0; i < kKeys; ++i) keys[i] = thread_keys[64 * i + lane];
       for (int bit = 31; bit >= kLowBit; --bit) {
         const uint32_t middle = bound | 1u << bit;
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) n += __popcll(__ballot(keys[i] >= middle));
+        for (int i = 0; i < kKeys; ++i) n += __popcll(__ballot(keys[i] >= middle));
         if (n >= k) bound = middle;
       }
       bound = exact(bound);
@@ -474,12 +488,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
     return;
   }
   unsigned char* to = a.parts + (int64_t)blockIdx.x * (sizeof(Part) + a.top * 8);
-  if (tid == 0) *reinterpret_cast<Part*>(to) = Part{sums, larger, 0};
+  if (tid == 0) *reinterpret_cast<Part*>(to) = Part{sums, larger};
   if (tid < a.top) reinterpret_cast<uint64_t*>(to + sizeof(Part))[tid] = best[tid];
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void join_kernel(LogprobsArgs a) {
+__global__ __launch_bounds__(kMany) void join_kernel(LogprobsArgs a) {
+  constexpr int kThreads = kMany, kWaves = kThreads / 64;
   extern __shared__ uint64_t candidates[];  // [num_parts * top]
   __shared__ uint64_t best[kMostTop];
   __shared__ int count;
@@ -496,12 +511,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(LogprobsArgs a) {
     in_vocab = t >= 0 && t < a.vocab;
     given = load1<DT>(x_row, in_vocab ? (int)t : 0);
   }
-  Sums sums = {kNone, 0.0f, 0.0f};
+  Sums sums = {kNone, 0.0, 0.0};
   int larger = 0;
   for (int p = 0; p < a.num_parts; ++p) {
     const Part part = *reinterpret_cast<const Part*>(from + (int64_t)p * step);
     sums = join(sums, part.sums);
-    larger += part.larger;
+    larger += (int)part.larger;
   }
   if (tid < kMostTop) best[tid] = 0;
   if (tid == 0) count = 0;
@@ -528,8 +543,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(LogprobsArgs a) {
   write_row(a, row, sums, given, in_vocab, larger, best);
 }
 
-template <int DT>
-hipError_t launch(const LogprobsArgs& args, hipStream_t stream) {
+template <int DT, int kThreads>
+hipError_t launch_threads(const LogprobsArgs& args, hipStream_t stream) {
+  constexpr int kBatch = kThreads * 8 * kUnits;
   const int batches = std::min(args.part_batches, (args.vocab + kBatch - 1) / kBatch);
   const int keys = args.top ? std::max(batches * kThreads * 4, kMostGroups * 32 * 8) : 0;
   // rows of a launch, so that its threads are counted in 32 bits; the parts of one are joined before
@@ -543,23 +559,29 @@ hipError_t launch(const LogprobsArgs& args, hipStream_t stream) {
     if (a.tokens) a.tokens += row, a.logprobs += row, a.ranks += row;
     if (a.top) a.top_logprobs += row * a.top, a.top_tokens += row * a.top;
     const int rows = (int)std::min<int64_t>(most, args.rows - row);
-    logprobs_kernel<DT><<<(unsigned)rows * (unsigned)a.num_parts, kThreads, keys, stream>>>(a);
-    if (a.num_parts > 1) join_kernel<DT><<<rows, kThreads, a.num_parts * a.top * 8, stream>>>(a);
+    logprobs_kernel<DT, kThreads>
+        <<<(unsigned)rows * (unsigned)a.num_parts, kThreads, keys, stream>>>(a);
+    if (a.num_parts > 1) join_kernel<DT><<<rows, kMany, a.num_parts * a.top * 8, stream>>>(a);
     if (const hipError_t e = hipGetLastError()) return e;
   }
   return hipSuccess;
+}
+template <int DT>
+hipError_t launch(const LogprobsArgs& a, hipStream_t stream) {
+  return a.threads == kFew ? launch_threads<DT, kFew>(a, stream) : launch_threads<DT, kMany>(a, stream);
 }
 
 }  // namespace
 
 // A workgroup a row, unless that leaves CUs without one: then parts of four batches or more, so many
-// that there are four workgroups a CU, at most 64.
+// that there are four workgroups a CU (one of 16 waves), at most 64.
 LogprobsPlan plan_token_logprobs(int rows, int vocab, int cus) {
-  const int batches = std::max(1, (int)(((int64_t)vocab + kBatch - 1) / kBatch));
-  int parts = (int)std::min<int64_t>((batches + 3) / 4, std::max<int64_t>(1, 4ll * cus / std::max(rows, 1)));
-  parts = std::min(parts, 64);
-  const int per = std::min(kMostBatches, (batches + parts - 1) / parts);
-  return {per, (batches + per - 1) / per};
+  const int threads = rows <= cus && vocab > 16384 ? kFew : kMany, batch = threads * 8 * kUnits;
+  const int batches = std::max(1, (int)(((int64_t)vocab + batch - 1) / batch));
+  const int64_t wanted = (threads == kFew ? 1ll : 4ll) * cus / std::max(rows, 1);
+  const int parts = (int)std::min<int64_t>({(batches + 3) / 4, std::max<int64_t>(1, wanted), 64});
+  const int per = std::min(kMostKept / threads, (batches + parts - 1) / parts);
+  return {threads, per, (batches + per - 1) / per};
 }
 
 size_t logprobs_part_bytes(int top) { return sizeof(Part) + (size_t)top * 8; }

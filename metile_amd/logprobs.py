@@ -5,6 +5,7 @@ The reference has no counterpart: its decode loop leaves sampling to MLX-LM.
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -50,7 +51,7 @@ def token_logprobs(logits, tokens=None, *, top=0, temperature=1.0):
         raise ValueError("tokens must be int64, one for each row of logits")
     device = logits.device
     _same_device(device, tokens)
-    flat = logits.reshape(-1, vocab)
+    flat = logits if logits.ndim == 2 else logits.reshape(-1, vocab)
     if vocab > 1 and flat.stride(1) != 1:
         flat = flat.contiguous()
     rows = flat.shape[0]
@@ -60,21 +61,21 @@ def token_logprobs(logits, tokens=None, *, top=0, temperature=1.0):
     logprobs = ranks = None
     if tokens is not None:
         tokens = tokens.contiguous()
-        logprobs, ranks = torch.empty_like(entropies), torch.empty(shape, dtype=torch.int32,
-                                                                   device=device)
+        logprobs, ranks = torch.empty_like(entropies), torch.empty_like(entropies, dtype=torch.int32)
     top_logprobs = torch.empty((*shape, top), dtype=torch.float32, device=device)
     top_tokens = torch.empty((*shape, top), dtype=torch.int64, device=device)
-    args = _lib.TOKEN_LOGPROBS_ARGS.pack(
+    need = _workspace_bytes(device.index, rows, vocab, top)
+    ws = _scratch(device, need) if need else None
+    _launch(device, _lib.lib().mt_token_logprobs, _lib.TOKEN_LOGPROBS_ARGS.pack(
         flat.data_ptr(), flat.stride(0), 0 if tokens is None else tokens.data_ptr(),
         0 if tokens is None else logprobs.data_ptr(), entropies.data_ptr(),
         0 if tokens is None else ranks.data_ptr(), top_logprobs.data_ptr(), top_tokens.data_ptr(),
-        rows, vocab, top, _DTYPES[logits.dtype], temperature)
-    lib = _lib.lib()
-
-    def call(stream):
-        need = lib.mt_token_logprobs_workspace_bytes(rows, vocab, top)
-        ws = _scratch(device, need) if need else None
-        return lib.mt_token_logprobs(args, None if ws is None else ws.data_ptr(), need, stream)
-
-    _launch(device, call)
+        rows, vocab, top, _DTYPES[logits.dtype], temperature), None if ws is None else ws.data_ptr(),
+        need)
     return TokenLogprobs(logprobs, entropies, ranks, top_logprobs, top_tokens)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(index, rows, vocab, top):
+    with torch.cuda.device(index):
+        return _lib.lib().mt_token_logprobs_workspace_bytes(rows, vocab, top)

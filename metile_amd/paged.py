@@ -117,7 +117,7 @@ class PagedCache:
             _CACHE_DTYPES[key.dtype], self.key_scale, self.value_scale)
         self._ref, self._address = ctypes.byref(self._desc), ctypes.addressof(self._desc)
         self._device, self._dtype, self._head_shape = key.device, key.dtype, key.shape[2:]
-        self._workspaces = {}  # (requests, heads, width, window) -> bytes
+        self._workspaces = {}  # ([tokens,] requests, heads, width, window) -> bytes
 
     @classmethod
     def allocate(cls, pages, page_size, kv_heads, head_dim, *, dtype=torch.bfloat16, device="cuda",
@@ -361,16 +361,26 @@ def paged_chunk_attention(query, cache, block_tables, lengths, starts, *, scale=
         lengths.data_ptr(), starts.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
         tokens, requests, heads, width, window, dim ** -0.5 if scale is None else scale,
         _DTYPES[dtype])
-    lib = _lib.lib()
-
-    def call(stream):
-        need = lib.mt_paged_chunk_attention_workspace_bytes(cache._ref, tokens, requests, heads, width,
-                                                            window)
-        ws = _scratch(device, need)
-        return lib.mt_paged_chunk_attention(cache._ref, args, ws.data_ptr(), need, stream)
-
-    _launch(device, call)
+    if device.index == _current_device():
+        _attend_chunks(cache, args, tokens, requests, heads, width, window)
+    else:
+        with torch.cuda.device(device):
+            _attend_chunks(cache, args, tokens, requests, heads, width, window)
     return (out, lse) if return_lse else out
+
+
+def _attend_chunks(cache, args, *shape):
+    lib, need = _lib.lib(), cache._workspaces.get(shape)
+    if need is None:  # (as many shapes as there are sizes of steps)
+        need = lib.mt_paged_chunk_attention_workspace_bytes(cache._ref, *shape)
+        if len(cache._workspaces) >= 256:
+            cache._workspaces.clear()
+        cache._workspaces[shape] = need
+    ws = _scratch(cache._device, need)
+    status = lib.mt_paged_chunk_attention(cache._ref, args, ws.data_ptr(), need,
+                                          _stream_handle(cache._device))
+    if status:
+        _lib.check(status)
 
 
 def paged_copy(caches, sources, targets):

@@ -212,6 +212,29 @@ def test_vocabulary_in_several_parts_and_the_largest():
     assert int(got.ranks) == 0 and int(got.top_tokens[0, 0]) == (1 << 24) - 1
 
 
+def test_ties_in_long_rows():
+    """Many equal maxima over several batches of a workgroup and several parts, of every kind of row."""
+    for rows, vocab in ((3, 70001), (3, 300007), (256, 70001), (257, 40000)):
+        x = torch.full((rows, vocab), -2.0, dtype=torch.bfloat16, device="cuda")
+        x[:, ::3] = 1.0
+        x[0, vocab - 5:] = 4.0
+        x[1, 60:90] = 5.0
+        check(x, torch.full((rows,), vocab - 1, device="cuda"), 32)
+
+
+def test_more_rows_than_one_launch_takes():
+    rows = (1 << 22) + 5
+    x = torch.zeros(rows, 9, dtype=torch.float16, device="cuda")
+    t = torch.arange(rows, device="cuda") % 9
+    x[torch.arange(rows, device="cuda"), t] = (t + 1).to(torch.float16)
+    got = mt.token_logprobs(x, t, top=2)
+    few = mt.token_logprobs(x[:9], t[:9], top=2)
+    want = ref.logprobs(x[:9], t[:9], 2)
+    assert bool(((few.logprobs.double().cpu() - want[0]).abs() <= 2.0 ** -20).all())
+    for a, b in zip(got, few):
+        assert torch.equal(a, b[t])
+
+
 def test_empty():
     got = mt.token_logprobs(torch.empty(0, 50, device="cuda"),
                             torch.empty(0, dtype=torch.int64, device="cuda"), top=3)
