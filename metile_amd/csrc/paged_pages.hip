@@ -347,6 +347,181 @@ __global__ __launch_bounds__(kThreads) void apply_compact_kernel(PagedCompactArg
     }
 }
 
+// ---- small pools: one launch -----------------------------------------------------------------------
+
+// One workgroup does it all where it needs no more time than the others' launches, with the marks in
+// LDS. (Free and compact, us: 64 requests over 1024 pages 9.0 -> 4.0 and 14.2 -> 5.6, 256 over 8192
+// 9.6 -> 6.4 and 15.9 -> 13.7, 64 over 16384 10.1 -> 9.0 and 18.2 -> 16.8; 1024 over 16384 took 15 and
+// 27 where the launches take 9.7 and 16.7. The host's part of a call is 17.4 -> 9.4 and 23.5 -> 12.7.)
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
+constexpr int kSmallPages = 16384, kSmallEntries = 32768, kSmallRequests = 256;
+constexpr int kAhead = 4;  // entries that a thread has under way
+
+// f(entry, column) for the columns [from(r), to(r)) of each row, 2^bits threads to a row.
+template <typename From, typename To, typename F>
+__device__ __forceinline__ void each_entry(const int32_t* tables, int64_t stride, int requests, int bits,
+                                           From from, To to, F f) {
+  const int threads = 1 << bits, me = threadIdx.x & (threads - 1);
+  for (int r = threadIdx.x >> bits; r < requests; r += kSmallThreads >> bits) {
+    const int32_t* row = tables + (int64_t)r * stride;
+    const int end = to(r);
+    for (int c = from(r) + me; c < end; c += threads * kAhead) {
+      int32_t p[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) p[i] = c + i * threads < end ? row[c + i * threads] : 0;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (c + i * threads < end) f(p[i], r, c + i * threads);
+    }
+  }
+}
+
+__device__ __forceinline__ void no_marks(unsigned char* marks) {
+  for (int i = threadIdx.x; i < kSmallPages / 16; i += kSmallThreads)
+    reinterpret_cast<u32x4*>(marks)[i] = (u32x4){0, 0, 0, 0};
+}
+
+// The pages of a wave are next to each other, 64 at a time. Sums over the waves before this one, and
+// over all, of how many pages have the marks.
+struct SmallScan {
+  int first, last;  // pages of the wave
+  Pair before, all;
+};
+__device__ __forceinline__ SmallScan scan_marks(const unsigned char* marks, int pages, int mark_a,
+                                                int mark_b, Pair* lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = (pages + kSmallThreads - 1) / kSmallThreads * 64;
+  SmallScan s;
+  s.first = wave * per;
+  s.last = min(s.first + per, pages);
+  Pair mine{0, 0};
+  for (int p = s.first; p < s.last; p += 64) {
+    const int mark = p + lane < s.last ? marks[p + lane] : 0;
+    mine.a += __popcll(__ballot(mark == mark_a));
+    mine.b += __popcll(__ballot(mark == mark_b));
+  }
+  if (lane == 0) lds[wave] = mine;
+  __syncthreads();
+  s.before = s.all = {0, 0};
+#pragma unroll
+  for (int w = 0; w < kSmallWaves; ++w) {
+    if (w < wave) s.before.a += lds[w].a, s.before.b += lds[w].b;
+    s.all.a += lds[w].a, s.all.b += lds[w].b;
+  }
+  return s;
+}
+__device__ __forceinline__ int lanes_before(uint64_t mask) {
+  return __popcll(mask & ((1ull << (threadIdx.x & 63)) - 1));
+}
+
+__global__ __launch_bounds__(kSmallThreads) void free_small_kernel(PagedFreeArgs a, DivMagic by_page,
+                                                                    int bits) {
+  __shared__ __attribute__((aligned(16))) unsigned char marks[kSmallPages];  // 1: dropped, 2: kept
+  __shared__ Pair lds[kSmallWaves];
+  const int64_t start = *a.free_start;
+  no_marks(marks);
+  __syncthreads();
+  auto used = [&](int r) { return columns_of(a.lengths[r], by_page, a.page_size, a.width); };
+  auto kept = [&](int r) {
+    return columns_of(min(a.kept[r], a.lengths[r]), by_page, a.page_size, a.width);
+  };
+  auto none = [](int) { return 0; };
+  each_entry(a.tables, a.table_stride, a.requests, bits, kept, used, [&](int32_t p, int, int) {
+    if ((uint32_t)p < (uint32_t)a.pages) marks[p] = 1;
+  });
+  __syncthreads();
+  each_entry(a.tables, a.table_stride, a.requests, bits, none, kept, [&](int32_t p, int, int) {
+    if ((uint32_t)p < (uint32_t)a.pages) marks[p] = 2;
+  });
+  __syncthreads();
+  const SmallScan s = scan_marks(marks, a.pages, 1, 3, lds);
+  int64_t at = start - s.all.a + s.before.a;
+  for (int p = s.first; p < s.last; p += 64) {
+    const int page = p + (threadIdx.x & 63);
+    const bool mine = page < s.last && marks[page] == 1;
+    const uint64_t mask = __ballot(mine);
+    const int64_t to = at + lanes_before(mask);
+    if (mine && to >= 0 && to < a.free_count) a.free_pages[to] = page;
+    at += __popcll(mask);
+  }
+  if (threadIdx.x == 0) *a.freed = s.all.a;
+}
+
+// As list_compact_kernel and those around it.
+__global__ __launch_bounds__(kSmallThreads) void compact_small_kernel(PagedCompactArgs a,
+                                                                       DivMagic by_page, int bits) {
+  __shared__ __attribute__((aligned(16))) unsigned char marks[kSmallPages];  // 1: free, 2: in use
+  __shared__ uint16_t number[kSmallPages];       // of a page in use: its move, or kStays
+  __shared__ uint16_t target_of[kSmallPages / 2];  // of a move
+  __shared__ Pair lds[kSmallWaves];
+  __shared__ int num_moves;
+  constexpr int kStays = 0xffff;
+  const int tid = threadIdx.x;
+  const int given = *a.free_start, start = max(given, 0);
+  if (tid == 0) num_moves = 0;
+  no_marks(marks);
+  __syncthreads();
+  for (int64_t i = (int64_t)start + tid; i < a.free_count; i += kSmallThreads) {
+    const int32_t p = a.free_pages[i];
+    if ((uint32_t)p < (uint32_t)a.pages) marks[p] = 1;
+  }
+  for (int i = tid; i < min(given, a.free_count); i += kSmallThreads) a.new_free[i] = a.free_pages[i];
+  __syncthreads();
+  auto columns = [&](int r) { return columns_of(a.lengths[r], by_page, a.page_size, a.width); };
+  auto none = [](int) { return 0; };
+  each_entry(a.tables, a.table_stride, a.requests, bits, none, columns, [&](int32_t p, int, int) {
+    if ((uint32_t)p < (uint32_t)a.pages) marks[p] = 2;
+  });
+  __syncthreads();
+  const SmallScan s = scan_marks(marks, a.pages, 2, 1, lds);
+  const int in_use = s.all.a;
+  int used_before = s.before.a, open_before = s.before.b;
+  for (int p = s.first; p < s.last; p += 64) {
+    const int page = p + (tid & 63), mark = page < s.last ? marks[page] : 0;
+    const uint64_t used = __ballot(mark == 2), open = __ballot(mark == 1);
+    const int before = used_before + lanes_before(used), opens = open_before + lanes_before(open);
+    const int rank = before + opens;
+    const bool low = rank < in_use;
+    if (mark) {
+      if (rank == in_use - 1) num_moves = opens + (mark == 1);
+      if (mark == 2) number[page] = low ? kStays : in_use - 1 - before;
+      if (mark == 2 && !low) a.sources[in_use - 1 - before] = page;
+      if (mark == 1 && low) {
+        a.targets[opens] = page;
+        target_of[opens] = page;
+      }
+      if (!low && (int64_t)start + rank - in_use < a.free_count) a.new_free[start + rank - in_use] = page;
+    }
+    used_before += __popcll(used);
+    open_before += __popcll(open);
+  }
+  __syncthreads();
+  const int moves = num_moves;
+  if (tid == 0) *a.moves = moves;
+  for (int i = moves + tid; i < a.most_moves; i += kSmallThreads) a.sources[i] = a.targets[i] = -1;
+  for (int64_t i = (int64_t)start + s.all.b + tid; i < a.free_count; i += kSmallThreads)
+    a.new_free[i] = -1;
+  each_entry(a.tables, a.table_stride, a.requests, bits, none, columns, [&](int32_t p, int r, int c) {
+    if ((uint32_t)p < (uint32_t)a.pages && number[p] != kStays) p = target_of[number[p]];
+    a.new_tables[(int64_t)r * a.width + c] = p;
+  });
+  auto width = [&](int) { return a.width; };
+  each_entry(a.tables, a.table_stride, a.requests, bits, columns, width, [&](int32_t p, int r, int c) {
+    a.new_tables[(int64_t)r * a.width + c] = p;
+  });
+}
+
+bool is_small(int pages, int requests, int width) {
+  return pages <= kSmallPages && requests <= kSmallRequests &&
+         (int64_t)requests * width <= kSmallEntries;
+}
+// Threads of a row, as many as there are for each.
+int row_bits(int requests) {
+  int bits = 10;
+  while (bits && (kSmallThreads >> bits) < requests) --bits;
+  return bits;
+}
+
 dim3 row_grid(int requests, int width) {
   const int rows = (requests + kWaves - 1) / kWaves;
   const int pieces = (int)(((int64_t)width + kRowPiece - 1) / kRowPiece);
@@ -395,6 +570,10 @@ size_t paged_free_work(int pages) {
 
 hipError_t launch_paged_free(const PagedFreeArgs& a, hipStream_t stream) {
   const DivMagic by_page = div_magic((uint32_t)a.page_size);
+  if (is_small(a.pages, a.requests, a.width)) {
+    free_small_kernel<<<1, kSmallThreads, 0, stream>>>(a, by_page, row_bits(a.requests));
+    return hipGetLastError();
+  }
   const size_t marks = padded(a.pages);
   unsigned char *keeps = a.work, *drops = a.work + marks;
   Pair* counts = reinterpret_cast<Pair*>(a.work + 2 * marks);
@@ -414,6 +593,11 @@ size_t paged_compact_work(int pages) {
 
 hipError_t launch_paged_compact(const PagedCompactArgs& a, hipStream_t stream) {
   const DivMagic by_page = div_magic((uint32_t)a.page_size);
+  if (is_small(a.pages, a.requests, a.width) && a.free_count <= 2 * kSmallPages &&
+      a.most_moves <= 2 * kSmallPages) {
+    compact_small_kernel<<<1, kSmallThreads, 0, stream>>>(a, by_page, row_bits(a.requests));
+    return hipGetLastError();
+  }
   const size_t marks = padded(a.pages);
   unsigned char *used = a.work, *open = a.work + marks;
   int32_t* number = reinterpret_cast<int32_t*>(a.work + 2 * marks);

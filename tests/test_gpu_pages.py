@@ -216,6 +216,29 @@ def test_free_of_a_large_pool_and_long_rows():
     check_free(s, [n // 3 if i % 2 else 0 for i, n in enumerate(s["lengths"])])
 
 
+@pytest.mark.parametrize("requests,longest,page,spare", [
+    (256, 500, 4, 0.2), (256, 512, 4, 0.2), (257, 500, 4, 0.2), (40, 900, 1, 0.2), (7, 2300, 1, 0.4),
+    (64, 700, 1, 0.1), (3, 20, 16, 3000.0), (1, 16300, 1, 0.0), (1, 16500, 1, 0.0)])
+def test_sizes_about_those_of_one_workgroup(requests, longest, page, spare):
+    s = state(requests, longest, page, seed=requests, spare=spare, stray=True)
+    rng = random.Random(requests)
+    check_free(s, [rng.choice((0, n, n // 2)) for n in s["lengths"]])
+    check_compact(s)
+
+
+@pytest.mark.parametrize("pages", [16383, 16384, 16385])
+def test_pools_about_those_of_one_workgroup(pages):
+    """Every page in use or free, moves from one end to the other."""
+    numbers = list(range(pages))
+    for used in (1, pages // 2, pages - 1, pages):
+        rows = [numbers[::-1][:used][i::4] for i in range(4)]
+        s = dict(tables=[row + [-1] * (used // 4 + 1 - len(row)) for row in rows],
+                 lengths=[len(row) for row in rows], free=[-1] * used + numbers[:pages - used], start=used,
+                 pages=pages, page=1)
+        check_compact(s)
+        check_free(s, [n // 2 for n in s["lengths"]])
+
+
 def test_free_without_requests():
     free = i32([-1, 4])
     freed = mt.paged_free(torch.empty(0, 3, dtype=torch.int32, device="cuda"), i32([]), i32([]), free,
