@@ -5,9 +5,16 @@ requests' lengths (``paged_tables``), then per layer the 4-bit projections (``af
 cache (``paged_append``, ``paged_attention``), the 4-bit MLP (``affine_mlp``) and the norms around
 them (``residual_norm``: each block's own norm, the scaled residual and the next block's norm in one
 pass). Lengths, tables and the free list stay on the device, so a step is captured once into a HIP
-graph and replayed. Weights are random; prompts go through the same one-token step.
+graph and replayed. Weights are random.
+
+Prompts go through the layers at once (``paged_chunk_attention``), or token by token through the same
+step. A prompt can be answered several times: its requests share its full pages (``paged_fork``,
+``paged_copy``) and begin with different tokens (``token_logprobs``), whose log probabilities are summed
+up. Requests that end give back their pages (``paged_free``), and those in use can be put together
+(``paged_compact``).
 
     python examples/paged_decode.py --requests 32 --steps 64
+    python examples/paged_decode.py --requests 32 --steps 64 --prompt 1000 --answers 4
 """
 
 from __future__ import annotations
@@ -90,6 +97,7 @@ class Batch:
         self.lengths = torch.zeros(requests, dtype=torch.int32, device=device)
         self.tokens = torch.zeros(requests, dtype=torch.int64, device=device)
         self.active = torch.ones(requests, dtype=torch.int32, device=device)
+        self.scores = torch.zeros(requests, dtype=torch.float32, device=device)
 
     def step(self):
         """Logits of every request's next token; ``self.tokens`` of the active ones enter the cache."""
@@ -101,8 +109,20 @@ class Batch:
                                page_size=self.page_size, tokens=requests, free_start=self.taken)
         # (rows are packed: row t is request plan.requests[t])
         owner = plan.requests.clamp(min=0).long()
-        residual = d.embedding[self.tokens[owner]]
         tables, lengths = self.tables[owner], torch.where(plan.requests >= 0, plan.positions + 1, 0)
+        h = self.layers(self.tokens[owner], plan, lambda q, cache: mt.paged_attention(
+            q, cache, tables, lengths.int()))
+        packed = mt.affine_qmv(h, *d.head)
+        logits = torch.zeros(requests + 1, c.vocab, dtype=packed.dtype, device=packed.device)
+        logits[torch.where(plan.requests >= 0, plan.requests.long(), requests)] = packed
+        self.lengths.copy_(plan.lengths)
+        self.taken.add_(plan.taken)
+        return logits[:requests]
+
+    def layers(self, tokens, plan, attend):
+        """The last norm of a packed batch of tokens, which enter the cache."""
+        d, c = self.decoder, self.decoder.config
+        residual = d.embedding[tokens]
         residual, h = mt.residual_norm(residual, weight=d.layers[0]["norms"][0])
         for i, (layer, cache) in enumerate(zip(d.layers, self.caches)):
             heads, kv = c.heads * c.head_dim, c.kv_heads * c.head_dim
@@ -110,7 +130,7 @@ class Batch:
             q = d.rotate(q.unflatten(1, (c.heads, c.head_dim)), plan.positions)
             k = d.rotate(k.unflatten(1, (c.kv_heads, c.head_dim)), plan.positions)
             mt.paged_append(k, v.unflatten(1, (c.kv_heads, c.head_dim)), cache, plan.slots)
-            mixed = mt.paged_attention(q, cache, tables, lengths.int())
+            mixed = attend(q, cache)
             block = mt.affine_qmv(mixed.flatten(1), *layer["out"])
             norms = layer["norms"]
             residual, h = mt.residual_norm(residual, block, post_weight=norms[1], weight=norms[2],
@@ -121,16 +141,77 @@ class Batch:
                 residual, block, post_weight=norms[3],
                 weight=d.final_norm if last else d.layers[i + 1]["norms"][0],
                 residual_scale=c.residual_scale)
-        packed = mt.affine_qmv(h, *d.head)
-        logits = torch.zeros(requests + 1, c.vocab, dtype=packed.dtype, device=packed.device)
-        logits[torch.where(plan.requests >= 0, plan.requests.long(), requests)] = packed
+        return h
+
+    def prefill(self, tokens, counts, *, score=False):
+        """Logits behind the last of each request's next ``counts`` tokens (int32 ``[requests]``; the
+        packed ``tokens`` are int64), which enter the cache. With ``score`` also the log probability of
+        each of ``tokens`` but a request's first (-inf there)."""
+        d = self.decoder
+        plan = mt.paged_tables(self.lengths, counts, self.tables, self.free,
+                               page_size=self.page_size, tokens=tokens.shape[0],
+                               free_start=self.taken)
+        h = self.layers(tokens, plan, lambda q, cache: mt.paged_chunk_attention(
+            q, cache, self.tables, plan.lengths, plan.starts))
         self.lengths.copy_(plan.lengths)
         self.taken.add_(plan.taken)
-        return logits[:requests]
+        last = plan.starts[1:].long() - 1
+        logits = mt.affine_qmv(h[last.clamp(min=0)], *d.head)
+        if not score:
+            return logits
+        # (row t has the distribution of token t + 1, if that is the same request's)
+        first = torch.ones_like(tokens, dtype=torch.bool)
+        first[1:] = plan.requests[1:] != plan.requests[:-1]
+        after = torch.where(first, -1, tokens).roll(-1)
+        scores = mt.token_logprobs(mt.affine_qmv(h, *d.head), after).logprobs.roll(1)
+        return logits, torch.where(first, float("-inf"), scores)
+
+    def fork(self, sources, targets):
+        """Requests ``targets`` (int32) go on from the tokens of ``sources``."""
+        plan = mt.paged_fork(self.tables, self.lengths, sources, targets, self.free,
+                             page_size=self.page_size, free_start=self.taken)
+        mt.paged_copy(self.caches, plan.sources, plan.targets)
+        self.taken.add_(plan.taken)
+        self.tokens[targets.long()] = self.tokens[sources.long()]
+        self.scores[targets.long()] = self.scores[sources.long()]
+
+    def release(self, kept):
+        """Requests give back the pages behind their first ``kept`` tokens (int32 ``[requests]``)."""
+        pages = self.caches[0].pages
+        freed = mt.paged_free(self.tables, self.lengths, kept, self.free, page_size=self.page_size,
+                              pages=pages, free_start=self.taken)
+        self.taken.sub_(freed)
+        self.lengths.copy_(kept)
+
+    def compact(self):
+        """The pages in use become the lowest ones."""
+        plan = mt.paged_compact(self.tables, self.lengths, self.free, page_size=self.page_size,
+                                pages=self.caches[0].pages, free_start=self.taken)
+        mt.paged_copy(self.caches, plan.sources, plan.targets)
+        self.tables.copy_(plan.block_tables)
+        self.free.copy_(plan.free_pages)
 
     def choose(self, logits):
         """Greedy next tokens of the active requests in place; idle ones keep theirs."""
         self.tokens.copy_(torch.where(self.active > 0, logits.argmax(-1), self.tokens))
+
+    def choose_scored(self, logits):
+        """The same, and the log probabilities of the chosen tokens onto ``self.scores``."""
+        best = mt.token_logprobs(logits, top=1)
+        on = self.active > 0
+        self.tokens.copy_(torch.where(on, best.top_tokens[:, 0], self.tokens))
+        self.scores.add_(torch.where(on, best.top_logprobs[:, 0], 0.0))
+
+    def answer(self, answers, logits):
+        """Requests ``answers * r`` have prompts, whose last logits these are: those behind each go on
+        from its tokens, with the likeliest next token, the second, and so on."""
+        requests = self.tokens.shape[0]
+        rows = torch.arange(requests, dtype=torch.int32, device=self.tokens.device)
+        at = rows % answers
+        self.fork((rows - at)[at > 0], rows[at > 0])
+        best = mt.token_logprobs(logits[::answers], top=answers)
+        self.tokens.copy_(best.top_tokens.flatten()[:requests])
+        self.scores.copy_(best.top_logprobs.flatten()[:requests])
 
 
 def main():
@@ -139,20 +220,40 @@ def main():
     p.add_argument("--steps", type=int, default=64)
     p.add_argument("--layers", type=int, default=Config.layers)
     p.add_argument("--cache", choices=("bf16", "fp8"), default="bf16")
+    p.add_argument("--prompt", type=int, default=0, help="tokens of each request's prompt")
+    p.add_argument("--answers", type=int, default=1, help="requests that answer one prompt")
     a = p.parse_args()
+    if a.answers < 1 or a.answers > 32 or a.requests % a.answers or (a.answers > 1 and not a.prompt):
+        p.error("answers must be 1 to 32 of a prompt and divide the requests")
     decoder = Decoder(Config(layers=a.layers))
-    pages = a.requests * -(-(a.steps + 2) // 16)
-    batch = Batch(decoder, a.requests, pages=pages, longest=a.steps + 2,
+    longest = a.prompt + a.steps + 2
+    pages = a.requests * -(-longest // 16)
+    batch = Batch(decoder, a.requests, pages=pages, longest=longest,
                   cache_dtype=torch.float8_e4m3fn if a.cache == "fp8" else None)
     batch.tokens.copy_(torch.arange(a.requests) + 1)
+    choose = batch.choose
+    if a.prompt:
+        choose = batch.choose_scored
+        counts = torch.zeros_like(batch.lengths)
+        counts[::a.answers] = a.prompt
+        tokens = torch.randint(decoder.config.vocab, (a.requests // a.answers * a.prompt,), device="cuda")
+        batch.prefill(tokens, counts)  # once before the clock runs
+        batch.release(torch.zeros_like(counts))
+        torch.cuda.synchronize()
+        began = time.perf_counter()
+        batch.answer(a.answers, batch.prefill(tokens, counts))
+        torch.cuda.synchronize()
+        seconds = time.perf_counter() - began
+        print(f"{tokens.shape[0]} tokens of prompts: {1e3 * seconds:.3f} ms, "
+              f"{tokens.shape[0] / seconds:.0f} tokens/s")
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
-        batch.choose(batch.step())  # once outside capture: the stream's workspace
+        choose(batch.step())  # once outside capture: the stream's workspace
         stream.synchronize()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
-            batch.choose(batch.step())
+            choose(batch.step())
         stream.synchronize()
         began = time.perf_counter()
         for _ in range(a.steps):
@@ -162,6 +263,12 @@ def main():
     print(f"{a.requests} requests, {a.layers} layers, {a.steps} steps: "
           f"{1e3 * seconds / a.steps:.3f} ms a step, {a.requests * a.steps / seconds:.0f} tokens/s, "
           f"lengths {batch.lengths.unique().tolist()}, pages taken {int(batch.taken)} of {pages}")
+    if a.answers > 1:
+        best = batch.scores.view(-1, a.answers).argmax(1, keepdim=True)
+        kept = torch.arange(a.answers, device="cuda") == best
+        batch.release(torch.where(kept.flatten(), batch.lengths, 0).int())
+        batch.compact()
+        print(f"the likeliest answers hold {int(batch.taken)} pages")
 
 
 if __name__ == "__main__":

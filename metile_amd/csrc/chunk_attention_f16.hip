@@ -1,3 +1,4 @@
+// Chunk attention of float16 queries over a cache of their type.
 #include "chunk_attention_kernel.h"
 
 namespace mt {

@@ -1,3 +1,4 @@
+// Chunk attention of float16 queries over an 8-bit cache.
 #include "chunk_attention_kernel.h"
 
 namespace mt {

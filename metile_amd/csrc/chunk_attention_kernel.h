@@ -18,14 +18,20 @@
 // Probabilities enter the second product rounded to 16 bits (at most 2^-8 of each in bf16, 2^-11 in
 // f16), as the result itself is; a second part of them would add half as many products again. Scores,
 // references, sums and results are fp32, and the sums are of the probabilities before that rounding.
+//
+// What bounds it: the matrix and the vector unit, each busy half of the time and together nearly all of it
+// (heads of 128: 32 products and 190 vector instructions a wave and block), and beneath them the power: the
+// same launch over zeros takes 0.73 of the time. A prompt of 8192 tokens, 32 heads of 128 over 8, in bf16,
+// takes 548 us (1000 TFLOP/s; a library's product of 8192 x 8192 x 8192 reaches 1225), 509 tokens behind
+// 130500 take 1108 us (984). 1024 tokens behind 16384 run at 866 TFLOP/s in heads of 128, 696 in those of
+// 64, whose products have half the steps for the same exponentials, and 527 in those of 256, whose wave
+// fills the registers of a SIMD. Three waves a SIMD instead of two for heads of 64 were slower (24 parts of
+// prompts 54 -> 61 us), as were parts of fewer than four blocks or two and three parts for each slot.
 #pragma once
 
 #include "chunk_attention.h"
 #include "common.h"
 
-#ifndef WAVES64
-#define WAVES64 2
-#endif
 namespace mt {
 namespace chunk {
 
@@ -244,7 +250,7 @@ struct Offset<false> {
 // DIM: the head's values. With GENERAL, that many or more (the rest count as zero), in caches of any size;
 // else the offsets of rows fit 32 bits.
 template <int DT, bool FP8, int DIM, bool GENERAL>
-__global__ __launch_bounds__(kThreads, DIM == 64 ? WAVES64 : DIM <= 128 ? 2 : 1) void attention_kernel(
+__global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel(
     ChunkAttentionArgs a) {
   constexpr int kChunks = DIM / 8, kSteps = DIM / 16, kTiles = DIM / 32;
   constexpr int kLoads = kChunks * kBlock / kThreads;  // of a thread, a side
@@ -287,7 +293,7 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? WAVES64 : DIM <= 128 ? 2 : 1)
   const int r = item.request, splits = item.splits;
   const Request q = item.q;
   const int tile = item.tile(a), split = item.in_request % splits;
-  if (tile < 0 || (splits > 1 && item.part >= a.most_parts)) return;
+  if (tile < 0 || (splits > 1 && (uint32_t)item.part >= (uint32_t)a.most_parts)) return;
   const int row0 = tile * kTile, rows = min(kTile, q.count * a.group - row0);
   const Blocks all = blocks_of(a, q, (int)div_by(row0, a.by_group),
                                (int)div_by(row0 + rows - 1, a.by_group));

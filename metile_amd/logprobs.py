@@ -35,10 +35,10 @@ def token_logprobs(logits, tokens=None, *, top=0, temperature=1.0):
     ``[...]``): a token of each row, whose log probability and rank (how many are likelier, or as likely
     with a lower index: 0 is the likeliest) are wanted; one outside the vocabulary (padding) has -inf and
     rank -1. ``top``: how many of the likeliest tokens (0 to 32, at most ``vocab``), equal ones by index.
-    Entropies are in nats; ``temperature`` is 1e-6 to 1e6. Logits of -inf (tokens that are not allowed) have no probability; a row of
-    them alone has log probabilities of -inf and an entropy of 0. A row with NaN or +inf has NaN for both,
-    and NaN is no alternative (token -1 where there are too few others). Returns a
-    :class:`TokenLogprobs`; there are no gradients.
+    Entropies are in nats; ``temperature`` is 1e-6 to 1e6. Logits of -inf (tokens that are not allowed)
+    have no probability; a row of them alone has log probabilities of -inf and an entropy of 0. A row with
+    NaN or +inf has NaN for both, and NaN is no alternative (token -1 where there are too few others).
+    Returns a :class:`TokenLogprobs`; there are no gradients.
     """
     if logits.dtype not in _DTYPES:
         raise ValueError("logits must be bfloat16, float16 or float32")

@@ -487,7 +487,9 @@ def paged_free(block_tables, lengths, kept, free_pages, *, page_size, pages, fre
     ascending order, are written to ``free_pages`` in place, in front of entry ``free_start`` (a device
     int32 tensor of one element: how many entries have been taken). Returns how many there are (int32
     ``[1]``); tables and lengths are not changed. A caller goes on with ``lengths.copy_(kept)`` and
-    ``free_start.sub_(freed)``. ``pages``: of the cache.
+    ``free_start.sub_(freed)``. ``pages``: of the cache. A request that is cut inside a page which others
+    share must not write on in place: :func:`paged_fork` with ``tokens`` lets a row go on from there with
+    a page of its own.
     """
     device = block_tables.device
     _same_device(device, lengths, kept, free_pages, free_start)
