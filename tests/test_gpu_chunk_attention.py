@@ -308,6 +308,29 @@ def test_calls_on_two_streams_at_once():
         assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
 
 
+def far_pool(pages, page, heads, dim, dtype, apart, seed):
+    """A cache whose pages lie `apart` values from each other."""
+    t = torch.empty(pages * apart, dtype=dtype, device="cuda").as_strided(
+        (pages, page, heads, dim), (apart, heads * dim, dim, 1))
+    t.copy_(pool(pages, page, heads, dim, dtype, "inner", seed=seed))
+    return t
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, torch.bfloat16), (80, FP8), (96, torch.bfloat16),
+                                       (128, torch.bfloat16), (128, FP8), (192, FP8),
+                                       (256, torch.bfloat16)])
+@pytest.mark.parametrize("size", [(1 << 32) - (1 << 20), (1 << 32) + (1 << 20), 11 << 30])
+def test_offsets_about_and_beyond_32_bits(dim, dtype, size):
+    """Keys and values that end just below 4 GiB, just above, and far above."""
+    pages, page, heads = 9, 16, 2
+    apart = size // (pages * dtype.itemsize) // 16 * 16
+    c = case([70, 1], [40, 10], heads=4, kv=heads, dim=dim, page=page, cache=dtype)
+    c["scales"] = (1.0, 1.0)
+    c["tables"] = i32([[8, 0, 7, 1, 6, 2, 5], [4, 8, 3, 0, 1, 2, 5]])
+    c["key"], c["value"] = (far_pool(pages, page, heads, dim, dtype, apart, s) for s in (1, 2))
+    compare(run(c), expect(c))
+
+
 def test_refusals():
     cache = mt.PagedCache.allocate(4, 16, 2, 64)
     q = torch.zeros(5, 4, 64, dtype=torch.bfloat16, device="cuda")

@@ -124,6 +124,20 @@ def test_copy_of_more_pairs_than_a_launch_counts():
         assert bool((bits[p] == held).all()), p
 
 
+@pytest.mark.parametrize("size", [(1 << 32) + (1 << 20), 11 << 30])
+def test_copy_beyond_32_bits(size):
+    apart = size // 9 // 2 // 16 * 16
+    cache = mt.PagedCache(*(torch.empty(9 * apart, dtype=torch.bfloat16, device="cuda").as_strided(
+        (9, 16, 2, 64), (apart, 128, 64, 1)) for _ in range(2)))
+    for t in (cache.key, cache.value):
+        t.copy_(torch.randn(9, 16, 2, 64, device="cuda"))
+    want = [as_bits(t) for t in (cache.key, cache.value)]
+    for bits in want:
+        bits[8], bits[7] = bits[0].clone(), bits[5].clone()
+    mt.paged_copy(cache, i32([0, 5]), i32([8, 7]))
+    assert all(torch.equal(as_bits(t), bits) for t, bits in zip((cache.key, cache.value), want))
+
+
 # ---- forks ---------------------------------------------------------------------------------------------
 
 
