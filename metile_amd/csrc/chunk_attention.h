@@ -12,9 +12,11 @@ namespace mt {
 // Rows (token, query head of a key-value head) of a tile, and keys of a block.
 constexpr int kChunkTile = 128;
 constexpr int kChunkBlock = 64;
-// Blocks that a part of a tile's keys has at least, and requests of a call whose work its workgroups count
-// up themselves.
-constexpr int kChunkLeastBlocks = 4;
+// Tiles of fewer blocks are not split, and a part has at least two (a draft of 6 tokens over 2049 keys, us:
+// 15.5 with four, 14.2), or four in calls with so many blocks that there would be more than 64 parts (over
+// 32768 keys 24.0 with four, 29.1).
+constexpr int kChunkLeastSplit = 4, kChunkLeastBlocks = 2;
+// Requests of a call whose work its workgroups count up themselves.
 constexpr int kChunkHere = 64;
 
 struct ChunkAttentionArgs {
@@ -30,7 +32,7 @@ struct ChunkAttentionArgs {
   const int32_t* starts;                // [requests + 1]
   uint16_t* out;                        // [tokens, heads, dim] contiguous
   float* lse;                           // [tokens, heads] or null
-  int32_t* plan;                        // kPlanHead + 2 (requests + 1) entries
+  int32_t* plan;                        // kPlanHead + 3 (requests + 1) entries
   float* parts;                         // slots of chunk_part_floats each
   int32_t tokens, requests, kv_heads, group, dim, pages, page_size, width, window;
   int32_t target;                       // items that the work is split into, if it can be
@@ -41,7 +43,8 @@ struct ChunkAttentionArgs {
   DivMagic by_page, by_group;
 };
 
-// In front of the plan: blocks of a split, items and parts of one key-value head.
+// In front of the plan: blocks of a split, then items and tiles with parts of one key-value head. Behind it
+// the sums of items, parts and tiles with parts of the requests before each.
 constexpr int kPlanHead = 4;
 // Floats of a part: 16 a lane and 32 dimensions, then reference and sum of each row.
 size_t chunk_part_floats(int dim);

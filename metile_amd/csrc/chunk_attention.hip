@@ -19,7 +19,7 @@ constexpr int kPlanThreads = 1024;
 __device__ __forceinline__ int64_t most31(int64_t v) { return v < 0x7fffffff ? v : 0x7fffffff; }
 
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkAttentionArgs a) {
-  __shared__ int64_t sums[2][kPlanThreads];
+  __shared__ int64_t sums[3][kPlanThreads];
   const int tid = threadIdx.x;
   const int run = (a.requests + kPlanThreads - 1) / kPlanThreads;
   const int begin = min(tid * run, a.requests), end = min(begin + run, a.requests);
@@ -36,43 +36,50 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ChunkAttentionArgs a
   }
   const int64_t total = sums[0][0];
   __syncthreads();
-  const int per = (int)most31(max((total + a.target - 1) / a.target, (int64_t)kChunkLeastBlocks));
-  int64_t items = 0, parts = 0;
+  const int per = (int)most31(max((total + a.target - 1) / a.target, (int64_t)least_blocks((float)total)));
+  int64_t items = 0, parts = 0, joins = 0;
   for (int r = begin; r < end; ++r) {
     const Request q = request_of(a, r);
     const int64_t tiles = tiles_of(a, q);
     const int splits = splits_of(most_blocks(a, q), per);
     items += tiles * splits;
-    if (splits > 1) parts += tiles * splits;
+    if (splits > 1) parts += tiles * splits, joins += tiles;
   }
   sums[0][tid] = items;
   sums[1][tid] = parts;
+  sums[2][tid] = joins;
   __syncthreads();
   for (int step = 1; step < kPlanThreads; step *= 2) {
     const int64_t x = tid >= step ? sums[0][tid - step] : 0;
     const int64_t y = tid >= step ? sums[1][tid - step] : 0;
+    const int64_t z = tid >= step ? sums[2][tid - step] : 0;
     __syncthreads();
     sums[0][tid] += x;
     sums[1][tid] += y;
+    sums[2][tid] += z;
     __syncthreads();
   }
   items = sums[0][tid] - items;
   parts = sums[1][tid] - parts;
+  joins = sums[2][tid] - joins;
   int32_t* item_sums = a.plan + kPlanHead;
   int32_t* part_sums = item_sums + a.requests + 1;
+  int32_t* join_sums = part_sums + a.requests + 1;
   for (int r = begin; r < end; ++r) {
     item_sums[r] = (int32_t)most31(items);
     part_sums[r] = (int32_t)most31(parts);
+    join_sums[r] = (int32_t)most31(joins);
     const Request q = request_of(a, r);
     const int64_t tiles = tiles_of(a, q);
     const int splits = splits_of(most_blocks(a, q), per);
     items += tiles * splits;
-    if (splits > 1) parts += tiles * splits;
+    if (splits > 1) parts += tiles * splits, joins += tiles;
   }
   if (tid == kPlanThreads - 1) {
     a.plan[0] = per;
     a.plan[1] = item_sums[a.requests] = (int32_t)most31(sums[0][tid]);
-    a.plan[2] = part_sums[a.requests] = (int32_t)most31(sums[1][tid]);
+    part_sums[a.requests] = (int32_t)most31(sums[1][tid]);
+    a.plan[2] = join_sums[a.requests] = (int32_t)most31(sums[2][tid]);
   }
 }
 
@@ -92,8 +99,9 @@ ChunkPlan plan_chunk_attention(int tokens, int requests, int kv_heads, int group
   const int slots = (dim <= 128 ? 2 : 1) * cus;
   p.target = (slots + kv_heads - 1) / kv_heads;
   if (window > 0) most_keys = std::min<int64_t>(most_keys, (int64_t)window + kChunkTile);
-  const int64_t blocks = (most_keys + kChunkBlock - 1) / kChunkBlock + 1;
-  const int64_t splits = (blocks + kChunkLeastBlocks - 1) / kChunkLeastBlocks;
+  const int64_t blocks = (most_keys + kChunkBlock - 1) / kChunkBlock + (window > 0);
+  const int64_t splits =
+      blocks < kChunkLeastSplit ? 1 : (blocks + kChunkLeastBlocks - 1) / kChunkLeastBlocks;
   p.parts = splits > 1 ? (int)std::min<int64_t>(2 * p.target, splits * p.tiles) : 0;
   return p;
 }

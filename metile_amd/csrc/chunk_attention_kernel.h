@@ -26,8 +26,10 @@
 // 130500 take 1108 us (984). 1024 tokens behind 16384 run at 866 TFLOP/s in heads of 128, 696 in those of
 // 64, whose products have half the steps for the same exponentials, and 527 in those of 256, whose wave
 // fills the registers of a SIMD. Three waves a SIMD instead of two for heads of 64 were slower (24 parts of
-// prompts 54 -> 61 us), as were parts of fewer than four blocks or two and three parts for each slot.
+// prompts 54 -> 61 us), as were two and three parts for each slot.
 #pragma once
+
+#include <algorithm>
 
 #include "chunk_attention.h"
 #include "common.h"
@@ -81,7 +83,11 @@ __device__ __forceinline__ int most_blocks(const ChunkAttentionArgs& a, const Re
 
 // Parts of each tile of a request whose tiles have up to `most` blocks.
 __device__ __forceinline__ int splits_of(int most, int per) {
-  return max((int)(((int64_t)most + per - 1) / per), 1);
+  return most < kChunkLeastSplit ? 1 : (int)(((int64_t)most + per - 1) / per);
+}
+// Blocks that a part has at least, of a call with so many.
+__device__ __forceinline__ int least_blocks(float total) {
+  return (int)fminf(fmaxf(total * (1.0f / 64.0f), (float)kChunkLeastBlocks), 4.0f);
 }
 
 // An item: a request's tile, or one part of `splits` of its keys; `part` is where a part is kept.
@@ -111,9 +117,10 @@ __device__ __forceinline__ T wave_scan(T v) {
 }
 __device__ __forceinline__ int readlane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 
-// Item n, or with PARTS the item that part n is of, of a call of up to 64 requests: each wave counts the
-// work up for itself, a lane a request. `behind` receives the packed row behind the last request's.
-template <bool PARTS>
+// Item n, or with JOIN the first part of the n-th tile that has parts, of a call of up to 64 requests: each
+// wave counts the work up for itself, a lane a request. `behind` receives the packed row behind the last
+// request's.
+template <bool JOIN>
 __device__ __forceinline__ Item find_here(const ChunkAttentionArgs& a, int n, int* behind) {
   const int lane = threadIdx.x & 63, r = min(lane, a.requests - 1);
   const Request q = request_of(a, r);
@@ -124,17 +131,18 @@ __device__ __forceinline__ Item find_here(const ChunkAttentionArgs& a, int n, in
       __builtin_bit_cast(float, readlane(__builtin_bit_cast(int, wave_scan((float)tiles * (float)most)),
                                          63));
   const int per =
-      max((int)fminf(total * 1.0001f / (float)a.target + 1.0f, 1073741824.0f), kChunkLeastBlocks);
+      max((int)fminf(total * 1.0001f / (float)a.target + 1.0f, 1073741824.0f), least_blocks(total));
   const int splits = splits_of(most, per);
   const int items = tiles * splits, parts = splits > 1 ? items : 0;
-  const int item_sums = wave_scan(items), part_sums = wave_scan(parts);
-  const uint64_t later = __ballot((PARTS ? part_sums : item_sums) > n);
+  const int count = !JOIN ? items : splits > 1 ? tiles : 0;
+  const int sums = wave_scan(count), part_sums = wave_scan(parts);
+  const uint64_t later = __ballot(sums > n);
   Item i{-1, 1, 0, 0, {}};
   if (!later) return i;
   const int l = __ffsll((unsigned long long)later) - 1;
   i.request = l;
   i.splits = readlane(splits, l);
-  i.in_request = n - readlane(PARTS ? part_sums - parts : item_sums - items, l);
+  i.in_request = (n - readlane(sums - count, l)) * (JOIN ? i.splits : 1);
   i.part = readlane(part_sums - parts, l) + i.in_request;
   i.q = {readlane(q.start, l), readlane(q.count, l), readlane(q.first, l), readlane(q.keys, l)};
   return i;
@@ -142,14 +150,14 @@ __device__ __forceinline__ Item find_here(const ChunkAttentionArgs& a, int n, in
 
 // The same of a call of more requests, from the sums that the plan holds: the last request whose sum of
 // those before it is at most n, 64 at a time, by a whole wave.
-template <bool PARTS>
+template <bool JOIN>
 __device__ __forceinline__ Item find_planned(const ChunkAttentionArgs& a, int n, int* behind) {
   const int lane = threadIdx.x & 63;
   const int32_t *items = a.plan + kPlanHead, *parts = items + a.requests + 1;
-  const int32_t* sums = PARTS ? parts : items;
+  const int32_t* sums = JOIN ? parts + a.requests + 1 : items;
   *behind = min(max(a.starts[a.requests], 0), a.tokens);
   Item i{-1, 1, 0, 0, {}};
-  if (n >= a.plan[PARTS ? 2 : 1]) return i;
+  if (n >= a.plan[JOIN ? 2 : 1]) return i;
   int lo = 0;
   for (int count = a.requests; count > 1;) {
     const int step = (count + 63) / 64;
@@ -161,13 +169,13 @@ __device__ __forceinline__ Item find_planned(const ChunkAttentionArgs& a, int n,
   i.request = lo;
   i.q = request_of(a, lo);
   i.splits = splits_of(most_blocks(a, i.q), a.plan[0]);
-  i.in_request = n - sums[lo];
+  i.in_request = (n - sums[lo]) * (JOIN ? i.splits : 1);
   i.part = parts[lo] + i.in_request;
   return i;
 }
-template <bool PARTS>
+template <bool JOIN>
 __device__ __forceinline__ Item find(const ChunkAttentionArgs& a, int n, int* behind) {
-  return a.requests <= kChunkHere ? find_here<PARTS>(a, n, behind) : find_planned<PARTS>(a, n, behind);
+  return a.requests <= kChunkHere ? find_here<JOIN>(a, n, behind) : find_planned<JOIN>(a, n, behind);
 }
 
 template <int DT>
@@ -759,24 +767,25 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
                              : (base + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
-// The parts of tiles whose keys were split, joined in order. Workgroup (part of one head, head, 32
-// dimensions); those of a tile's first part do it, a wave 32 rows, in the layout that they were stored.
-template <int DT, int DIM>
-__global__ __launch_bounds__(kThreads) void join_kernel(ChunkAttentionArgs a) {
+// The parts of a tile whose keys were split, joined in an order that does not change. Workgroup (tile of
+// those, head; 32 dimensions; 32 rows): its waves take the parts in turn, in the layout that they were
+// stored, and what they have is joined through LDS. With kWaves of 1 there are four to a workgroup, each
+// with all parts of 32 rows.
+template <int DT, int DIM, int kWaves>
+__global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void join_kernel(ChunkAttentionArgs a) {
   constexpr int kTiles = DIM / 32, kPart = kTile * (DIM + 2), kBatch = 4;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, in_group = uniform(threadIdx.x >> 6);
+  const int wave = kWaves == 1 ? 0 : in_group, slab = kWaves == 1 ? in_group : blockIdx.z;
   const int col = lane & 31, half = lane >> 5;
-  const int head = (int)(blockIdx.x % (unsigned)a.kv_heads);
-  const int part = (int)(blockIdx.x / (unsigned)a.kv_heads), t = blockIdx.y;
+  const int head = (int)(blockIdx.x % (unsigned)a.kv_heads), t = blockIdx.y;
   int behind;
-  const Item item = find<true>(a, part, &behind);
+  const Item item = find<true>(a, (int)(blockIdx.x / (unsigned)a.kv_heads), &behind);
   if (item.request < 0) return;
   const Request q = item.q;
-  const int splits = item.splits, tile = item.tile(a);
-  if (item.in_request % splits || part + splits > a.most_parts) return;
-  if (tile < 0) return;
+  const int splits = item.splits, tile = item.tile(a), part = item.part;
+  if (tile < 0 || part < 0 || part + splits > a.most_parts) return;
   const int row0 = tile * kTile, rows = min(kTile, q.count * a.group - row0);
-  if (32 * wave >= rows) return;
+  if (32 * slab >= rows) return;
   const float* from = a.parts + ((int64_t)part * a.kv_heads + head) * kPart;
   const int64_t step = (int64_t)a.kv_heads * kPart;
 
@@ -784,45 +793,70 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ChunkAttentionArgs a) {
   float acc[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-  for (int n0 = 0; n0 < splits; n0 += kBatch) {
+  auto fix_of = [](float from, float to) { return fmaxf(__builtin_amdgcn_exp2f(from - to), kTiny); };
+  for (int n0 = wave; n0 < splits; n0 += kBatch * kWaves) {
     float b[kBatch], l[kBatch], v[kBatch][16];
 #pragma unroll
     for (int n = 0; n < kBatch; ++n) {
-      const float* p = from + min(n0 + n, splits - 1) * step;
-      b[n] = p[kTile * DIM + 32 * wave + col];
-      l[n] = p[kTile * (DIM + 1) + 32 * wave + col];
+      const float* p = from + min(n0 + n * kWaves, splits - 1) * step;
+      b[n] = p[kTile * DIM + 32 * slab + col];
+      l[n] = p[kTile * (DIM + 1) + 32 * slab + col];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[n][i] = p[((wave * kTiles + t) * 16 + i) * 64 + lane];
+      for (int i = 0; i < 16; ++i) v[n][i] = p[((slab * kTiles + t) * 16 + i) * 64 + lane];
     }
 #pragma unroll
     for (int n = 0; n < kBatch; ++n) {
-      if (n0 + n >= splits || b[n] == -__builtin_inff()) continue;
+      if (n0 + n * kWaves >= splits || b[n] == -__builtin_inff()) continue;
       const float next = fmaxf(base, b[n]);
-      const float old = fmaxf(__builtin_amdgcn_exp2f(base - next), kTiny);
-      const float now = fmaxf(__builtin_amdgcn_exp2f(b[n] - next), kTiny);
+      const float old = fix_of(base, next), now = fix_of(b[n], next);
       sum = sum * old + l[n] * now;
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[i] = acc[i] * old + v[n][i] * now;
       base = next;
     }
   }
-  if (32 * wave + col >= rows) return;
-  const int my_row = row0 + 32 * wave + col;
+  const bool has_row = 32 * slab + col < rows;
+  const int my_row = row0 + min(32 * slab + col, rows - 1);
   const int token = (int)div_by(my_row, a.by_group);
   const int64_t row = (int64_t)(q.start + token) * a.kv_heads * a.group + head * a.group +
                       (my_row - token * a.group);
-  const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
-#pragma unroll
-  for (int i = 0; i < 16; i += 4) {
-    const int d = 32 * t + 2 * i + 4 * half;
-    if (d < a.dim)
+  // values 4 g .. 4 g + 3 of a lane
+  auto write = [&](int g, float x0, float x1, float x2, float x3) {
+    const float inv = sum == 0.0f ? 0.0f : a.value_scale / sum;
+    const int d = 32 * t + 8 * g + 4 * half;
+    if (has_row && d < a.dim)
       *reinterpret_cast<u32x2*>(a.out + row * a.dim + d) =
-          (u32x2){pack2<DT>(acc[i] * inv, acc[i + 1] * inv),
-                  pack2<DT>(acc[i + 2] * inv, acc[i + 3] * inv)};
+          (u32x2){pack2<DT>(x0 * inv, x1 * inv), pack2<DT>(x2 * inv, x3 * inv)};
+    if (has_row && a.lse && half == 0 && t == 0 && g == 0)
+      a.lse[row] = sum == 0.0f ? -__builtin_inff()
+                               : (base + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+  };
+  if constexpr (kWaves == 1) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) write(g, acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]);
+  } else {
+    __shared__ float kept[kWaves][16][64], bases[kWaves][64], sums[kWaves][64];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) kept[wave][i][lane] = acc[i];
+    bases[wave][lane] = base;
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave >= 4) return;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) base = fmaxf(base, bases[w][lane]);
+    sum = 0.0f;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float b = bases[w][lane];
+      if (b == -__builtin_inff()) continue;
+      const float now = fix_of(b, base);
+      sum += sums[w][lane] * now;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += kept[w][4 * wave + e][lane] * now;
+    }
+    write(wave, x[0], x[1], x[2], x[3]);
   }
-  if (a.lse && half == 0 && t == 0)
-    a.lse[row] = sum == 0.0f ? -__builtin_inff()
-                             : (base + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
 template <int DT, bool FP8, int DIM>
@@ -831,9 +865,23 @@ hipError_t launch_dim(const ChunkAttentionArgs& a, hipStream_t stream) {
   if (a.dim == DIM && a.narrow)
     attention_kernel<DT, FP8, DIM, false><<<items, kThreads, 0, stream>>>(a);
   else attention_kernel<DT, FP8, DIM, true><<<items, kThreads, 0, stream>>>(a);
-  if (a.most_parts > 0)
-    join_kernel<DT, DIM><<<dim3((unsigned)a.most_parts * (unsigned)a.kv_heads, DIM / 32), kThreads,
-                           0, stream>>>(a);
+  if (a.most_parts > 0) {
+    // (a tile that has parts has two or more)
+    const int tiles = std::min(a.most_tiles, a.most_parts / 2);
+    const int slabs = (int)((std::min<int64_t>(kTile, (int64_t)a.tokens * a.group) + 31) / 32);
+    dim3 grid((unsigned)tiles * (unsigned)a.kv_heads, DIM / 32, slabs);
+    const int parts = std::min(a.target, a.most_parts) / tiles;  // of a tile
+    // (us of a draft of 6 tokens with 4 waves and with 16: 33 parts 16.9 and 17.9, 128 28.0 and 24.7; of
+    // 24 parts of prompts, which have one part or few, with 1 and with 4: 49.7 and 55.4)
+    if (parts > 64) {
+      join_kernel<DT, DIM, 16><<<grid, 1024, 0, stream>>>(a);
+    } else if (parts > 4) {
+      join_kernel<DT, DIM, 4><<<grid, 256, 0, stream>>>(a);
+    } else {
+      grid.z = 1;
+      join_kernel<DT, DIM, 1><<<grid, 256, 0, stream>>>(a);
+    }
+  }
   return hipGetLastError();
 }
 

@@ -131,7 +131,7 @@ int plan_chunks(const char* op, const mt_paged_cache* c, int tokens, int request
   call->plan = mt::plan_chunk_attention(tokens, requests, c->heads, heads / c->heads, c->dim,
                                         (int64_t)width * c->page_size, window,
                                         mt::current_device_cus());
-  const size_t ints = mt::kPlanHead + 2 * ((size_t)requests + 1);
+  const size_t ints = mt::kPlanHead + 3 * ((size_t)requests + 1);
   call->plan_bytes = (ints * 4 + 255) / 256 * 256;
   call->bytes = call->plan_bytes +
                 (size_t)call->plan.parts * c->heads * mt::chunk_part_floats(c->dim) * 4;

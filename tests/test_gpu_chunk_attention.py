@@ -129,6 +129,20 @@ def test_long_context_is_split(dtype, cache):
     check([30], [4000], heads=3, kv=1, dim=256, dtype=dtype, cache=cache, window=3000)
 
 
+@pytest.mark.parametrize("past", [120, 185, 190, 250, 2000, 9000, 33000, 70000])
+@pytest.mark.parametrize("heads,kv,dim", [(12, 2, 128), (3, 1, 64), (40, 1, 80), (2, 1, 256)])
+def test_few_rows_in_few_and_many_parts(heads, kv, dim, past):
+    check([6], [past], heads=heads, kv=kv, dim=dim, page=64, dtype=torch.float16)
+
+
+def test_many_parts_beside_requests_with_none():
+    """Some tiles of a call are split and some are not, in both ways of counting them."""
+    for requests in (60, 70):
+        new = [(r % 4) * 3 for r in range(requests)]
+        past = [9000 if r % 9 == 5 else r for r in range(requests)]
+        check(new, past, heads=4, kv=1, dim=64, padding=5, seed=requests)
+
+
 def test_large_scores_and_f16_probabilities():
     """Scores of hundreds, in rising and falling order along the keys."""
     for dtype in (torch.bfloat16, torch.float16):
