@@ -547,8 +547,9 @@ int mt_paged_free(const mt_paged_free_args* args, void* workspace, size_t worksp
  * numbers. The highest in use moves to the lowest free one, and so on: sources and targets [most_moves]
  * (at least min(pages / 2, requests * width); -1 behind the last) for mt_paged_copy, moves [1] how many.
  * new_tables [requests, width] receives the block tables as they are then, new_free [free_count] the free
- * list (up to *free_start as it was, then ascending; -1 behind the last where a page was listed twice or in use). Inputs are not changed. Pages neither in use nor free are left alone. The
- * workspace need not be cleared. width * page_size is below 2^31. Outputs overlap no input. */
+ * list (up to *free_start as it was, then ascending; -1 behind the last where a page was listed twice or in
+ * use). Inputs are not changed. Pages neither in use nor free are left alone. The workspace need not be
+ * cleared. width * page_size is below 2^31. Outputs overlap no input. */
 typedef struct mt_paged_compact_args {
   const int32_t* block_tables;
   int64_t table_stride;
@@ -573,8 +574,9 @@ int mt_paged_compact(const mt_paged_compact_args* args, void* workspace, size_t 
  * logprobs and ranks may be NULL together. Logits of -inf have no probability and no part in the entropy;
  * a token outside the vocabulary has -inf and rank -1. A row of -inf alone has log probabilities of -inf
  * and an entropy of 0. A row with NaN or +inf has NaN for both; NaN is no alternative (token -1 where there
- * are too few others). All sums are fp32 in a fixed order. Logits need the alignment of their type only.
- * vocab is at most 2^24, temperature 1e-6 to 1e6. The workspace need not be cleared; its size depends on the shapes alone. */
+ * are too few others). A thread's sums are fp32, those of threads 64 bits, in a fixed order. Logits need the
+ * alignment of their type only. vocab is at most 2^24, temperature 1e-6 to 1e6. The workspace need not be
+ * cleared; its size depends on the shapes alone. */
 typedef struct mt_token_logprobs_args {
   const void* logits;
   int64_t row_stride;

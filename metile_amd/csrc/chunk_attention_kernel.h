@@ -67,7 +67,7 @@ struct Blocks {
 __device__ __forceinline__ Blocks blocks_of(const ChunkAttentionArgs& a, const Request& q, int t0,
                                             int t1) {
   const int hi = min(q.first + t1 + 1, q.keys);
-  const int lo = a.window ? max(q.first + t0 + 1 - a.window, 0) : 0;
+  const int lo = a.window ? max(max(q.first + t0 + 1, 0) - a.window, 0) : 0;  // (in 32 bits)
   Blocks b;
   b.first = lo / kBlock;
   b.count = hi > lo ? (hi + kBlock - 1) / kBlock - b.first : 0;
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   const int my_head = head * a.group + (my_row - my_token * a.group);
   const bool has_row = 32 * wave + col < rows;
   const int my_end = min(q.first + my_token + 1, q.keys);  // keys below
-  const int my_begin = a.window ? max(q.first + my_token + 1 - a.window, 0) : 0;
+  const int my_begin = a.window ? max(max(q.first + my_token + 1, 0) - a.window, 0) : 0;
   // (rows are in order of their tokens, so the ends of lanes 0 and 31 bound the wave's; readlane of
   // lanes whose row repeats the last one)
   const int first_end = __builtin_amdgcn_readlane(my_end, 0);
@@ -356,7 +356,8 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
     uint32_t slot;
   };
   auto look_up = [&](int block) __attribute__((always_inline)) {
-    const uint32_t token = (uint32_t)min(block * kBlock + lane, last_key);
+    // (blocks past the end may be past 2^31 too)
+    const uint32_t token = min((uint32_t)block * kBlock + (uint32_t)lane, (uint32_t)last_key);
     const uint32_t column = div_by(token, a.by_page);
     return Place{table[column], token - column * (uint32_t)a.page_size};
   };
@@ -744,7 +745,8 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
 #pragma unroll
       for (int i = 0; i < 16; ++i) to[((wave * kTiles + t) * 16 + i) * 64 + lane] = acc[t][i];
     if (half == 0) {
-      to[kTile * DIM + 32 * wave + col] = base;
+      // (a sum that is no number has no reference, but is not nothing)
+      to[kTile * DIM + 32 * wave + col] = sum != sum && base == -__builtin_inff() ? 0.0f : base;
       to[kTile * (DIM + 1) + 32 * wave + col] = sum;
     }
     return;

@@ -345,6 +345,58 @@ def test_offsets_about_and_beyond_32_bits(dim, dtype, size):
     compare(run(c), expect(c))
 
 
+def test_largest_window_of_a_chunk_longer_than_its_request():
+    c = case([300], [0], heads=2, kv=1, dim=64, window=(1 << 31) - 1)
+    c["lengths"].copy_(i32([200]))
+    compare(run(c), expect(c))
+
+
+def test_longest_table():
+    """2^31 - 128 keys, all of them one page's: the page's result. A part's sums have 2^16 equal terms (blocks),
+    each rounded by at most 2^-24 of the sum, so they are off by 2^-8 of it at most."""
+    page, dim = 64, 16
+    key, value = (pool(1, page, 1, dim, torch.bfloat16, "inner", seed=s) for s in (1, 2))
+    cache = mt.PagedCache(key, value)
+    width = (1 << 25) - 2
+    tables = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 1, dim, device="cuda").bfloat16()
+    one, starts = i32([page]), i32([0, 1])
+    out, lse = mt.paged_chunk_attention(q, cache, tables, i32([width * page]), starts, return_lse=True)
+    want, want_lse = mt.paged_chunk_attention(q, cache, tables, one, starts, return_lse=True)
+    assert float((lse - want_lse - math.log(width)).abs().max()) <= 2.0 ** -8 + 2.0 ** -20
+    # (numerator and denominator, a rounding of either result)
+    assert float((out.float() - want.float()).abs().max()) <= (2.0 ** -7 + 2.0 ** -7) * float(value.abs().max())
+    over = mt.paged_chunk_attention(q, cache, tables, i32([(1 << 31) - 1]), starts)
+    assert torch.equal(over, out)
+
+
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+def test_queries_that_are_no_numbers_keep_to_themselves(odd):
+    c = case([40, 3], [200, 3000], heads=4, kv=2, dim=64)
+    clean = run(c)
+    want = expect(c)
+    c["query"][5, 2, 7] = odd
+    c["query"][41, 0, 0] = odd
+    out, lse = run(c)
+    for row, head in ((5, 2), (41, 0)):
+        assert bool(torch.isnan(out[row, head]).all()) and not bool(torch.isfinite(lse[row, head]))
+        out[row, head], lse[row, head] = clean[0][row, head], clean[1][row, head]
+    compare((out, lse), want)
+
+
+def test_8_bit_nan_that_no_token_sees():
+    c = case([30], [70], heads=4, kv=2, dim=64, cache=FP8, extra_columns=1)
+    want = expect(c)
+    used = set(c["tables"][0, :7].tolist())
+    for t in (c["key"], c["value"]):
+        bits = t.view(torch.uint8)
+        for p in range(t.shape[0]):
+            if p not in used:
+                bits[p] = 0x7f
+        bits[int(c["tables"][0, 6]), 4:] = 0x7f  # behind the 100 tokens
+    compare(run(c), want)
+
+
 def test_refusals():
     cache = mt.PagedCache.allocate(4, 16, 2, 64)
     q = torch.zeros(5, 4, 64, dtype=torch.bfloat16, device="cuda")
