@@ -36,6 +36,7 @@ struct ChunkAttentionArgs {
   float* parts;                         // slots of chunk_part_floats each
   int32_t tokens, requests, kv_heads, group, dim, pages, page_size, width, window;
   int32_t target;                       // items that the work is split into, if it can be
+  int32_t slots;                        // workgroups that run at once
   int32_t most_tiles, most_parts;       // of one key-value head
   float scale_log2, value_scale;
   bool narrow;                          // every row of a head begins less than 4 GiB behind its first
@@ -51,7 +52,7 @@ size_t chunk_part_floats(int dim);
 
 // Bounds of a call's tiles and parts of one key-value head, and the items wanted of it, from shapes.
 struct ChunkPlan {
-  int tiles, parts, target;
+  int tiles, parts, target, slots;
 };
 ChunkPlan plan_chunk_attention(int tokens, int requests, int kv_heads, int group, int dim,
                                int64_t most_keys, int window, int cus);

@@ -96,8 +96,8 @@ ChunkPlan plan_chunk_attention(int tokens, int requests, int kv_heads, int group
                                int64_t most_keys, int window, int cus) {
   ChunkPlan p;
   p.tiles = (int)((int64_t)tokens * group / kChunkTile) + std::min(requests, tokens);
-  const int slots = (dim <= 128 ? 2 : 1) * cus;
-  p.target = (slots + kv_heads - 1) / kv_heads;
+  p.slots = (dim <= 128 ? 2 : 1) * cus;
+  p.target = (p.slots + kv_heads - 1) / kv_heads;
   if (window > 0) most_keys = std::min<int64_t>(most_keys, (int64_t)window + kChunkTile);
   const int64_t blocks = (most_keys + kChunkBlock - 1) / kChunkBlock + (window > 0);
   const int64_t splits =

@@ -23,9 +23,9 @@
 // (heads of 128: 32 products and 190 vector instructions a wave and block), and beneath them the power: the
 // same launch over zeros takes 0.73 of the time. A prompt of 8192 tokens, 32 heads of 128 over 8, in bf16,
 // takes 548 us (1000 TFLOP/s; a library's product of 8192 x 8192 x 8192 reaches 1225), 509 tokens behind
-// 130500 take 1108 us (984). 1024 tokens behind 16384 run at 866 TFLOP/s in heads of 128, 696 in those of
-// 64, whose products have half the steps for the same exponentials, and 527 in those of 256, whose wave
-// fills the registers of a SIMD. Three waves a SIMD instead of two for heads of 64 were slower (24 parts of
+// 130500 take 1108 us (984). 1024 tokens behind 16384 run at 860 TFLOP/s in heads of 128, 690 in those of
+// 64, whose products have half the steps for the same exponentials, and 575 and 675 in those of 192 and 256,
+// whose wave fills the registers of a SIMD (256 with results in accumulation registers: 531). Three waves a SIMD instead of two for heads of 64 were slower (24 parts of
 // prompts 54 -> 61 us), as were two and three parts for each slot.
 #pragma once
 
@@ -117,6 +117,28 @@ __device__ __forceinline__ T wave_scan(T v) {
 }
 __device__ __forceinline__ int readlane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 
+// Blocks of a part of one request's tiles, so that the last round of workgroups is not left nearly empty: a
+// lane a choice, from twice to a third of an even share, the last one `per`, which is kept unless another
+// promises a seventh less. A round takes as long as an item and its start; one that leaves half of the slots
+// free (of two a CU) three quarters of that.
+__device__ __forceinline__ int best_parts(const ChunkAttentionArgs& a, int lane, float even, int per,
+                                          int tiles, int most) {
+  constexpr float kStart = 3.0f;  // in blocks
+  const int mine = lane == 63 ? per : (int)fmaxf(even * 16.0f / (float)(lane % 40 + 8), kChunkLeastBlocks);
+  const int splits = splits_of(most, mine);
+  const float items = (float)tiles * (float)splits;
+  const float rounds = items * (float)a.kv_heads / (float)a.slots, whole = floorf(rounds);
+  const float rest = rounds - whole;
+  const float last = rest == 0.0f ? 0.0f : a.dim <= 128 && rest <= 0.5f ? 0.75f : 1.0f;
+  float cost = (whole + last) * (ceilf((float)most / (float)splits) + kStart);
+  if (splits > 1 && items > (float)a.most_parts) cost = 3.0e38f;
+  if (lane == 63) cost *= 0.85f;
+  float least = cost;
+  for (int d = 32; d; d /= 2) least = fminf(least, __shfl_xor(least, d));
+  // (of equal ones the first lane's, which has the fewest parts; `per` has room for its own)
+  return readlane(mine, __ffsll((unsigned long long)__ballot(cost == least)) - 1);
+}
+
 // Item n, or with JOIN the first part of the n-th tile that has parts, of a call of up to 64 requests: each
 // wave counts the work up for itself, a lane a request. `behind` receives the packed row behind the last
 // request's.
@@ -130,8 +152,12 @@ __device__ __forceinline__ Item find_here(const ChunkAttentionArgs& a, int n, in
   const float total =
       __builtin_bit_cast(float, readlane(__builtin_bit_cast(int, wave_scan((float)tiles * (float)most)),
                                          63));
-  const int per =
-      max((int)fminf(total * 1.0001f / (float)a.target + 1.0f, 1073741824.0f), least_blocks(total));
+  const float even = total * 1.0001f / (float)a.target;  // blocks of an item, if all were the same
+  int per = max((int)fminf(even + 1.0f, 1073741824.0f), least_blocks(total));
+  // (us of 1024 tokens behind 16384 without and with the choice: 14 heads of 64 on 2 129 and 108, 24 of 96 on 3
+  // 261 and 221, 20 of 192 on 5 588 and 460)
+  if (a.requests == 1 && even > 16.0f)
+    per = best_parts(a, lane, even, per, readlane(tiles, 0), readlane(most, 0));
   const int splits = splits_of(most, per);
   const int items = tiles * splits, parts = splits > 1 ? items : 0;
   const int count = !JOIN ? items : splits > 1 ? tiles : 0;
@@ -863,7 +889,9 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void join_kernel(C
 
 template <int DT, bool FP8, int DIM>
 hipError_t launch_dim(const ChunkAttentionArgs& a, hipStream_t stream) {
-  const unsigned items = (unsigned)(a.most_tiles + a.target) * (unsigned)a.kv_heads;
+  // Items: no more than there are tiles and, on top of them, even shares; or one request's tiles or parts.
+  const int most = a.requests > 1 ? a.most_tiles + a.target : std::max(a.most_tiles, a.most_parts);
+  const unsigned items = (unsigned)most * (unsigned)a.kv_heads;
   if (a.dim == DIM && a.narrow)
     attention_kernel<DT, FP8, DIM, false><<<items, kThreads, 0, stream>>>(a);
   else attention_kernel<DT, FP8, DIM, true><<<items, kThreads, 0, stream>>>(a);

@@ -445,6 +445,7 @@ int mt_paged_chunk_attention(const mt_paged_cache* cache, const mt_paged_chunk_a
   a.width = in.width;
   a.window = in.window;
   a.target = call.plan.target;
+  a.slots = call.plan.slots;
   a.most_tiles = call.plan.tiles;
   a.most_parts = call.plan.parts;
   // A scale below zero is the query's; one of zero stands for the smallest, whose products are as

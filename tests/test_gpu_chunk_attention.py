@@ -135,6 +135,15 @@ def test_few_rows_in_few_and_many_parts(heads, kv, dim, past):
     check([6], [past], heads=heads, kv=kv, dim=dim, page=64, dtype=torch.float16)
 
 
+@pytest.mark.parametrize("new,past", [(300, 8000), (1100, 3000)])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(14, 2, 64, torch.float16), (24, 3, 96, torch.bfloat16),
+                                                (20, 5, 192, torch.bfloat16), (16, 1, 256, FP8),
+                                                (9, 1, 128, torch.float16)])
+def test_one_request_in_parts_that_fill_rounds(heads, kv, dim, dtype, new, past):
+    check([new], [past], heads=heads, kv=kv, dim=dim, page=64, cache=dtype,
+          dtype=torch.bfloat16 if dtype == FP8 else dtype)
+
+
 def test_many_parts_beside_requests_with_none():
     """Some tiles of a call are split and some are not, in both ways of counting them."""
     for requests in (60, 70):
