@@ -122,9 +122,10 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(PagedForkArgs a, DivMagi
   }
 }
 
+// ---- marks -----------------------------------------------------------------------------------------
+
 // Freeing and compaction are bound by launches and round trips, 2 to 5 us each: with marks in memory, whose
 // stores from many CUs meet there, every step of them is a launch.
-// ---- marks -----------------------------------------------------------------------------------------
 
 // Pages of a thread. (Free and compact of 24000 pages, us: 9.8 and 15.6, with 16 10.2 and 17.4, with 4 9.6
 // and 14.7; of 4000000: 52 and 149, with 16 49 and 157, with 4 60 and 153.)
