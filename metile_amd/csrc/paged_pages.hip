@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(PagedForkArgs a, DivMagi
   if (f.source < 0) return;
   const int32_t* from = a.tables + (int64_t)f.source * a.table_stride;
   int32_t* to = a.tables + (int64_t)f.target * a.table_stride;
-  for (int c = tid; c < full; c += kThreads) to[c] = from[c];
+  for (uint32_t c = tid; c < (uint32_t)full; c += kThreads) to[c] = from[c];
   if (tid == 0) {
     if (partial) to[full] = fresh;
     a.lengths[f.target] = f.tokens;
@@ -148,23 +148,29 @@ __device__ __forceinline__ int columns_of(int tokens, DivMagic by_page, int page
   return min(c + (c * page_size != n), width);
 }
 
-// A wave a row of a block table, several side by side for long ones.
-constexpr int kRowPiece = 1024;  // entries
+// A wave a row of a block table, several side by side for long ones, which count columns past 2^31: f(column)
+// for those below `end`.
+constexpr uint32_t kRowPiece = 1024;  // entries
+
+template <typename F>
+__device__ __forceinline__ void each_column(int end, F f) {
+  const uint32_t lane = threadIdx.x & 63;
+  for (uint32_t c0 = blockIdx.y * kRowPiece; c0 < (uint32_t)end; c0 += gridDim.y * kRowPiece)
+    for (uint32_t c = c0 + lane; c < min(c0 + kRowPiece, (uint32_t)end); c += 64) f(c);
+}
 
 __global__ __launch_bounds__(kThreads) void mark_free_kernel(PagedFreeArgs a, DivMagic by_page,
                                                               unsigned char* keeps,
                                                               unsigned char* drops) {
-  const int r = blockIdx.x * kWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r = blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (r >= a.requests) return;
   const int length = a.lengths[r], kept = min(a.kept[r], length);
-  const int used = columns_of(length, by_page, a.page_size, a.width);
-  const int keep = columns_of(kept, by_page, a.page_size, a.width);
+  const uint32_t keep = columns_of(kept, by_page, a.page_size, a.width);
   const int32_t* row = a.tables + (int64_t)r * a.table_stride;
-  for (int c0 = (int)blockIdx.y * kRowPiece; c0 < used; c0 += (int)gridDim.y * kRowPiece)
-    for (int c = c0 + lane; c < min(c0 + kRowPiece, used); c += 64) {
-      const int32_t p = row[c];
-      if ((uint32_t)p < (uint32_t)a.pages) (c < keep ? keeps : drops)[p] = 1;
-    }
+  each_column(columns_of(length, by_page, a.page_size, a.width), [&](uint32_t c) {
+    const int32_t p = row[c];
+    if ((uint32_t)p < (uint32_t)a.pages) (c < keep ? keeps : drops)[p] = 1;
+  });
 }
 
 // A thread's marks, bytes of 0 or 1.
@@ -274,7 +280,6 @@ __global__ __launch_bounds__(kThreads) void begin_compact_kernel(PagedCompactArg
 __global__ __launch_bounds__(kThreads) void mark_compact_kernel(PagedCompactArgs a, DivMagic by_page,
                                                                  int row_blocks, unsigned char* used,
                                                                  unsigned char* open) {
-  const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x >= row_blocks) {  // the free list
     const int64_t step = (int64_t)(gridDim.x - row_blocks) * gridDim.y * kThreads;
     const int64_t start = max(*a.free_start, 0);
@@ -288,13 +293,11 @@ __global__ __launch_bounds__(kThreads) void mark_compact_kernel(PagedCompactArgs
   }
   const int r = blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (r >= a.requests) return;
-  const int columns = columns_of(a.lengths[r], by_page, a.page_size, a.width);
   const int32_t* row = a.tables + (int64_t)r * a.table_stride;
-  for (int c0 = (int)blockIdx.y * kRowPiece; c0 < columns; c0 += (int)gridDim.y * kRowPiece)
-    for (int c = c0 + lane; c < min(c0 + kRowPiece, columns); c += 64) {
-      const int32_t p = row[c];
-      if ((uint32_t)p < (uint32_t)a.pages) used[p] = 1;
-    }
+  each_column(columns_of(a.lengths[r], by_page, a.page_size, a.width), [&](uint32_t c) {
+    const int32_t p = row[c];
+    if ((uint32_t)p < (uint32_t)a.pages) used[p] = 1;
+  });
 }
 
 __global__ __launch_bounds__(kThreads) void count_compact_kernel(const unsigned char* used,
@@ -347,20 +350,19 @@ __global__ __launch_bounds__(kThreads) void list_compact_kernel(PagedCompactArgs
 
 __global__ __launch_bounds__(kThreads) void apply_compact_kernel(PagedCompactArgs a, DivMagic by_page,
                                                                   const int32_t* number) {
-  const int r = blockIdx.x * kWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r = blockIdx.x * kWaves + (threadIdx.x >> 6);
   if (r >= a.requests) return;
-  const int columns = columns_of(a.lengths[r], by_page, a.page_size, a.width);
+  const uint32_t columns = columns_of(a.lengths[r], by_page, a.page_size, a.width);
   const int32_t* row = a.tables + (int64_t)r * a.table_stride;
   int32_t* to = a.new_tables + (int64_t)r * a.width;
-  for (int c0 = (int)blockIdx.y * kRowPiece; c0 < a.width; c0 += (int)gridDim.y * kRowPiece)
-    for (int c = c0 + lane; c < min(c0 + kRowPiece, a.width); c += 64) {
-      int32_t p = row[c];
-      if (c < columns && (uint32_t)p < (uint32_t)a.pages) {
-        const int move = number[p];
-        if (move >= 0) p = a.targets[move];
-      }
-      to[c] = p;
+  each_column(a.width, [&](uint32_t c) {
+    int32_t p = row[c];
+    if (c < columns && (uint32_t)p < (uint32_t)a.pages) {
+      const int move = number[p];
+      if (move >= 0) p = a.targets[move];
     }
+    to[c] = p;
+  });
 }
 
 // ---- small pools: one launch -----------------------------------------------------------------------
@@ -540,7 +542,7 @@ int row_bits(int requests) {
 
 dim3 row_grid(int requests, int width) {
   const int rows = (requests + kWaves - 1) / kWaves;
-  const int pieces = (int)(((int64_t)width + kRowPiece - 1) / kRowPiece);
+  const int pieces = (int)(((int64_t)width + kRowPiece - 1) / (int64_t)kRowPiece);
   return dim3(rows, std::max(1, std::min({pieces, 64, (1 << 20) / std::max(rows, 1)})));
 }
 unsigned fill_grid(int64_t vectors) {

@@ -1,0 +1,57 @@
+"""The serving operators where counts of tokens, pages, columns and forks come near 2^31, or near the most that
+is accepted."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import metile_amd as mt
+from tests.test_gpu_paged import i32
+
+pytestmark = pytest.mark.gpu
+MOST = (1 << 31) - 1
+
+
+def long_row(rows=1):
+    """Rows of 2^31 - 1 pages of a token each: the first 30000 again and again, and two others near the end."""
+    tables = torch.empty(rows, MOST, dtype=torch.int32, device="cuda")
+    torch.arange(MOST, dtype=torch.int32, device="cuda", out=tables[0])
+    tables[0].remainder_(30000)
+    tables[0, -70000], tables[0, -1] = 39998, 39999
+    return tables
+
+
+def test_free_of_the_longest_rows():
+    tables = long_row()
+    free = torch.full((40000,), -1, dtype=torch.int32, device="cuda")
+    free[30002:] = torch.arange(30000, 39998, device="cuda")
+    before = free.clone()
+    for kept, gone in ((MOST - 70001, [39998, 39999]), (MOST - 1, [39999]), (MOST, [])):
+        list_ = before.clone()
+        freed = mt.paged_free(tables, i32([MOST]), i32([kept]), list_, page_size=1, pages=40000,
+                              free_start=i32([30002]))
+        assert freed.tolist() == [len(gone)]
+        assert list_[30002 - len(gone):30002].tolist() == gone
+        assert torch.equal(list_[30002:], before[30002:]) and bool((list_[:30002 - len(gone)] == -1).all())
+
+
+def test_compaction_of_the_longest_rows():
+    tables = long_row()
+    free = torch.full((40000,), -1, dtype=torch.int32, device="cuda")
+    free[30002:] = torch.arange(30000, 39998, device="cuda")
+    plan = mt.paged_compact(tables, i32([MOST]), free, page_size=1, pages=40000, free_start=i32([30002]))
+    assert plan.moves.tolist() == [2]
+    assert plan.sources[:3].tolist() == [39999, 39998, -1] and plan.targets[:3].tolist() == [30000, 30001, -1]
+    assert plan.free_pages[30002:].tolist() == list(range(30002, 40000))
+    tables[0, -70000], tables[0, -1] = 30001, 30000
+    assert torch.equal(plan.block_tables, tables)
+
+
+def test_fork_of_the_longest_rows():
+    tables = long_row(2)
+    tables[1].fill_(-1)
+    lengths = i32([MOST, 0])
+    fork = mt.paged_fork(tables, lengths, i32([0]), i32([1]), i32([]), page_size=1)
+    assert [t.tolist() for t in fork] == [[-1], [-1], [0]] and lengths.tolist() == [MOST, MOST]
+    assert torch.equal(tables[0], tables[1])
