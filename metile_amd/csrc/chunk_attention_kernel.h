@@ -311,10 +311,10 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   int behind;
   const Item item = find<false>(a, (int)(blockIdx.x / (unsigned)a.kv_heads), &behind);
 
-  // ---- rows that belong to no request ----
+  // ---- rows that belong to no request (counted in 32 unsigned bits: with gridDim.x they may pass 2^31) ----
   {
     const int row_words = a.kv_heads * a.group * (dim / 8);
-    for (int row = behind + (int)blockIdx.x; row < a.tokens; row += (int)gridDim.x) {
+    for (uint32_t row = (uint32_t)behind + blockIdx.x; row < (uint32_t)a.tokens; row += gridDim.x) {
       u32x4* to = reinterpret_cast<u32x4*>(a.out) + (int64_t)row * row_words;
       for (int i = tid; i < row_words; i += kThreads) to[i] = (u32x4){0, 0, 0, 0};
       if (a.lse)

@@ -55,3 +55,18 @@ def test_fork_of_the_longest_rows():
     fork = mt.paged_fork(tables, lengths, i32([0]), i32([1]), i32([]), page_size=1)
     assert [t.tolist() for t in fork] == [[-1], [-1], [0]] and lengths.tolist() == [MOST, MOST]
     assert torch.equal(tables[0], tables[1])
+
+
+def test_nearly_2_31_rows_of_padding():
+    """A call of one request and the most rows that are accepted for it: all but its own are zeros."""
+    tokens, dim = 128 * ((1 << 24) - (1 << 16)) - 129, 16
+    cache = mt.PagedCache.allocate(1, 16, 1, dim)
+    cache.key.normal_(), cache.value.normal_()
+    query = torch.randn(1, 1, dim, device="cuda").bfloat16().expand(tokens, 1, dim)
+    tables, lengths = i32([[0]]), i32([16])
+    few = mt.paged_chunk_attention(query[:5], cache, tables, lengths, i32([0, 5]))
+    out, lse = mt.paged_chunk_attention(query, cache, tables, lengths, i32([0, 5]), return_lse=True)
+    assert torch.equal(out[:5], few)
+    assert bool((lse[5:] == -float("inf")).all())
+    rest = out[5:].flatten().view(torch.int16)
+    assert not any(bool(part.any()) for part in rest.split(1 << 30))
