@@ -326,12 +326,15 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
   }
   if (in_vocab && token >= begin && token < end && tid == 0)  // those of the token's own eight
     for (int i = token & ~7; i < token; ++i) larger += load1<DT>(x_row, i) == given;
-  if (in_vocab && given == -__builtin_inff()) {
-    // (nothing is below -inf: the larger ones have been counted, those before the token are as large)
+  // The rank's count by the definition, of the wave.
+  auto count_larger = [&]() {
     larger = 0;
-    for (int i = begin + tid; i < end; i += kThreads)
-      larger += __popcll(__ballot(load1<DT>(x_row, i) > given || i < token));
-  }
+    for (int i = begin + tid; i < end; i += kThreads) {
+      const float x = load1<DT>(x_row, i);
+      larger += __popcll(__ballot(x > given || (x == given && i < token)));
+    }
+  };
+  if (in_vocab && given == -__builtin_inff()) count_larger();  // (nothing is below -inf)
   if (lane == 0) wave_count[0][wave] = larger;
   if (tid < kMostTop) best[tid] = 0;
   if (tid == 0) counts[0] = counts[1] = 0, flagged = 0;
@@ -341,7 +344,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
   uint32_t own_key = key_of(own_top);
   if (!(sums.s > 0.0 && sums.s < (double)__builtin_inff())) {
     // NaN or infinities, logits too large for c times them, or none that is allowed: again, with
-    // references in 64 bits and maxima by whole numbers
+    // references in 64 bits and maxima by whole numbers, and the rank's count without maxima
     Sums own = {kNone, 0.0, 0.0};
     own_key = 0;
 #pragma unroll 1
@@ -362,6 +365,10 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
       }
       if (a.top) group_keys[b * kThreads + tid] = key;
       own_key = max(own_key, key);
+    }
+    if (in_vocab) {  // (maxima that a signalling NaN had part in may have hidden larger values)
+      count_larger();
+      if (lane == 0) wave_count[0][wave] = larger;
     }
     __syncthreads();
     sums = of_waves(of_lanes(own, 32));
