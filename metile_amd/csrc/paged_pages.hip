@@ -86,21 +86,70 @@ __device__ __forceinline__ Fork fork_of(const PagedForkArgs& a, int i) {
 
 __global__ void zero_int_kernel(int32_t* to) { *to = 0; }
 
-// A workgroup a fork. Each counts the forks before its own that take a page. Round trips bound it: a fork 2.2
-// us, 256 5.1.
+// Calls of so many forks or more count those before each in a launch of one workgroup before: in the forks'
+// own workgroups, which is one launch less, the work grows with their number's square. (us without and with
+// that launch: 256 forks 3.4 and 5.7, 2048 6.2 and 7.2, 4096 12.8 and 10.3, 16384 108 and 28.5; 65536 101,
+// 8388607 15361.)
+constexpr int kForksCounted = 2560;
+constexpr int kCountThreads = 1024, kCountRun = 4;  // forks of a thread, next to each other
+
+__device__ __forceinline__ int begun_of(const PagedForkArgs& a, const Fork& f, DivMagic by_page) {
+  return f.tokens - (int)div_by(f.tokens, by_page) * a.page_size;
+}
+
+// The forks before each that take a page, where the fork's own page will be written.
+__global__ __launch_bounds__(kCountThreads) void count_forks_kernel(PagedForkArgs a, DivMagic by_page) {
+  __shared__ int lds[2][kCountThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int carry = 0, turn = 0;
+  for (int base = 0; base < a.forks; base += kCountThreads * kCountRun, turn ^= 1) {
+    const int first = base + tid * kCountRun;
+    int takes[kCountRun], mine = 0;
+#pragma unroll
+    for (int k = 0; k < kCountRun; ++k) {
+      const Fork f = fork_of(a, min(first + k, a.forks - 1));
+      takes[k] = begun_of(a, f, by_page) > 0 && first + k < a.forks;
+      mine += takes[k];
+    }
+    int sum = mine;
+    for (int d = 1; d < 64; d *= 2) {
+      const int x = __shfl_up(sum, d);
+      if (lane >= d) sum += x;
+    }
+    if (lane == 63) lds[turn][wave] = sum;
+    __syncthreads();
+    int before = carry + sum - mine;
+#pragma unroll
+    for (int w = 0; w < kCountThreads / 64; ++w) {
+      if (w < wave) before += lds[turn][w];
+      carry += lds[turn][w];
+    }
+#pragma unroll
+    for (int k = 0; k < kCountRun; ++k) {
+      if (first + k < a.forks) a.to[first + k] = before;
+      before += takes[k];
+    }
+  }
+}
+
+// A workgroup a fork. Each counts the forks before its own that take a page, unless they have been counted.
+// Round trips bound it: a fork 2.2 us, 256 5.1.
+template <bool kCounted>
 __global__ __launch_bounds__(kThreads) void fork_kernel(PagedForkArgs a, DivMagic by_page) {
   __shared__ int lds[kWaves];
   const int i = blockIdx.x, tid = threadIdx.x;
   const bool last = i == a.forks - 1;
-  auto begun = [&](const Fork& f) {
-    return f.tokens - (int)div_by(f.tokens, by_page) * a.page_size;
-  };
   int before = 0;
-  for (int j = tid; j < i; j += kThreads) before += begun(fork_of(a, j)) > 0;
-  before = block_sum(before, lds);
+  if constexpr (kCounted) {
+    before = a.to[i];
+    __syncthreads();
+  } else {
+    for (int j = tid; j < i; j += kThreads) before += begun_of(a, fork_of(a, j), by_page) > 0;
+    before = block_sum(before, lds);
+  }
   const Fork f = fork_of(a, i);
   const int full = (int)div_by(f.tokens, by_page);
-  const bool partial = begun(f) > 0;
+  const bool partial = begun_of(a, f, by_page) > 0;
   if (last && tid == 0) *a.taken = before + partial;
   int32_t fresh = -1, old = -1;
   if (partial) {
@@ -577,7 +626,13 @@ hipError_t launch_zero_int(int32_t* to, hipStream_t stream) {
 }
 
 hipError_t launch_paged_fork(const PagedForkArgs& a, hipStream_t stream) {
-  fork_kernel<<<a.forks, kThreads, 0, stream>>>(a, div_magic((uint32_t)a.page_size));
+  const DivMagic by_page = div_magic((uint32_t)a.page_size);
+  if (a.forks >= kForksCounted) {
+    count_forks_kernel<<<1, kCountThreads, 0, stream>>>(a, by_page);
+    fork_kernel<true><<<a.forks, kThreads, 0, stream>>>(a, by_page);
+  } else {
+    fork_kernel<false><<<a.forks, kThreads, 0, stream>>>(a, by_page);
+  }
   return hipGetLastError();
 }
 

@@ -70,3 +70,42 @@ def test_nearly_2_31_rows_of_padding():
     assert bool((lse[5:] == -float("inf")).all())
     rest = out[5:].flatten().view(torch.int16)
     assert not any(bool(part.any()) for part in rest.split(1 << 30))
+
+
+@pytest.mark.parametrize("forks", [1023, 2559, 2560, 4095, 4096, 4097, 50001, (1 << 23) - 1])
+def test_many_forks(forks):
+    """Sources with and without a begun page, some forks left out, the list too short for the last."""
+    g = torch.Generator("cuda").manual_seed(forks)
+    live, page = 1000, 4
+    requests = live + forks
+    lengths = torch.zeros(requests, dtype=torch.int32, device="cuda")
+    lengths[:live] = torch.randint(0, 9, (live,), generator=g, device="cuda")
+    tables = torch.full((requests, 3), -1, dtype=torch.int32, device="cuda")
+    tables[:live] = torch.randint(0, 5000, (live, 3), generator=g, device="cuda", dtype=torch.int32)
+    sources = torch.randint(-20, live, (forks,), generator=g, device="cuda", dtype=torch.int32)
+    targets = live + torch.randperm(forks, generator=g, device="cuda").int()
+    targets[5::97] = requests
+    kept = torch.randint(0, 12, (forks,), generator=g, device="cuda", dtype=torch.int32)
+    ok = (sources >= 0) & (targets < requests)
+    source = sources.clamp(min=0).long()
+    n = torch.where(ok, torch.minimum(lengths[source], kept), 0)
+    begun = n % page > 0
+    before = begun.long().cumsum(0) - begun.long()
+    free = torch.randperm(int(begun.sum()), generator=g, device="cuda").int()  # from entry 2 on: two short
+    at = before + 2
+    there = begun & (at < free.numel())
+    fresh = torch.where(there, free[at.clamp(max=free.numel() - 1)], -1)
+    full = (n // page).long()
+    old = tables[source].gather(1, full.clamp(max=2)[:, None])[:, 0]
+    want_tables, want_lengths = tables.clone(), lengths.clone()
+    column = torch.arange(3, device="cuda")
+    rows = torch.where(column < full[:, None], tables[source], -1)
+    rows = torch.where((column == full[:, None]) & begun[:, None], fresh[:, None], rows)
+    want_tables[targets[ok].long()] = rows[ok]
+    want_lengths[targets[ok].long()] = n[ok]
+    fork = mt.paged_fork(tables, lengths, sources, targets, free, page_size=page, free_start=i32([2]),
+                         tokens=kept)
+    assert torch.equal(fork.sources, torch.where(there, old, -1))
+    assert torch.equal(fork.targets, fresh.int())
+    assert int(fork.taken) == int(begun.sum())
+    assert torch.equal(tables, want_tables) and torch.equal(lengths, want_lengths)
