@@ -94,10 +94,17 @@ class Batch:
         self.tables = torch.full((requests, width), -1, dtype=torch.int32, device=device)
         self.free = torch.arange(pages, dtype=torch.int32, device=device)
         self.taken = torch.zeros(1, dtype=torch.int32, device=device)
+        self.missing = torch.zeros(1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(requests, dtype=torch.int32, device=device)
         self.tokens = torch.zeros(requests, dtype=torch.int64, device=device)
         self.active = torch.ones(requests, dtype=torch.int32, device=device)
         self.scores = torch.zeros(requests, dtype=torch.float32, device=device)
+
+    def take(self, pages):
+        """Counts pages that were taken: the list's end where it held fewer, and how many were missing."""
+        most = self.free.shape[0]
+        self.missing.add_((self.taken + pages - most).clamp(min=0))
+        self.taken.add_(pages).clamp_(max=most)
 
     def step(self):
         """Logits of every request's next token; ``self.tokens`` of the active ones enter the cache."""
@@ -116,7 +123,7 @@ class Batch:
         logits = torch.zeros(requests + 1, c.vocab, dtype=packed.dtype, device=packed.device)
         logits[torch.where(plan.requests >= 0, plan.requests.long(), requests)] = packed
         self.lengths.copy_(plan.lengths)
-        self.taken.add_(plan.taken)
+        self.take(plan.taken)
         return logits[:requests]
 
     def layers(self, tokens, plan, attend):
@@ -154,7 +161,7 @@ class Batch:
         h = self.layers(tokens, plan, lambda q, cache: mt.paged_chunk_attention(
             q, cache, self.tables, plan.lengths, plan.starts))
         self.lengths.copy_(plan.lengths)
-        self.taken.add_(plan.taken)
+        self.take(plan.taken)
         last = plan.starts[1:].long() - 1
         logits = mt.affine_qmv(h[last.clamp(min=0)], *d.head)
         if not score:
@@ -171,7 +178,7 @@ class Batch:
         plan = mt.paged_fork(self.tables, self.lengths, sources, targets, self.free,
                              page_size=self.page_size, free_start=self.taken)
         mt.paged_copy(self.caches, plan.sources, plan.targets)
-        self.taken.add_(plan.taken)
+        self.take(plan.taken)
         self.tokens[targets.long()] = self.tokens[sources.long()]
         self.scores[targets.long()] = self.scores[sources.long()]
 
@@ -262,7 +269,8 @@ def main():
         seconds = time.perf_counter() - began
     print(f"{a.requests} requests, {a.layers} layers, {a.steps} steps: "
           f"{1e3 * seconds / a.steps:.3f} ms a step, {a.requests * a.steps / seconds:.0f} tokens/s, "
-          f"lengths {batch.lengths.unique().tolist()}, pages taken {int(batch.taken)} of {pages}")
+          f"lengths {batch.lengths.unique().tolist()}, pages taken {int(batch.taken)} of {pages}"
+          + (f", {int(batch.missing)} missing" if int(batch.missing) else ""))
     if a.answers > 1:
         best = batch.scores.view(-1, a.answers).argmax(1, keepdim=True)
         kept = torch.arange(a.answers, device="cuda") == best

@@ -385,7 +385,8 @@ typedef struct mt_paged_cache {
  * taken [1], the pages that the step needed as far as the tables reach. Tokens behind the last
  * request's (padding) get slot -1, position 0, request -1; tokens that the table's width or the free
  * list has no page for get slot -1. An exhausted list writes -1 into the table, and `taken` tells the
- * shortage; a table that is too narrow shows in lengths beyond width * page_size alone. Tokens beyond
+ * shortage: *free_start + taken is beyond free_count then, and the caller goes on with a start of
+ * free_count. A table that is too narrow shows in lengths beyond width * page_size alone. Tokens beyond
  * `tokens` are dropped with the table entries of the pages they open. width * page_size is below
  * 2^31; sums of counts stop at 2^31 - 1. requests or tokens may be 0. Outputs
  * overlap no input. */
@@ -504,9 +505,10 @@ int mt_paged_copy(const mt_paged_cache* const* caches, int num_caches, const mt_
  * has been begun is the target's own, taken from free_pages ([free_count]) beginning with entry
  * *free_start (NULL: 0), fork by fork; what it holds is to be copied from page copy_sources[i] to
  * copy_targets[i] (mt_paged_copy; -1 where nothing is). lengths[targets[i]] is set; taken [1] receives the
- * pages that were needed. An exhausted list writes -1 as the begun page. Forks with a request that is none
- * of the batch's are left out. Targets are distinct and none of the sources. width * page_size is below
- * 2^31, requests below 2^24 (also below) and forks below 2^23. */
+ * pages that were needed. An exhausted list writes -1 as the begun page; the start is then free_count, as
+ * for mt_paged_tables. Forks with a request that is none of the batch's are left out. Targets are distinct
+ * and none of the sources. width * page_size is below 2^31, requests below 2^24 (also below) and forks
+ * below 2^23. */
 typedef struct mt_paged_fork_args {
   int32_t* block_tables;
   int64_t table_stride;
@@ -525,10 +527,10 @@ int mt_paged_fork(const mt_paged_fork_args* args, void* stream);
 
 /* Frees the pages of tokens behind the first kept[r] of each request's lengths[r] (0: all of them): those
  * that no request has among its kept tokens' pages. Their numbers, ascending, are written to free_pages
- * ([free_count]) in front of entry *free_start (entries before the first are dropped); freed [1] receives
- * how many there are. Tables and lengths are not changed: the caller sets lengths to kept and takes
- * `freed` from the start. Entries that are no pages (of `pages`) are left out. The workspace need not be
- * cleared. width * page_size is below 2^31. */
+ * ([free_count]) in front of entry *free_start, which is at most free_count (numbers whose entry would be
+ * outside the list are dropped); freed [1] receives how many there are. Tables and lengths are not
+ * changed: the caller sets lengths to kept and takes `freed` from the start. Entries that are no pages (of
+ * `pages`) are left out. The workspace need not be cleared. width * page_size is below 2^31. */
 typedef struct mt_paged_free_args {
   const int32_t* block_tables;
   int64_t table_stride;

@@ -171,7 +171,9 @@ def paged_tables(cached, new, block_tables, free_pages, *, page_size, tokens, fr
     ``taken`` (the pages that the step needs and the tables have room for) is more than the list holds
     from ``free_start`` on; where a table is too narrow, ``lengths`` is more than ``width *
     page_size``, and ``taken`` does not count the pages beyond: a caller sees either shortage when it
-    next looks. Returns a :class:`PagedStep`; nothing is synchronised.
+    next looks. A caller goes on with ``free_start.add_(step.taken).clamp_(max=free_pages.shape[0])``:
+    after a shortage the whole list has been taken, and no more. Returns a :class:`PagedStep`; nothing is
+    synchronised.
     """
     device = block_tables.device
     _same_device(device, cached, new, free_pages, free_start)
@@ -445,10 +447,11 @@ def paged_fork(block_tables, lengths, sources, targets, free_pages, *, page_size
     has been begun is the target's own, taken from ``free_pages`` as :func:`paged_tables` does;
     ``paged_copy(caches, fork.sources, fork.targets)`` copies what it holds. The targets' rows of
     ``block_tables`` and their ``lengths`` are set in place; entries behind the last page stay as they
-    were. Where the list is exhausted the begun page is -1, and ``taken`` is more than the list holds.
-    Forks of or onto rows that there are not (-1) are left out. A request may be forked any number of
-    times at once; targets must be distinct, and none of them a source. Pages of a target's former
-    tokens are not freed: :func:`paged_free` does that. Returns a :class:`PagedFork`.
+    were. Where the list is exhausted the begun page is -1, and ``taken`` is more than the list holds; a
+    caller goes on with ``free_start.add_(fork.taken).clamp_(max=free_pages.shape[0])``. Forks of or onto
+    rows that there are not (-1) are left out. A request may be forked any number of times at once;
+    targets must be distinct, and none of them a source. Pages of a target's former tokens are not freed:
+    :func:`paged_free` does that. Returns a :class:`PagedFork`.
     """
     device = block_tables.device
     _same_device(device, lengths, sources, targets, free_pages, free_start, tokens)
@@ -485,11 +488,12 @@ def paged_free(block_tables, lengths, kept, free_pages, *, page_size, pages, fre
 
     A page that any request still has among its kept tokens' pages stays. The numbers of the others, in
     ascending order, are written to ``free_pages`` in place, in front of entry ``free_start`` (a device
-    int32 tensor of one element: how many entries have been taken). Returns how many there are (int32
-    ``[1]``); tables and lengths are not changed. A caller goes on with ``lengths.copy_(kept)`` and
-    ``free_start.sub_(freed)``. ``pages``: of the cache. A request that is cut inside a page which others
-    share must not write on in place: :func:`paged_fork` with ``tokens`` lets a row go on from there with
-    a page of its own.
+    int32 tensor of one element: how many entries have been taken, so at most as many as there are; numbers
+    that would come to lie outside the list are dropped). Returns how many there are (int32 ``[1]``);
+    tables and lengths are not changed. A caller goes on with ``lengths.copy_(kept)`` (the smaller of both,
+    where ``kept`` may be more than the length) and ``free_start.sub_(freed)``. ``pages``: of the cache. A
+    request that is cut inside a page which others share must not write on in place: :func:`paged_fork`
+    with ``tokens`` lets a row go on from there with a page of its own.
     """
     device = block_tables.device
     _same_device(device, lengths, kept, free_pages, free_start)
