@@ -455,15 +455,16 @@ int mt_paged_attention(const mt_paged_cache* cache, const mt_paged_attention_arg
                        void* workspace, size_t workspace_bytes, void* stream);
 
 /* Attention of a chunk of new tokens of each request over its pages: a prompt, a part of one, a draft.
- * Request r's new tokens are rows starts[r] .. starts[r + 1] - 1 of the packed batch (starts[0] is 0, as
+ * Request r's new tokens are rows starts[r] .. starts[r + 1] - 1 of the packed batch (ascending, as
  * mt_paged_tables writes them) and the last of its lengths[r] tokens in the cache, whose keys and values
  * are appended first. Each attends to the tokens up to itself, of them the last `window` (0: all):
  * out[t, h] = sum_j p_j v_j with p = softmax(scale * q[t, h] . k_j), of the key-value head h / (heads /
  * cache heads). Keys are limited to width * page_size, which is at most 2^31 - 64; tokens whose entry is
  * not a page of the cache are left out, and neither what slots behind the last token hold nor what
  * later tokens do matters to a token, NaN and infinities too. Tokens without a key, and rows of the batch
- * that belong to no request, get 0. lse (or NULL) [tokens, heads] receives log sum exp of the scaled
- * scores, -inf for such rows. Lengths, starts, tables and the cache must not change while the call runs.
+ * that belong to no request (in front of starts[0] and behind the last), get 0. lse (or NULL) [tokens,
+ * heads] receives log sum exp of the scaled scores, -inf for such rows. Lengths, starts, tables and the
+ * cache must not change while the call runs.
  * query [tokens, heads, dim] with element strides per token and head (multiples of 16 bytes), out
  * [tokens, heads, dim] contiguous, 16-byte aligned, both in dtype; a 16-bit cache has the same. tokens *
  * heads is below 2^31, and tokens * heads / 128 + requests * cache heads below 2^24 - 2^16. Scores, maxima

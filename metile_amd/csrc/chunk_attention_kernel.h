@@ -311,10 +311,14 @@ __global__ __launch_bounds__(kThreads, DIM <= 128 ? 2 : 1) void attention_kernel
   int behind;
   const Item item = find<false>(a, (int)(blockIdx.x / (unsigned)a.kv_heads), &behind);
 
-  // ---- rows that belong to no request (counted in 32 unsigned bits: with gridDim.x they may pass 2^31) ----
+  // ---- rows that belong to no request, in front of the first one's and behind the last one's (counted in 32
+  // unsigned bits: with gridDim.x they may pass 2^31) ----
   {
     const int row_words = a.kv_heads * a.group * (dim / 8);
-    for (uint32_t row = (uint32_t)behind + blockIdx.x; row < (uint32_t)a.tokens; row += gridDim.x) {
+    const uint32_t front = (uint32_t)min(max(a.starts[0], 0), a.tokens);
+    const uint32_t none = front + (uint32_t)(a.tokens - behind);
+    for (uint32_t n = blockIdx.x; n < none; n += gridDim.x) {
+      const uint32_t row = n < front ? n : n - front + (uint32_t)behind;
       u32x4* to = reinterpret_cast<u32x4*>(a.out) + (int64_t)row * row_words;
       for (int i = tid; i < row_words; i += kThreads) to[i] = (u32x4){0, 0, 0, 0};
       if (a.lse)

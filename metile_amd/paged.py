@@ -314,12 +314,13 @@ def paged_chunk_attention(query, cache, block_tables, lengths, starts, *, scale=
 
     ``query`` ``[tokens, heads, head_dim]`` (bfloat16 or float16; ``heads`` a multiple of the cache's) is
     a packed batch: request ``r``'s new tokens are rows ``starts[r]`` to ``starts[r + 1] - 1`` (int32
-    ``[requests + 1]``, beginning with 0) and the last of its ``lengths[r]`` tokens in the cache (int32
+    ``[requests + 1]``, ascending) and the last of its ``lengths[r]`` tokens in the cache (int32
     ``[requests]``), as :func:`paged_tables` gives both. Each attends to its request's tokens up to
     itself, with ``window`` to the last so many of them only; what later tokens hold does not matter to
     it. ``block_tables`` and ``scale`` are as in :func:`paged_attention`. Returns the output in
     ``query``'s shape and dtype and, with ``return_lse``, the log of the sum of exponentials (float32
-    ``[tokens, heads]``). Rows that belong to no request give zeros and -inf.
+    ``[tokens, heads]``). Rows that belong to no request, in front of the first one's and behind the last
+    one's, give zeros and -inf.
     """
     dtype = query.dtype
     if dtype not in _DTYPES:
