@@ -45,7 +45,8 @@ struct ChunkAttentionArgs {
 };
 
 // In front of the plan: blocks of a split, then items and tiles with parts of one key-value head. Behind it
-// the sums of items, parts and tiles with parts of the requests before each.
+// the sums of items, parts and tiles with parts of the requests before each. Calls of up to kChunkHere requests
+// have the first alone, from the attention for the join.
 constexpr int kPlanHead = 4;
 // Floats of a part: 16 a lane and 32 dimensions, then reference and sum of each row.
 size_t chunk_part_floats(int dim);

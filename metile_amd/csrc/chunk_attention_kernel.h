@@ -148,16 +148,23 @@ __device__ __forceinline__ Item find_here(const ChunkAttentionArgs& a, int n, in
   const Request q = request_of(a, r);
   *behind = readlane(min(max(a.starts[r + 1], 0), a.tokens), a.requests - 1);
   const int tiles = lane < a.requests ? tiles_of(a, q) : 0, most = most_blocks(a, q);
-  // (rounded up, so that there are no more than `target` parts on top of the tiles)
-  const float total =
-      __builtin_bit_cast(float, readlane(__builtin_bit_cast(int, wave_scan((float)tiles * (float)most)),
-                                         63));
-  const float even = total * 1.0001f / (float)a.target;  // blocks of an item, if all were the same
-  int per = max((int)fminf(even + 1.0f, 1073741824.0f), least_blocks(total));
-  // (us of 1024 tokens behind 16384 without and with the choice: 14 heads of 64 on 2 129 and 108, 24 of 96 on 3
-  // 261 and 221, 20 of 192 on 5 588 and 460)
-  if (a.requests == 1 && even > 16.0f)
-    per = best_parts(a, lane, even, per, readlane(tiles, 0), readlane(most, 0));
+  int per;
+  if constexpr (JOIN) {
+    // (as the attention kernel found it: the parts lie where it put them, however its sums were rounded)
+    per = a.plan[0];
+  } else {
+    // (rounded up, so that there are no more than `target` parts on top of the tiles)
+    const float total =
+        __builtin_bit_cast(float, readlane(__builtin_bit_cast(int, wave_scan((float)tiles * (float)most)),
+                                           63));
+    const float even = total * 1.0001f / (float)a.target;  // blocks of an item, if all were the same
+    per = max((int)fminf(even + 1.0f, 1073741824.0f), least_blocks(total));
+    // (us of 1024 tokens behind 16384 without and with the choice: 14 heads of 64 on 2 129 and 108, 24 of 96 on
+    // 3 261 and 221, 20 of 192 on 5 588 and 460)
+    if (a.requests == 1 && even > 16.0f)
+      per = best_parts(a, lane, even, per, readlane(tiles, 0), readlane(most, 0));
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = per;
+  }
   const int splits = splits_of(most, per);
   const int items = tiles * splits, parts = splits > 1 ? items : 0;
   const int count = !JOIN ? items : splits > 1 ? tiles : 0;

@@ -109,3 +109,26 @@ def test_many_forks(forks):
     assert torch.equal(fork.targets, fresh.int())
     assert int(fork.taken) == int(begun.sum())
     assert torch.equal(tables, want_tables) and torch.equal(lengths, want_lengths)
+
+
+def test_parts_of_more_blocks_than_fp32_counts():
+    """Requests of up to 110 million keys, all of them one page's, whose blocks sum up past 2^24, in parts of
+    which a lost or misplaced one would show: the page's result. A part's sums have some 2^16 equal terms
+    (blocks), each rounded by at most 2^-24 of the sum."""
+    page, dim, heads = 64, 16, 130
+    cache = mt.PagedCache.allocate(1, page, 1, dim)
+    g = torch.Generator("cuda").manual_seed(3)
+    cache.key.normal_(generator=g), cache.value.normal_(generator=g)
+    widths, new = [1699999, 300001, 77777, 1234567], [9, 1, 1, 5]
+    starts = i32([0, 9, 10, 11, 16])
+    tables = torch.zeros(4, max(widths), dtype=torch.int32, device="cuda")
+    q = torch.randn(1, heads, dim, generator=g, device="cuda").bfloat16().repeat(16, 1, 1)
+    # (each request's new tokens are its page's last: a token sees `widths` whole pages and some)
+    out, lse = mt.paged_chunk_attention(q, cache, tables, i32([w * page for w in widths]), starts,
+                                        return_lse=True)
+    want, want_lse = mt.paged_chunk_attention(q[:1], cache, tables[:1], i32([page]), i32([0, 1]),
+                                              return_lse=True)
+    blocks = torch.tensor([float(w) for w, n in zip(widths, new) for _ in range(n)]).log().cuda()
+    assert float((lse - want_lse - blocks[:, None]).abs().max()) <= 2.0 ** -8 + 2.0 ** -16
+    assert float((out.float() - want.float()).abs().max()) <= (2.0 ** -7 + 2.0 ** -7) * float(
+        cache.value.abs().max())
