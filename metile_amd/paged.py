@@ -117,7 +117,9 @@ class PagedCache:
             _CACHE_DTYPES[key.dtype], self.key_scale, self.value_scale)
         self._ref, self._address = ctypes.byref(self._desc), ctypes.addressof(self._desc)
         self._device, self._dtype, self._head_shape = key.device, key.dtype, key.shape[2:]
-        self._workspaces = {}  # ([tokens,] requests, heads, width, window) -> bytes
+        # (requests, heads, width, window) -> bytes; of chunks (tokens, requests, ...), which come in as many
+        # sizes as steps have, apart from those
+        self._workspaces, self._chunk_workspaces = {}, {}
 
     @classmethod
     def allocate(cls, pages, page_size, kv_heads, head_dim, *, dtype=torch.bfloat16, device="cuda",
@@ -133,10 +135,21 @@ class PagedCache:
         need = self._workspaces.get(shape)
         if need is None:
             need = _lib.lib().mt_paged_attention_workspace_bytes(self._ref, *shape)
-            if len(self._workspaces) >= 256:
-                self._workspaces.clear()
-            self._workspaces[shape] = need
+            _remember(self._workspaces, shape, need)
         return need
+
+    def _chunk_workspace_bytes(self, *shape):
+        need = self._chunk_workspaces.get(shape)
+        if need is None:
+            need = _lib.lib().mt_paged_chunk_attention_workspace_bytes(self._ref, *shape)
+            _remember(self._chunk_workspaces, shape, need)
+        return need
+
+
+def _remember(sizes, shape, need):
+    if len(sizes) >= 256:
+        sizes.clear()
+    sizes[shape] = need
 
 
 class PagedStep(NamedTuple):
@@ -373,15 +386,10 @@ def paged_chunk_attention(query, cache, block_tables, lengths, starts, *, scale=
 
 
 def _attend_chunks(cache, args, *shape):
-    lib, need = _lib.lib(), cache._workspaces.get(shape)
-    if need is None:  # (as many shapes as there are sizes of steps)
-        need = lib.mt_paged_chunk_attention_workspace_bytes(cache._ref, *shape)
-        if len(cache._workspaces) >= 256:
-            cache._workspaces.clear()
-        cache._workspaces[shape] = need
+    need = cache._chunk_workspace_bytes(*shape)
     ws = _scratch(cache._device, need)
-    status = lib.mt_paged_chunk_attention(cache._ref, args, ws.data_ptr(), need,
-                                          _stream_handle(cache._device))
+    status = _lib.lib().mt_paged_chunk_attention(cache._ref, args, ws.data_ptr(), need,
+                                                 _stream_handle(cache._device))
     if status:
         _lib.check(status)
 
