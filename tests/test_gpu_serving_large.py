@@ -132,3 +132,65 @@ def test_parts_of_more_blocks_than_fp32_counts():
     assert float((lse - want_lse - blocks[:, None]).abs().max()) <= 2.0 ** -8 + 2.0 ** -16
     assert float((out.float() - want.float()).abs().max()) <= (2.0 ** -7 + 2.0 ** -7) * float(
         cache.value.abs().max())
+
+
+def test_pools_of_nearly_2_31_pages():
+    """Pages of one token, the highest numbers in use, freed and compacted."""
+    pages = MOST
+    rows = [[pages - 1, 7, pages - 3], [pages - 3, 1 << 30, -1]]
+    tables, lengths, start = i32(rows), i32([3, 2]), i32([4])
+    listed = [-1, -1, -1, -1, pages - 2, 5, 1 << 20, 3]
+    free = i32(listed)
+    freed = mt.paged_free(tables, lengths, i32([1, 1]), free, page_size=1, pages=pages, free_start=start)
+    assert freed.tolist() == [2]  # (the second keeps what the first gives up)
+    assert free.tolist() == [-1, -1, 7, 1 << 30] + listed[4:]
+    plan = mt.paged_compact(tables, lengths, i32(listed), page_size=1, pages=pages, free_start=start)
+    # in use 7, 2^30, and two of the highest; free 3, 5, 2^20 and the highest but one
+    assert plan.moves.tolist() == [3]
+    assert plan.sources.tolist() == [pages - 1, pages - 3, 1 << 30, -1, -1, -1]
+    assert plan.targets.tolist() == [3, 5, 1 << 20, -1, -1, -1]
+    assert plan.block_tables.tolist() == [[3, 7, 5], [5, 1 << 20, -1]]
+    assert plan.free_pages.tolist() == [-1, -1, -1, -1, 1 << 30, pages - 3, pages - 2, pages - 1]
+
+
+def test_many_forks_in_a_replayed_graph():
+    live, forks, page = 50, 3000, 4
+    tables = torch.zeros(live + forks, 3, dtype=torch.int32, device="cuda")
+    lengths = torch.zeros(live + forks, dtype=torch.int32, device="cuda")
+    sources = torch.zeros(forks, dtype=torch.int32, device="cuda")
+    targets = live + torch.arange(forks, dtype=torch.int32, device="cuda")
+    free, start = torch.arange(forks, device="cuda").int(), i32([0])
+
+    def call():
+        return mt.paged_fork(tables, lengths, sources, targets, free, page_size=page, free_start=start)
+
+    def fill(seed):
+        g = torch.Generator("cuda").manual_seed(seed)
+        tables.copy_(torch.randint(0, 900, tables.shape, generator=g, device="cuda"))
+        lengths.copy_(torch.randint(0, 12, lengths.shape, generator=g, device="cuda"))
+        sources.copy_(torch.randint(-3, live, sources.shape, generator=g, device="cuda"))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = call()
+    torch.cuda.synchronize()
+    for seed in range(4):
+        fill(seed)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        after = [t.clone() for t in (*got, tables, lengths)]
+        fill(seed)
+        eager = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(after, (*eager, tables, lengths)))
+        source, known = sources.clamp(min=0).long(), sources >= 0
+        begun = known & (lengths[source] % page > 0)
+        assert int(eager.taken) == int(begun.sum())
+        before = (begun.long().cumsum(0) - begun.long()).int()
+        assert torch.equal(eager.targets, torch.where(begun, before, -1))
