@@ -6,7 +6,7 @@
 // than total / target blocks are split. Up to 64 requests are counted up by every wave of the attention
 // for itself (a draft of 6 tokens over 2049 keys 25.7 -> 21.4 us without a launch before it), more by
 // a launch of one workgroup, in whose sums the attention's then search. A last launch joins the parts, a
-// workgroup a tile (that draft 16.9 -> 14.1 us with smaller parts; over 131072 keys 99 -> 44).
+// workgroup a tile (that draft 16.9 -> 14.2 us with smaller parts; over 131072 keys 99 -> 44).
 #include <algorithm>
 
 #include "chunk_attention.h"

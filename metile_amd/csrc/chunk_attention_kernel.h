@@ -19,14 +19,16 @@
 // f16), as the result itself is; a second part of them would add half as many products again. Scores,
 // references, sums and results are fp32, and the sums are of the probabilities before that rounding.
 //
-// What bounds it: the matrix and the vector unit, each busy half of the time and together nearly all of it
-// (heads of 128: 32 products and 190 vector instructions a wave and block), and beneath them the power: the
-// same launch over zeros takes 0.73 of the time. A prompt of 8192 tokens, 32 heads of 128 over 8, in bf16,
-// takes 548 us (1000 TFLOP/s; a library's product of 8192 x 8192 x 8192 reaches 1225), 509 tokens behind
-// 130500 take 1108 us (984). 1024 tokens behind 16384 run at 860 TFLOP/s in heads of 128, 690 in those of
-// 64, whose products have half the steps for the same exponentials, and 575 and 675 in those of 192 and 256,
-// whose wave fills the registers of a SIMD (256 with results in accumulation registers: 531). Three waves a SIMD instead of two for heads of 64 were slower (24 parts of
-// prompts 54 -> 61 us), as were two and three parts for each slot.
+// What bounds it: the matrix and the vector unit, each busy a little more than half of the time (heads of 128:
+// 32 products and 190 vector instructions a wave and block), and beneath them the power: the same launch over
+// zeros takes 0.73 of the time. A prompt of 8192 tokens, 32 heads of 128 over 8, in bf16, takes 558 us (986
+// TFLOP/s; a library's product of 8192 x 8192 x 8192 reaches 1271), 509 tokens behind 130500 take 1098 us
+// (993). 1024 tokens behind 16384 in a stream of 600 calls, in which that product reaches 1412 TFLOP/s: 953 in
+// 32 heads of 128 over 8, 787 in 24 of 96 over 3, 673 in 16 of 80, 754 in 32 of 64 over 8, whose products have
+// half the steps for the same exponentials, 704 in 20 of 192 over 5 and 833 in 16 of 256 over 1, whose wave
+// fills the registers of a SIMD (256 with results in accumulation registers: 1.27 times the time); over 8-bit
+// caches 3% less to 1% more. Three waves a SIMD instead of two for heads of 64 were slower (24 parts of prompts
+// 54 -> 61 us), as were two and three parts for each slot.
 #pragma once
 
 #include <algorithm>
@@ -160,7 +162,8 @@ __device__ __forceinline__ Item find_here(const ChunkAttentionArgs& a, int n, in
     const float even = total * 1.0001f / (float)a.target;  // blocks of an item, if all were the same
     per = max((int)fminf(even + 1.0f, 1073741824.0f), least_blocks(total));
     // (us of 1024 tokens behind 16384 without and with the choice: 14 heads of 64 on 2 129 and 108, 24 of 96 on
-    // 3 261 and 221, 20 of 192 on 5 588 and 460)
+    // 3 261 and 221, 20 of 192 on 5 588 and 460; for 2 to 8 requests, a choice a time over all of them, it cost
+    // more than it gave: 3 prompts 60 and 77)
     if (a.requests == 1 && even > 16.0f)
       per = best_parts(a, lane, even, per, readlane(tiles, 0), readlane(most, 0));
     if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = per;
@@ -237,7 +240,7 @@ __device__ __forceinline__ u32x4 fp8_eight(u32x2 w) {
         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true))};
 }
 
-// Two 16-bit floats, 0 in place of infinities and NaN; and whether there is any.
+// Two 16-bit floats, 0 in place of infinities and NaN.
 template <int DT>
 __device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
   constexpr uint32_t kExponent = DT == kBF16 ? 0x7f80u : 0x7c00u;

@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kCountThreads) void count_forks_kernel(PagedForkArg
 }
 
 // A workgroup a fork. Each counts the forks before its own that take a page, unless they have been counted.
-// Round trips bound it: a fork 2.2 us, 256 5.1.
+// Round trips bound it: a fork 2.5 us, 256 5.1.
 template <bool kCounted>
 __global__ __launch_bounds__(kThreads) void fork_kernel(PagedForkArgs a, DivMagic by_page) {
   __shared__ int lds[kWaves];
@@ -267,7 +267,8 @@ __device__ __forceinline__ Pair scan_pair(Pair v, Pair* total, Pair (*lds)) {
   *total = all;
   return {before.a + s.a - v.a, before.b + s.b - v.b};
 }
-// Sums of the blocks' counts before this one, and of all.
+// Sums of the blocks' counts before this one, and of all. (Every workgroup reads all counts: nothing beside a
+// launch in ordinary pools, 7.6 ms a call in one of 2^28 pages, 0.57 s in one of 2^31 - 1.)
 __device__ __forceinline__ Pair blocks_before(const Pair* counts, int blocks, Pair* total, Pair* lds) {
   Pair before{0, 0}, all{0, 0};
   for (int i = threadIdx.x; i < blocks; i += kThreads) {
